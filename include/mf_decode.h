@@ -76,6 +76,62 @@ int mf_swap_blocks(void* host_cache, void* device_cache, const int64_t* pairs, i
                    int64_t block_bytes, int64_t host_blocks, int64_t device_blocks, int device_to_host,
                    void* stream);
 
+/* ---- blocks that sequences share (beam search) ------------------------------------------------------- */
+
+/* Block tables of a step that goes on from `parents`: int32 tables [rows, width] (-1 = no block) and lens [rows] (tokens in the
+ * cache) -> tables_out, lens_out, new tensors of the same shapes.  No counterpart in the reference, whose block tables
+ * (mindformers/modules/block_tables.py:24-126) share nothing.  The tables are the only state: a block is in use if an entry names it.
+ *   - row s continues row parents[s] (NULL: itself); a parent outside [0, rows) leaves the row empty (-1, length 0): its blocks are
+ *     given back.  Entries behind the length, and outside [0, num_blocks), become -1.
+ *   - a last block that is not full is open: the lowest child keeps it, every other child gets a block of its own and the
+ *     list `copies` int32 [rows, 3] an entry (its parent's block, its own, rows to copy); entries in row order, then (-1, -1, 0).
+ *   - window > 0: entries whose tokens all lie in front of the window of the next query (which sits at the old length and sees
+ *     `window` tokens with itself) become -1, but for those with one of the first `sinks` tokens.
+ *   - new_tokens more tokens a row: blocks for them, their slots int32 [rows, new_tokens] (-1: none), lens_out = length + new_tokens
+ *     (at most width * block_size).
+ *   - new blocks are the lowest that no kept entry names and `held` (a byte a block, may be NULL: blocks of other tables) does
+ *     not mark, handed out row by row: in a row the copied open block first.  Where they, or the table's width, do not suffice, the
+ *     entries stay -1 and *missing counts them.
+ * Distinct rows must not share an open block in `tables` unless one is copied from the other by this call.  num_blocks <= 2^20;
+ * workspace: mf_fork_blocks_workspace_bytes. */
+size_t mf_fork_blocks_workspace_bytes(int rows, int block_size, int new_tokens);
+int mf_fork_blocks(int32_t* tables_out, int32_t* lens_out, int32_t* slots, int32_t* copies, int32_t* missing,
+                   const int32_t* tables, const int32_t* lens, const int32_t* parents, const uint8_t* held, int rows, int width,
+                   int num_blocks, int block_size, int new_tokens, int window, int sinks, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* Closes up a pool: the n blocks that the tables name and `held` does not mark (*live = n) go to the n lowest blocks that are
+ * not held; one that is there stays, the others go, ascending, to the blocks left, ascending.  copies int32
+ * [num_blocks / 2, 3]: (source, destination, block_size), then (-1, -1, 0).  tables_out may be tables. */
+size_t mf_compact_blocks_workspace_bytes(int num_blocks);
+int mf_compact_blocks(int32_t* tables_out, int32_t* copies, int32_t* live, const int32_t* tables, const uint8_t* held,
+                      int rows, int width, int num_blocks, int block_size, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/* Copies within caches [num_blocks, block_size, row] of any number of layers: for every entry (source, destination, rows) of the
+ * DEVICE list copies int32 [n_copies, 3], up to the first negative source, the first `rows` token rows of block `source` to block
+ * `destination`, in each of the caches.  host_caches / host_row_bytes: HOST arrays [n_caches] of device pointers and of bytes per
+ * token row.  A destination must not be named by another entry (the entries are copied in no order).  Entries outside the
+ * caches are skipped. */
+int mf_copy_blocks(void* const* host_caches, const int32_t* host_row_bytes, int n_caches, const int32_t* copies, int n_copies,
+                   int num_blocks, int block_size, void* stream);
+
+/* ---- beam search --------------------------------------------------------------------------------------- */
+
+/* The n best continuations of every group of beams, over (beam, token):
+ *     score(b, v) = beam_scores[b] + log_softmax(logits[b])[v]          ties to the lowest b * vocab + v
+ * logits [groups * beams, vocab] (dtype MF_BF16 / MF_FP16 / MF_FP32, rows row_stride elements apart, 0 = dense), beam_scores fp32
+ * [groups, beams].  scores fp32, beam_ids, tokens int32 [groups, n], best first; next_scores, next_rows (group * beams + beam),
+ * next_tokens [groups, beams]: the first `beams` of them whose token is not eos (eos < 0: the first ones).  Scores are compared in
+ * float64 (tokens of one beam by their logits) and rounded once.  A NaN logit counts as -inf, +inf as the largest float; a
+ * beam whose running score is not in (-1e30, 1e30) is out: its candidates score -inf.  beams, n <= 64; n >= beams, with
+ * eos >= 0 n >= 2 beams. */
+size_t mf_beam_search_workspace_bytes(int groups, int beams, int vocab, int n, int dtype);
+int mf_beam_search_select(float* scores, int32_t* beam_ids, int32_t* tokens, float* next_scores, int32_t* next_rows,
+                          int32_t* next_tokens, const void* logits, int64_t row_stride, const float* beam_scores, int groups,
+                          int beams, int vocab, int n, int eos, int dtype, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
 /* ---- paged attention (decode) --------------------------------------------------------------------- */
 
 /* Bytes of scratch mf_paged_attention_decode needs for this shape (0 when the context fits one partition). */

@@ -25,6 +25,13 @@ SIGNATURES = {
     "mf_rope_rows": (_I, [_P, _P, _P, _P, _I, _I, _I, _P]),
     "mf_rope_and_cache": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _L, _L, _L, _L, _I, _I, _P]),
     "mf_swap_blocks": (_I, [_P, _P, _P, _L, _L, _L, _L, _I, _P]),
+    "mf_fork_blocks_workspace_bytes": (_Z, [_I, _I, _I]),
+    "mf_fork_blocks": (_I, [_P] * 9 + [_I] * 7 + [_P, _Z, _P]),
+    "mf_compact_blocks_workspace_bytes": (_Z, [_I]),
+    "mf_compact_blocks": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _Z, _P]),
+    "mf_copy_blocks": (_I, [_P, _P, _I, _P, _I, _I, _I, _P]),
+    "mf_beam_search_workspace_bytes": (_Z, [_I, _I, _I, _I, _I]),
+    "mf_beam_search_select": (_I, [_P] * 7 + [_L, _P] + [_I] * 6 + [_P, _Z, _P]),
     "mf_paged_attention_workspace_bytes": (_Z, [_I, _I, _I, _I]),
     "mf_paged_attention_decode_dynamic_quant": (_I, [_P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I,
                                                      _F, _L, _I, _P, _Z, _P]),

@@ -4,7 +4,10 @@ Each wrapper checks shapes, dtypes, contiguity and device on the host (a kernel 
 not expect can fault the GPU), allocates the output with torch (device-memory plumbing only) and enqueues
 the kernel on torch's current stream.  Nothing is computed in Python.
 """
+import contextlib
+import ctypes
 import math
+from typing import NamedTuple
 
 import torch
 
@@ -62,6 +65,14 @@ def _dev_of(*tensors):
         elif t.device != dev:
             raise ValueError("all tensors must be on the same device")
     return dev
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(dev):
+    """A context in which kernels go to ``dev``: its default stream has the handle of every device's, so the current device decides."""
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def rows_of(x, width):
@@ -636,6 +647,184 @@ def swap_cache(host_cache, device_cache, block_mapping, is_device_to_host):
     check(lib.mf_swap_blocks(host_cache.data_ptr(), ptr(device_cache), pairs.ctypes.data, pairs.shape[0], block_bytes,
                              host_cache.shape[0], device_cache.shape[0], int(bool(is_device_to_host)),
                              stream_ptr(dev)), "mf_swap_blocks")
+
+
+# --------------------------------------------------------------------------------------------- shared blocks, beam search
+class ForkedBlocks(NamedTuple):
+    """What ``fork_blocks`` returns, all int32: block_tables [S, M], context_lens [S], slot_mapping [S * new_tokens] (-1 = none),
+    copies [S, 3] (source block, destination block, rows; unused entries (-1, -1, 0) behind the used ones), missing [1]."""
+    block_tables: torch.Tensor
+    context_lens: torch.Tensor
+    slot_mapping: torch.Tensor
+    copies: torch.Tensor
+    missing: torch.Tensor
+
+
+def _table_args(block_tables, num_blocks, held):
+    dev = _dev_ok(block_tables, held)
+    _need(block_tables.dtype == torch.int32 and block_tables.dim() == 2 and block_tables.numel() > 0,
+          "block_tables must be a non-empty int32 [rows, max_blocks]")
+    if not 0 < num_blocks <= 1 << 20:
+        raise ValueError(f"num_blocks must be 1 to {1 << 20}, got {num_blocks}")
+    _need(held is None or (held.dtype in (torch.bool, torch.uint8) and held.dim() == 1 and held.numel() == num_blocks),
+          "held must be bool or uint8 [num_blocks]")
+    return dev
+
+
+def fork_blocks(block_tables, context_lens, num_blocks, block_size, parents=None, new_tokens=0, window=None, sinks=0, held=None):
+    """The block tables of a step in which row s goes on from row ``parents[s]`` (None: from itself) and gets ``new_tokens`` more
+    tokens: the device-side form of ``BlockTables`` for sequences that share blocks, without a host synchronisation.
+
+    ``context_lens`` int32 [S] counts the tokens in the cache before the step.  A parent outside [0, S) leaves the row empty and gives
+    its blocks back.  Full blocks are shared; a block that is not full goes to the lowest child of a row, the others get blocks of
+    their own, to be filled with ``copy_blocks(caches, copies)`` before the step writes.  With a ``window`` the blocks behind the
+    one of the step's first new token are given back too, but for those of the first ``sinks`` tokens.  New blocks are the
+    lowest ids that the kept entries do not name and ``held`` (bool or uint8 [num_blocks], blocks of other tables) does not
+    mark.  Nothing is changed in place; rows that found no block have -1 entries and slots, and ``missing`` counts them."""
+    lib = _lib.load()
+    dev = _table_args(block_tables, num_blocks, held)
+    s, m = block_tables.shape
+    for t, name in ((context_lens, "context_lens"), (parents, "parents")):
+        if t is not None:
+            if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.dim() == 1 and t.numel() == s and t.is_contiguous()):
+                raise ValueError(f"{name} must be a contiguous int32 [{s}]")
+            _need(t.device == dev, "all tensors must be on the same device")
+    _need(block_size > 0 and new_tokens >= 0 and sinks >= 0, "block_size must be positive, new_tokens and sinks not negative")
+    _need(window is None or window > 0, "window must be positive (None: no window)")
+    _need(window is not None or sinks == 0, "sinks go with a window")
+    out = torch.empty(s * (m + new_tokens + 4) + 1, dtype=torch.int32, device=dev)
+    a, b, c, d = s * m, s * (m + 1), s * (m + 4), s * (m + 4) + 1
+    res = ForkedBlocks(out[:a].view(s, m), out[a:b], out[d:], out[b:c].view(s, 3), out[c:d])
+    need = lib.mf_fork_blocks_workspace_bytes(s, block_size, new_tokens)
+    ws = workspace(need, dev, "fork")
+    at = out.data_ptr()
+    with _on(dev):
+        check(lib.mf_fork_blocks(at, at + 4 * a, at + 4 * d, at + 4 * b, at + 4 * c, ptr(block_tables), ptr(context_lens), ptr(parents),
+                                 ptr(held), s, m, num_blocks, block_size, new_tokens, min(window or 0, 0x7fffffff), min(sinks, 0x7fffffff),
+                                 ptr(ws), ws.numel(), stream_ptr(dev)), "mf_fork_blocks")
+    return res
+
+
+def compact_blocks(block_tables, num_blocks, block_size, held=None):
+    """Plan that closes up a cache's pool: the n blocks in use move to the n lowest ids that are not ``held``.  Returns
+    (block_tables [S, M], copies [num_blocks // 2, 3] for ``copy_blocks``, live [1] = n), int32.  The tables hold once the
+    copies are made; blocks that the new tables do not name are free, blocks held by others stay where they are."""
+    lib = _lib.load()
+    dev = _table_args(block_tables, num_blocks, held)
+    _need(block_size > 0, "block_size must be positive")
+    s, m = block_tables.shape
+    most = num_blocks // 2
+    out = torch.empty(s * m + 3 * most + 1, dtype=torch.int32, device=dev)
+    tables, copies, live = out[:s * m].view(s, m), out[s * m:-1].view(most, 3), out[-1:]
+    ws = workspace(lib.mf_compact_blocks_workspace_bytes(num_blocks), dev, "compact")
+    with _on(dev):
+        check(lib.mf_compact_blocks(ptr(tables), ptr(copies), ptr(live), ptr(block_tables), ptr(held), s, m, num_blocks, block_size,
+                                    ptr(ws), ws.numel(), stream_ptr(dev)), "mf_compact_blocks")
+    return tables, copies, live
+
+
+def copy_blocks(caches, copies):
+    """Copy blocks within each of ``caches`` (tensors [num_blocks, block_size, ...] of one geometry: the key and value caches of
+    all layers, int8 caches with their scale caches), in one launch.  ``copies``: the list of ``fork_blocks`` /
+    ``compact_blocks``, int32 [n, 3] on the device (source, destination, rows; it ends at the first negative source), or host
+    integers [n, 2] (whole blocks) or [n, 3].  A block that one entry writes must not be named by another: a host list is
+    checked, a device list is taken at its word."""
+    lib = _lib.load()
+    caches = list(caches)
+    _need(len(caches) > 0, "caches must not be empty")
+    dev = _dev_ok(*caches)
+    first = caches[0].shape[:2]
+    nb, bs = first if len(first) == 2 else (0, 0)
+    _need(nb > 0 and bs > 0, "caches must be [num_blocks, block_size, ...]")
+    rows = []
+    for c in caches:
+        _need(c.shape[:2] == first and c.numel() > 0, "all caches must share num_blocks and block_size")
+        rows.append(c.numel() // (nb * bs) * c.element_size())
+    if not (isinstance(copies, torch.Tensor) and copies.is_cuda):
+        copies = _host_copies(copies, nb, bs)
+        if copies.shape[0] == 0:
+            return
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a host list of copies cannot be captured: a replay would read it from a buffer given back")
+        copies = torch.from_numpy(copies).pin_memory().to(dev, non_blocking=True)
+    _need(copies.dtype == torch.int32 and copies.dim() == 2 and copies.shape[1] == 3 and copies.is_contiguous() and copies.device == dev,
+          "copies must be a contiguous int32 [n, 3] on the caches' device, or host integers")
+    n = len(caches)
+    with _on(dev):
+        check(lib.mf_copy_blocks((ctypes.c_void_p * n)(*[c.data_ptr() for c in caches]), (ctypes.c_int32 * n)(*rows), n, ptr(copies),
+                                 copies.shape[0], nb, bs, stream_ptr(dev)), "mf_copy_blocks")
+
+
+def _host_copies(copies, nb, bs):
+    """A host list as int32 [n, 3], checked."""
+    import numpy as np
+    a = np.asarray(copies.numpy() if isinstance(copies, torch.Tensor) else copies)
+    if a.size == 0:
+        return np.zeros((0, 3), np.int32)
+    _need(a.ndim == 2 and a.shape[1] in (2, 3) and a.dtype.kind in "iu", "copies must be integers [n, 2] or [n, 3]")
+    if a.shape[1] == 2:
+        a = np.concatenate([a, np.full((len(a), 1), bs)], axis=1)
+    a = a.astype(np.int64)
+    if not (a[:, :2].min() >= 0 and a[:, :2].max() < nb and a[:, 2].min() >= 0 and a[:, 2].max() <= bs):
+        raise ValueError(f"copies name blocks outside [0, {nb}) or more than {bs} rows")
+    dst = a[:, 1]
+    if len(np.unique(dst)) != len(dst) or np.isin(dst, a[:, 0]).any():
+        raise ValueError("a block that is written must not be named by another entry")
+    return np.ascontiguousarray(a.astype(np.int32))
+
+
+class BeamSelection(NamedTuple):
+    """What ``beam_search_select`` returns: the candidates [B, n], best first (scores fp32, beams and tokens int32), and the K of them
+    that go on [B, K]: next_scores fp32, next_rows int32 (the row b * K + beam that each goes on from), next_tokens int32."""
+    scores: torch.Tensor
+    beams: torch.Tensor
+    tokens: torch.Tensor
+    next_scores: torch.Tensor
+    next_rows: torch.Tensor
+    next_tokens: torch.Tensor
+
+
+def beam_search_select(logits, beam_scores, eos_token_id=-1, n_candidates=None):
+    """One step of beam search over B groups of K beams: the ``n_candidates`` (default 2 K) best of
+    beam_scores[b, k] + log_softmax(logits[b * K + k])[v] over (k, v), ties to the lowest k * vocab + v, and the first K of them
+    whose token is not ``eos_token_id`` (negative: no such token).  logits [B * K, vocab] or [B, K, vocab], bf16, fp16 or fp32,
+    may be a slice of wider rows; beam_scores fp32 [B, K].  NaN logits count as -inf; a beam whose score is -inf, NaN or beyond
+    +-1e30 is out of the search: its candidates score -inf."""
+    lib = _lib.load()
+    dev = _dev_of(logits, beam_scores)
+    _need(beam_scores.dtype == torch.float32 and beam_scores.dim() == 2 and beam_scores.is_contiguous(),
+          "beam_scores must be a contiguous fp32 [groups, beams]")
+    g, k = beam_scores.shape
+    _need(logits.dtype in _ACT or logits.dtype == torch.float32, "logits must be bf16, fp16 or fp32")
+    if logits.dim() == 3:
+        _need(logits.shape[:2] == (g, k) and (logits.stride(0) == k * logits.stride(1) or g == 1),
+              "logits must be [groups, beams, vocab] with evenly spaced rows")
+        v, stride = logits.shape[2], logits.stride(1)
+    else:
+        _need(logits.dim() == 2 and logits.shape[0] == g * k, "logits must hold a row for every beam")
+        v, stride = logits.shape[1], logits.stride(0)
+    if g * k == 1:
+        stride = v                                            # one row: whatever its stride says
+    _need(v > 0 and (logits.stride(-1) == 1 or v == 1) and stride >= v, "logits rows must have a unit column stride and not overlap")
+    n = 2 * k if n_candidates is None else int(n_candidates)
+    eos = -1 if eos_token_id is None else int(eos_token_id)
+    if not (1 <= k <= 64 and k * (2 if eos >= 0 else 1) <= n <= min(64, k * v)):
+        raise ValueError(f"{n} candidates of {k} beams and {v} tokens: one a beam at least (two with an end token), 64 or all at most")
+    scores = torch.empty((g * (n + k),), dtype=torch.float32, device=dev)
+    ids = torch.empty((2 * g * (n + k),), dtype=torch.int32, device=dev)
+    gn, gk = g * n, g * k
+    res = BeamSelection(scores[:gn].view(g, n), ids[:gn].view(g, n), ids[gn:2 * gn].view(g, n), scores[gn:].view(g, k),
+                        ids[2 * gn:2 * gn + gk].view(g, k), ids[2 * gn + gk:].view(g, k))
+    if g == 0:
+        return res
+    code = dtype_code(logits.dtype)
+    ws = workspace(lib.mf_beam_search_workspace_bytes(g, k, v, n, code), dev, "beam")
+    a, i = scores.data_ptr(), ids.data_ptr()
+    with _on(dev):
+        check(lib.mf_beam_search_select(a, i, i + 4 * gn, a + 4 * gn, i + 8 * gn, i + 8 * gn + 4 * gk, ptr(logits), stride,
+                                        ptr(beam_scores), g, k, v, n, eos, code, ptr(ws), ws.numel(), stream_ptr(dev)),
+              "mf_beam_search_select")
+    return res
 
 
 # --------------------------------------------------------------------------------------------- norm / activation
