@@ -181,6 +181,33 @@ int mf_paged_attention_decode_static(void* out, const void* query, const void* k
                                      int max_blocks_per_seq, int num_blocks, float scale, int64_t q_row_stride,
                                      int dtype, void* stream);
 
+/* ---- attention through a sliding window with sinks ---------------------------------------------------- */
+
+/* mf_paged_attention_decode and its forms where a query at position p sees the tokens j <= p with j > p - window (`window` tokens
+ * with its own) or j < sinks, at their own positions.  FlashAttentionScore's band (sparse_mode 4, pre_tokens = window - 1,
+ * mindformers/parallel_core/inference/transformer/flash_attention.py:96-104) plus the first tokens, which keep the softmax's weight
+ * where training put it.  Entries of the block table whose block holds no visible token are not read (-1 where the block was given
+ * back), nor are the cache rows of hidden tokens.  kv_quant: 0 = 16-bit caches, 1 = int8 with key_scale = antiquant_scale
+ * [2, n_kv * D] and value_scale = antiquant_offset (may be NULL), 2 = int8 with one key and one value scale per slot.  xq (may be
+ * NULL; 16-bit caches), x_scale, smooth, xq_layout: as mf_paged_attention_decode_dynamic_quant. */
+size_t mf_window_attention_workspace_bytes(int batch, int n_heads, int head_dim, int max_context, int window, int sinks);
+int mf_window_attention_decode(void* out, int8_t* xq, float* x_scale, const float* smooth, int xq_layout, const void* query,
+                               const void* key_cache, const void* value_cache, const float* key_scale,
+                               const float* value_scale, int kv_quant, const int32_t* block_tables,
+                               const int32_t* context_lens, int batch, int n_heads, int n_kv_heads, int head_dim,
+                               int block_size, int max_blocks_per_seq, int num_blocks, float scale, int window, int sinks,
+                               int64_t q_row_stride, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+/* The same for several query rows per sequence: mf_paged_attention_prefill and its int8 forms (packed rows with block_tables ==
+ * NULL, 16-bit only).  head_dim 32, 64 or 128.  max_context as for mf_paged_attention_prefill_workspace_bytes. */
+size_t mf_window_attention_prefill_workspace_bytes(int batch, int total_q, int n_heads, int n_kv_heads, int head_dim,
+                                                   int max_context, int window, int sinks);
+int mf_window_attention_prefill(void* out, const void* query, const void* key, const void* value, const float* key_scale,
+                                const float* value_scale, int kv_quant, const int32_t* block_tables,
+                                const int32_t* context_lens, const int32_t* q_starts, int batch, int total_q, int n_heads,
+                                int n_kv_heads, int head_dim, int block_size, int max_blocks_per_seq, int num_blocks,
+                                float scale, int window, int sinks, int64_t q_row_stride, int64_t kv_row_stride, int dtype,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- int8 KV cache (kvcache_dtype = int8, per-channel) ------------------------------------------------ */
 
 /* The reference sizes an int8 cache (mindformers/model_runner.py:364-368, kvcache_dtype in the quantization

@@ -37,6 +37,10 @@ SIGNATURES = {
                                                      _F, _L, _I, _P, _Z, _P]),
     "mf_paged_attention_decode": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _L, _I, _P, _Z, _P]),
     "mf_paged_attention_decode_static": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _L, _I, _P]),
+    "mf_window_attention_workspace_bytes": (_Z, [_I] * 6),
+    "mf_window_attention_decode": (_I, [_P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I, _P, _P] + [_I] * 7 + [_F, _I, _I, _L, _I, _P, _Z, _P]),
+    "mf_window_attention_prefill_workspace_bytes": (_Z, [_I] * 8),
+    "mf_window_attention_prefill": (_I, [_P] * 6 + [_I] + [_P] * 3 + [_I] * 8 + [_F, _I, _I, _L, _L, _I, _P, _Z, _P]),
     "mf_quant_reshape_and_cache": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _L, _L, _L, _I, _P]),
     "mf_paged_attention_decode_int8kv": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _L, _I, _P,
                                               _Z, _P]),

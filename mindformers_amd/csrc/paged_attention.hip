@@ -40,29 +40,44 @@ struct PaQuantArgs {
     int layout;
 };
 
-template <typename T, int D, int KVQ>
+// Tokens a partition and partitions of a decode step with a window, over contexts of up to max_ctx tokens.
+struct PaWinPlan {
+    int part_tokens, max_parts;
+};
+static inline PaWinPlan pa_win_plan(int64_t max_ctx, int kvq, int64_t batch_kv_groups, PaWindow win) {
+    const int64_t walk = pa_win_tiles(max_ctx, 1, win) * PA_TILE;
+    const int part = pa_launch_tiles_per_wave(walk, kvq, batch_kv_groups) * PA_WAVE_TOKENS;
+    return {part, (int)((walk + part - 1) / part)};
+}
+
+template <typename T, int D, int KVQ, bool WIN = false>
 int launch_pa(void* out, const void* query, const void* key_cache, const void* value_cache,
               const int32_t* block_tables, const int32_t* context_lens, int batch, int n_heads, int n_kv,
               int block_size, int max_blocks, int num_blocks, float scale, int64_t q_stride, void* workspace,
-              hipStream_t st, const float* kv_scale, const float* kv_offset, const PaQuantArgs* qa = nullptr) {
+              hipStream_t st, const float* kv_scale, const float* kv_offset, const PaQuantArgs* qa = nullptr, PaWindow win = {}) {
     const int n_rep = n_heads / n_kv;
     const int head_groups = (n_rep + 15) / 16;
     const int64_t max_ctx = (int64_t)max_blocks * block_size;
-    const int tpw = pa_launch_tiles_per_wave(max_ctx, KVQ, (int64_t)batch * n_kv * head_groups);
-    const int part_tokens = tpw * PA_WAVE_TOKENS;
-    const int max_parts = (int)((max_ctx + part_tokens - 1) / part_tokens);
+    const int tpw = WIN ? 0 : pa_launch_tiles_per_wave(max_ctx, KVQ, (int64_t)batch * n_kv * head_groups);
+    PaWinPlan plan = {tpw * PA_WAVE_TOKENS, 0};
+    if constexpr (WIN) plan = pa_win_plan(max_ctx, KVQ, (int64_t)batch * n_kv * head_groups, win);
+    const int part_tokens = plan.part_tokens;
+    const int max_parts = WIN ? plan.max_parts : (int)((max_ctx + part_tokens - 1) / part_tokens);
     float* part_out = (float*)workspace;
     float* part_ml = part_out ? part_out + (int64_t)batch * n_heads * max_parts * D : nullptr;
     const float scale_log2 = scale * 1.4426950408889634f;
     dim3 grid((unsigned)((int64_t)batch * max_parts * n_kv * head_groups));
     const bool tib = block_size % PA_TILE == 0;               // a 32-token tile never straddles two blocks
 #define PA_LAUNCH(TPWV, TIBV)                                                                                    \
-    hipLaunchKernelGGL((paged_attention_kernel<T, D, TPWV, false, KVQ, TIBV>), grid, dim3(PA_WAVES * 64), 0, st,  \
+    hipLaunchKernelGGL((paged_attention_kernel<T, D, TPWV, false, KVQ, TIBV, WIN>), grid, dim3(PA_WAVES * 64), 0, st,  \
                        (uint16_t*)out, part_out, part_ml, (const uint16_t*)query, (const uint16_t*)key_cache,      \
                        (const uint16_t*)value_cache, block_tables, context_lens, n_heads, n_kv, n_rep, head_groups, \
                        block_size, max_blocks, num_blocks, max_parts, scale_log2, q_stride, batch,                 \
-                       (const int32_t*)nullptr, 0, (int64_t)0, 0, kv_scale, kv_offset)
-    if (tpw == 16) {
+                       (const int32_t*)nullptr, WIN ? part_tokens : 0, (int64_t)0, 0, kv_scale, kv_offset, win)
+    if constexpr (WIN) {
+        if (tib) PA_LAUNCH(0, true);
+        else PA_LAUNCH(0, false);
+    } else if (tpw == 16) {
         if (tib) PA_LAUNCH(16, true);
         else PA_LAUNCH(16, false);
     } else if (tpw == 8) {
@@ -80,16 +95,16 @@ int launch_pa(void* out, const void* query, const void* key_cache, const void* v
     if (rc) return rc;
     if (qa && max_parts > 1 && max_parts <= 16 && n_heads * D <= PA_RQ_THREADS * 8) {
         // combine of the partitions and quantisation of the row in one kernel
-        hipLaunchKernelGGL((paged_attention_reduce_quant_kernel<T, D>), dim3(batch), dim3(PA_RQ_THREADS), 0, st,
+        hipLaunchKernelGGL((paged_attention_reduce_quant_kernel<T, D, WIN>), dim3(batch), dim3(PA_RQ_THREADS), 0, st,
                            (uint16_t*)out, qa->xq, qa->x_scale, part_out, part_ml, context_lens, qa->smooth, n_heads,
-                           max_parts, part_tokens, qa->layout);
+                           max_parts, part_tokens, qa->layout, (int)max_ctx, win);
         return MF_LAUNCH_CHECK();
     }
     if (max_parts > 1) {
-        hipLaunchKernelGGL((paged_attention_reduce_kernel<T, D, false>), dim3(n_heads, batch),
+        hipLaunchKernelGGL((paged_attention_reduce_kernel<T, D, false, WIN>), dim3(n_heads, batch),
                            dim3(PA_REDUCE_THREADS<D>), 0, st,
                            (uint16_t*)out, part_out, part_ml, context_lens, n_heads, max_parts, part_tokens,
-                           (const int32_t*)nullptr, batch, false, 0);
+                           (const int32_t*)nullptr, batch, false, WIN ? (int)max_ctx : 0, PaWinCombine{win, n_rep, 1});
         rc = MF_LAUNCH_CHECK();
         if (rc) return rc;
     }
@@ -111,7 +126,8 @@ static int pa_decode_entry(void* out, const void* query, const void* key_cache, 
                            int n_kv_heads, int head_dim, int block_size, int max_blocks_per_seq, int num_blocks,
                            float scale, int64_t q_row_stride, int dtype, void* workspace, size_t workspace_bytes,
                            void* stream, int kvq, const float* kv_scale, const float* kv_offset,
-                           const PaQuantArgs* qa = nullptr) {
+                           const PaQuantArgs* qa = nullptr, PaWindow win = {}) {
+    // win.window 0: the whole context.
     // kvq: 0 = 16-bit caches, 1 = int8 with per-channel scale / offset, 2 = int8 with per-token key scales
     // (kv_scale) and value scales (kv_offset), one float per cache slot
     MF_REQUIRE(dtype == MF_BF16 || dtype == MF_FP16, "paged_attention: dtype must be bf16 or fp16");
@@ -134,16 +150,19 @@ static int pa_decode_entry(void* out, const void* query, const void* key_cache, 
     MF_REQUIRE((((uintptr_t)out | (uintptr_t)query | (uintptr_t)key_cache | (uintptr_t)value_cache) & 15) == 0,
                "paged_attention: out / query / caches must be 16-byte aligned");
     if (batch == 0) return 0;
-    const size_t need = mf_paged_attention_workspace_bytes(batch, n_heads, head_dim, max_blocks_per_seq * block_size);
+    const size_t need =
+        win.window ? mf_window_attention_workspace_bytes(batch, n_heads, head_dim, max_blocks_per_seq * block_size, win.window, win.sinks)
+                   : mf_paged_attention_workspace_bytes(batch, n_heads, head_dim, max_blocks_per_seq * block_size);
     MF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
                "paged_attention: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
     MF_REQUIRE(need == 0 || ((uintptr_t)workspace & 15) == 0, "paged_attention: workspace must be 16-byte aligned");
     hipStream_t st = (hipStream_t)stream;
     void* ws = need ? workspace : nullptr;
-#define PA_CASE_Q(TT, DD, QQ)                                                                                   \
-    return launch_pa<TT, DD, QQ>(out, query, key_cache, value_cache, block_tables, context_lens, batch, n_heads,  \
-                                 n_kv_heads, block_size, max_blocks_per_seq, num_blocks, scale, q_row_stride, ws, st, \
-                                 kvq ? kv_scale : nullptr, kvq ? kv_offset : nullptr, qa)
+#define PA_CASE_W(TT, DD, QQ, WW)                                                                               \
+    launch_pa<TT, DD, QQ, WW>(out, query, key_cache, value_cache, block_tables, context_lens, batch, n_heads,     \
+                              n_kv_heads, block_size, max_blocks_per_seq, num_blocks, scale, q_row_stride, ws, st, \
+                              kvq ? kv_scale : nullptr, kvq ? kv_offset : nullptr, qa, win)
+#define PA_CASE_Q(TT, DD, QQ) return win.window ? PA_CASE_W(TT, DD, QQ, true) : PA_CASE_W(TT, DD, QQ, false)
 #define PA_CASE(TT, DD)                                                                                        \
     {                                                                                                          \
         if (kvq == 2) PA_CASE_Q(TT, DD, 2);                                                                    \
@@ -161,6 +180,7 @@ static int pa_decode_entry(void* out, const void* query, const void* key_cache, 
     }
 #undef PA_CASE
 #undef PA_CASE_Q
+#undef PA_CASE_W
 }
 
 extern "C" int mf_paged_attention_decode(void* out, const void* query, const void* key_cache,
@@ -218,6 +238,38 @@ extern "C" int mf_paged_attention_decode_int8kv_per_token(void* out, const void*
     return pa_decode_entry(out, query, key_cache, value_cache, block_tables, context_lens, batch, n_heads,
                            n_kv_heads, head_dim, block_size, max_blocks_per_seq, num_blocks, scale, q_row_stride,
                            dtype, workspace, workspace_bytes, stream, 2, key_scale_cache, value_scale_cache);
+}
+
+// ---- decode attention through a sliding window with sinks ----------------------------------------------------------
+// The kernels of a full context on another walk over its tiles (PaWindow).
+extern "C" size_t mf_window_attention_workspace_bytes(int batch, int n_heads, int head_dim, int max_context, int window, int sinks) {
+    if (batch <= 0 || n_heads <= 0 || head_dim <= 0 || max_context <= 0 || window <= 0 || sinks < 0) return 0;
+    // the smallest partition that the launch rule may choose
+    const int64_t walk = pa_win_tiles(max_context, 1, {window, sinks}) * PA_TILE;
+    const int part_tokens = pa_tiles_per_wave(walk) * PA_WAVE_TOKENS;
+    const int64_t max_parts = (walk + part_tokens - 1) / part_tokens;
+    if (max_parts <= 1) return 0;
+    return (size_t)batch * n_heads * max_parts * (head_dim + 2) * sizeof(float);
+}
+
+extern "C" int mf_window_attention_decode(void* out, int8_t* xq, float* x_scale, const float* smooth, int xq_layout,
+                                          const void* query, const void* key_cache, const void* value_cache,
+                                          const float* key_scale, const float* value_scale, int kv_quant,
+                                          const int32_t* block_tables, const int32_t* context_lens, int batch, int n_heads,
+                                          int n_kv_heads, int head_dim, int block_size, int max_blocks_per_seq, int num_blocks,
+                                          float scale, int window, int sinks, int64_t q_row_stride, int dtype, void* workspace,
+                                          size_t workspace_bytes, void* stream) {
+    if (batch == 0) return 0;
+    MF_REQUIRE(window > 0 && sinks >= 0, "window_attention: window %d must be positive, sinks %d not negative", window, sinks);
+    MF_REQUIRE(kv_quant >= 0 && kv_quant <= 2, "window_attention: kv_quant must be 0 (16-bit), 1 (per channel) or 2 (per token)");
+    MF_REQUIRE(!xq || (kv_quant == 0 && x_scale && (xq_layout == 0 || xq_layout == 1)),
+               "window_attention: a quantised output needs a 16-bit cache, its scales and a layout of 0 or 1");
+    MF_REQUIRE(((uintptr_t)xq & 7) == 0 && ((uintptr_t)smooth & 15) == 0,
+               "window_attention: xq must be 8-byte aligned, smooth 16-byte aligned");
+    const PaQuantArgs qa = {xq, x_scale, smooth, xq_layout};
+    return pa_decode_entry(out, query, key_cache, value_cache, block_tables, context_lens, batch, n_heads, n_kv_heads, head_dim,
+                           block_size, max_blocks_per_seq, num_blocks, scale, q_row_stride, dtype, workspace, workspace_bytes,
+                           stream, kv_quant, key_scale, value_scale, xq ? &qa : nullptr, PaWindow{window, sinks});
 }
 
 // ---- decode attention for callers that cannot allocate ----------------------------------------------------------

@@ -43,6 +43,46 @@ struct PaSmem {
     static_assert(16 * D * 4 <= PA_TILE * VSTRIDE, "a wave's accumulators must fit its staging tile");
 };
 
+// ---- sliding window with sinks -----------------------------------------------------------------------------------
+// A row at position p sees token j <= p where j > p - window or j < sinks.  The rows of a workgroup sit at consecutive positions, so
+// the tokens that any of them sees are the sinks in front of the first row's window and everything from there to the last
+// row: two runs of 32-token tiles, which the kernels walk as one.  Tile v of a walk is tile v of the sequence while v < ns
+// and tile v - ns + w0 from there on; partitions are cut in this order too.  Tiles between the runs are neither loaded nor
+// looked up (their blocks may have been given back), and the rows of the runs' tiles that no row sees are replaced by one that
+// some row sees, whatever the cache holds there.
+struct PaWindow {
+    int window, sinks;                                        // window 0: none
+};
+struct PaWinRange {
+    int lo, sv;                                               // first token of the first row's window; sinks in front of it
+    int ns, w0, tiles;                                        // tiles with sinks, first tile of the windows, tiles of the walk
+    __device__ __forceinline__ int tile(int v) const { return v < ns ? v : v - ns + w0; }
+};
+__device__ __forceinline__ PaWinRange pa_win_range(int first_pos, int last_pos, PaWindow win) {
+    PaWinRange r;
+    r.lo = first_pos >= win.window ? first_pos - win.window + 1 : 0;
+    r.sv = win.sinks < r.lo ? win.sinks : r.lo;
+    r.ns = (r.sv + PA_TILE - 1) / PA_TILE;
+    r.w0 = r.lo / PA_TILE > r.ns ? r.lo / PA_TILE : r.ns;
+    r.tiles = r.ns + last_pos / PA_TILE + 1 - r.w0;
+    return r;
+}
+// The same for one of `cols` consecutive (query, head of the kv group) columns of a sequence: its queries' positions
+// start at ctx_before.
+__device__ __forceinline__ PaWinRange pa_win_group(int group, int cols, int n_rep, int ctx_before, int q_len, PaWindow win) {
+    const int last = min(q_len, (group * cols + cols - 1) / n_rep + 1) - 1;
+    return pa_win_range(ctx_before + group * cols / n_rep, ctx_before + last, win);
+}
+// Most tiles that a walk over a context of max_ctx tokens takes, for `rows` consecutive rows: a run of n tokens touches
+// (n + 30) / 32 + 1 tiles at most.
+__host__ __device__ __forceinline__ int64_t pa_win_tiles(int64_t max_ctx, int rows, PaWindow win) {
+    const int64_t all = (max_ctx + PA_TILE - 1) / PA_TILE;
+    const int64_t some = ((int64_t)win.sinks + PA_TILE - 1) / PA_TILE + ((int64_t)win.window + rows - 1 + PA_TILE - 2) / PA_TILE + 1;
+    return all < some ? all : some;
+}
+// most rows that `cols` consecutive columns belong to
+__host__ __device__ __forceinline__ int pa_group_rows(int cols, int n_rep) { return (cols - 2 + n_rep) / n_rep + 1; }
+
 // Prefill bookkeeping of sequence s: first query row, number of query rows and context length, made safe
 // (never more queries than context; query rows, and with them contiguous keys, never leave the `rows` passed).
 __device__ inline void pf_seq(int s, const int32_t* __restrict__ q_starts, const int32_t* __restrict__ ctx_lens,
@@ -84,7 +124,9 @@ __device__ __forceinline__ u32x4 pa_stream_load(const uint8_t* p) { return __bui
 // of a token is multiplied by its key scale, its probability by its value scale before it is rounded to T for the PV
 // product (the denominator sums the unscaled probabilities).  The scales of a tile are loaded one tile ahead, like
 // the tile itself.  KVQ = 1 is the per-channel form above, 0 a 16-bit cache.
-template <typename T, int D, int TPW, bool PF, int KVQ, bool TIB>
+// WIN: a sliding window with sinks (see PaWindow); the tile order, and with it part_start and tile numbers, is the walk's, and the
+// partition size is pf_part_tokens in decode too.
+template <typename T, int D, int TPW, bool PF, int KVQ, bool TIB, bool WIN = false>
 // Decode over an int8 cache keeps half the prefetch registers of a 16-bit one and fits four workgroups on a compute
 // unit (128 registers; measured 6 % faster than with three); the 16-bit kernel needs 166 registers for its two
 // prefetched tiles and gained nothing from a one-tile variant that fits four, so it stays at three.
@@ -94,14 +136,14 @@ __global__ __launch_bounds__(PA_WAVES * 64, (!PF && KVQ == 1 && TIB) ? 4 : 3) vo
     const int32_t* __restrict__ block_tables, const int32_t* __restrict__ ctx_lens, int n_heads, int n_kv,
     int n_rep, int head_groups, int block_size, int max_blocks, int num_blocks, int max_parts,
     float scale_log2, int64_t q_stride, int batch, const int32_t* __restrict__ q_starts, int pf_part_tokens,
-    int64_t pf_kv_stride, int pf_rows, const float* __restrict__ kv_scale, const float* __restrict__ kv_offset) {
+    int64_t pf_kv_stride, int pf_rows, const float* __restrict__ kv_scale, const float* __restrict__ kv_offset, PaWindow win) {
     using vec8 = typename T::vec8;
     constexpr bool KV8 = KVQ != 0;
     constexpr int KS = D / 32;
     constexpr int VSTRIDE = PaSmem<D>::VSTRIDE;
     // tokens per partition: fixed by TPW in decode, chosen by the host (a multiple of 128) in PF, where the
     // query rows already supply the parallelism and one partition may span the whole context
-    const int PART = PF ? pf_part_tokens : TPW * PA_WAVE_TOKENS;
+    const int PART = PF || WIN ? pf_part_tokens : TPW * PA_WAVE_TOKENS;
     constexpr int EB = KV8 ? 1 : 2;                           // bytes per cache element
     constexpr int CPR = D * EB / 16;                          // 16-byte chunks per row
     constexpr int RPI = 64 / CPR;                             // rows one wave-wide load covers
@@ -135,6 +177,12 @@ __global__ __launch_bounds__(PA_WAVES * 64, (!PF && KVQ == 1 && TIB) ? 4 : 3) vo
                 len = bb < batch ? min(ctx_lens[bb], max_blocks * block_size) : 0;   // the table holds no more
             }
             int np = len > 0 ? (len + PART - 1) / PART : 0;
+            if constexpr (WIN) {                              // PF: the most of the sequence's column groups
+                if (len > 0) {
+                    const int tiles = PF ? (int)pa_win_tiles(len, pa_group_rows(16, n_rep), win) : pa_win_range(len - 1, len - 1, win).tiles;
+                    np = (tiles * PA_TILE + PART - 1) / PART;
+                }
+            }
             np = np < max_parts ? np : max_parts;
             const int per_seq = np * (PF ? n_kv * ncg : nkg);
             int incl = per_seq;
@@ -214,7 +262,12 @@ __global__ __launch_bounds__(PA_WAVES * 64, (!PF && KVQ == 1 && TIB) ? 4 : 3) vo
     if constexpr (PF) {
         const int last_q = min(q_len, (hg * 16 + 15) / n_rep + 1);
         L = ctx_before + last_q;
-        if (part_start >= L) return;
+        if (!WIN && part_start >= L) return;
+    }
+    PaWinRange wr = {};
+    if constexpr (WIN) {
+        wr = PF ? pa_win_group(hg, 16, n_rep, ctx_before, q_len, win) : pa_win_range(L - 1, L - 1, win);
+        if (part_start >= wr.tiles * PA_TILE) return;
     }
     if (threadIdx.x == 0) sm_count = 0;
     __syncthreads();                                          // the only barrier: all waves are still in step here
@@ -236,6 +289,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, (!PF && KVQ == 1 && TIB) ? 4 : 3) vo
     // tiles that end at or before the smallest limit of the group's live columns need no mask (columns past the
     // sequence's queries are never written)
     const int Lmask = PF ? ctx_before + (hg * 16) / n_rep + 1 : L;
+    [[maybe_unused]] const int lo_col = WIN ? Lcol - win.window : 0;    // the column sees tokens >= lo_col and sinks
     vec8 qreg[KS];
     {
         const uint16_t* qp = q + (int64_t)q_row * q_stride + (int64_t)head * D + 8 * g;
@@ -277,26 +331,35 @@ __global__ __launch_bounds__(PA_WAVES * 64, (!PF && KVQ == 1 && TIB) ? 4 : 3) vo
     int ntiles = 0;
     {
         const int first = part_start + wu * PA_TILE;
-        if (first < L) {
-            const int last_tok = min(L, part_start + PART) - 1;
+        const int end = WIN ? wr.tiles * PA_TILE : L;
+        if (first < end) {
+            const int last_tok = min(end, part_start + PART) - 1;
             ntiles = (last_tok - first) / (PA_WAVES * PA_TILE) + 1;
         }
     }
     // slot of a tile's first token when the tile lies inside one block (uniform: a scalar load), looked up
     // two tiles ahead so that no K/V load ever waits on a table load
     auto tile_slot = [&](int ts) -> int64_t {
-        if (!tile_in_block || ts >= L) return 0;
+        if (!tile_in_block || ts >= (WIN ? wr.tiles * PA_TILE : L)) return 0;
+        if constexpr (WIN) ts = wr.tile(ts / PA_TILE) * PA_TILE;
         if (contiguous) return (int64_t)q_start + ts;
         const int bi = ts / block_size;
         int blk = table[bi];
         blk = (blk < 0 || blk >= num_blocks) ? 0 : blk;       // never leave the cache allocation
         return (int64_t)blk * block_size + (ts - bi * block_size);
     };
+    // WIN: row of tile `ts` (a token) whose values stand in for row `row` where no column sees that one
+    [[maybe_unused]] auto seen_row = [&](int ts, int row) -> int {
+        const int lo = wr.lo - ts, sv = wr.sv - ts;
+        row = lo >= PA_TILE ? min(row, sv - 1) : (row < sv ? row : max(row, lo));
+        return min(row, L - 1 - ts);
+    };
     // byte offset of chunk lchunk of token (tstart + lrow + RPI*i); tokens past the context re-read the last
     // valid row (their scores are masked)
     auto row_offset = [&](int64_t slot0, int tstart, int i) -> int64_t {
         int tok = tstart + lrow + RPI * i;
-        tok = tok < L ? tok : L - 1;
+        if constexpr (WIN) tok = tstart + seen_row(tstart, lrow + RPI * i);
+        else tok = tok < L ? tok : L - 1;
         int64_t slot;
         if (tile_in_block) {
             slot = slot0 + (tok - tstart);
@@ -317,7 +380,13 @@ __global__ __launch_bounds__(PA_WAVES * 64, (!PF && KVQ == 1 && TIB) ? 4 : 3) vo
     const uint32_t lane_col = (uint32_t)(kvh * D * EB + 16 * lchunk);
     const uint32_t lane_off = (uint32_t)(lrow * (int)row_bytes) + lane_col;
     auto load_tile = [&](u32x4* reg, const uint16_t* __restrict__ cache, int64_t slot0, int tstart) {
-        if constexpr (TIB) {
+        if constexpr (WIN) tstart = wr.tile(tstart / PA_TILE) * PA_TILE;
+        if constexpr (TIB && WIN) {
+            const uint8_t* base = (const uint8_t*)cache + slot0 * row_bytes;       // wave-uniform
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+                reg[i] = pa_stream_load(base + (uint32_t)(seen_row(tstart, lrow + RPI * i) * (int)row_bytes) + lane_col);
+        } else if constexpr (TIB) {
             const uint8_t* base = (const uint8_t*)cache + slot0 * row_bytes;       // wave-uniform
             if (tstart + PA_TILE <= L) {                                           // whole tile: constant lane offset
 #pragma unroll
@@ -349,6 +418,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, (!PF && KVQ == 1 && TIB) ? 4 : 3) vo
     // Groups past the context read the scales of the sequence's first tokens: their scores are masked and their
     // value scales replaced by zero where they are used.
     auto load_scales = [&](f32x4* reg, const float* __restrict__ cache, int64_t slot0, int tstart) {
+        if constexpr (WIN) tstart = wr.tile(tstart / PA_TILE) * PA_TILE;
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2) {
             if constexpr (TIB) {
@@ -386,8 +456,8 @@ __global__ __launch_bounds__(PA_WAVES * 64, (!PF && KVQ == 1 && TIB) ? 4 : 3) vo
     // around the prefetch inside the loop would make the compiler wait for every outstanding load at the join.
     auto tile_body = [&](int it, auto more_c) {
         constexpr bool more = decltype(more_c)::value;
-        const int tstart = tfirst + it * tstep;
-        const int tnext = tstart + tstep;
+        const int tnext = tfirst + it * tstep + tstep;
+        const int tstart = WIN ? wr.tile((tnext - tstep) / PA_TILE) * PA_TILE : tnext - tstep;
         const int64_t slot_nn = more ? tile_slot(tnext + tstep) : 0;
 
         // ---- stage K row-major in LDS, read it back as MFMA A operands (lane = token row r, 8 d per k-step)
@@ -424,7 +494,9 @@ __global__ __launch_bounds__(PA_WAVES * 64, (!PF && KVQ == 1 && TIB) ? 4 : 3) vo
             }
         }
         float tmax = PA_NEG;
-        if (tstart + PA_TILE <= Lmask) {                      // every token of the tile is visible to every column
+        bool whole = tstart + PA_TILE <= Lmask;               // every token of the tile is visible to every column
+        if constexpr (WIN) whole = whole && (tstart >= L - win.window || tstart + PA_TILE <= win.sinks);
+        if (whole) {
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -441,11 +513,11 @@ __global__ __launch_bounds__(PA_WAVES * 64, (!PF && KVQ == 1 && TIB) ? 4 : 3) vo
                     float scaled;
                     if constexpr (KVQ == 2) {
                         scaled = sc[s][i] * kts[s][i];
-                        if (tok >= L) vts[s][i] = 0.f;        // whatever the cache holds there
+                        if (tok >= L || (WIN && tok >= win.sinks && tok < wr.lo)) vts[s][i] = 0.f;   // whatever the cache holds there
                     } else {
                         scaled = sc[s][i] * scale_log2;
                     }
-                    const float v = tok < Lcol ? scaled : PA_NEG;
+                    const float v = tok < Lcol && (!WIN || tok >= lo_col || tok < win.sinks) ? scaled : PA_NEG;
                     sc[s][i] = v;
                     tmax = fmaxf(tmax, v);
                 }
@@ -579,10 +651,11 @@ __global__ __launch_bounds__(PA_WAVES * 64, (!PF && KVQ == 1 && TIB) ? 4 : 3) vo
 }
 
 // Causal limit (number of cache tokens visible) of query row `row` in a prefill step; 0 for a row that belongs to
-// no sequence (before q_starts[0], from q_starts[batch] on, or beyond its sequence's context).
+// no sequence (before q_starts[0], from q_starts[batch] on, or beyond its sequence's context).  The row is number *query of
+// the *count that its sequence brings.
 __device__ inline int pf_row_limit(int row, const int32_t* __restrict__ q_starts,
                                    const int32_t* __restrict__ ctx_lens, bool contiguous, int rows, int max_ctx,
-                                   int batch) {
+                                   int batch, int* query = nullptr, int* count = nullptr) {
     const int lane = threadIdx.x & 63;
     int lo = -1;                                              // last sequence with q_starts[s] <= row: all lanes call
     for (int s0 = 0; s0 < batch && batch > 1; s0 += 64) {     // (one sequence: no read in front of its own)
@@ -593,7 +666,29 @@ __device__ inline int pf_row_limit(int row, const int32_t* __restrict__ q_starts
     int qs, ql, len;
     pf_seq(lo, q_starts, ctx_lens, contiguous, rows, max_ctx, batch, qs, ql, len);
     const int qi = row - qs;
+    if (query) {
+        *query = qi;
+        *count = ql;
+    }
     return (qi >= 0 && qi < ql) ? len - ql + qi + 1 : 0;
+}
+
+// Partitions of (row, head) in a step with a window: those of its column group's walk.  cols: columns a group.
+struct PaWinCombine {
+    PaWindow win;
+    int n_rep, cols;
+};
+__device__ __forceinline__ int pf_win_parts(int L, int query, int q_len, int head, int part_tokens, PaWinCombine wc) {
+    if (L <= 0) return 0;
+    const int group = (query * wc.n_rep + head % wc.n_rep) / wc.cols;
+    const int tiles = pa_win_group(group, wc.cols, wc.n_rep, L - 1 - query, q_len, wc.win).tiles;
+    return (tiles * PA_TILE + part_tokens - 1) / part_tokens;
+}
+
+// the same in decode, where a row's walk is its own; max_ctx: what the block table holds
+__device__ __forceinline__ int pa_decode_win_parts(int L, int max_ctx, int part_tokens, PaWindow win) {
+    L = min(L, max_ctx);
+    return L <= 0 ? 0 : (pa_win_range(L - 1, L - 1, win).tiles * PA_TILE + part_tokens - 1) / part_tokens;
 }
 
 // Combine the partitions of one (sequence, head): out = sum_p 2^(m_p - M) acc_p / sum_p 2^(m_p - M) l_p.
@@ -623,22 +718,29 @@ __device__ __forceinline__ float pa_combine16(const float* mv, const float* lv, 
 template <int D>
 constexpr int PA_REDUCE_THREADS = D < 64 ? 64 : D;
 
-template <typename T, int D, bool PF>
+template <typename T, int D, bool PF, bool WIN = false>
 __global__ __launch_bounds__(PA_REDUCE_THREADS<D>) void paged_attention_reduce_kernel(uint16_t* __restrict__ out,
                                                                   const float* __restrict__ part_out,
                                                                   const float* __restrict__ part_ml,
                                                                   const int32_t* __restrict__ ctx_lens, int n_heads,
                                                                   int max_parts, int part_tokens,
                                                                   const int32_t* __restrict__ q_starts, int batch,
-                                                                  bool contiguous, int max_ctx) {
+                                                                  bool contiguous, int max_ctx, PaWinCombine wc) {
     __shared__ float s_f[64];
     const int h = blockIdx.x, b = blockIdx.y;                 // b: sequence (decode) or query row (PF)
     const bool own = (int)threadIdx.x < D;                    // this thread owns an output column
     const int d = own ? threadIdx.x : 0;
     const int lane = threadIdx.x & 63;
-    const int L = PF ? pf_row_limit(b, q_starts, ctx_lens, contiguous, gridDim.y, max_ctx, batch) : ctx_lens[b];
+    int query = 0, q_len = 1;
+    int L;
+    if constexpr (WIN && PF) L = pf_row_limit(b, q_starts, ctx_lens, contiguous, gridDim.y, max_ctx, batch, &query, &q_len);
+    else L = PF ? pf_row_limit(b, q_starts, ctx_lens, contiguous, gridDim.y, max_ctx, batch) : ctx_lens[b];
     const int64_t gh = (int64_t)b * n_heads + h;
     int np = L <= 0 ? 0 : (L + part_tokens - 1) / part_tokens;
+    if constexpr (WIN) {
+        if (PF) np = pf_win_parts(L, query, q_len, h, part_tokens, wc);
+        else np = pa_decode_win_parts(L, max_ctx, part_tokens, wc.win);
+    }
     np = np < max_parts ? np : max_parts;
     if (np == 0) {
         if (own) out[gh * D + d] = 0;
@@ -701,16 +803,18 @@ __global__ __launch_bounds__(PA_REDUCE_THREADS<D>) void paged_attention_reduce_k
 // lane instead of a binary search: 1531 rows of 28 heads, 2 partitions 42 us with a workgroup per (row, head), 12 us here; 1048
 // rows of 32 heads 36 / 10 us.
 constexpr int PF_REDUCE_THREADS = 256;
-template <typename T, int D, int NB>
+template <typename T, int D, int NB, bool WIN = false>
 __global__ __launch_bounds__(PF_REDUCE_THREADS) void prefill_reduce_kernel(
     uint16_t* __restrict__ out, const float* __restrict__ part_out, const float* __restrict__ part_ml,
     const int32_t* __restrict__ ctx_lens, int n_heads, int max_parts, int part_tokens,
-    const int32_t* __restrict__ q_starts, int batch, bool contiguous, int max_ctx, int rows) {
+    const int32_t* __restrict__ q_starts, int batch, bool contiguous, int max_ctx, int rows, PaWinCombine wc) {
     const int row = blockIdx.x;
-    const int L = pf_row_limit(row, q_starts, ctx_lens, contiguous, rows, max_ctx, batch);
+    int query = 0, q_len = 1;
+    const int L = pf_row_limit(row, q_starts, ctx_lens, contiguous, rows, max_ctx, batch, WIN ? &query : nullptr, &q_len);
     const int c = 4 * (blockIdx.y * PF_REDUCE_THREADS + threadIdx.x);
     if (c >= n_heads * D) return;
     int np = L <= 0 ? 0 : (L + part_tokens - 1) / part_tokens;
+    if constexpr (WIN) np = pf_win_parts(L, query, q_len, c / D, part_tokens, wc);
     np = np < max_parts ? np : max_parts;
     uint16_t* dst = out + (int64_t)row * n_heads * D + c;
     if (np == 0) {
@@ -751,11 +855,11 @@ __global__ __launch_bounds__(PF_REDUCE_THREADS) void prefill_reduce_kernel(
 // elements of one head; at most 16 partitions and 512 threads (n_heads * D <= 4096).  out receives the same bits as
 // paged_attention_reduce_kernel writes, xq / x_scale what the per-token quantisation kernel makes of that row.
 constexpr int PA_RQ_THREADS = 512;
-template <typename T, int D>
+template <typename T, int D, bool WIN = false>
 __global__ __launch_bounds__(PA_RQ_THREADS) void paged_attention_reduce_quant_kernel(
     uint16_t* __restrict__ out, int8_t* __restrict__ xq, float* __restrict__ x_scale,
     const float* __restrict__ part_out, const float* __restrict__ part_ml, const int32_t* __restrict__ ctx_lens,
-    const float* __restrict__ smooth, int n_heads, int max_parts, int part_tokens, int tiled) {
+    const float* __restrict__ smooth, int n_heads, int max_parts, int part_tokens, int tiled, int max_ctx, PaWindow win) {
     __shared__ float red[PA_RQ_THREADS / 64];
     const int b = quant_row(blockIdx.x, gridDim.x, tiled);
     const int cols = n_heads * D;
@@ -763,6 +867,7 @@ __global__ __launch_bounds__(PA_RQ_THREADS) void paged_attention_reduce_quant_ke
     const bool on_row = c * 8 < cols;
     const int L = ctx_lens[b];
     int np = L <= 0 ? 0 : (L + part_tokens - 1) / part_tokens;
+    if constexpr (WIN) np = pa_decode_win_parts(L, max_ctx, part_tokens, win);
     np = np < max_parts ? np : max_parts;
     float v[8];
 #pragma unroll

@@ -86,14 +86,16 @@ struct PfRope {
 // sub-tile of the keys from where `rope` says.  The rotary part that all heads share is read where it lies: writing it behind
 // every head's 128 up-projected values took 102 us of a layer's 930 (2025 rows, 128 heads: 66 MB read, 100 MB written), and its rows
 // come out of L2 here instead of 128 copies out of memory.
-template <typename T, int D, bool TIB, int DV = D, int KVQ = 0>
+// WIN: a sliding window with sinks: tiles are numbered, and partitions cut, in the order of the walk (PaWindow).
+template <typename T, int D, bool TIB, int DV = D, int KVQ = 0, bool WIN = false>
 __global__ __launch_bounds__(PA_WAVES * 64, D == 192 ? 2 : 3) void prefill_attention_kernel(
     uint16_t* __restrict__ out, float* __restrict__ part_out, float* __restrict__ part_ml,
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ kc, const uint16_t* __restrict__ vc,
     const int32_t* __restrict__ block_tables, const int32_t* __restrict__ ctx_lens, int n_heads, int n_kv,
     int n_rep, int block_size, int max_blocks, int num_blocks, int max_parts, float scale_log2, int64_t q_stride,
     int batch, const int32_t* __restrict__ q_starts, int part_tokens, int64_t kv_stride, int rows,
-    int64_t v_stride, const float* __restrict__ kv_scale, const float* __restrict__ kv_offset, float lazy_log2, PfRope rope) {
+    int64_t v_stride, const float* __restrict__ kv_scale, const float* __restrict__ kv_offset, float lazy_log2, PfRope rope,
+    PaWindow win) {
     using vec8 = typename T::vec8;
     using S = PfSmem<D>;
     // Type of the probabilities and of the widened values in the PV product.  int8 values are exact in either type and fp16 rounds
@@ -128,6 +130,10 @@ __global__ __launch_bounds__(PA_WAVES * 64, D == 192 ? 2 : 3) void prefill_atten
             pf_seq(bb, q_starts, ctx_lens, block_tables == nullptr, rows, max_blocks * block_size, batch, qs, ql, len);
             const int ncg = (ql * n_rep + PF_COLS - 1) / PF_COLS;
             int np = len > 0 ? (len + part_tokens - 1) / part_tokens : 0;
+            if constexpr (WIN) {                              // the most of the sequence's column groups
+                const int tiles = (int)pa_win_tiles(len, pa_group_rows(PF_COLS, n_rep), win);
+                np = len > 0 ? (tiles * PF_TOK + part_tokens - 1) / part_tokens : 0;
+            }
             np = np < max_parts ? np : max_parts;
             const int per_seq = np * n_kv * ncg;
             int incl = per_seq;
@@ -173,7 +179,19 @@ __global__ __launch_bounds__(PA_WAVES * 64, D == 192 ? 2 : 3) void prefill_atten
     // the farthest token any column of this group may see; partitions past it have nothing to do (the reduce kernel
     // counts partitions per query row and never reads them)
     const int Lwg = ctx_before + min(q_len, (hg * PF_COLS + PF_COLS - 1) / n_rep + 1);
-    if (part_start >= Lwg) return;                            // uniform over the workgroup
+    if (!WIN && part_start >= Lwg) return;                    // uniform over the workgroup
+    PaWinRange wr = {};
+    if constexpr (WIN) {
+        wr = pa_win_group(hg, PF_COLS, n_rep, ctx_before, q_len, win);
+        if (part_start >= wr.tiles * PF_TOK) return;
+    }
+    // first token of tile t of the partition
+    auto tile_start = [&](int t) { return WIN ? wr.tile(part_start / PF_TOK + t) * PF_TOK : part_start + t * PF_TOK; };
+    // WIN: row of the tile at ts whose values stand in for row `row` where no column sees that one (rows past the range aside)
+    [[maybe_unused]] auto seen_row = [&](int ts, int row) -> int {
+        const int lo = wr.lo - ts, sv = wr.sv - ts;
+        return lo >= PF_TOK ? min(row, sv - 1) : (row < sv ? row : max(row, lo));
+    };
 
     const int tid = threadIdx.x;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -190,7 +208,10 @@ __global__ __launch_bounds__(PA_WAVES * 64, D == 192 ? 2 : 3) void prefill_atten
     const int Lcol = col_ok ? ctx_before + qi + 1 : 0;        // causal limit of this lane's column
     const int q_first = c0 / n_rep;                           // first query of the wave
     // a wave none of whose columns sees a token of this partition only helps with the loads
-    const bool wave_live = q_first < q_len && ctx_before + min(q_len, (c0 + 31) / n_rep + 1) > part_start;
+    const int wave_end = ctx_before + min(q_len, (c0 + 31) / n_rep + 1);      // one past what the wave's columns see
+    const bool wave_live = q_first < q_len && (WIN || wave_end > part_start);
+    // WIN: the tokens in front of these are hidden from all of the wave's columns, from some of them, from this lane's, sinks aside
+    [[maybe_unused]] const int lo_all = ctx_before + q_first + 1 - win.window, lo_some = wave_end - win.window, lo_col = Lcol - win.window;
     const int Lmask = ctx_before + q_first + 1;               // tiles that end at or before it need no mask
     vec8 qreg[KS];
     {
@@ -245,13 +266,13 @@ __global__ __launch_bounds__(PA_WAVES * 64, D == 192 ? 2 : 3) void prefill_atten
         kofs[i] = (uint32_t)(row * (int)((SPLIT && second ? rope.stride : kv_stride) * 2)) + kcol[i];   // offsets within a whole tile
         vofs[i] = (uint32_t)(row * (int)(v_stride * 2)) + vcol[i];
     });
-    const int part_end = min(Lwg, part_start + part_tokens);
+    const int part_end = min(WIN ? wr.tiles * PF_TOK : Lwg, part_start + part_tokens);
     const int ntiles = (part_end - part_start + PF_TOK - 1) / PF_TOK;
 
     // rows past the group's range re-read its last row (their scores are masked)
     auto issue_tile = [&](int t) {
         if (S0::LW < PA_WAVES && w >= S0::LW) return;         // narrow heads: a tile is fewer loads than waves
-        const int ts = part_start + t * PF_TOK;
+        const int ts = tile_start(t);
         uint8_t* kdst = pf_smem + (t % PF_RING) * S::BUF;
         int64_t slot0 = 0;
         if constexpr (TIB) {                                  // the tile lies inside one block: one uniform lookup
@@ -265,7 +286,9 @@ __global__ __launch_bounds__(PA_WAVES * 64, D == 192 ? 2 : 3) void prefill_atten
             }
         }
         const int last_row = Lwg - 1 - ts;
-        if (TIB && last_row >= PF_TOK - 1) {                  // whole tile inside one block: constant lane offsets
+        // WIN: the same two paths, the second for tiles with rows to replace
+        const bool all_rows = last_row >= PF_TOK - 1 && (!WIN || ts >= wr.lo || ts + PF_TOK <= wr.sv);
+        if (TIB && all_rows) {                                // whole tile inside one block: constant lane offsets
             const uint8_t* kb = (const uint8_t*)kc + slot0 * row_bytes;
             const uint8_t* vb = (const uint8_t*)vc + slot0 * v_row_bytes;
             static_for<NI>([&](auto ic) {
@@ -290,7 +313,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, D == 192 ? 2 : 3) void prefill_atten
             constexpr int li = i - (second ? S0::NI : 0);
             const int r0 = (SS::LW * li + w) * SS::RPI;
             uint8_t* dst = kdst + (second ? S::SUB1 : 0) + r0 * SS::ROWB;
-            const int rc = min(r0 + lane / SS::CPR, last_row);
+            const int rc = min(WIN ? seen_row(ts, r0 + lane / SS::CPR) : r0 + lane / SS::CPR, last_row);
             const uint8_t *kp, *vp;
             if constexpr (TIB) {                              // uniform base, 32-bit lane offset
                 const int64_t krow = SPLIT && second ? rope_row_bytes : row_bytes;
@@ -320,8 +343,8 @@ __global__ __launch_bounds__(PA_WAVES * 64, D == 192 ? 2 : 3) void prefill_atten
     [[maybe_unused]] u32x4 kraw, vraw;
     auto load_regs = [&](int t) {
         if (!piece) return;
-        const int ts = part_start + t * PF_TOK;
-        const int rc = min(prow, Lwg - 1 - ts);               // rows past the group's range re-read its last row
+        const int ts = tile_start(t);
+        const int rc = min(WIN ? seen_row(ts, prow) : prow, Lwg - 1 - ts);    // rows past the group's range re-read its last row
         int64_t slot;
         if constexpr (TIB) {
             const int bi = ts / block_size;
@@ -399,7 +422,9 @@ __global__ __launch_bounds__(PA_WAVES * 64, D == 192 ? 2 : 3) void prefill_atten
     auto step = [&](int t, auto ring_c) {
         constexpr int R = decltype(ring_c)::value;
         constexpr int OFF = R * S::BUF, P = 4;
-        const int ts = part_start + t * PF_TOK;
+        const int ts = tile_start(t);
+        if constexpr (WIN)                                    // a tile that none of the wave's columns sees
+            if (ts >= wave_end || (ts + PF_TOK <= lo_all && ts >= win.sinks)) return;
 
         // ---- S^T[token, col] = K[token, :] . Q[col, :]
         f32x16 sc;
@@ -427,11 +452,13 @@ __global__ __launch_bounds__(PA_WAVES * 64, D == 192 ? 2 : 3) void prefill_atten
                 fetch(std::integral_constant<int, m + P>{});
             });
         }
-        if (ts + PF_TOK > Lmask) {                            // tokens hidden from a column leave its scores
+        bool hides = ts + PF_TOK > Lmask;
+        if constexpr (WIN) hides = hides || (ts < lo_some && ts + PF_TOK > win.sinks);
+        if (hides) {                                          // tokens hidden from a column leave its scores
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int tok = ts + 8 * (i >> 2) + 4 * h + (i & 3);
-                sc[i] = tok < Lcol ? sc[i] : PA_NEG;
+                sc[i] = tok < Lcol && (!WIN || tok >= lo_col || tok < win.sinks) ? sc[i] : PA_NEG;
             }
         }
         float tmax = sc[0];
@@ -691,24 +718,31 @@ __global__ void pf_zero_rows_kernel(uint16_t* __restrict__ out, const int32_t* _
     }
 }
 
-template <typename T, int D, int KVQ, int DV = D>
+// Plan of a step with a window: that of a context as long as the longest walk.
+static inline int64_t pf_win_walk(int64_t max_ctx, int cols, int n_rep, PaWindow win) {
+    return pa_win_tiles(max_ctx, pa_group_rows(cols, n_rep), win) * PF_TOK;
+}
+
+template <typename T, int D, int KVQ, int DV = D, bool WIN = false>
 int launch_pf(void* out, const void* query, const void* key_cache, const void* value_cache,
               const int32_t* block_tables, const int32_t* context_lens, const int32_t* q_starts, int batch,
               int total_q, int n_heads, int n_kv, int block_size, int max_blocks, int num_blocks, float scale,
               int64_t q_stride, int64_t kv_stride, void* workspace, hipStream_t st, const float* kv_scale,
-              const float* kv_offset, int64_t v_stride = 0, PfRope rope = {}) {
+              const float* kv_offset, int64_t v_stride = 0, PfRope rope = {}, PaWindow win = {}) {
     static_assert(DV == D || KVQ == 0, "value heads narrower than the key heads: 16-bit packed rows only");
     if (v_stride <= 0) v_stride = kv_stride;
     const int n_rep = n_heads / n_kv;
     const bool contiguous = block_tables == nullptr;
     const int64_t max_ctx = contiguous ? total_q : (int64_t)max_blocks * block_size;
     const bool tib_tok = contiguous || block_size % PF_TOK == 0;       // a staged tile never straddles two blocks
-    const PfPlan plan = KVQ == 0 ? pf_plan16(batch, total_q, n_heads, n_kv, D, max_ctx, contiguous, tib_tok)
-                                 : pf_plan(batch, total_q, n_heads, n_kv, max_ctx);
+    // int8 caches with per-channel scales and a window take the 128-column kernel at any number of rows
+    const bool cols16 = KVQ == 2 || (KVQ == 1 && !WIN && pf_cols16(pf_plan(batch, total_q, n_heads, n_kv, max_ctx), batch, n_kv, D, max_ctx));
+    const int64_t walk = WIN ? pf_win_walk(max_ctx, cols16 ? 16 : PF_COLS, n_rep, win) : max_ctx;
+    const PfPlan plan = KVQ == 0 ? pf_plan16(batch, total_q, n_heads, n_kv, D, walk, contiguous, tib_tok)
+                                 : pf_plan(batch, total_q, n_heads, n_kv, walk);
     float* part_out = plan.max_parts > 1 ? (float*)workspace : nullptr;
     float* part_ml = part_out ? part_out + (int64_t)total_q * n_heads * plan.max_parts * DV : nullptr;
     const float scale_log2 = scale * 1.4426950408889634f;
-    const bool cols16 = KVQ == 2 || (KVQ == 1 && pf_cols16(plan, batch, n_kv, D, max_ctx));
     const int64_t wgs = (cols16 ? plan.col_groups16 : plan.col_groups128) * n_kv * plan.max_parts;
     if (wgs > 0x7fffffffLL) {
         mf_set_error("paged_attention_prefill: %lld workgroups exceed the grid limit", (long long)wgs);
@@ -720,15 +754,15 @@ int launch_pf(void* out, const void* query, const void* key_cache, const void* v
         int rc = MF_LAUNCH_CHECK();
         if (rc) return rc;
     }
-    if constexpr (KVQ != 0) if (cols16) {
+    if constexpr (KVQ == 2 || (KVQ == 1 && !WIN)) if (cols16) {
         const bool tib = block_size % PA_TILE == 0;           // a 32-token tile never straddles two blocks
 #define PF_LAUNCH(TIBV)                                                                                           \
-    hipLaunchKernelGGL((paged_attention_kernel<T, D, 2, true, KVQ, TIBV>), dim3((unsigned)wgs),                    \
+    hipLaunchKernelGGL((paged_attention_kernel<T, D, 2, true, KVQ, TIBV, WIN>), dim3((unsigned)wgs),               \
                        dim3(PA_WAVES * 64), 0, st, (uint16_t*)out, part_out, part_ml, (const uint16_t*)query,      \
                        (const uint16_t*)key_cache, (const uint16_t*)value_cache, block_tables, context_lens,       \
                        n_heads, n_kv, n_rep, (n_rep + 15) / 16, block_size, max_blocks, num_blocks, plan.max_parts, \
                        scale_log2, q_stride, batch, q_starts, plan.part_tokens, kv_stride, total_q, kv_scale,      \
-                       kv_offset)
+                       kv_offset, win)
         if (tib) PF_LAUNCH(true);
         else PF_LAUNCH(false);
 #undef PF_LAUNCH
@@ -740,7 +774,7 @@ int launch_pf(void* out, const void* query, const void* key_cache, const void* v
         if (e != hipSuccess) return (int)e;
 #define PF_LAUNCH(TIBV)                                                                                           \
     {                                                                                                             \
-        auto kern = prefill_attention_kernel<T, D, TIBV, DV, KVQ>;                                                    \
+        auto kern = prefill_attention_kernel<T, D, TIBV, DV, KVQ, WIN>;                                               \
         if (dev < 0 || dev >= MF_MAX_DEVICES || !lds_set[TIBV][dev]) {                                            \
             e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize,                \
                                     PfSmem<D>::BYTES);                                                            \
@@ -752,7 +786,7 @@ int launch_pf(void* out, const void* query, const void* key_cache, const void* v
                            (const uint16_t*)value_cache, block_tables, context_lens, n_heads, n_kv, n_rep,        \
                            block_size, max_blocks, num_blocks, plan.max_parts, scale_log2, q_stride, batch,       \
                            q_starts, plan.part_tokens, kv_stride, total_q, v_stride, kv_scale, kv_offset, plan.lazy_log2, \
-                           rope);                                                                                  \
+                           rope, win);                                                                             \
     }
         if (tib_tok) PF_LAUNCH(true)
         else PF_LAUNCH(false)
@@ -764,16 +798,17 @@ int launch_pf(void* out, const void* query, const void* key_cache, const void* v
         // 1024 elements a workgroup where that gives every compute unit two, else a workgroup per (row, head), which spreads a
         // row over more of them (one row of 8 heads, 62 | 16 partitions: 3 | 0.6 us less); more than 16 partitions come with
         // fewer than 4096 (row, head) pairs only (pf_plan)
+        const PaWinCombine wc = {win, n_rep, cols16 ? 16 : PF_COLS};
         const int per_row = (n_heads * DV + 4 * PF_REDUCE_THREADS - 1) / (4 * PF_REDUCE_THREADS);
         if (plan.max_parts > 16 || (int64_t)total_q * per_row < 512) {
-            hipLaunchKernelGGL((paged_attention_reduce_kernel<T, DV, true>), dim3(n_heads, total_q),
+            hipLaunchKernelGGL((paged_attention_reduce_kernel<T, DV, true, WIN>), dim3(n_heads, total_q),
                                dim3(PA_REDUCE_THREADS<DV>), 0, st, (uint16_t*)out, part_out, part_ml, context_lens, n_heads,
-                               plan.max_parts, plan.part_tokens, q_starts, batch, contiguous, (int)max_ctx);
+                               plan.max_parts, plan.part_tokens, q_starts, batch, contiguous, (int)max_ctx, wc);
         } else {
 #define PFR_LAUNCH(NB)                                                                                            \
-    hipLaunchKernelGGL((prefill_reduce_kernel<T, DV, NB>), dim3((unsigned)total_q, (unsigned)per_row), dim3(PF_REDUCE_THREADS), \
+    hipLaunchKernelGGL((prefill_reduce_kernel<T, DV, NB, WIN>), dim3((unsigned)total_q, (unsigned)per_row), dim3(PF_REDUCE_THREADS), \
                        0, st, (uint16_t*)out, part_out, part_ml, context_lens, n_heads, plan.max_parts, plan.part_tokens, \
-                       q_starts, batch, contiguous, (int)max_ctx, total_q)
+                       q_starts, batch, contiguous, (int)max_ctx, total_q, wc)
             if (plan.max_parts <= 4) PFR_LAUNCH(4);
             else PFR_LAUNCH(16);
 #undef PFR_LAUNCH
@@ -813,7 +848,8 @@ static int pa_prefill_entry(void* out, const void* query, const void* key_cache,
                             int batch, int total_q, int n_heads, int n_kv_heads, int head_dim, int block_size,
                             int max_blocks_per_seq, int num_blocks, float scale, int64_t q_row_stride,
                             int64_t kv_row_stride, int dtype, void* workspace, size_t workspace_bytes, void* stream,
-                            int kvq, const float* kv_scale, const float* kv_offset) {
+                            int kvq, const float* kv_scale, const float* kv_offset, PaWindow win = {}) {
+    // win.window 0: the whole context.
     // kvq: 0 = 16-bit rows or caches, 1 = int8 caches with per-channel scale / offset, 2 = int8 caches with per-token
     // key scales (kv_scale) and value scales (kv_offset), one float per cache slot
     const bool kv8 = kvq != 0;
@@ -847,18 +883,22 @@ static int pa_prefill_entry(void* out, const void* query, const void* key_cache,
                "paged_attention_prefill: query row stride must be >= n_heads*head_dim and a multiple of 8 elements");
     MF_REQUIRE((((uintptr_t)out | (uintptr_t)query | (uintptr_t)key_cache | (uintptr_t)value_cache) & 15) == 0,
                "paged_attention_prefill: out / query / caches must be 16-byte aligned");
-    const size_t need = mf_paged_attention_prefill_workspace_bytes(
-        batch, total_q, n_heads, n_kv_heads, head_dim, contiguous ? total_q : max_blocks_per_seq * block_size);
+    MF_REQUIRE(!win.window || head_dim != 192, "paged_attention_prefill: a window goes with heads of 32, 64 or 128");
+    const int max_ctx = contiguous ? total_q : max_blocks_per_seq * block_size;
+    const size_t need = win.window ? mf_window_attention_prefill_workspace_bytes(batch, total_q, n_heads, n_kv_heads, head_dim, max_ctx,
+                                                                                win.window, win.sinks)
+                                   : mf_paged_attention_prefill_workspace_bytes(batch, total_q, n_heads, n_kv_heads, head_dim, max_ctx);
     MF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
                "paged_attention_prefill: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
     MF_REQUIRE(need == 0 || ((uintptr_t)workspace & 15) == 0,
                "paged_attention_prefill: workspace must be 16-byte aligned");
     hipStream_t st = (hipStream_t)stream;
-#define PF_CASE_Q(TT, DD, QQ)                                                                                      \
-    return launch_pf<TT, DD, QQ>(out, query, key_cache, value_cache, block_tables, context_lens, q_starts, batch,  \
-                                 total_q, n_heads, n_kv_heads, block_size, max_blocks_per_seq, num_blocks, scale,  \
-                                 q_row_stride, kv_row_stride, workspace, st, kvq ? kv_scale : nullptr,             \
-                                 kvq ? kv_offset : nullptr)
+#define PF_CASE_W(TT, DD, QQ, WW)                                                                                  \
+    launch_pf<TT, DD, QQ, DD, WW>(out, query, key_cache, value_cache, block_tables, context_lens, q_starts, batch, \
+                                  total_q, n_heads, n_kv_heads, block_size, max_blocks_per_seq, num_blocks, scale, \
+                                  q_row_stride, kv_row_stride, workspace, st, kvq ? kv_scale : nullptr,            \
+                                  kvq ? kv_offset : nullptr, 0, PfRope{}, win)
+#define PF_CASE_Q(TT, DD, QQ) return win.window ? PF_CASE_W(TT, DD, QQ, true) : PF_CASE_W(TT, DD, QQ, false)
 #define PF_CASE(TT, DD)                                                                                            \
     {                                                                                                              \
         if (kvq == 2) PF_CASE_Q(TT, DD, 2);                                                                        \
@@ -883,6 +923,31 @@ static int pa_prefill_entry(void* out, const void* query, const void* key_cache,
 #undef PF_CASE192
 #undef PF_CASE
 #undef PF_CASE_Q
+#undef PF_CASE_W
+}
+
+extern "C" size_t mf_window_attention_prefill_workspace_bytes(int batch, int total_q, int n_heads, int n_kv_heads, int head_dim,
+                                                              int max_context, int window, int sinks) {
+    if (batch <= 0 || total_q <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || max_context <= 0 || window <= 0 || sinks < 0)
+        return 0;
+    int most = 1;                                             // 16 or 128 columns a group, by the cache's type
+    for (const int cols : {16, PF_COLS})
+        most = std::max(most, pf_plan(batch, total_q, n_heads, n_kv_heads,
+                                      pf_win_walk(max_context, cols, n_heads / n_kv_heads, {window, sinks})).max_parts);
+    return most <= 1 ? 0 : (size_t)total_q * n_heads * most * (head_dim + 2) * sizeof(float);
+}
+
+extern "C" int mf_window_attention_prefill(void* out, const void* query, const void* key, const void* value, const float* key_scale,
+                                           const float* value_scale, int kv_quant, const int32_t* block_tables,
+                                           const int32_t* context_lens, const int32_t* q_starts, int batch, int total_q, int n_heads,
+                                           int n_kv_heads, int head_dim, int block_size, int max_blocks_per_seq, int num_blocks,
+                                           float scale, int window, int sinks, int64_t q_row_stride, int64_t kv_row_stride, int dtype,
+                                           void* workspace, size_t workspace_bytes, void* stream) {
+    MF_REQUIRE(window > 0 && sinks >= 0, "window_attention: window %d must be positive, sinks %d not negative", window, sinks);
+    MF_REQUIRE(kv_quant >= 0 && kv_quant <= 2, "window_attention: kv_quant must be 0 (16-bit), 1 (per channel) or 2 (per token)");
+    return pa_prefill_entry(out, query, key, value, block_tables, context_lens, q_starts, batch, total_q, n_heads, n_kv_heads, head_dim,
+                            block_size, max_blocks_per_seq, num_blocks, scale, q_row_stride, kv_row_stride, dtype, workspace,
+                            workspace_bytes, stream, kv_quant, key_scale, value_scale, PaWindow{window, sinks});
 }
 
 extern "C" int mf_paged_attention_prefill(void* out, const void* query, const void* key_cache,

@@ -181,11 +181,23 @@ def rope_and_cache(query, key, value, cos, sin, key_cache, value_cache, slot_map
 
 
 # --------------------------------------------------------------------------------------------- attention
+def check_window(window, sinks):
+    """(window, sinks) as the library takes them, window 0 = none.  A query at position p sees the tokens j <= p with
+    j > p - window (``window`` tokens with its own) or j < sinks."""
+    if window is None:
+        _need(sinks == 0, "sinks go with a window")
+        return 0, 0
+    if not (int(window) == window and window > 0 and int(sinks) == sinks and sinks >= 0):
+        raise ValueError(f"window must be a positive integer and sinks not negative, got {window!r} and {sinks!r}")
+    return min(int(window), 0x7fffffff), min(int(sinks), 0x7fffffff)
+
+
 def paged_attention(query, key_cache, value_cache, block_tables, context_lens, n_heads, n_kv_heads, scale, out=None,
-                    quant=None):
+                    quant=None, window=None, sinks=0):
     """PagedAttention(head_num, scale, kv_head_num)(query, key_cache, value_cache, block_tables, context_lens).
     ``quant`` = (smooth or None, tiled): also quantise every output row per token, as ``dynamic_quant`` would; the
-    call then returns (out, xq, scale)."""
+    call then returns (out, xq, scale).  ``window`` (None: all of the context): a query sees its own and the window - 1 tokens
+    in front of it, and the first ``sinks`` tokens; block table entries whose blocks hold none of them may be -1."""
     lib = _lib.load()
     _dev_of(query)
     dev = _dev_ok(key_cache, value_cache, block_tables, context_lens, out)
@@ -206,6 +218,9 @@ def paged_attention(query, key_cache, value_cache, block_tables, context_lens, n
         out = query.new_empty(query.shape)
     else:
         _need(out.shape == query.shape and out.dtype == query.dtype, "out mismatch")
+    if window is not None or sinks:
+        return _window_decode(lib, dev, out, quant, query, key_cache, value_cache, None, None, 0, block_tables, context_lens, n_heads,
+                              n_kv_heads, scale, window, sinks, qs)
     need = lib.mf_paged_attention_workspace_bytes(b, n_heads, d, max_blocks * bs)
     ws = workspace(need, dev, "pa") if need else None
     if quant is not None:
@@ -224,6 +239,50 @@ def paged_attention(query, key_cache, value_cache, block_tables, context_lens, n
                                         ptr(context_lens), b, n_heads, n_kv_heads, d, bs, max_blocks, nb,
                                         float(scale), qs, dtype_code(query.dtype), ptr(ws), ws.numel() if ws is not None else 0,
                                         stream_ptr(dev)), "mf_paged_attention_decode")
+    return out
+
+
+def _window_decode(lib, dev, out, quant, query, key_cache, value_cache, key_scale, value_scale, kvq, block_tables, context_lens, n_heads,
+                   n_kv_heads, scale, window, sinks, q_stride):
+    """The windowed form of ``paged_attention`` / ``paged_attention_int8kv``, behind their checks."""
+    window, sinks = check_window(window, sinks)
+    nb, bs, _, d = key_cache.shape
+    b, max_blocks = block_tables.shape
+    need = lib.mf_window_attention_workspace_bytes(b, n_heads, d, max_blocks * bs, window, sinks)
+    ws = workspace(need, dev, "pa") if need else None
+    smooth, tiled = quant if quant is not None else (None, False)
+    xq = xs = None
+    if quant is not None:
+        cols = n_heads * d
+        _need(smooth is None or (smooth.dtype == torch.float32 and smooth.numel() == cols and smooth.device == dev),
+              "smooth must be fp32 [n_heads * D]")
+        xq, xs = _quant_out(lib, (b, cols), b, cols, tiled, dev)
+    with _on(dev):
+        check(lib.mf_window_attention_decode(
+            ptr(out), ptr(xq), ptr(xs), ptr(smooth), 1 if tiled else 0, ptr(query), ptr(key_cache), ptr(value_cache), ptr(key_scale),
+            ptr(value_scale), kvq, ptr(block_tables), ptr(context_lens), b, n_heads, n_kv_heads, d, bs, max_blocks, nb, float(scale),
+            window, sinks, q_stride, dtype_code(query.dtype), ptr(ws), ws.numel() if ws is not None else 0, stream_ptr(dev)),
+            "mf_window_attention_decode")
+    if quant is None:
+        return out
+    return out, (TiledInt8Activations(xq, (b, cols)) if tiled else xq), xs
+
+
+def _window_prefill(lib, dev, out, query, key, value, key_scale, value_scale, kvq, block_tables, context_lens, q_starts, n_heads,
+                    n_kv_heads, d, scale, window, sinks, q_stride, kv_stride):
+    """The windowed form of the attention of several query rows per sequence, behind the checks of its callers; block_tables None:
+    packed keys and values."""
+    window, sinks = check_window(window, sinks)
+    b, total_q = q_starts.numel() - 1, out.numel() // (n_heads * d)
+    nb, bs, max_blocks = (key.shape[0], key.shape[1], block_tables.shape[1]) if block_tables is not None else (0, 0, 0)
+    need = lib.mf_window_attention_prefill_workspace_bytes(b, total_q, n_heads, n_kv_heads, d,
+                                                           max_blocks * bs if block_tables is not None else total_q, window, sinks)
+    ws = workspace(need, dev, "pa_prefill") if need else None
+    with _on(dev):
+        check(lib.mf_window_attention_prefill(
+            ptr(out), ptr(query), ptr(key), ptr(value), ptr(key_scale), ptr(value_scale), kvq, ptr(block_tables), ptr(context_lens),
+            ptr(q_starts), b, total_q, n_heads, n_kv_heads, d, bs, max_blocks, nb, float(scale), window, sinks, q_stride, kv_stride,
+            dtype_code(query.dtype), ptr(ws), ws.numel() if ws is not None else 0, stream_ptr(dev)), "mf_window_attention_prefill")
     return out
 
 
@@ -417,11 +476,13 @@ def _token_scale_caches(key_scale_cache, value_scale_cache, nb, bs):
 
 
 def paged_attention_int8kv(query, key_cache, value_cache, block_tables, context_lens, antiquant_scale,
-                           antiquant_offset, n_heads, n_kv_heads, scale, q_starts=None, out=None, token_scales=None):
+                           antiquant_offset, n_heads, n_kv_heads, scale, q_starts=None, out=None, token_scales=None,
+                           window=None, sinks=0):
     """PagedAttention(...)(query, key_cache, value_cache, block_tables, context_lens, antiquant_scale,
     antiquant_offset[, mask, q_seq_lens]) on int8 caches; ``q_starts`` selects the several-rows-per-sequence form.
     ``token_scales`` = (key_scale_cache, value_scale_cache), fp32 [num_blocks, block_size]: caches quantised per
-    token (``dynamic_quant_reshape_and_cache``); antiquant_scale / antiquant_offset are then None."""
+    token (``dynamic_quant_reshape_and_cache``); antiquant_scale / antiquant_offset are then None.  ``window`` / ``sinks``:
+    as in ``paged_attention``."""
     lib = _lib.load()
     _dev_of(query)
     dev = _dev_ok(key_cache, value_cache, block_tables, context_lens, out)
@@ -447,9 +508,17 @@ def paged_attention_int8kv(query, key_cache, value_cache, block_tables, context_
         out = torch.empty((rows, n_heads * d), dtype=query.dtype, device=dev)
     else:
         _need(out.numel() == rows * n_heads * d and out.dtype == query.dtype, "out mismatch")
+    if q_starts is None and rows != b:
+        raise ValueError(f"query has {rows} rows for {b} sequences")
+    if window is not None or sinks:
+        kvq, ks, vs = (1, antiquant_scale, antiquant_offset) if token_scales is None else (2, *token_scales)
+        if q_starts is None:
+            return _window_decode(lib, dev, out, None, query, key_cache, value_cache, ks, vs, kvq, block_tables, context_lens, n_heads,
+                                  n_kv_heads, scale, window, sinks, qs)
+        _need(_q_starts(q_starts, dev) == b, "q_starts must have batch + 1 entries")
+        return _window_prefill(lib, dev, out, query, key_cache, value_cache, ks, vs, kvq, block_tables, context_lens, q_starts, n_heads,
+                               n_kv_heads, d, scale, window, sinks, qs, 0)
     if q_starts is None:
-        if rows != b:
-            raise ValueError(f"query has {rows} rows for {b} sequences")
         need = lib.mf_paged_attention_workspace_bytes(b, n_heads, d, max_blocks * bs)
         ws = workspace(need, dev, "pa") if need else None
         if token_scales is not None:
@@ -519,10 +588,11 @@ def q_starts_from_lens(q_seq_lens):
 
 
 def paged_attention_prefill(query, key_cache, value_cache, block_tables, context_lens, q_starts, n_heads,
-                            n_kv_heads, scale, out=None):
+                            n_kv_heads, scale, out=None, window=None, sinks=0):
     """Causal attention of several new tokens per sequence over the paged cache (their keys/values already
     scattered): PagedAttention(...)(query, key_cache, value_cache, block_tables, batch_valid_length, None, None,
-    causal_mask, q_seq_lens) with q_starts = [0, cumsum(q_seq_lens)]."""
+    causal_mask, q_seq_lens) with q_starts = [0, cumsum(q_seq_lens)].  ``window`` / ``sinks``: as in ``paged_attention``, heads of
+    32, 64 or 128."""
     lib = _lib.load()
     _dev_of(query)
     dev = _dev_ok(key_cache, value_cache, block_tables, context_lens, out)
@@ -542,6 +612,9 @@ def paged_attention_prefill(query, key_cache, value_cache, block_tables, context
         out = torch.empty((total_q, n_heads * d), dtype=query.dtype, device=dev)
     else:
         _need(out.numel() == total_q * n_heads * d and out.dtype == query.dtype and out.is_contiguous(), "out mismatch")
+    if window is not None or sinks:
+        return _window_prefill(lib, dev, out, query, key_cache, value_cache, None, None, 0, block_tables, context_lens, q_starts, n_heads,
+                               n_kv_heads, d, scale, window, sinks, qs, 0)
     need = lib.mf_paged_attention_prefill_workspace_bytes(b, total_q, n_heads, n_kv_heads, d, max_blocks * bs)
     ws = workspace(need, dev, "pa_prefill") if need else None
     check(lib.mf_paged_attention_prefill(ptr(out), ptr(query), ptr(key_cache), ptr(value_cache), ptr(block_tables),
@@ -552,12 +625,12 @@ def paged_attention_prefill(query, key_cache, value_cache, block_tables, context
     return out
 
 
-def causal_attention_varlen(query, key, value, q_starts, n_heads, n_kv_heads, scale, out=None):
+def causal_attention_varlen(query, key, value, q_starts, n_heads, n_kv_heads, scale, out=None, window=None, sinks=0):
     """FlashAttentionScore in the TH layout with a causal mask and actual_seq_qlen == actual_seq_kvlen: packed
     rows, sequence b owns rows q_starts[b] .. q_starts[b+1]-1 of query, key and value.  key / value may be column
     slices of a fused projection output (equal row strides).  With 192-wide query / key heads the value heads may be
     128 wide (multi-latent attention): the result then has 128-wide heads, the numbers the 192-wide call gives on
-    zero-padded values in its first 128 columns."""
+    zero-padded values in its first 128 columns.  ``window`` / ``sinks``: as in ``paged_attention``, heads of 32, 64 or 128."""
     lib = _lib.load()
     dev = _dev_of(query, key, value)
     _dev_ok(out)
@@ -571,6 +644,7 @@ def causal_attention_varlen(query, key, value, q_starts, n_heads, n_kv_heads, sc
     b = _q_starts(q_starts, dev)
     if value.shape[1] != key.shape[1]:
         # value heads narrower than the key heads: the prefill of multi-latent attention (192-wide keys, 128-wide values)
+        _need(window is None and sinks == 0, "a window goes with value heads as wide as the key heads")
         _need(d == 192 and value.shape[1] == n_kv_heads * 128, "narrower value heads are built for 192-wide keys with 128-wide values")
         value, vs = _rows(value, n_kv_heads * 128, "value")
         _need(key.shape[0] == total_q and value.shape[0] == total_q, "query, key and value must have the same number of rows")
@@ -592,6 +666,9 @@ def causal_attention_varlen(query, key, value, q_starts, n_heads, n_kv_heads, sc
         out = torch.empty((total_q, n_heads * d), dtype=query.dtype, device=dev)
     else:
         _need(out.numel() == total_q * n_heads * d and out.dtype == query.dtype and out.is_contiguous(), "out mismatch")
+    if window is not None or sinks:
+        return _window_prefill(lib, dev, out, query, key, value, None, None, 0, None, None, q_starts, n_heads, n_kv_heads, d, scale,
+                               window, sinks, qs, ks)
     need = lib.mf_paged_attention_prefill_workspace_bytes(b, total_q, n_heads, n_kv_heads, d, total_q)
     ws = workspace(need, dev, "pa_prefill") if need else None
     check(lib.mf_paged_attention_prefill(ptr(out), ptr(query), ptr(key), ptr(value), None, None, ptr(q_starts), b,

@@ -89,3 +89,24 @@ def compact_blocks(tables, num_blocks, block_size, held=None):
     copies = [(a, b, block_size) for a, b in zip(moves, holes)]
     copies += [(-1, -1, 0)] * (num_blocks // 2 - len(copies))
     return out, np.array(copies).reshape(-1, 3), len(live)
+
+
+def window_attention(query, keys, values, lens, q_lens, n_heads, n_kv, scale, window, sinks, of="value"):
+    """Attention where the row at position p sees the tokens j <= p with j > p - window or j < sinks, float64.  query [T, H * D], the
+    sequences' rows packed; keys / values: per sequence [L, n_kv, D].  ``of``: "value", "magnitude" (the same of |values|) or "sum" (the
+    visible |values| added up)."""
+    t = query.shape[0]
+    d = query.shape[1] // n_heads
+    out, row = np.zeros((t, n_heads, d)), 0
+    for k, v, n, ql in zip(keys, values, lens, q_lens):
+        for i in range(int(ql)):
+            p = int(n) - int(ql) + i
+            if p >= 0:
+                seen = [j for j in range(p + 1) if j > p - window or j < sinks]
+                kk, vv = (np.repeat(x[seen].astype(np.float64), n_heads // n_kv, axis=1) for x in (k, v if of == "value" else np.abs(v)))
+                s = np.einsum("hd,jhd->hj", query[row].reshape(n_heads, d).astype(np.float64), kk) * scale
+                w = np.exp(s - s.max(axis=1, keepdims=True))
+                w = w * 0 + 1 if of == "sum" else w / w.sum(axis=1, keepdims=True)
+                out[row] = np.einsum("hj,jhd->hd", w, vv)
+            row += 1
+    return out.reshape(t, -1)

@@ -276,3 +276,256 @@ def test_copies_of_more_caches_than_a_launch_names_and_past_4_gib():
     ops.copy_blocks([big, wide], [[4998, 4999, 127], [0, 1, 128]])
     for c in (big, wide):
         assert (c[4999, :127] == 7).all() and (c[4999, 127] == 0).all() and (c[1] == 0).all()
+
+
+# --------------------------------------------------------------------------------------------- sliding window with sinks
+# Tolerance: probabilities are rounded in front of the product with the values (half a step of sum p |v|), the denominator
+# sums them rounded (half a step of the result at most), the result is rounded (half a step): three half steps of sum p |v|,
+# which helpers.EPS is one of.  Below 2^-14 fp16 is off by up to 2^-25 whatever the value (the smallest step's half): that much of the
+# sum of the visible |v| more, as the largest probability is 1 at least; where the values' scale of an int8 cache rides on the
+# probability, of the sum of the visible int8 values.  int8 caches with a scale a channel go through fp16 in both types.  The scales of
+# int8 caches are powers of two here, so that folding them into the query rounds nothing.
+def _hold(got, args, dtype, what, kind="16", steps=None):
+    from helpers import assert_within
+    extra = 0.0
+    if dtype == torch.float16 or kind == "channel":
+        q, keys, values, *rest = args
+        extra = 2.0 ** -25 * G.window_attention(q, keys, values if steps is None else steps, *rest, of="sum")
+        if dtype == torch.float16:                            # the result itself
+            extra = extra + 2.0 ** -25
+    assert_within(got, G.window_attention(*args), G.window_attention(*args, of="magnitude"), dtype, ulps=3.0, extra=extra, what=what)
+
+
+ACT = [torch.bfloat16, torch.float16]
+
+
+def _paged(rng, dtype, lens, q_lens, nh, nkv, d, block, window, sinks, kind="16", poison=True):
+    """Queries and a paged cache of the given lengths in a shuffled pool.  Blocks without a visible token are given back (-1) and
+    everything that no row sees holds NaN (16-bit values, scales) or garbage."""
+    from helpers import rounded
+    lens, q_lens = np.asarray(lens), np.asarray(q_lens)
+    need = [-(-max(int(n), 0) // block) for n in lens]
+    width = max(max(need), 1) + 1
+    nb = sum(need) + 3
+    perm = rng.permutation(nb)
+    tables = np.full((len(lens), width), -1)
+    at = 0
+    shape = (nb, block, nkv, d)
+    if kind == "16":
+        cache = [rounded(rng.normal(0, 1, shape), dtype) for _ in range(2)]
+        scales = None
+    else:
+        cache = [rng.integers(-127, 128, shape).astype(np.float32) for _ in range(2)]
+        scales = 2.0 ** -rng.integers(5, 8, (2, nb, block) if kind == "token" else (2, nkv * d)).astype(np.float64)
+    keys, values = [], []
+    visible = np.zeros((nb, block), dtype=bool)
+    for b, n in enumerate(lens):
+        pages = perm[at:at + need[b]]
+        at += need[b]
+        tables[b, :need[b]] = pages
+        for store, c, i in ((keys, cache[0], 0), (values, cache[1], 1)):
+            rows = c[pages].astype(np.float64)
+            if kind == "token":
+                rows = rows * scales[i][pages][:, :, None, None]
+            rows = rows.reshape(-1, nkv, d)[:max(int(n), 0)]
+            store.append(rows * scales[i].reshape(nkv, d) if kind == "channel" else rows)
+        for p in range(max(int(n - q_lens[b]), 0), int(n)):
+            for j in list(range(max(p - window + 1, 0), p + 1)) + list(range(min(sinks, p + 1))):
+                visible[pages[j // block], j % block] = True
+    if poison:
+        for c in cache:
+            c[~visible] = np.nan if kind == "16" else -128
+        if kind == "token":
+            scales[:, ~visible] = np.nan
+        hidden = ~visible.any(axis=1)
+        tables = np.where((tables >= 0) & hidden[tables], -1, tables)
+    q = rounded(rng.normal(0, 1, (int(q_lens.sum()), nh * d)), dtype)
+    return q, cache, scales, tables, keys, values
+
+
+def _windowed(dtype, lens, q_lens, nh, nkv, d, block, window, sinks, kind="16", seed=0, strided=False):
+    from mindformers_amd import ops
+    rng = np.random.default_rng(seed + window)
+    q, cache, scales, tables, keys, values = _paged(rng, dtype, lens, q_lens, nh, nkv, d, block, window, sinks, kind)
+    dq = torch.from_numpy(q).to(dtype).cuda()
+    if strided:
+        wide = torch.full((dq.shape[0], dq.shape[1] + 24), float("nan"), dtype=dtype, device="cuda")
+        wide[:, 8:-16] = dq
+        dq = wide[:, 8:-16]
+    kc, vc = (torch.from_numpy(c).to(dtype if kind == "16" else torch.int8).cuda() for c in cache)
+    t, n = _i32(tables), _i32(lens)
+    scale, view = 1 / np.sqrt(d), dict(window=window, sinks=sinks)
+    several = max(q_lens) > 1
+    starts = _i32(np.concatenate([[0], np.cumsum(q_lens)]))
+    if kind == "16":
+        got = (ops.paged_attention_prefill(dq, kc, vc, t, n, starts, nh, nkv, scale, **view) if several else
+               ops.paged_attention(dq, kc, vc, t, n, nh, nkv, scale, **view))
+    else:
+        s = torch.from_numpy(scales).float().cuda()
+        par = dict(token_scales=(s[0].contiguous(), s[1].contiguous())) if kind == "token" else {}
+        got = ops.paged_attention_int8kv(dq, kc, vc, t, n, None if par else s, None, nh, nkv, scale, q_starts=starts if several else None,
+                                         **par, **view)
+    args = (q, keys, values, lens, q_lens, nh, nkv, scale, window, sinks)
+    steps = [np.full_like(v, 127.0) for v in values] if kind == "token" else None      # no int8 value is larger
+    _hold(_np(got), args, dtype, f"window {window}, sinks {sinks}", kind, steps)
+    return got
+
+
+@pytest.mark.parametrize("dtype", ACT)
+@pytest.mark.parametrize("nh,nkv,d,block", [(8, 2, 64, 16), (7, 1, 128, 128), (4, 4, 32, 7), (40, 2, 128, 32)])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (5, 3), (32, 32), (33, 0), (100, 4), (130, 70), (513, 17), (4000, 1)])
+def test_windowed_decode_matches_the_oracle(dtype, nh, nkv, d, block, window, sinks):
+    lens = [1, 2, 31, 32, 33, 97, 0, 129, 300, 517, 64, 131, 1030]
+    got = _windowed(dtype, lens, [1] * len(lens), nh, nkv, d, block, window, sinks, strided=block == 16)
+    assert (got[6] == 0).all()
+
+
+@pytest.mark.parametrize("kind", ["channel", "token"])
+@pytest.mark.parametrize("dtype", ACT)
+@pytest.mark.parametrize("nh,nkv,d,block", [(8, 2, 64, 16), (7, 1, 128, 128), (4, 4, 32, 12)])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (5, 3), (33, 40), (100, 4), (513, 17)])
+def test_windowed_decode_over_int8_caches_matches_the_oracle(kind, dtype, nh, nkv, d, block, window, sinks):
+    lens = [1, 32, 33, 97, 0, 129, 300, 1517]
+    _windowed(dtype, lens, [1] * len(lens), nh, nkv, d, block, window, sinks, kind)
+
+
+@pytest.mark.parametrize("kind", ["16", "channel", "token"])
+@pytest.mark.parametrize("dtype", ACT)
+@pytest.mark.parametrize("nh,nkv,d,block", [(8, 2, 64, 16), (7, 1, 128, 128), (4, 4, 32, 12), (3, 3, 128, 32)])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (3, 5), (32, 1), (40, 33), (200, 64)])
+def test_windowed_chunks_match_the_oracle(kind, dtype, nh, nkv, d, block, window, sinks):
+    lens, q_lens = [1, 40, 300, 97, 700, 5, 128], [1, 40, 1, 33, 150, 2, 64]
+    _windowed(dtype, lens, q_lens, nh, nkv, d, block, window, sinks, kind)
+
+
+@pytest.mark.parametrize("dtype", ACT)
+@pytest.mark.parametrize("window,sinks", [(100, 4), (1500, 300)])
+def test_a_few_rows_behind_a_long_context_are_cut_and_joined(dtype, window, sinks):
+    """Few column groups: the walk is cut into partitions, whose number differs from row to row."""
+    _windowed(dtype, [1700, 2050, 130], [3, 9, 2], 8, 2, 64, 32, window, sinks)
+    _windowed(dtype, [1700, 2050, 130], [3, 9, 2], 7, 1, 64, 20, window, sinks)
+    _windowed(dtype, [2000], [21], 7, 1, 128, 128, window, sinks, "token")
+    _windowed(dtype, [2000, 900], [21, 40], 6, 2, 64, 16, window, sinks, "channel")
+
+
+def _packed(dtype, q_lens, nh, nkv, d, window, sinks, seed=0, sliced=False, extra=0):
+    from helpers import rounded
+    from mindformers_amd import ops
+    rng = np.random.default_rng(seed)
+    t = int(np.sum(q_lens))
+    q, k, v = (rounded(rng.normal(0, 1, (t + extra, h * d)), dtype) for h in (nh, nkv, nkv))
+    dq, dk, dv = (torch.from_numpy(x).to(dtype).cuda() for x in (q, k, v))
+    if sliced:
+        fused = torch.cat([dq, dk, dv], dim=1)
+        dq, dk, dv = fused[:, :nh * d], fused[:, nh * d:(nh + nkv) * d], fused[:, (nh + nkv) * d:]
+    starts = _i32(np.concatenate([[0], np.cumsum(q_lens)]))
+    got = ops.causal_attention_varlen(dq, dk, dv, starts, nh, nkv, 1 / np.sqrt(d), window=window, sinks=sinks)
+    split = lambda x: np.split(x[:t].reshape(t, nkv, d), np.cumsum(q_lens)[:-1])  # noqa: E731
+    args = (q[:t], split(k), split(v), q_lens, q_lens, nh, nkv, 1 / np.sqrt(d), window, sinks)
+    _hold(_np(got)[:t], args, dtype, "packed rows")
+    assert (got[t:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ACT)
+@pytest.mark.parametrize("nh,nkv,d", [(8, 2, 64), (7, 1, 128), (4, 4, 32)])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 2), (31, 3), (64, 0), (129, 33), (5000, 7)])
+def test_windowed_prompts_match_the_oracle(dtype, nh, nkv, d, window, sinks):
+    _packed(dtype, [1, 300, 33, 2, 450], nh, nkv, d, window, sinks, sliced=nh == 7)
+
+
+def test_windowed_prompts_of_one_row_and_rows_of_no_sequence():
+    _packed(torch.bfloat16, [1], 8, 2, 64, 1, 0)
+    _packed(torch.bfloat16, [1], 8, 2, 64, 7, 9, extra=5)
+    _packed(torch.float16, [200, 3], 28, 4, 128, 50, 4, extra=3)
+
+
+def test_a_window_as_long_as_the_context_is_the_whole_context():
+    from mindformers_amd import ops
+    rng = np.random.default_rng(1)
+    q, cache, _, tables, _, _ = _paged(rng, torch.bfloat16, [700, 64, 1], [1, 1, 1], 8, 2, 128, 128, 10 ** 6, 0, poison=False)
+    dq, kc, vc = (torch.from_numpy(x).bfloat16().cuda() for x in (q, *cache))
+    t, n = _i32(tables), _i32([700, 64, 1])
+    whole = ops.paged_attention(dq, kc, vc, t, n, 8, 2, 0.09)
+    for window, sinks in ((700, 0), (2 ** 40, 2 ** 40), (1, 700)):
+        got = ops.paged_attention(dq, kc, vc, t, n, 8, 2, 0.09, window=window, sinks=sinks)
+        assert (got.float() - whole.float()).abs().max() <= 2 * 2.0 ** -8 * vc.float().abs().max()
+
+
+@pytest.mark.parametrize("tiled", [False, True])
+@pytest.mark.parametrize("b,hi,window", [(3, 40, 20), (5, 1500, 900), (70, 200, 64)])
+def test_windowed_decode_with_quantised_output_equals_two_calls(tiled, b, hi, window):
+    from mindformers_amd import ops
+    rng = np.random.default_rng(b)
+    lens = rng.integers(1, hi + 1, b)
+    q, cache, _, tables, _, _ = _paged(rng, torch.bfloat16, lens, [1] * b, 8, 2, 64, 16, window, 5)
+    dq, kc, vc = (torch.from_numpy(x).bfloat16().cuda() for x in (q, *cache))
+    smooth = torch.rand(512, device="cuda") + 0.5
+    args = (dq, kc, vc, _i32(tables), _i32(lens), 8, 2, 0.1)
+    want = ops.paged_attention(*args, window=window, sinks=5)
+    out, xq, xs = ops.paged_attention(*args, quant=(smooth, tiled), window=window, sinks=5)
+    wq, ws = ops.dynamic_quant(want, smooth, tiled=tiled)
+    raw = lambda x: x.data if tiled else x  # noqa: E731
+    assert torch.equal(out, want) and torch.equal(xs, ws)
+    if b % 16 == 0 or not tiled:
+        assert torch.equal(raw(xq), raw(wq))
+
+
+def test_windowed_attention_of_a_cache_past_4_gib():
+    """Blocks whose offsets pass 32 bits in bytes and in elements."""
+    from mindformers_amd import ops
+    nb, bs = 40000, 128                                       # 10.5 GB a cache, 5.2e9 elements
+    kc, vc = (torch.empty(nb, bs, 8, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    low = torch.arange(0, 6, dtype=torch.int32, device="cuda")
+    high = torch.arange(nb - 6, nb, dtype=torch.int32, device="cuda")
+    for c in (kc, vc):
+        c[low.long()] = torch.randn(6, bs, 8, 128, device="cuda").bfloat16()
+        c[high.long()] = c[low.long()]
+    q = torch.randn(2, 4096, device="cuda").bfloat16()
+    lens = _i32([700, 555])
+    for window, sinks in ((300, 4), (64, 200)):
+        a, b = (ops.paged_attention(q, kc, vc, x[None].repeat(2, 1), lens, 32, 8, 0.09, window=window, sinks=sinks) for x in (low, high))
+        assert torch.equal(a, b) and a.float().abs().sum() > 0
+        starts = _i32([0, 40, 60])
+        rows = torch.randn(60, 4096, device="cuda").bfloat16()
+        a, b = (ops.paged_attention_prefill(rows, kc, vc, x[None].repeat(2, 1), lens, starts, 32, 8, 0.09, window=window, sinks=sinks)
+                for x in (low, high))
+        assert torch.equal(a, b) and a.float().abs().sum() > 0
+
+
+def test_windowed_attention_replayed_in_a_graph():
+    from mindformers_amd import ops
+    rng = np.random.default_rng(6)
+    lens = rng.integers(1, 900, 9)
+    q, cache, _, tables, _, _ = _paged(rng, torch.float16, lens, [1] * 9, 8, 2, 64, 16, 300, 4, poison=False)
+    dq, kc, vc = (torch.from_numpy(x).half().cuda() for x in (q, *cache))
+    t, n = _i32(tables), _i32(lens)
+    call = lambda: ops.paged_attention(dq, kc, vc, t, n, 8, 2, 0.1, window=300, sinks=4)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    for _ in range(3):
+        n.copy_(_i32(np.minimum(rng.integers(1, 900, 9), lens)))
+        dq.copy_(torch.randn_like(dq))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, call())
+
+
+def test_windows_that_are_refused():
+    from mindformers_amd import ops
+    q = torch.zeros(2, 512, dtype=torch.bfloat16, device="cuda")
+    kc = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16, device="cuda")
+    t, n, starts = _i32(np.zeros((2, 2))), _i32([3, 4]), _i32([0, 1, 2])
+    for view in (dict(window=0), dict(window=-4), dict(window=2.5), dict(window=4, sinks=-1), dict(sinks=3)):
+        for call in (lambda: ops.paged_attention(q, kc, kc, t, n, 8, 2, 0.1, **view),
+                     lambda: ops.paged_attention_prefill(q, kc, kc, t, n, starts, 8, 2, 0.1, **view),
+                     lambda: ops.causal_attention_varlen(q, q[:, :128], q[:, :128], starts, 8, 2, 0.1, **view)):
+            with pytest.raises(ValueError):
+                call()
+    wide = torch.zeros(2, 384, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError, match="heads of 32, 64 or 128"):
+        ops.causal_attention_varlen(wide, wide, wide, starts, 2, 2, 0.1, window=4)
+    with pytest.raises(ValueError):
+        ops.causal_attention_varlen(wide, wide, torch.zeros(2, 256, dtype=torch.bfloat16, device="cuda"), starts, 2, 2, 0.1, window=4)
