@@ -713,7 +713,8 @@ int mf_grouped_w8a8_gemm_silu_mul_sources(void* y, const int8_t* xq, const float
                                           int n_experts, int total_rows, int n, int k, int out_dtype, void* stream);
 
 /* A decode step of a weight-only layer (QuantDecodeLayer.forward with 16-bit caches and one token a sequence) from one call:
- * the launches of mf_rmsnorm (unless `normed` brings the normed input), mf_w8a16_qkv_rope_and_cache, mf_paged_attention_decode,
+ * the launches of mf_rmsnorm (unless `normed` brings the normed input), mf_w8a16_qkv_rope_and_cache, mf_paged_attention_decode (with a
+ * window > 0: mf_window_attention_decode),
  * mf_w8a16_gemm_add_rmsnorm, mf_w8a16_gemm_silu_mul and mf_w8a16_gemm (with next_gamma: mf_w8a16_gemm_add_rmsnorm, whose norm goes to
  * norm_out), the intermediate rows in `scratch` (16-byte aligned).  The rows of fc1_w are interleaved gate / up.  Every field is
  * 8 bytes wide. */
@@ -728,6 +729,7 @@ typedef struct {
     int64_t rows, hidden, n_heads, n_kv_heads, head_dim, ffn, block_size, num_blocks, max_blocks;
     int64_t dtype, table_dtype, attn_gamma_dtype, ffn_gamma_dtype, next_gamma_dtype;
     int64_t scratch_bytes, workspace_bytes, attn_workspace_bytes;
+    int64_t window, sinks;
     double eps, next_eps, scale;
 } mf_decode_layer_args;
 size_t mf_decode_layer_args_bytes(void);                     /* what this library takes the struct to be */

@@ -124,7 +124,7 @@ DECODE_LAYER_FIELDS = {
           "context_lens", "out", "norm_out", "scratch", "workspace", "attn_workspace", "stream"),
     "q": ("rows", "hidden", "n_heads", "n_kv_heads", "head_dim", "ffn", "block_size", "num_blocks", "max_blocks", "dtype",
           "table_dtype", "attn_gamma_dtype", "ffn_gamma_dtype", "next_gamma_dtype", "scratch_bytes", "workspace_bytes",
-          "attn_workspace_bytes"),
+          "attn_workspace_bytes", "window", "sinks"),
     "d": ("eps", "next_eps", "scale"),
 }
 DECODE_LAYER_ARGS = struct.Struct("@" + "".join(f"{len(names)}{kind}" for kind, names in DECODE_LAYER_FIELDS.items()))

@@ -23,13 +23,19 @@ class QuantDecodeLayer(nn.Module):
 
     Parameters are plain buffers: ``{qkv,wo,fc1,fc2}_w`` int8 [out, in], ``*_s`` fp32 [out], optional
     ``*_b`` bias, optional ``*_smooth`` fp32 [in] (W8A8), ``attn_norm`` / ``ffn_norm`` gammas.
+
+    ``window`` (None: the whole context): attention through a sliding window of that many tokens, the query's own among
+    them, with the first ``sinks`` tokens of a sequence visible throughout.
     """
 
     NAMES = ("qkv", "wo", "fc1", "fc2")
+    window, sinks = None, 0                                   # layers built before there were windows
 
     def __init__(self, hidden, n_head, n_kv_head, head_dim, ffn, eps=1e-5, dtype=torch.bfloat16, act_quant=False,
-                 qkv_bias=False, device="cuda"):
+                 qkv_bias=False, device="cuda", window=None, sinks=0):
         super().__init__()
+        ops.check_window(window, sinks)
+        self.window, self.sinks = window, sinks
         self.hidden, self.n_head, self.n_kv_head, self.head_dim, self.ffn = hidden, n_head, n_kv_head, head_dim, ffn
         self.eps, self.dtype, self.act_quant = eps, dtype, act_quant
         self.scale_value = 1.0 / math.sqrt(head_dim)
@@ -103,6 +109,10 @@ class QuantDecodeLayer(nn.Module):
         self.kv_offset = None if offset is None else offset.to(torch.float32).contiguous()
         return self
 
+    def _view(self):
+        """The window of this layer's attention, as the operators take it."""
+        return {} if self.window is None else {"window": self.window, "sinks": self.sinks}
+
     def attend(self, q, key_cache, value_cache, block_tables, batch_valid_length, q_starts=None):
         """Attention of this step's queries over the caches (16-bit or int8)."""
         if key_cache.dtype == torch.int8:
@@ -110,12 +120,12 @@ class QuantDecodeLayer(nn.Module):
                 raise RuntimeError("int8 caches need set_kv_quant(scale, offset)")
             return ops.paged_attention_int8kv(q, key_cache, value_cache, block_tables, batch_valid_length,
                                               self.kv_scale, self.kv_offset, self.n_head, self.n_kv_head,
-                                              self.scale_value, q_starts=q_starts)
+                                              self.scale_value, q_starts=q_starts, **self._view())
         if q_starts is None:
             return ops.paged_attention(q, key_cache, value_cache, block_tables, batch_valid_length, self.n_head,
-                                       self.n_kv_head, self.scale_value)
+                                       self.n_kv_head, self.scale_value, **self._view())
         return ops.paged_attention_prefill(q, key_cache, value_cache, block_tables, batch_valid_length, q_starts,
-                                           self.n_head, self.n_kv_head, self.scale_value)
+                                           self.n_head, self.n_kv_head, self.scale_value, **self._view())
 
     def forward(self, x, key_cache, value_cache, block_tables, batch_valid_length, slot_mapping, cos, sin,
                 q_starts=None, normed=None, next_norm=None):
@@ -136,7 +146,7 @@ class QuantDecodeLayer(nn.Module):
             step = ops.decode_layer_step(x, normed, buffers["attn_norm"], buffers["ffn_norm"], next_norm,
                                          [packed.get(name) for name in self.NAMES], self.qkv_b, cos, sin, key_cache, value_cache,
                                          slot_mapping, block_tables, batch_valid_length, self.n_head, self.n_kv_head,
-                                         self.head_dim, self.eps, self.scale_value)
+                                         self.head_dim, self.eps, self.scale_value, **self._view())
             if step is not None:
                 return step[0] if next_norm is None else step
         nq, nkv = self.n_head * self.head_dim, self.n_kv_head * self.head_dim
@@ -179,7 +189,7 @@ class QuantDecodeLayer(nn.Module):
             # W8A8 decode: the attention output is only read by wo's per-token quantisation, done with the combine of
             # the partitions
             _, aq, a_s = ops.paged_attention(q, key_cache, value_cache, block_tables, batch_valid_length, self.n_head,
-                                             self.n_kv_head, self.scale_value, quant=(self.wo_smooth, True))
+                                             self.n_kv_head, self.scale_value, quant=(self.wo_smooth, True), **self._view())
             attn = None
         else:
             attn = self.attend(q, key_cache, value_cache, block_tables, batch_valid_length, q_starts)

@@ -1,4 +1,5 @@
 """Drop-in modules of the decode path (same constructor / call surface as the reference's cells)."""
+from .beam_search import BeamSearch
 from .block_tables import BlockMemPool, BlockTables, CacheEngine
 from .flash_attention import FlashAttention
 from .infer_attention import InferAttention, InferRotaryEmbedding

@@ -11,12 +11,20 @@ class FlashAttention(nn.Module):
     """ReshapeAndCache, then FlashAttentionScore (prefill) or PagedAttention (decode; with q_seq_lens: several new
     tokens per sequence; with pa_mla_v_dim > 0: multi-latent decode over the single latent cache, whose prefill runs as
     ordinary attention on the up-projected keys and values).  Masks are causal: `attn_mask` is accepted for signature parity and taken to be the lower
-    triangle the reference's models build; sparse modes other than the causal default are not built."""
+    triangle the reference's models build; sparse modes other than the causal default are not built.  ``window`` (None: the
+    whole context) / ``sinks``: a query sees its own and the window - 1 tokens in front of it, and the first ``sinks`` tokens
+    (not with multi-latent attention)."""
+
+    window, sinks = None, 0
 
     def __init__(self, head_num, head_dim=None, kv_head_num=None, keep_prob=1.0, scale_value=1.0,
                  pre_tokens=2147483647, next_tokens=2147483647, sparse_mode=0, input_layout="TH",
-                 pa_kv_head_num=None, pa_mla_v_dim=0):
+                 pa_kv_head_num=None, pa_mla_v_dim=0, window=None, sinks=0):
         super().__init__()
+        ops.check_window(window, sinks)
+        if window is not None and pa_mla_v_dim > 0:
+            raise NotImplementedError("a window over a latent cache is not built")
+        self.window, self.sinks = window, sinks
         if input_layout not in ("TH", "TND"):
             raise ValueError(f"input_layout must be TH or TND, got {input_layout}")
         self.head_num = head_num
@@ -50,6 +58,7 @@ class FlashAttention(nn.Module):
         if kv8 and self.use_multi_latent_attention:
             raise NotImplementedError("an int8 latent cache is not built")
         token_scales = (key_scale_cache, value_scale_cache) if per_token else None
+        view = {} if self.window is None else {"window": self.window, "sinks": self.sinks}
         if per_token:
             ops.dynamic_quant_reshape_and_cache(key, value, key_cache, value_cache, key_scale_cache, value_scale_cache,
                                                 slot_mapping)
@@ -78,7 +87,7 @@ class FlashAttention(nn.Module):
             if q2.shape[1] != self.head_num * d or k2.shape[1] % d or (v2.shape[1] != k2.shape[1] and not narrow_v):
                 raise ValueError(f"query / key / value widths {q2.shape[1]} / {k2.shape[1]} / {v2.shape[1]} do not "
                                  f"fit {self.head_num} heads")
-            out = ops.causal_attention_varlen(q2, k2, v2, starts, self.head_num, k2.shape[1] // d, self.scale_value)
+            out = ops.causal_attention_varlen(q2, k2, v2, starts, self.head_num, k2.shape[1] // d, self.scale_value, **view)
             if narrow_v:                                      # 128-wide value heads of multi-latent attention, unpadded
                 return out
             return out.reshape(shape)
@@ -90,15 +99,15 @@ class FlashAttention(nn.Module):
             starts = None if q_seq_lens is None else ops.q_starts_from_lens(q_seq_lens)
             out = ops.paged_attention_int8kv(q2, key_cache, value_cache, block_tables, batch_valid_length,
                                              antiquant_scale, antiquant_offset, self.head_num, self.pa_kv_head_num,
-                                             self.scale_value, q_starts=starts, token_scales=token_scales)
+                                             self.scale_value, q_starts=starts, token_scales=token_scales, **view)
             return out.reshape(shape)
         if q_seq_lens is not None:                            # several new tokens per sequence (flash_attention.py:140-143)
             out = ops.paged_attention_prefill(q2, key_cache, value_cache, block_tables, batch_valid_length,
                                               ops.q_starts_from_lens(q_seq_lens), self.head_num,
-                                              self.pa_kv_head_num, self.scale_value)
+                                              self.pa_kv_head_num, self.scale_value, **view)
             return out.reshape(shape)
         out = ops.paged_attention(q2, key_cache, value_cache, block_tables, batch_valid_length, self.head_num,
-                                  self.pa_kv_head_num, self.scale_value)
+                                  self.pa_kv_head_num, self.scale_value, **view)
         return out.reshape(shape)
 
     construct = forward

@@ -39,13 +39,14 @@ class InferAttention(nn.Module):
     context length including the token written by this call.  Prefill (`is_first_iteration`): causal attention over
     this call's own keys; in the TH layout `batch_valid_length` (the lengths of the packed sequences, or their
     increasing row ends) is what the reference hands to FlashAttentionScore (infer_attention.py:459-461), in BSH
-    every batch row is a full sequence of S tokens.  Masks are causal; `attn_mask` is not read."""
+    every batch row is a full sequence of S tokens.  Masks are causal; `attn_mask` is not read.  ``window`` / ``sinks``: as in
+    PagedAttentionMgr, for every form of the attention."""
 
     def __init__(self, n_head, head_dim, n_kv_head, pa_n_head_split=None, pa_n_kv_head_split=None, keep_prob=1.0,
                  scale_value=1.0, pre_tokens=2147483647, next_tokens=2147483647, sparse_mode=0, block_size=16,
                  num_blocks=1024, seq_length=-1, is_dynamic=True, use_flash_attention=True, use_alibi_mask=False,
                  use_rope_rotary_emb=True, rotary_cos_format=0, compute_dtype=torch.float16, parallel_decoding=False,
-                 chunk_prefill=False, device="cuda"):
+                 chunk_prefill=False, device="cuda", window=None, sinks=0):
         super().__init__()
         if use_alibi_mask:
             raise NotImplementedError("alibi attention is not built")
@@ -78,7 +79,7 @@ class InferAttention(nn.Module):
         self.paged_attention_mgr = PagedAttentionMgr(self.pa_n_head_split, self.head_dim, self.pa_n_kv_head_split,
                                                      kv_shape, seq_length, compute_dtype=self.compute_dtype,
                                                      parallel_decoding=parallel_decoding, chunk_prefill=chunk_prefill,
-                                                     device=device)
+                                                     device=device, window=window, sinks=sinks)
         if use_rope_rotary_emb:
             self.rotary_embedding = InferRotaryEmbedding(self.rotary_cos_format, n_head, n_kv_head, head_dim)
 
@@ -127,7 +128,9 @@ class InferAttention(nn.Module):
         else:                                                 # BSH: every batch row is one sequence of S tokens
             bsz, seq = shape[0], shape[1]
             starts = torch.arange(0, bsz + 1, dtype=torch.int32, device=query.device) * seq
-        return ops.causal_attention_varlen(query, key, value, starts, self.n_head, self.n_kv_head, self.scale_value)
+        mgr = self.paged_attention_mgr                        # may have been replaced by a quantised one, with the same window
+        view = {} if getattr(mgr, "window", None) is None else {"window": mgr.window, "sinks": mgr.sinks}
+        return ops.causal_attention_varlen(query, key, value, starts, self.n_head, self.n_kv_head, self.scale_value, **view)
 
     construct = forward
 

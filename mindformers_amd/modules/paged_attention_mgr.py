@@ -11,11 +11,16 @@ from .. import ops
 
 class PagedAttentionMgr(nn.Module):
     """Owns the key/value caches [num_blocks, block_size, n_kv_heads, head_dim] and runs
-    reshape_and_cache / paged_attention on them (paged_attention_mgr.py:29-58)."""
+    reshape_and_cache / paged_attention on them (paged_attention_mgr.py:29-58).  ``window`` (None: the whole context) / ``sinks``:
+    a query sees its own and the window - 1 tokens in front of it, and the first ``sinks`` tokens."""
+
+    window, sinks = None, 0
 
     def __init__(self, n_heads, head_dim, n_kv_heads, kv_shape, seq_length=-1, compute_dtype=torch.float16,
-                 parallel_decoding=False, chunk_prefill=False, device="cuda"):
+                 parallel_decoding=False, chunk_prefill=False, device="cuda", window=None, sinks=0):
         super().__init__()
+        ops.check_window(window, sinks)
+        self.window, self.sinks = window, sinks
         if len(kv_shape) != 4:
             raise ValueError(f"kv_shape must be (num_blocks, block_size, n_kv_heads, head_dim), got {kv_shape}")
         if kv_shape[2] != n_kv_heads or kv_shape[3] != head_dim:
@@ -37,6 +42,10 @@ class PagedAttentionMgr(nn.Module):
 
     construct = forward
 
+    def _view(self):
+        """The window of the attention, as the operators take it."""
+        return {} if self.window is None else {"window": self.window, "sinks": self.sinks}
+
     def paged_attn(self, query, batch_valid_length, block_tables, attn_mask=None, q_seq_lens=None):
         """The forward compute of Paged Attention (paged_attention_mgr.py:64-70).  With parallel_decoding or
         chunk_prefill every sequence brings q_seq_lens[b] new tokens, masked causally among themselves: `attn_mask` is
@@ -48,10 +57,10 @@ class PagedAttentionMgr(nn.Module):
                 raise ValueError("parallel_decoding / chunk_prefill need q_seq_lens")
             out = ops.paged_attention_prefill(q2, self.key_cache, self.value_cache, block_tables, batch_valid_length,
                                               ops.q_starts_from_lens(q_seq_lens), self.n_heads, self.n_kv_heads,
-                                              self.scale_value)
+                                              self.scale_value, **self._view())
         else:
             out = ops.paged_attention(q2, self.key_cache, self.value_cache, block_tables, batch_valid_length,
-                                      self.n_heads, self.n_kv_heads, self.scale_value)
+                                      self.n_heads, self.n_kv_heads, self.scale_value, **self._view())
         return out if out.shape == shape else out.reshape(shape)
 
     def paged_attn_with_alibi(self, query, batch_valid_length, block_tables, alibi_tensor):
@@ -77,9 +86,9 @@ class QuantPagedAttentionMgr(PagedAttentionMgr):
     in ``key_scale_cache`` / ``value_scale_cache`` float32 [num_blocks, block_size]."""
 
     def __init__(self, n_heads, head_dim, n_kv_heads, kv_shape, seq_length=-1, compute_dtype=torch.float16,
-                 parallel_decoding=False, chunk_prefill=False, device="cuda", granularity="per_channel"):
+                 parallel_decoding=False, chunk_prefill=False, device="cuda", granularity="per_channel", window=None, sinks=0):
         super().__init__(n_heads, head_dim, n_kv_heads, (1,) + tuple(kv_shape[1:]), seq_length, compute_dtype,
-                         parallel_decoding, chunk_prefill, device)
+                         parallel_decoding, chunk_prefill, device, window=window, sinks=sinks)
         if granularity not in ("per_channel", "per_token"):
             raise ValueError(f"kvcache_quant_granularity must be per_channel or per_token, got {granularity!r}")
         self.granularity = granularity
@@ -101,7 +110,8 @@ class QuantPagedAttentionMgr(PagedAttentionMgr):
         """A quantised manager with the geometry of a float one."""
         kc = mgr.key_cache
         return cls(mgr.n_heads, mgr.head_dim, mgr.n_kv_heads, tuple(kc.shape), mgr.seq_length, kc.dtype,
-                   mgr.parallel_decoding, mgr.chunk_prefill, kc.device, granularity=granularity)
+                   mgr.parallel_decoding, mgr.chunk_prefill, kc.device, granularity=granularity, window=mgr.window,
+                   sinks=mgr.sinks)
 
     def set_kv_quant(self, scale, offset=None):
         if self.granularity == "per_token":
@@ -134,5 +144,5 @@ class QuantPagedAttentionMgr(PagedAttentionMgr):
                                          self.kv_scale, self.kv_offset, self.n_heads, self.n_kv_heads,
                                          self.scale_value, q_starts=starts,
                                          token_scales=(self.key_scale_cache, self.value_scale_cache)
-                                         if self.granularity == "per_token" else None)
+                                         if self.granularity == "per_token" else None, **self._view())
         return out.reshape(shape)

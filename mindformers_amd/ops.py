@@ -1625,10 +1625,10 @@ def grouped_w8a8_linear(xq, x_scale, w, offsets, out_dtype=torch.bfloat16, retur
 
 
 def decode_layer_step(x, normed, attn_norm, ffn_norm, next_norm, weights, qkv_bias, cos, sin, key_cache, value_cache, slots, tables,
-                      lens, n_heads, n_kv_heads, head_dim, eps, scale):
+                      lens, n_heads, n_kv_heads, head_dim, eps, scale, window=None, sinks=0):
     """A decode step of a weight-only layer in one native call, or None where an operand is not of the plain form that it takes (the
     caller then goes through the separate operators, which say what is wrong or take the other form).  x [T, hidden]; ``weights``:
-    the packed (qkv, wo, fc1, fc2), fc1 gated; ``next_norm`` None or (gamma, eps).  Returns (out, normed output or None)."""
+    the packed (qkv, wo, fc1, fc2), fc1 gated; ``next_norm`` None or (gamma, eps); ``window`` / ``sinks`` as in ``paged_attention``.  Returns (out, normed output or None)."""
     dt, dev = x.dtype, x.get_device()
     rows = lens.numel()
     if dt not in _ACT or dev < 0 or x.dim() != 2 or rows == 0 or key_cache.dim() != 4:
@@ -1664,7 +1664,9 @@ def decode_layer_step(x, normed, attn_norm, ffn_norm, next_norm, weights, qkv_bi
     sizes = (rows, hidden, n_heads, n_kv, d, ffn)
     need = lib.mf_decode_layer_workspace_bytes(*sizes)
     ws = workspace(need, device, "gemm") if need else None
-    need = lib.mf_paged_attention_workspace_bytes(rows, n_heads, d, tables.shape[1] * bs)
+    window, sinks = check_window(window, sinks)
+    need = lib.mf_window_attention_workspace_bytes(rows, n_heads, d, tables.shape[1] * bs, window, sinks) if window else \
+        lib.mf_paged_attention_workspace_bytes(rows, n_heads, d, tables.shape[1] * bs)
     pws = workspace(need, device, "pa") if need else None
     scratch_bytes = lib.mf_decode_layer_scratch_bytes(*sizes)
     scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=device)
@@ -1681,7 +1683,7 @@ def decode_layer_step(x, normed, attn_norm, ffn_norm, next_norm, weights, qkv_bi
         rows, hidden, n_heads, n_kv, d, ffn, bs, nb, tables.shape[1],
         dtype_code(dt), dtype_code(cos.dtype), dtype_code(attn_norm.dtype), dtype_code(ffn_norm.dtype),
         0 if gamma is None else dtype_code(gamma.dtype), scratch_bytes, 0 if ws is None else ws.numel(),
-        0 if pws is None else pws.numel(), float(eps), float(next_eps), float(scale))
+        0 if pws is None else pws.numel(), window, sinks, float(eps), float(next_eps), float(scale))
     check(lib.mf_decode_layer_step(args), "mf_decode_layer_step")
     return out, norm_out
 

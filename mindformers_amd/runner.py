@@ -94,6 +94,7 @@ class DecodeStackRunner:
         d = self.head_size
         inv = 1.0 / (theta ** (torch.arange(0, d, 2, dtype=torch.float32, device=self.device) / d))
         self._rope_theta, self._inv_freq = theta, inv.cpu().numpy()
+        self._freq_dev = inv                                  # for steps whose arrays are on the device: whole since .cpu(), never written again
 
     def _rope_rows(self, positions, inv_freq):
         if positions.dtype == torch.int32 and positions.is_contiguous():
@@ -162,7 +163,24 @@ class DecodeStackRunner:
         slots = there["slots"] if "slots" in there else torch.as_tensor(slot_mapping, dtype=torch.int32, device=self.device)
         pos_t = there["pos"] if "pos" in there else torch.as_tensor(position_ids, device=self.device).reshape(-1)
         cos, sin = self._rope_rows(pos_t, there["freq"].view(torch.float32))
-        h = hidden_states
+        h = self._run_layers(hidden_states, tables, lens_t, slots, cos, sin, q_starts)
+        if prefill:
+            self.add_flags_custom(is_first_iteration=False)
+        return h
+
+    def decode(self, hidden_states, context_lens, block_tables, slot_mapping):
+        """One decode step whose arrays are on the device, int32: what a loop that never comes back to the host has (``BeamSearch``).  Row i
+        brings the token at position context_lens[i] - 1; empty rows have length 0 and slot -1.  No host synchronisation; can be
+        captured into a graph."""
+        for t, n, name in ((context_lens, 1, "context_lens"), (slot_mapping, 1, "slot_mapping"), (block_tables, 2, "block_tables")):
+            if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.int32 and t.dim() == n and t.is_contiguous()
+                    and t.shape[0] == hidden_states.shape[0]):
+                raise ValueError(f"{name} must be a contiguous int32 device tensor with a row for each of {hidden_states.shape[0]} tokens")
+        self.add_flags_custom(is_first_iteration=False)
+        cos, sin = self._rope_rows(torch.clamp(context_lens - 1, min=0), self._freq_dev)
+        return self._run_layers(hidden_states, block_tables, context_lens, slot_mapping, cos, sin, None)
+
+    def _run_layers(self, h, tables, lens_t, slots, cos, sin, q_starts):
         normed = None
         for i, layer in enumerate(self.layers):
             # layer i also computes layer i + 1's attention norm (W8A8: and its quantisation), in the kernel that
@@ -175,9 +193,16 @@ class DecodeStackRunner:
             out = layer(h, self.key_cache[i], self.value_cache[i], tables, lens_t, slots, cos, sin, q_starts=q_starts,
                         normed=normed, next_norm=nn)
             h, normed = out if chain else (out, None)
-        if prefill:
-            self.add_flags_custom(is_first_iteration=False)
         return h
+
+    def caches(self):
+        """Every cache tensor of every layer, as ``ops.copy_blocks`` and ``BeamSearch`` take them."""
+        return self.key_cache + self.value_cache
+
+    def copy_blocks(self, copies):
+        """Copy blocks within the key and value caches of all layers (``ops.copy_blocks``): the list of a fork or of a
+        compaction, or host integers (source, destination[, rows])."""
+        ops.copy_blocks(self.caches(), copies)
 
     def swap(self, block_tables, swap_type):
         """Swap key/value cache blocks between host and device for every layer (model_runner.py:477-491).

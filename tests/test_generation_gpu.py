@@ -529,3 +529,178 @@ def test_windows_that_are_refused():
         ops.causal_attention_varlen(wide, wide, wide, starts, 2, 2, 0.1, window=4)
     with pytest.raises(ValueError):
         ops.causal_attention_varlen(wide, wide, torch.zeros(2, 256, dtype=torch.bfloat16, device="cuda"), starts, 2, 2, 0.1, window=4)
+
+
+# --------------------------------------------------------------------------------------------- the operators together
+def _stack(window, sinks, act_quant=False, dtype=torch.bfloat16, seed=3, n=2):
+    from mindformers_amd import synthetic
+    from mindformers_amd.decode_layer import QuantDecodeLayer
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(seed)
+    return [synthetic.fill_layer(QuantDecodeLayer(512, 8, 2, 64, 1024, 1e-5, dtype, act_quant, window=window, sinks=sinks), gen)
+            for _ in range(n)]
+
+
+@pytest.mark.parametrize("window,sinks", [(None, 0), (24, 3)])
+def test_a_beam_search_over_shared_blocks_is_one_over_private_ones(window, sinks):
+    """Beam search of three prompts through a two-layer stack whose beams share blocks, against the same search with every beam's
+    cache copied as a whole to blocks of its own: the same tokens, and the layers' outputs bit for bit."""
+    from mindformers_amd import ops
+    from mindformers_amd.modules import BeamSearch, BlockTables
+    from mindformers_amd.runner import DecodeStackRunner
+    bs, width, k, vocab, steps = 8, 9, 3, 211, 30
+    layers = _stack(window, sinks)
+    shared, private = (DecodeStackRunner(layers, npu_mem_size=0.004, cpu_mem_size=0, block_size=bs) for _ in range(2))
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(11)
+    embed = torch.randn(vocab, 512, generator=gen, device="cuda").bfloat16()
+    head = torch.randn(512, vocab, generator=gen, device="cuda") / 16
+    lens = np.array([13, 1, 32])
+    blocks = BlockTables(shared.npu_num_blocks, bs, width * bs)
+    blocks.init_cache_engine(3)
+    tables, slots = blocks.assemble_pa_full_inputs(32, lens, [False] * 3)
+    slots = slots.reshape(3, -1)
+    words = [torch.randint(0, vocab, (int(n),), generator=gen, device="cuda") for n in lens]
+    x = embed[torch.cat(words)]
+    hidden = shared.forward(x, lens, tables, np.concatenate([slots[i, :n] for i, n in enumerate(lens)]), prefill=True)
+    first = hidden[torch.tensor(np.cumsum(lens) - 1, device="cuda")].float() @ head
+
+    rows = 3 * k
+    own = torch.arange(rows * width, device="cuda", dtype=torch.int32).view(rows, width)
+    assert private.npu_num_blocks >= rows * width
+    for a, b in zip(shared.caches(), private.caches()):
+        for r in range(rows):
+            for j in range(-(-int(lens[r // k]) // bs)):
+                b[own[r, j].item()] = a[int(tables[r // k, j])]
+
+    search = BeamSearch(shared.caches(), k, eos_token_id=5, window=window, sinks=sinks)
+    tokens = search.start(tables, lens, first)
+    beams = [[] for _ in range(rows)]                         # the tokens of every row, kept on the host
+    scores = torch.full((3, k), -torch.inf, device="cuda")
+    scores[:, 0] = 0
+    logits, n = first.repeat_interleave(k, 0), torch.from_numpy(lens).cuda().repeat_interleave(k)
+    finished = [[] for _ in range(3)]
+    for step in range(steps):
+        sel = ops.beam_search_select(logits, scores, eos_token_id=5)
+        assert torch.equal(sel.next_tokens.view(-1), tokens)
+        for g in range(3):
+            for s, b, t in zip(sel.scores[g, :k].tolist(), sel.beams[g, :k].tolist(), sel.tokens[g, :k].tolist()):
+                if t == 5 and np.isfinite(s):
+                    finished[g].append((s / (step + 1), beams[g * k + b] + [5]))
+        parents, scores = sel.next_rows.view(-1), sel.next_scores
+        beams = [beams[p] + [t] for p, t in zip(parents.tolist(), tokens.tolist())]
+        for c in private.caches():
+            c[:rows * width] = c[:rows * width].view(rows, width, *c.shape[1:])[parents.long()].view(rows * width, *c.shape[1:])
+        n = n + 1
+        slot = own[torch.arange(rows, device="cuda"), (n - 1) // bs] * bs + ((n - 1) % bs).int()
+        got = shared.decode(embed[tokens.long()], search.context_lens, search.block_tables, search.slot_mapping)
+        want = private.decode(embed[tokens.long()], n.int(), own, slot.int())
+        assert torch.equal(got, want), f"step {step}"
+        if step == 12:
+            before = torch.unique(search.block_tables[search.block_tables >= 0]).numel()
+            assert int(search.compact()) == before and int(search.block_tables.max()) == before - 1
+        logits = got.float() @ head
+        if step + 1 < steps:
+            tokens = search.step(logits)
+    used = torch.unique(search.block_tables[search.block_tables >= 0]).numel()
+    assert used < 9 * 6 and (window is None or used <= 9 * 4 + 9)
+    live = [[(s / steps, beams[g * k + i]) for i, s in enumerate(scores[g].tolist())] for g in range(3)]
+    for g, found in enumerate(search.hypotheses()):
+        assert sorted(t for _, t in found) == sorted(t for _, t in finished[g] + live[g])
+        assert [s for s, _ in found] == sorted((s for s, _ in found), reverse=True)
+        np.testing.assert_allclose(sorted(s for s, _ in found), sorted(s for s, _ in finished[g] + live[g]), rtol=1e-12)
+    search.release([1])
+    search.step(logits)
+    assert (search.block_tables[k:2 * k] == -1).all() and (search.slot_mapping[k:2 * k] == -1).all()
+    assert (search.context_lens[k:2 * k] == 0).all() and (search.slot_mapping[:k] >= 0).all()
+    again = shared.decode(embed[tokens.long()], search.context_lens, search.block_tables, search.slot_mapping)
+    assert torch.isfinite(again.float()).all()
+
+
+def test_a_beam_search_without_blocks_says_so():
+    from mindformers_amd.modules import BeamSearch
+    caches = [torch.zeros(4, 4, 1, 32, dtype=torch.float16, device="cuda")]
+    search = BeamSearch(caches, 4)
+    search.start(np.array([[0, 1, -1, -1]]), np.array([7]), torch.randn(1, 50, device="cuda"))
+    with pytest.raises(RuntimeError, match="short"):          # 1 prompt block and 4 open ones do not fit 4 blocks
+        search.hypotheses()
+
+
+@pytest.mark.parametrize("act_quant", [False, True])
+@pytest.mark.parametrize("rows", [3, 40])
+def test_a_windowed_layer_is_a_full_one_on_the_tokens_that_it_sees(act_quant, rows, dtype=torch.bfloat16):
+    """A decode step through a window without sinks against the same layer without a window on a cache that holds the window's
+    tokens only: the same operands in another place (the tiles of a walk start at multiples of 32, so do the copies here)."""
+    bs, window = 32, 64
+    layer, = _stack(window, 0, act_quant, dtype, n=1)
+    full, = _stack(None, 0, act_quant, dtype, n=1)
+    nb = rows * 8
+    kc, vc = (torch.randn(nb, bs, 2, 64, device="cuda").to(dtype) for _ in range(2))
+    tables = torch.randperm(nb, device="cuda").int().view(rows, 8)
+    n = torch.full((rows,), 160, dtype=torch.int32, device="cuda")       # the window is tokens 96 to 159: blocks 3 and 4
+    slots = tables[:, 4] * bs + 31
+    x = torch.randn(rows, 512, device="cuda").to(dtype)
+    cos, sin = torch.ones(rows, 64, device="cuda").to(dtype), torch.zeros(rows, 64, device="cuda").to(dtype)
+    k2, v2 = kc.clone(), vc.clone()
+    hidden = tables.clone()
+    hidden[:, :3] = -1
+    got = layer(x, kc, vc, hidden, n, slots, cos, sin)
+    want = full(x, k2, v2, tables[:, 3:].contiguous(), torch.full_like(n, 64), slots, cos, sin)
+    assert torch.equal(kc, k2) and torch.equal(vc, v2)
+    assert torch.equal(got, want)
+
+
+def test_the_modules_pass_their_window_on():
+    """InferAttention and FlashAttention in every form of their attention, a manager and its quantised successor."""
+    from mindformers_amd import ops
+    from mindformers_amd.modules import FlashAttention, InferAttention, PagedAttentionMgr, QuantPagedAttentionMgr
+    nh, nkv, d, bs, nb, view = 4, 2, 64, 16, 12, dict(window=20, sinks=2)
+    t = torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4)
+    n = _i32([50, 33])
+    mk = lambda r, h: torch.randn(r, h * d, device="cuda").half()  # noqa: E731
+    q, k, v = mk(2, nh), mk(2, nkv), mk(2, nkv)
+    slots = torch.tensor([3 * 16 + 1, 4 * 16 + 2 * 16], dtype=torch.int32, device="cuda")
+    attn = InferAttention(nh, d, nkv, scale_value=0.1, block_size=bs, num_blocks=nb, use_rope_rotary_emb=False, **view)
+    mgr = attn.paged_attention_mgr
+    mgr.scale_value = 0.1
+    mgr.key_cache.normal_()
+    mgr.value_cache.normal_()
+    attn.is_first_iteration = False
+    got = attn(q, k, v, n, t, slots)
+    want = ops.paged_attention(q, mgr.key_cache, mgr.value_cache, t, n, nh, nkv, 0.1, **view)
+    assert torch.equal(got, want) and not torch.equal(got, ops.paged_attention(q, mgr.key_cache, mgr.value_cache, t, n, nh, nkv, 0.1))
+    flash = FlashAttention(nh, d, nkv, scale_value=0.1, **view)
+    flash.is_prefill = False
+    assert torch.equal(flash(q, k, v, slots, t, n, key_cache=mgr.key_cache, value_cache=mgr.value_cache), want)
+    # prompts
+    q, k, v = mk(60, nh), mk(60, nkv), mk(60, nkv)
+    ends, starts = _i32([37, 60]), _i32([0, 37, 60])
+    want = ops.causal_attention_varlen(q, k, v, starts, nh, nkv, 0.1, **view)
+    none = torch.full((60,), -1, dtype=torch.int32, device="cuda")
+    flash.is_prefill = attn.is_first_iteration = True
+    assert torch.equal(flash(q, k, v, none, actual_seq_qlen=ends, key_cache=mgr.key_cache, value_cache=mgr.value_cache), want)
+    assert torch.equal(attn(q, k, v, ends, t, none), want)
+    # chunks
+    q, lens = mk(9, nh), _i32([5, 4])
+    chunked = PagedAttentionMgr(nh, d, nkv, (nb, bs, nkv, d), chunk_prefill=True, **view)
+    chunked.key_cache.copy_(mgr.key_cache)
+    chunked.value_cache.copy_(mgr.value_cache)
+    want = ops.paged_attention_prefill(q, mgr.key_cache, mgr.value_cache, t, n, _i32([0, 5, 9]), nh, nkv, chunked.scale_value, **view)
+    assert torch.equal(chunked.paged_attn(q, n, t, q_seq_lens=lens), want)
+    for gran in ("per_channel", "per_token"):
+        quant = QuantPagedAttentionMgr.from_float(chunked, gran)
+        assert (quant.window, quant.sinks) == (20, 2)
+        quant.key_cache.random_(-100, 100)
+        quant.value_cache.random_(-100, 100)
+        if gran == "per_token":
+            quant.key_scale_cache.fill_(0.01)
+            quant.value_scale_cache.fill_(0.01)
+        out = quant.paged_attn(q, n, t, q_seq_lens=lens)
+        quant.window = None
+        assert not torch.equal(out, quant.paged_attn(q, n, t, q_seq_lens=lens))
+    with pytest.raises(NotImplementedError):
+        FlashAttention(nh, d, nkv, pa_mla_v_dim=512, **view)
+    for make in (lambda: InferAttention(nh, d, nkv, window=0), lambda: FlashAttention(nh, d, nkv, sinks=3),
+                 lambda: PagedAttentionMgr(nh, d, nkv, (nb, bs, nkv, d), window=-1)):
+        with pytest.raises(ValueError):
+            make()
