@@ -92,7 +92,7 @@ int mf_swap_blocks(void* host_cache, void* device_cache, const int64_t* pairs, i
  *   - new blocks are the lowest that no kept entry names and `held` (a byte a block, may be NULL: blocks of other tables) does
  *     not mark, handed out row by row: in a row the copied open block first.  Where they, or the table's width, do not suffice, the
  *     entries stay -1 and *missing counts them.
- * Distinct rows must not share an open block in `tables` unless one is copied from the other by this call.  num_blocks <= 2^20;
+ * Distinct rows must not share an open block in `tables` unless one is copied from the other by this call.  num_blocks <= 2^20, rows <= 4096;
  * workspace: mf_fork_blocks_workspace_bytes. */
 size_t mf_fork_blocks_workspace_bytes(int rows, int block_size, int new_tokens);
 int mf_fork_blocks(int32_t* tables_out, int32_t* lens_out, int32_t* slots, int32_t* copies, int32_t* missing,

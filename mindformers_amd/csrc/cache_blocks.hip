@@ -13,12 +13,13 @@ namespace {
 constexpr int CB_THREADS = 1024;
 constexpr int CB_WAVES = CB_THREADS / 64;
 constexpr int CB_MAX_BLOCKS = 1 << 20;                        // bits of the bitmap: 128 KB of LDS
+constexpr int CB_MAX_ROWS = 4096;                             // rows of a fork: 16 KB of LDS beside it
 
 struct ForkArgs {
     int32_t *tables_out, *lens_out, *slots, *copies, *missing;
     const int32_t *tables, *lens, *parents;
     const uint8_t* held;
-    int32_t *split, *fresh;                                   // workspace: [rows], [fresh blocks asked for]
+    int32_t* fresh;                                           // workspace: the blocks that are handed out
     int rows, width, num_blocks, block_size, new_tokens, window, sinks;
 };
 
@@ -41,26 +42,15 @@ __device__ __forceinline__ bool fork_keeps(const ForkArgs& a, int j, int len) {
     return (int64_t)(j + 1) * a.block_size > (int64_t)len - a.window + 1 || (int64_t)j * a.block_size < a.sinks;
 }
 
-// One row of the new tables without the blocks that are still to be found, by one wave: the open block (the last one,
-// where it is not full) goes to the lowest child of a parent, which `split` says.
+// One row of the new tables without the blocks that are still to be found, by one wave.  The open block (the last one, where
+// it is not full) is every child's here.
 __device__ __forceinline__ void fork_gather_row(const ForkArgs& a, int s) {
-    const int lane = threadIdx.x & 63;
     const ForkRow r = fork_row(a, s);
-    bool elder = false;                                       // a lower row with the same parent
-    const bool open = r.parent >= 0 && r.len % a.block_size != 0;
-    if (open && a.parents) {
-        for (int t0 = 0; t0 < s && !elder; t0 += 64) elder = __ballot(t0 + lane < s && a.parents[min(t0 + lane, s)] == r.parent) != 0;
-    }
     const int32_t* from = a.tables + (int64_t)max(r.parent, 0) * a.width;
-    if (elder) {
-        const int page = from[r.used - 1];
-        elder = page >= 0 && page < a.num_blocks;             // nothing to copy where the parent has no block
-    }
-    if (lane == 0) a.split[s] = elder;
     int32_t* to = a.tables_out + (int64_t)s * a.width;
-    for (int j = lane; j < a.width; j += 64) {
+    for (int j = threadIdx.x & 63; j < a.width; j += 64) {
         int page = -1;
-        if (j < r.used && fork_keeps(a, j, r.len) && !(elder && j == r.used - 1)) {
+        if (j < r.used && fork_keeps(a, j, r.len)) {
             page = from[j];
             if (page >= a.num_blocks) page = -1;
         }
@@ -98,16 +88,22 @@ __device__ __forceinline__ int block_scan(int v, int* red, int& total) {
 
 __device__ __forceinline__ void mark(uint32_t* bits, int page, int num_blocks) {
     if (page < 0 || page >= num_blocks) return;
-    const uint32_t m = 1u << (page & 31);
-    if (!(bits[page >> 5] & m)) atomicOr(&bits[page >> 5], m);
+    atomicOr(&bits[page >> 5], 1u << (page & 31));            // nothing waits for it; looking first took half as long again
 }
 // the bits of all entries of a table
 __device__ __forceinline__ void mark_table(uint32_t* bits, const int32_t* t, int64_t n, int num_blocks) {
     const int64_t n4 = ((uintptr_t)t & 15) == 0 ? n / 4 : 0;
-    for (int64_t i = threadIdx.x; i < n4; i += CB_THREADS) {
-        const i32x4 v = ((const i32x4*)t)[i];
+    for (int64_t i0 = threadIdx.x; i0 < n4; i0 += 8 * CB_THREADS) {
+        i32x4 v[8];                                           // eight reads on their way at a time: one workgroup waits for each
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mark(bits, v[e], num_blocks);
+        for (int k = 0; k < 8; ++k) {
+            const int64_t i = i0 + k * CB_THREADS;
+            v[k] = i < n4 ? ((const i32x4*)t)[i] : (i32x4){-1, -1, -1, -1};
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mark(bits, v[k][e], num_blocks);
     }
     for (int64_t i = 4 * n4 + threadIdx.x; i < n; i += CB_THREADS) mark(bits, t[i], num_blocks);
 }
@@ -125,25 +121,46 @@ __device__ __forceinline__ uint32_t in_range(int w, int num_blocks) {
 
 // The blocks that a fork's rows ask for: rows ascending, in a row the copy of its open block first, then the blocks of its
 // new tokens; request i gets the i-th lowest free block.  GATHER: the rows are gathered here too (small tables: one launch).
+struct ForkRequest {
+    ForkRow r;
+    int open, wanted;                                         // block to copy (-1: none), blocks behind it
+};
 template <bool GATHER>
 __global__ __launch_bounds__(CB_THREADS) void fork_assign_kernel(ForkArgs a) {
     extern __shared__ uint32_t bits[];
     __shared__ int red[CB_WAVES];
     const int tid = threadIdx.x;
     const int words = (a.num_blocks + 31) / 32;
+    int* eldest = (int*)(bits + words);                       // lowest child of every row
     for (int w = tid; w < words; w += CB_THREADS) bits[w] = held_word(a.held, w, a.num_blocks);
+    for (int s = tid; s < a.rows; s += CB_THREADS) eldest[s] = a.rows;
     if constexpr (GATHER) {
         for (int s = tid >> 6; s < a.rows; s += CB_WAVES) fork_gather_row(a, s);
         __threadfence_block();
     }
     __syncthreads();
-    mark_table(bits, a.tables_out, (int64_t)a.rows * a.width, a.num_blocks);
-
-    // how many blocks are asked for
-    int asked = 0;
     for (int s = tid; s < a.rows; s += CB_THREADS) {
-        const ForkRow r = fork_row(a, s);
-        if (r.parent >= 0) asked += a.split[s] + (int)(((int64_t)r.len + a.new_tokens + a.block_size - 1) / a.block_size) - r.used;
+        const int p = a.parents ? a.parents[s] : s;
+        if (p >= 0 && p < a.rows) atomicMin(&eldest[p], s);
+    }
+    mark_table(bits, a.tables_out, (int64_t)a.rows * a.width, a.num_blocks);
+    __syncthreads();
+
+    auto request = [&](int s) -> ForkRequest {
+        ForkRequest q = {{-1, 0, 0}, -1, 0};
+        if (s >= a.rows) return q;
+        q.r = fork_row(a, s);
+        if (q.r.parent < 0) return q;
+        q.wanted = (int)(((int64_t)q.r.len + a.new_tokens + a.block_size - 1) / a.block_size) - q.r.used;
+        if (q.r.len % a.block_size != 0 && eldest[q.r.parent] != s) q.open = a.tables_out[(int64_t)s * a.width + q.r.used - 1];
+        return q;
+    };
+    // how many blocks are asked for
+    const ForkRequest first = request(tid);
+    int asked = (first.open >= 0) + first.wanted;
+    for (int s = tid + CB_THREADS; s < a.rows; s += CB_THREADS) {
+        const ForkRequest q = request(s);
+        asked += (q.open >= 0) + q.wanted;
     }
     int total;
     (void)block_scan(asked, red, total);
@@ -169,28 +186,27 @@ __global__ __launch_bounds__(CB_THREADS) void fork_assign_kernel(ForkArgs a) {
     int base = 0, base_copy = 0, given = 0;
     for (int s0 = 0; s0 < a.rows; s0 += CB_THREADS) {
         const int s = s0 + tid;
-        ForkRow r = {-1, 0, 0};
-        int split = 0, wanted = 0;
-        if (s < a.rows) r = fork_row(a, s);
-        if (r.parent >= 0) {
-            split = a.split[s];
-            wanted = (int)(((int64_t)r.len + a.new_tokens + a.block_size - 1) / a.block_size) - r.used;
-        }
+        const ForkRequest q = s0 == 0 ? first : request(s);
+        const ForkRow r = q.r;
+        const bool split = q.open >= 0;
         int all, copies;
-        const int begin = base + block_scan(split + wanted, red, all);
+        const int begin = base + block_scan(split + q.wanted, red, all);
         const bool copied = split && begin < found;
         const int at = base_copy + block_scan(copied, red, copies);
         if (s < a.rows) {
             int32_t* row = a.tables_out + (int64_t)s * a.width;
-            if (copied) {
-                const int page = a.fresh[begin];
-                row[r.used - 1] = page;
-                a.copies[3 * at] = a.tables[(int64_t)r.parent * a.width + r.used - 1];
-                a.copies[3 * at + 1] = page;
-                a.copies[3 * at + 2] = r.len % a.block_size;
-                ++given;
+            int last = -1;                                    // block of the first new token, where the open one takes it
+            if (split) {
+                last = copied ? a.fresh[begin] : -1;
+                row[r.used - 1] = last;
+                if (copied) {
+                    a.copies[3 * at] = q.open;
+                    a.copies[3 * at + 1] = last;
+                    a.copies[3 * at + 2] = r.len % a.block_size;
+                    ++given;
+                }
             }
-            for (int i = 0; i < wanted && r.used + i < a.width; ++i) {
+            for (int i = 0; i < q.wanted && r.used + i < a.width; ++i) {
                 const int rank = begin + split + i;
                 if (rank >= found) break;
                 row[r.used + i] = a.fresh[rank];
@@ -202,7 +218,7 @@ __global__ __launch_bounds__(CB_THREADS) void fork_assign_kernel(ForkArgs a) {
                 const int64_t pos = (int64_t)r.len + i;
                 int slot = -1;
                 if (r.parent >= 0 && pos < cap) {
-                    const int page = row[pos / a.block_size];
+                    const int page = split && pos / a.block_size == r.used - 1 ? last : row[pos / a.block_size];
                     if (page >= 0) slot = page * a.block_size + (int)(pos % a.block_size);
                 }
                 a.slots[(int64_t)s * a.new_tokens + i] = slot;
@@ -293,10 +309,11 @@ __global__ __launch_bounds__(256) void compact_remap_kernel(int32_t* __restrict_
 }
 
 // Block copies within the cache tensors of all layers in one launch.  The list is on the device and may be longer than
-// what is used of it (it ends at the first negative source), so the grid is fixed and its workgroups take (copy, tensor,
-// piece) in turn.
+// what is used of it (it ends at the first negative source), so the workgroups look for its end and take (copy, tensor, piece) in
+// turn.  Bound: memory.  24 open blocks of 64 caches, 420 MB read and written: 87 us (4.8 TB/s; a plain copy of 200 MB reaches 5.4, the
+// library's), 96 through the caches with 32 KB pieces on 2048 workgroups; 192 whole blocks of 16 caches, 1.6 GB: 280 us.
 constexpr int COPY_TENSORS = 128;
-constexpr int COPY_PIECE = 32768;                             // bytes of a block that a workgroup copies at a time
+constexpr int COPY_PIECE = 16384;                             // bytes of a block that a workgroup copies at a time
 constexpr int COPY_THREADS = 256;
 struct CopyTensors {
     uint8_t* base[COPY_TENSORS];
@@ -305,15 +322,15 @@ struct CopyTensors {
 __global__ __launch_bounds__(COPY_THREADS) void copy_blocks_kernel(CopyTensors t, const int32_t* __restrict__ copies, int most,
                                                                    int tensors, int pieces, int num_blocks, int block_size) {
     const int lane = threadIdx.x & 63;
-    int n = 0;                                                // copies in use: the list's leading entries
-    for (; n < most; n += 64) {
-        const uint64_t m = __ballot(n + lane >= most || copies[3 * (int64_t)min(n + lane, most - 1)] < 0);
-        if (m) {
-            n += __builtin_ctzll(m);
-            break;
-        }
+    int n = 0, end = most;                                    // copies in use: the list's leading entries; between n and end of them
+    while (n < end) {
+        const int step = (end - n + 63) / 64;
+        const int64_t at = n + (int64_t)lane * step;
+        const int used = __popcll(__ballot(at < end && copies[3 * at] >= 0));      // of the probes, one a lane
+        if (!used) break;
+        n += (used - 1) * step + 1;
+        end = min(end, n - 1 + step);
     }
-    n = min(n, most);
     const int64_t items = (int64_t)n * tensors * pieces;
     for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
         const int piece = (int)(it % pieces);
@@ -334,12 +351,11 @@ __global__ __launch_bounds__(COPY_THREADS) void copy_blocks_kernel(CopyTensors t
             constexpr int STEP = COPY_THREADS * 16;
             i += threadIdx.x * 16;
             for (; i + 3 * STEP < end; i += 4 * STEP) {
-                const u32x4 v0 = *(const u32x4*)(s + i), v1 = *(const u32x4*)(s + i + STEP);
-                const u32x4 v2 = *(const u32x4*)(s + i + 2 * STEP), v3 = *(const u32x4*)(s + i + 3 * STEP);
-                *(u32x4*)(d + i) = v0;
-                *(u32x4*)(d + i + STEP) = v1;
-                *(u32x4*)(d + i + 2 * STEP) = v2;
-                *(u32x4*)(d + i + 3 * STEP) = v3;
+                u32x4 v[4];                                   // past the caches: neither side is read again soon
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = __builtin_nontemporal_load((const u32x4*)(s + i + k * STEP));
+#pragma unroll
+                for (int k = 0; k < 4; ++k) __builtin_nontemporal_store(v[k], (u32x4*)(d + i + k * STEP));
             }
             for (; i < end; i += STEP) *(u32x4*)(d + i) = *(const u32x4*)(s + i);
             i = max(end, from);
@@ -355,7 +371,7 @@ int set_lds(K kern, size_t bytes, bool (&done)[MF_MAX_DEVICES]) {
     hipError_t e = hipGetDevice(&dev);
     if (e != hipSuccess) return (int)e;
     if (dev >= 0 && dev < MF_MAX_DEVICES && done[dev]) return 0;
-    e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, CB_MAX_BLOCKS / 8);
+    e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, CB_MAX_BLOCKS / 8 + 4 * CB_MAX_ROWS);
     if (e == hipSuccess && dev >= 0 && dev < MF_MAX_DEVICES) done[dev] = true;
     return (int)e;
 }
@@ -364,8 +380,8 @@ int set_lds(K kern, size_t bytes, bool (&done)[MF_MAX_DEVICES]) {
 
 extern "C" size_t mf_fork_blocks_workspace_bytes(int rows, int block_size, int new_tokens) {
     if (rows <= 0 || block_size <= 0 || new_tokens < 0) return 0;
-    // `split` and, at most, a copied block and the blocks of the new tokens for every row
-    return (size_t)rows * sizeof(int32_t) * (2 + ((size_t)new_tokens + block_size - 1) / block_size);
+    // at most a copied block and the blocks of the new tokens for every row
+    return (size_t)rows * sizeof(int32_t) * (1 + ((size_t)new_tokens + block_size - 1) / block_size);
 }
 
 extern "C" int mf_fork_blocks(int32_t* tables_out, int32_t* lens_out, int32_t* slots, int32_t* copies, int32_t* missing,
@@ -374,6 +390,7 @@ extern "C" int mf_fork_blocks(int32_t* tables_out, int32_t* lens_out, int32_t* s
                               size_t workspace_bytes, void* stream) {
     MF_REQUIRE(rows > 0 && width > 0 && block_size > 0 && new_tokens >= 0 && window >= 0 && sinks >= 0, "fork_blocks: bad sizes");
     MF_REQUIRE(num_blocks > 0 && num_blocks <= CB_MAX_BLOCKS, "fork_blocks: %d blocks, 1 to %d are served", num_blocks, CB_MAX_BLOCKS);
+    MF_REQUIRE(rows <= CB_MAX_ROWS, "fork_blocks: %d rows, up to %d are served", rows, CB_MAX_ROWS);
     MF_REQUIRE((int64_t)width * block_size + new_tokens <= 0x7fffffffLL && (int64_t)num_blocks * block_size <= 0x7fffffffLL &&
                    (int64_t)rows * (2 + ((int64_t)new_tokens + block_size - 1) / block_size) <= 0x7fffffffLL,
                "fork_blocks: positions or slots overflow 32 bits");
@@ -384,10 +401,10 @@ extern "C" int mf_fork_blocks(int32_t* tables_out, int32_t* lens_out, int32_t* s
     MF_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 3) == 0,
                "fork_blocks: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
     int32_t* ws = (int32_t*)workspace;
-    const ForkArgs a = {tables_out, lens_out, slots, copies, missing, tables, lens, parents, held, ws, ws + rows,
+    const ForkArgs a = {tables_out, lens_out, slots, copies, missing, tables, lens, parents, held, ws,
                         rows, width, num_blocks, block_size, new_tokens, window, sinks};
     hipStream_t st = (hipStream_t)stream;
-    const size_t lds = ((size_t)num_blocks + 31) / 32 * 4;
+    const size_t lds = (((size_t)num_blocks + 31) / 32 + rows) * 4;
     const bool small = (int64_t)rows * width <= 8192;
     static bool set[2][MF_MAX_DEVICES] = {};
     int rc;
@@ -454,7 +471,7 @@ extern "C" int mf_copy_blocks(void* const* host_caches, const int32_t* host_row_
         }
         const int pieces = (int)((block + COPY_PIECE - 1) / COPY_PIECE);
         const int64_t items = (int64_t)n_copies * n * pieces;
-        hipLaunchKernelGGL(copy_blocks_kernel, dim3((unsigned)std::min<int64_t>(items, 2048)), dim3(COPY_THREADS), 0, st, t, copies,
+        hipLaunchKernelGGL(copy_blocks_kernel, dim3((unsigned)std::min<int64_t>(items, 65536)), dim3(COPY_THREADS), 0, st, t, copies,
                            n_copies, n, pieces, num_blocks, block_size);
         const int rc = MF_LAUNCH_CHECK();
         if (rc) return rc;

@@ -771,7 +771,9 @@ def fork_blocks(block_tables, context_lens, num_blocks, block_size, parents=None
     _need(window is not None or sinks == 0, "sinks go with a window")
     out = torch.empty(s * (m + new_tokens + 4) + 1, dtype=torch.int32, device=dev)
     a, b, c, d = s * m, s * (m + 1), s * (m + 4), s * (m + 4) + 1
-    res = ForkedBlocks(out[:a].view(s, m), out[a:b], out[d:], out[b:c].view(s, 3), out[c:d])
+    part = out.as_strided                                     # half the time of a slice and a view
+    res = ForkedBlocks(part((s, m), (m, 1), 0), part((s,), (1,), a), part((s * new_tokens,), (1,), d), part((s, 3), (3, 1), b),
+                       part((1,), (1,), c))
     need = lib.mf_fork_blocks_workspace_bytes(s, block_size, new_tokens)
     ws = workspace(need, dev, "fork")
     at = out.data_ptr()
@@ -890,8 +892,9 @@ def beam_search_select(logits, beam_scores, eos_token_id=-1, n_candidates=None):
     scores = torch.empty((g * (n + k),), dtype=torch.float32, device=dev)
     ids = torch.empty((2 * g * (n + k),), dtype=torch.int32, device=dev)
     gn, gk = g * n, g * k
-    res = BeamSelection(scores[:gn].view(g, n), ids[:gn].view(g, n), ids[gn:2 * gn].view(g, n), scores[gn:].view(g, k),
-                        ids[2 * gn:2 * gn + gk].view(g, k), ids[2 * gn + gk:].view(g, k))
+    val, num = scores.as_strided, ids.as_strided              # half the time of a slice and a view
+    res = BeamSelection(val((g, n), (n, 1), 0), num((g, n), (n, 1), 0), num((g, n), (n, 1), gn), val((g, k), (k, 1), gn),
+                        num((g, k), (k, 1), 2 * gn), num((g, k), (k, 1), 2 * gn + gk))
     if g == 0:
         return res
     code = dtype_code(logits.dtype)
