@@ -338,6 +338,20 @@ __device__ __forceinline__ f16x8 dequant8<FP16>(uint32_t lo, uint32_t hi) {
     return v;
 }
 
+// The same in five instructions for four values: byte ^ 0x80 under the exponent of 1024 is 1152 + q.
+__device__ __forceinline__ f16x8 i8x8_to_f16x8(uint32_t lo, uint32_t hi) {
+    typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
+    const f16x2_t bias = {(_Float16)1152.f, (_Float16)1152.f};
+    u32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = (i < 2 ? lo : hi) ^ 0x80808080u;
+        const uint32_t u = __builtin_amdgcn_perm(0x64646464u, w, i & 1 ? 0x04030402u : 0x04010400u);
+        v[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, u) - bias);
+    }
+    return __builtin_bit_cast(f16x8, v);
+}
+
 // bytes shift / 8 and shift / 8 + 1 of w as a pair of T, exact
 template <typename T>
 __device__ __forceinline__ uint32_t i8x2_to(uint32_t w, int shift) {
