@@ -79,6 +79,29 @@ struct PfRope {
     int head, key_head;                                       // elements from head to head, here and in the key rows
 };
 
+// Zero the rows the single-partition prefill path never writes (rows of no sequence): one workgroup per sequence
+// takes the rows between the sequence's last query and the next sequence's first (the end of the output for the
+// last sequence), the first workgroup also those before the first sequence.  Usually there are none.
+// A launch of its own, or, with a window, the first workgroups of the attention's launch (the launch took 4.5 us of 48).
+__device__ __forceinline__ void pf_zero_rows(uint16_t* __restrict__ out, const int32_t* __restrict__ q_starts,
+                                             const int32_t* __restrict__ ctx_lens, bool contiguous, int max_ctx, int batch,
+                                             int row, int rows, int s) {
+    int qs, ql, len;
+    pf_seq(s, q_starts, ctx_lens, contiguous, rows, max_ctx, batch, qs, ql, len);
+    const int64_t lo = qs < 0 ? 0 : (int64_t)qs + ql;
+    int64_t hi = s + 1 < batch ? q_starts[s + 1] : rows;
+    hi = hi > rows ? rows : hi;
+    const u32x4 z = {0u, 0u, 0u, 0u};
+    for (int64_t r = lo; r < hi; ++r)
+        for (int i = threadIdx.x * 8; i < row; i += blockDim.x * 8) *(u32x4*)(out + r * row + i) = z;
+    if (s == 0) {
+        int64_t first = q_starts[0];
+        first = first > rows ? rows : first;
+        for (int64_t r = 0; r < first; ++r)
+            for (int i = threadIdx.x * 8; i < row; i += blockDim.x * 8) *(u32x4*)(out + r * row + i) = z;
+    }
+}
+
 // Three workgroups per compute unit; two at 192-wide heads (72 KB of LDS and 96 accumulator registers each).
 // (int8 caches at heads of 128: the tile in registers takes them past 168, and 144 bytes a lane are spilled.)
 // DV: width of a value head and of an output head.  DV < D (the prefill of multi-latent attention: 192-wide queries
@@ -95,7 +118,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, D == 192 ? 2 : 3) void prefill_atten
     int n_rep, int block_size, int max_blocks, int num_blocks, int max_parts, float scale_log2, int64_t q_stride,
     int batch, const int32_t* __restrict__ q_starts, int part_tokens, int64_t kv_stride, int rows,
     int64_t v_stride, const float* __restrict__ kv_scale, const float* __restrict__ kv_offset, float lazy_log2, PfRope rope,
-    PaWindow win) {
+    PaWindow win, int zero_blocks) {
     using vec8 = typename T::vec8;
     using S = PfSmem<D>;
     // Type of the probabilities and of the widened values in the PV product.  int8 values are exact in either type and fp16 rounds
@@ -118,10 +141,16 @@ __global__ __launch_bounds__(PA_WAVES * 64, D == 192 ? 2 : 3) void prefill_atten
 
     extern __shared__ __attribute__((aligned(16))) uint8_t pf_smem[];
 
+    if constexpr (WIN) {
+        if ((int)blockIdx.x < zero_blocks) {
+            pf_zero_rows(out, q_starts, ctx_lens, block_tables == nullptr, max_blocks * block_size, batch, n_heads * DV, rows, blockIdx.x);
+            return;
+        }
+    }
     // work list: see paged_attention_kernel; a sequence has ceil(q_len * n_rep / 128) column groups
     int b = -1, part = 0, L = 0, kg = 0, q_len = 1, q_start = 0, col_groups = 1;
     {
-        const int pidx = blockIdx.x;
+        const int pidx = blockIdx.x - (WIN ? zero_blocks : 0);
         const int ln = threadIdx.x & 63;
         int base = 0;
         for (int c0 = 0; c0 < batch; c0 += 64) {
@@ -695,32 +724,43 @@ static inline bool pf_cols16(const PfPlan& p, int batch, int n_kv, int head_dim,
            200.f + std::min<int64_t>(p.part_tokens, max_ctx) * width;
 }
 
-// Zero the rows the single-partition prefill path never writes (rows of no sequence): one workgroup per sequence
-// takes the rows between the sequence's last query and the next sequence's first (the end of the output for the
-// last sequence), the first workgroup also those before the first sequence.  Usually there are none.
 __global__ void pf_zero_rows_kernel(uint16_t* __restrict__ out, const int32_t* __restrict__ q_starts,
                                     const int32_t* __restrict__ ctx_lens, bool contiguous, int max_ctx, int batch,
                                     int row, int rows) {
-    const int s = blockIdx.x;
-    int qs, ql, len;
-    pf_seq(s, q_starts, ctx_lens, contiguous, rows, max_ctx, batch, qs, ql, len);
-    const int64_t lo = qs < 0 ? 0 : (int64_t)qs + ql;
-    int64_t hi = s + 1 < batch ? q_starts[s + 1] : rows;
-    hi = hi > rows ? rows : hi;
-    const u32x4 z = {0u, 0u, 0u, 0u};
-    for (int64_t r = lo; r < hi; ++r)
-        for (int i = threadIdx.x * 8; i < row; i += blockDim.x * 8) *(u32x4*)(out + r * row + i) = z;
-    if (s == 0) {
-        int64_t first = q_starts[0];
-        first = first > rows ? rows : first;
-        for (int64_t r = 0; r < first; ++r)
-            for (int i = threadIdx.x * 8; i < row; i += blockDim.x * 8) *(u32x4*)(out + r * row + i) = z;
-    }
+    pf_zero_rows(out, q_starts, ctx_lens, contiguous, max_ctx, batch, row, rows, blockIdx.x);
 }
 
-// Plan of a step with a window: that of a context as long as the longest walk.
+// Tokens of the longest walk of a step with a window, `cols` columns a group.
 static inline int64_t pf_win_walk(int64_t max_ctx, int cols, int n_rep, PaWindow win) {
     return pa_win_tiles(max_ctx, pa_group_rows(cols, n_rep), win) * PF_TOK;
+}
+
+// Plan of a step with a window on the 128-column kernel.  Walks are about equally long (no short causal ranges), so the time is priced
+// for every number of partitions: 8 us a round of 768 workgroups, and the tiles of one chain at 0.72 us or of a compute unit at
+// 0.54 us each (heads of 128), whichever is more; a cut adds 2.5 us and 0.33 us for every megabyte of partials written and read
+// back.  Measured, us with the plan of a full context | uncut | this one | best: chunks of 512 rows beside 24 decoding sequences through 1024,
+// 32/8 heads 68 | 48 | 44 | 44, one chunk of 64 through 2048 22.9 | 62.6 | 23.1 | 22.9, one of 32 beside 24 through 512, 28/4 heads, blocks of
+// 16 24.4 | 32.8 | 19.4 | 19.4, a prompt of 2048 rows through 1024, 8/1 heads 32.3 | 34.5 | 30.6 | 30.6, one of 4096 through 512, 8/8 30.5 |
+// 28.4 | 24.7 | 24.7 (the uncut ones here without the launch for rows of no sequence).
+static inline PfPlan pf_win_plan(int batch, int64_t total_q, int n_heads, int n_kv, int head_dim, int64_t walk) {
+    PfPlan best = pf_plan(batch, total_q, n_heads, n_kv, walk);
+    const int64_t groups = std::max<int64_t>((total_q * (n_heads / n_kv) + PF_COLS - 1) / PF_COLS, std::min<int64_t>(batch, total_q));
+    const int64_t wgs = std::max<int64_t>(1, groups) * n_kv;
+    const float width = (0.012f + 0.000058f * head_dim) / 0.0194f, tiles = (float)(walk / PF_TOK);
+    const float mb = 4e-6f * (head_dim + 2) * total_q * n_heads;
+    float best_us = 0.f;
+    for (int64_t parts = 1; parts <= std::max<int64_t>(1, std::min<int64_t>(32, walk / PA_WAVE_TOKENS)); ++parts) {
+        PfPlan p = best;
+        pf_cut(p, walk, parts);
+        const int64_t n = wgs * p.max_parts;
+        float us = 8.f * ((n + 767) / 768) + width * std::max(0.72f * std::min(tiles, (float)p.part_tokens / PF_TOK), 0.54f * wgs * tiles / 256.f);
+        if (p.max_parts > 1) us += 2.5f + 0.33f * mb * p.max_parts;
+        if (parts == 1 || us < best_us) {
+            best = p;
+            best_us = us;
+        }
+    }
+    return best;
 }
 
 template <typename T, int D, int KVQ, int DV = D, bool WIN = false>
@@ -738,17 +778,20 @@ int launch_pf(void* out, const void* query, const void* key_cache, const void* v
     // int8 caches with per-channel scales and a window take the 128-column kernel at any number of rows
     const bool cols16 = KVQ == 2 || (KVQ == 1 && !WIN && pf_cols16(pf_plan(batch, total_q, n_heads, n_kv, max_ctx), batch, n_kv, D, max_ctx));
     const int64_t walk = WIN ? pf_win_walk(max_ctx, cols16 ? 16 : PF_COLS, n_rep, win) : max_ctx;
-    const PfPlan plan = KVQ == 0 ? pf_plan16(batch, total_q, n_heads, n_kv, D, walk, contiguous, tib_tok)
-                                 : pf_plan(batch, total_q, n_heads, n_kv, walk);
+    const PfPlan plan = WIN && KVQ != 2 ? pf_win_plan(batch, total_q, n_heads, n_kv, D, walk)
+                        : KVQ == 0      ? pf_plan16(batch, total_q, n_heads, n_kv, D, walk, contiguous, tib_tok)
+                                        : pf_plan(batch, total_q, n_heads, n_kv, walk);
     float* part_out = plan.max_parts > 1 ? (float*)workspace : nullptr;
     float* part_ml = part_out ? part_out + (int64_t)total_q * n_heads * plan.max_parts * DV : nullptr;
     const float scale_log2 = scale * 1.4426950408889634f;
     const int64_t wgs = (cols16 ? plan.col_groups16 : plan.col_groups128) * n_kv * plan.max_parts;
-    if (wgs > 0x7fffffffLL) {
+    // rows of no sequence: written by the first workgroups with a window, else by a launch of their own
+    const int zero_blocks = WIN && !cols16 && plan.max_parts == 1 ? batch : 0;
+    if (wgs + zero_blocks > 0x7fffffffLL) {
         mf_set_error("paged_attention_prefill: %lld workgroups exceed the grid limit", (long long)wgs);
         return 1;
     }
-    if (plan.max_parts == 1) {
+    if (plan.max_parts == 1 && !zero_blocks) {
         hipLaunchKernelGGL(pf_zero_rows_kernel, dim3(batch), dim3(256), 0, st, (uint16_t*)out, q_starts, context_lens,
                            contiguous, max_blocks * block_size, batch, n_heads * DV, total_q);
         int rc = MF_LAUNCH_CHECK();
@@ -781,12 +824,12 @@ int launch_pf(void* out, const void* query, const void* key_cache, const void* v
             if (e != hipSuccess) return (int)e;                                                                   \
             if (dev >= 0 && dev < MF_MAX_DEVICES) lds_set[TIBV][dev] = true;                                      \
         }                                                                                                         \
-        hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(PA_WAVES * 64), PfSmem<D>::BYTES, st, (uint16_t*)out,  \
+        hipLaunchKernelGGL(kern, dim3((unsigned)(wgs + zero_blocks)), dim3(PA_WAVES * 64), PfSmem<D>::BYTES, st, (uint16_t*)out, \
                            part_out, part_ml, (const uint16_t*)query, (const uint16_t*)key_cache,                 \
                            (const uint16_t*)value_cache, block_tables, context_lens, n_heads, n_kv, n_rep,        \
                            block_size, max_blocks, num_blocks, plan.max_parts, scale_log2, q_stride, batch,       \
                            q_starts, plan.part_tokens, kv_stride, total_q, v_stride, kv_scale, kv_offset, plan.lazy_log2, \
-                           rope, win);                                                                             \
+                           rope, win, zero_blocks);                                                                \
     }
         if (tib_tok) PF_LAUNCH(true)
         else PF_LAUNCH(false)
@@ -930,10 +973,10 @@ extern "C" size_t mf_window_attention_prefill_workspace_bytes(int batch, int tot
                                                               int max_context, int window, int sinks) {
     if (batch <= 0 || total_q <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || max_context <= 0 || window <= 0 || sinks < 0)
         return 0;
-    int most = 1;                                             // 16 or 128 columns a group, by the cache's type
-    for (const int cols : {16, PF_COLS})
-        most = std::max(most, pf_plan(batch, total_q, n_heads, n_kv_heads,
-                                      pf_win_walk(max_context, cols, n_heads / n_kv_heads, {window, sinks})).max_parts);
+    const int n_rep = n_heads / n_kv_heads;                   // 16 or 128 columns a group, by the cache's type
+    const int most = std::max(
+        pf_plan(batch, total_q, n_heads, n_kv_heads, pf_win_walk(max_context, 16, n_rep, {window, sinks})).max_parts,
+        pf_win_plan(batch, total_q, n_heads, n_kv_heads, head_dim, pf_win_walk(max_context, PF_COLS, n_rep, {window, sinks})).max_parts);
     return most <= 1 ? 0 : (size_t)total_q * n_heads * most * (head_dim + 2) * sizeof(float);
 }
 
