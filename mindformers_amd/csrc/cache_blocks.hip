@@ -13,13 +13,15 @@ namespace {
 constexpr int CB_THREADS = 1024;
 constexpr int CB_WAVES = CB_THREADS / 64;
 constexpr int CB_MAX_BLOCKS = 1 << 20;                        // bits of the bitmap: 128 KB of LDS
+constexpr int FORK_FILL = 16;                                 // more new tokens than this a row are placed by a kernel of their own
 constexpr int CB_MAX_ROWS = 4096;                             // rows of a fork: 16 KB of LDS beside it
 
 struct ForkArgs {
     int32_t *tables_out, *lens_out, *slots, *copies, *missing;
     const int32_t *tables, *lens, *parents;
     const uint8_t* held;
-    int32_t* fresh;                                           // workspace: the blocks that are handed out
+    int32_t *fresh, *ranks;                                   // workspace: the blocks that are handed out; with FORK_FILL, [1 + rows]:
+                                                              // how many, and the place of each row's first block behind its open one
     int rows, width, num_blocks, block_size, new_tokens, window, sinks;
 };
 
@@ -206,15 +208,14 @@ __global__ __launch_bounds__(CB_THREADS) void fork_assign_kernel(ForkArgs a) {
                     ++given;
                 }
             }
-            for (int i = 0; i < q.wanted && r.used + i < a.width; ++i) {
-                const int rank = begin + split + i;
-                if (rank >= found) break;
-                row[r.used + i] = a.fresh[rank];
-                ++given;
-            }
+            const int got = max(min(min(q.wanted, a.width - r.used), found - begin - split), 0);
+            given += got;
             const int cap = a.width * a.block_size;
             a.lens_out[s] = r.parent >= 0 ? (int)min((int64_t)r.len + a.new_tokens, (int64_t)cap) : 0;
-            for (int i = 0; i < a.new_tokens; ++i) {
+            if (a.new_tokens > FORK_FILL) a.ranks[1 + s] = begin + split;
+            const bool here = a.new_tokens <= FORK_FILL;
+            for (int i = 0; here && i < got; ++i) row[r.used + i] = a.fresh[begin + split + i];
+            for (int i = 0; here && i < a.new_tokens; ++i) {
                 const int64_t pos = (int64_t)r.len + i;
                 int slot = -1;
                 if (r.parent >= 0 && pos < cap) {
@@ -234,7 +235,27 @@ __global__ __launch_bounds__(CB_THREADS) void fork_assign_kernel(ForkArgs a) {
     }
     int got;
     (void)block_scan(given, red, got);
-    if (tid == 0) *a.missing = total - got;
+    if (tid == 0) {
+        *a.missing = total - got;
+        if (a.new_tokens > FORK_FILL) a.ranks[0] = found;
+    }
+}
+// Blocks and slots of many new tokens (a prompt's): a workgroup a row.
+__global__ __launch_bounds__(256) void fork_fill_kernel(ForkArgs a) {
+    const int s = blockIdx.x, tid = threadIdx.x;
+    const ForkRow r = fork_row(a, s);
+    int32_t* row = a.tables_out + (int64_t)s * a.width;
+    const int64_t last = (int64_t)r.len + a.new_tokens;
+    const int rank = a.ranks[1 + s], wanted = (int)((last + a.block_size - 1) / a.block_size) - r.used;
+    const int got = r.parent < 0 ? 0 : max(min(min(wanted, a.width - r.used), a.ranks[0] - rank), 0);
+    for (int i = tid; i < got; i += 256) row[r.used + i] = a.fresh[rank + i];
+    for (int i = tid; i < a.new_tokens; i += 256) {           // a slot's block by its rank: the row may still be on its way
+        const int64_t pos = (int64_t)r.len + i;
+        const int j = (int)(pos / a.block_size), b = j - r.used;
+        int page = -1;
+        if (r.parent >= 0 && j < a.width) page = b < 0 ? row[j] : (b < got ? a.fresh[rank + b] : -1);
+        a.slots[(int64_t)s * a.new_tokens + i] = page >= 0 ? page * a.block_size + (int)(pos % a.block_size) : -1;
+    }
 }
 
 // Closing up a pool: the n live blocks that may move go to the n lowest blocks that are not held; one that is there
@@ -380,8 +401,8 @@ int set_lds(K kern, size_t bytes, bool (&done)[MF_MAX_DEVICES]) {
 
 extern "C" size_t mf_fork_blocks_workspace_bytes(int rows, int block_size, int new_tokens) {
     if (rows <= 0 || block_size <= 0 || new_tokens < 0) return 0;
-    // at most a copied block and the blocks of the new tokens for every row
-    return (size_t)rows * sizeof(int32_t) * (1 + ((size_t)new_tokens + block_size - 1) / block_size);
+    // `ranks`; at most a copied block and the blocks of the new tokens for every row
+    return sizeof(int32_t) * (1 + (size_t)rows * (2 + ((size_t)new_tokens + block_size - 1) / block_size));
 }
 
 extern "C" int mf_fork_blocks(int32_t* tables_out, int32_t* lens_out, int32_t* slots, int32_t* copies, int32_t* missing,
@@ -401,7 +422,7 @@ extern "C" int mf_fork_blocks(int32_t* tables_out, int32_t* lens_out, int32_t* s
     MF_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 3) == 0,
                "fork_blocks: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
     int32_t* ws = (int32_t*)workspace;
-    const ForkArgs a = {tables_out, lens_out, slots, copies, missing, tables, lens, parents, held, ws,
+    const ForkArgs a = {tables_out, lens_out, slots, copies, missing, tables, lens, parents, held, ws + 1 + rows, ws,
                         rows, width, num_blocks, block_size, new_tokens, window, sinks};
     hipStream_t st = (hipStream_t)stream;
     const size_t lds = (((size_t)num_blocks + 31) / 32 + rows) * 4;
@@ -417,6 +438,8 @@ extern "C" int mf_fork_blocks(int32_t* tables_out, int32_t* lens_out, int32_t* s
         if ((rc = set_lds(fork_assign_kernel<false>, lds, set[0]))) return rc;
         hipLaunchKernelGGL(fork_assign_kernel<false>, dim3(1), dim3(CB_THREADS), lds, st, a);
     }
+    if ((rc = MF_LAUNCH_CHECK())) return rc;
+    if (new_tokens > FORK_FILL) hipLaunchKernelGGL(fork_fill_kernel, dim3(rows), dim3(256), 0, st, a);
     return MF_LAUNCH_CHECK();
 }
 

@@ -95,6 +95,14 @@ def workspace(nbytes, device, tag="default"):
     return buf
 
 
+def _scratch(nbytes, device, tag):
+    """``workspace``, but a buffer of its own inside a stream capture: graphs that are replayed at once must not share one, and this
+    one belongs to the graph's memory."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+    return workspace(nbytes, device, tag)
+
+
 # --------------------------------------------------------------------------------------------- KV cache
 def reshape_and_cache(key, value, key_cache, value_cache, slot_mapping):
     """ReshapeAndCache(key, value, key_cache, value_cache, slot_mapping) -> key.
@@ -249,7 +257,7 @@ def _window_decode(lib, dev, out, quant, query, key_cache, value_cache, key_scal
     nb, bs, _, d = key_cache.shape
     b, max_blocks = block_tables.shape
     need = lib.mf_window_attention_workspace_bytes(b, n_heads, d, max_blocks * bs, window, sinks)
-    ws = workspace(need, dev, "pa") if need else None
+    ws = _scratch(need, dev, "pa") if need else None
     smooth, tiled = quant if quant is not None else (None, False)
     xq = xs = None
     if quant is not None:
@@ -277,7 +285,7 @@ def _window_prefill(lib, dev, out, query, key, value, key_scale, value_scale, kv
     nb, bs, max_blocks = (key.shape[0], key.shape[1], block_tables.shape[1]) if block_tables is not None else (0, 0, 0)
     need = lib.mf_window_attention_prefill_workspace_bytes(b, total_q, n_heads, n_kv_heads, d,
                                                            max_blocks * bs if block_tables is not None else total_q, window, sinks)
-    ws = workspace(need, dev, "pa_prefill") if need else None
+    ws = _scratch(need, dev, "pa_prefill") if need else None
     with _on(dev):
         check(lib.mf_window_attention_prefill(
             ptr(out), ptr(query), ptr(key), ptr(value), ptr(key_scale), ptr(value_scale), kvq, ptr(block_tables), ptr(context_lens),
@@ -775,7 +783,7 @@ def fork_blocks(block_tables, context_lens, num_blocks, block_size, parents=None
     res = ForkedBlocks(part((s, m), (m, 1), 0), part((s,), (1,), a), part((s * new_tokens,), (1,), d), part((s, 3), (3, 1), b),
                        part((1,), (1,), c))
     need = lib.mf_fork_blocks_workspace_bytes(s, block_size, new_tokens)
-    ws = workspace(need, dev, "fork")
+    ws = _scratch(need, dev, "fork")
     at = out.data_ptr()
     with _on(dev):
         check(lib.mf_fork_blocks(at, at + 4 * a, at + 4 * d, at + 4 * b, at + 4 * c, ptr(block_tables), ptr(context_lens), ptr(parents),
@@ -795,7 +803,7 @@ def compact_blocks(block_tables, num_blocks, block_size, held=None):
     most = num_blocks // 2
     out = torch.empty(s * m + 3 * most + 1, dtype=torch.int32, device=dev)
     tables, copies, live = out[:s * m].view(s, m), out[s * m:-1].view(most, 3), out[-1:]
-    ws = workspace(lib.mf_compact_blocks_workspace_bytes(num_blocks), dev, "compact")
+    ws = _scratch(lib.mf_compact_blocks_workspace_bytes(num_blocks), dev, "compact")
     with _on(dev):
         check(lib.mf_compact_blocks(ptr(tables), ptr(copies), ptr(live), ptr(block_tables), ptr(held), s, m, num_blocks, block_size,
                                     ptr(ws), ws.numel(), stream_ptr(dev)), "mf_compact_blocks")
@@ -898,7 +906,7 @@ def beam_search_select(logits, beam_scores, eos_token_id=-1, n_candidates=None):
     if g == 0:
         return res
     code = dtype_code(logits.dtype)
-    ws = workspace(lib.mf_beam_search_workspace_bytes(g, k, v, n, code), dev, "beam")
+    ws = _scratch(lib.mf_beam_search_workspace_bytes(g, k, v, n, code), dev, "beam")
     a, i = scores.data_ptr(), ids.data_ptr()
     with _on(dev):
         check(lib.mf_beam_search_select(a, i, i + 4 * gn, a + 4 * gn, i + 8 * gn, i + 8 * gn + 4 * gk, ptr(logits), stride,

@@ -704,3 +704,76 @@ def test_the_modules_pass_their_window_on():
                  lambda: PagedAttentionMgr(nh, d, nkv, (nb, bs, nkv, d), window=-1)):
         with pytest.raises(ValueError):
             make()
+
+
+@pytest.mark.parametrize("rows,width,block,new", [(3, 40, 16, 500), (70, 30, 8, 17), (5, 6, 4, 40), (1, 1, 1, 300)])
+def test_fork_with_the_tokens_of_a_prompt(rows, width, block, new):
+    """More new tokens than a thread places by itself, and more than the table or the pool holds."""
+    rng = np.random.default_rng(new)
+    blocks = rows * (width + 1)
+    tables, lens = _tables(rng, rows, width, block, blocks, groups=2)
+    lens[0] = 0
+    for parents in (None, rng.integers(-1, rows, rows)):
+        _fork(tables, lens, blocks, block, parents=parents, new_tokens=new)
+        _fork(tables, lens, max(blocks // 3, int(tables.max()) + 1, 1), block, parents=parents, new_tokens=new)
+
+
+def test_graphs_replayed_at_once_share_no_workspace():
+    """Two captures of each operator, replayed together on two streams over and over: the answers of one are never the other's."""
+    from mindformers_amd import ops
+    rng = np.random.default_rng(3)
+    sets = []
+    for seed in (1, 2):
+        lens = rng.integers(1000, 1500, 8)
+        q, cache, _, tables, _, _ = _paged(rng, torch.bfloat16, lens, [1] * 8, 8, 2, 64, 16, 900, 4, poison=False)
+        q, kc, vc = (torch.from_numpy(x).bfloat16().cuda() for x in (q, *cache))
+        logits, scores = _beams(4, 4, 60000, torch.float32, seed)
+        t, l = _tables(rng, 200, 64, 4, 200 * 70, groups=4)
+        sets.append((q, kc, vc, _i32(tables), _i32(lens), logits, scores, _i32(t), _i32(l), _i32(rng.integers(-1, 200, 200))))
+
+    def calls(q, kc, vc, tables, lens, logits, scores, t, l, p):
+        fork = ops.fork_blocks(t, l, 200 * 70, 4, parents=p, new_tokens=1)
+        return [ops.paged_attention(q, kc, vc, tables, lens, 8, 2, 0.1, window=900, sinks=4), *ops.beam_search_select(logits, scores),
+                *fork, *ops.compact_blocks(fork.block_tables, 200 * 70, 4)]
+
+    want = [[x.clone() for x in calls(*s)] for s in sets]
+    graphs, got = [], []
+    for s in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got.append(calls(*s))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(20):
+        for g, st in zip(graphs, streams):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for w, h in zip(want, got):
+            assert all(torch.equal(a, b) for a, b in zip(w, h))
+
+
+def test_a_device_side_decode_step_replayed_in_a_graph():
+    from mindformers_amd.runner import DecodeStackRunner
+    run = DecodeStackRunner(_stack(40, 3), npu_mem_size=0.004, cpu_mem_size=0, block_size=16)
+    for c in run.caches():
+        c.normal_()
+    tables = torch.arange(32, dtype=torch.int32, device="cuda").view(4, 8)
+    lens, slots = _i32([5, 0, 128, 77]), _i32([4, -1, 2 * 128 + 127, 3 * 128 + 76])
+    x = torch.randn(4, 512, device="cuda").bfloat16()
+    run.decode(x, lens, tables, slots)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run.decode(x, lens, tables, slots)
+    for _ in range(3):
+        x.copy_(torch.randn_like(x))
+        graph.replay()
+        torch.cuda.synchronize()
+        again = got.clone()
+        assert torch.equal(again, run.decode(x, lens, tables, slots))
+    with pytest.raises(ValueError):
+        run.decode(x, lens.long(), tables, slots)
+    with pytest.raises(ValueError):
+        run.decode(x, lens, tables[:3], slots)
