@@ -83,6 +83,13 @@ __host__ __device__ __forceinline__ int64_t pa_win_tiles(int64_t max_ctx, int ro
 // most rows that `cols` consecutive columns belong to
 __host__ __device__ __forceinline__ int pa_group_rows(int cols, int n_rep) { return (cols - 2 + n_rep) / n_rep + 1; }
 
+// Exponent x of a query's largest value, in [2^(x - 1), 2^x), by which 2^(15 - x) brings it below 2^15.  Zero, infinity and the far
+// ends are left to themselves: the scores of a query below 2^-60 vanish beside any other's, and the mask's value times the scale
+// of the column, 2^(x - 15) of the call's, stays far below every score.
+__device__ __forceinline__ int pa_query_exponent(float top) {
+    return top > 0x1p-60f && top < 0x1p100f ? __builtin_amdgcn_frexp_expf(top) : 15;
+}
+
 // Prefill bookkeeping of sequence s: first query row, number of query rows and context length, made safe
 // (never more queries than context; query rows, and with them contiguous keys, never leave the `rows` passed).
 __device__ inline void pf_seq(int s, const int32_t* __restrict__ q_starts, const int32_t* __restrict__ ctx_lens,
@@ -315,8 +322,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, (!PF && KVQ == 1 && TIB) ? 4 : 3) vo
         }
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
-        // top in [2^(x - 1), 2^x) -> 2^(15 - x); zero, infinity and the far ends are left to themselves
-        const int x = top > 0x1p-100f && top < 0x1p100f ? __builtin_amdgcn_frexp_expf(top) : 15;
+        const int x = pa_query_exponent(top);
         const float up = ldexpf(1.f, 15 - x);
         col_scale_log2 = ldexpf(scale_log2, x - 15);
 #pragma unroll

@@ -119,7 +119,12 @@ __global__ __launch_bounds__(PA_WAVES * 64, D == 192 ? 2 : 3) void prefill_atten
     int batch, const int32_t* __restrict__ q_starts, int part_tokens, int64_t kv_stride, int rows,
     int64_t v_stride, const float* __restrict__ kv_scale, const float* __restrict__ kv_offset, float lazy_log2, PfRope rope,
     PaWindow win, int zero_blocks) {
-    using vec8 = typename T::vec8;
+    // With a window, the score product over int8 caches is in fp16 too, on a query scaled to its range as in the 16-column kernel.  RMS
+    // error against float64 over the result, 300 bf16 rows behind 2700 tokens, 32/8 heads of 128, window 1024: 1.68e-3 (the rounding
+    // of the result alone 1.66e-3) where the query rounded to bf16 gives 2.39e-3, in 39.1 us instead of 38.3.
+    constexpr bool QF16 = WIN && KVQ == 1;
+    using QT = std::conditional_t<QF16, FP16, T>;
+    using vec8 = typename QT::vec8;
     using S = PfSmem<D>;
     // Type of the probabilities and of the widened values in the PV product.  int8 values are exact in either type and fp16 rounds
     // the probabilities eight times finer than bf16, in the same time.  RMS error against float64, bf16, 512 rows over 4096 tokens,
@@ -243,7 +248,33 @@ __global__ __launch_bounds__(PA_WAVES * 64, D == 192 ? 2 : 3) void prefill_atten
     [[maybe_unused]] const int lo_all = ctx_before + q_first + 1 - win.window, lo_some = wave_end - win.window, lo_col = Lcol - win.window;
     const int Lmask = ctx_before + q_first + 1;               // tiles that end at or before it need no mask
     vec8 qreg[KS];
-    {
+    float col_scale = scale_log2, col_neg = PA_NEG;           // of this lane's column: a score's scale, and what a hidden one is set to
+    if constexpr (QF16) {
+        const uint16_t* qp = q + (int64_t)(q_start + (col_ok ? qi : 0)) * q_stride +
+                             (int64_t)(kvh * n_rep + (col_ok ? hcol : 0)) * D + 8 * h;
+        const float* ks = kv_scale + kvh * D + 8 * h;
+        float f[KS][8], top = 0.f;
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+            u32x4 v = {0u, 0u, 0u, 0u};
+            if (col_ok) v = *(const u32x4*)(qp + 16 * j);
+            unpack8<T>(v, f[j]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                f[j][e] *= ks[16 * j + e];
+                top = fmaxf(top, fabsf(f[j][e]));
+            }
+        }
+        top = max_xor32(top);
+        const int x = pa_query_exponent(top);
+        const float up = ldexpf(1.f, 15 - x);
+        col_scale = ldexpf(scale_log2, x - 15);
+        if (x > 15) col_neg = ldexpf(PA_NEG, 15 - x);         // its product with the scale stays finite
+#pragma unroll
+        for (int j = 0; j < KS; ++j)
+            qreg[j] = bitcast<vec8>((u32x4){pack2<QT>(f[j][0] * up, f[j][1] * up), pack2<QT>(f[j][2] * up, f[j][3] * up),
+                                            pack2<QT>(f[j][4] * up, f[j][5] * up), pack2<QT>(f[j][6] * up, f[j][7] * up)});
+    } else {
         const uint16_t* qp = q + (int64_t)(q_start + (col_ok ? qi : 0)) * q_stride +
                              (int64_t)(kvh * n_rep + (col_ok ? hcol : 0)) * D + 8 * h;
 #pragma unroll
@@ -399,8 +430,15 @@ __global__ __launch_bounds__(PA_WAVES * 64, D == 192 ? 2 : 3) void prefill_atten
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int c = 2 * pc + i;
-            *(vec8*)(kdst + 16 * (c ^ key)) = dequant8<T>(kraw[2 * i], kraw[2 * i + 1]);
-            *(pvec8*)(vdst + 16 * ((c + 4 * key4) & (S0::CPR - 1))) = dequant8<PT>(vraw[2 * i], vraw[2 * i + 1]);
+            vec8& kd = *(vec8*)(kdst + 16 * (c ^ key));
+            pvec8& vd = *(pvec8*)(vdst + 16 * ((c + 4 * key4) & (S0::CPR - 1)));
+            if constexpr (QF16) {
+                kd = i8x8_to_f16x8(kraw[2 * i], kraw[2 * i + 1]);
+                vd = i8x8_to_f16x8(vraw[2 * i], vraw[2 * i + 1]);
+            } else {
+                kd = dequant8<T>(kraw[2 * i], kraw[2 * i + 1]);
+                vd = dequant8<PT>(vraw[2 * i], vraw[2 * i + 1]);
+            }
         }
     };
 
@@ -439,10 +477,10 @@ __global__ __launch_bounds__(PA_WAVES * 64, D == 192 ? 2 : 3) void prefill_atten
     // seen).  The token at the reference point has probability 1, which needs no rounding, and the 16-column kernel has more such
     // tokens than a lazy or a running maximum would give here (four waves with a maximum each): RMS error as above 3.37e-4 there,
     // 3.52e-4 lazily, 3.45e-4 with the running maximum, 3.27e-4 here, for 2 % (1024 tokens) to 10 % (16384) of the time.
-    float m_run = 0.5f * PA_NEG, l_run = 0.f;
+    float m_run = 0.5f * col_neg, l_run = 0.f;
     [[maybe_unused]] float m_peak = m_run;
     constexpr bool TILE_REF = KVQ == 1 && std::is_same<T, FP16>::value;
-    const float lazy = (TILE_REF ? 32.0f : lazy_log2) / scale_log2;
+    const float lazy = (TILE_REF ? 32.0f : lazy_log2) / col_scale;
 
     // One tile, living in ring buffer R = t mod 3 (a compile-time constant of the step): scores, softmax, PV product,
     // one phase after the other.  A wave does not overlap its own MFMAs with its own vector instructions, so nothing
@@ -473,9 +511,9 @@ __global__ __launch_bounds__(PA_WAVES * 64, D == 192 ? 2 : 3) void prefill_atten
                     f32x16 z;
 #pragma unroll
                     for (int e = 0; e < 16; ++e) z[e] = 0.f;
-                    sc = T::mfma32(bitcast<vec8>(ka[m % P]), qreg[m], z);
+                    sc = QT::mfma32(bitcast<vec8>(ka[m % P]), qreg[m], z);
                 } else {
-                    sc = T::mfma32(bitcast<vec8>(ka[m % P]), qreg[m], sc);
+                    sc = QT::mfma32(bitcast<vec8>(ka[m % P]), qreg[m], sc);
                 }
                 __builtin_amdgcn_sched_barrier(0);
                 fetch(std::integral_constant<int, m + P>{});
@@ -487,7 +525,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, D == 192 ? 2 : 3) void prefill_atten
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int tok = ts + 8 * (i >> 2) + 4 * h + (i & 3);
-                sc[i] = tok < Lcol && (!WIN || tok >= lo_col || tok < win.sinks) ? sc[i] : PA_NEG;
+                sc[i] = tok < Lcol && (!WIN || tok >= lo_col || tok < win.sinks) ? sc[i] : col_neg;
             }
         }
         float tmax = sc[0];
@@ -502,19 +540,19 @@ __global__ __launch_bounds__(PA_WAVES * 64, D == 192 ? 2 : 3) void prefill_atten
             m_new = tmax > m_run + lazy ? tmax : m_run;
         }
         if (__builtin_amdgcn_ballot_w64(m_new != m_run) != 0) {      // the reference point moves: rare
-            const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * scale_log2);
+            const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * col_scale);
             l_run *= alpha;
 #pragma unroll
             for (int db = 0; db < DB; ++db) acc[db] *= alpha;
             m_run = m_new;
         }
-        const float nm = -m_run * scale_log2;
+        const float nm = -m_run * col_scale;
         // probabilities, rounded to T; the denominator sums them as the PV product sees them
         uint32_t pp[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[2 * k], scale_log2, nm));
-            const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[2 * k + 1], scale_log2, nm));
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[2 * k], col_scale, nm));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[2 * k + 1], col_scale, nm));
             pp[k] = pack2<PT>(p0, p1);
             l_run = PT::sum2(pp[k], l_run);
         }
@@ -634,7 +672,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, D == 192 ? 2 : 3) void prefill_atten
                 *(f32x4*)(dst + 32 * db + 8 * q4) =
                     (f32x4){acc[db][4 * q4], acc[db][4 * q4 + 1], acc[db][4 * q4 + 2], acc[db][4 * q4 + 3]};
         if (h == 0) {
-            part_ml[pi * 2] = m_run * scale_log2;
+            part_ml[pi * 2] = m_run * col_scale;
             part_ml[pi * 2 + 1] = l_run;
         }
     }

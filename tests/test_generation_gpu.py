@@ -398,6 +398,32 @@ def test_windowed_chunks_match_the_oracle(kind, dtype, nh, nkv, d, block, window
     _windowed(dtype, lens, q_lens, nh, nkv, d, block, window, sinks, kind)
 
 
+# The largest key of the queries' channel is the first token that the window leaves, which takes the whole probability where the
+# scores are 2^31 apart; where they are 2^-40 the probabilities are equal.
+@pytest.mark.parametrize("dtype,size", [(torch.bfloat16, 2.0 ** 40), (torch.bfloat16, 2.0 ** -50), (torch.bfloat16, 2.0 ** 25), (torch.float16, 2.0 ** 15),
+                                        (torch.float16, 2.0 ** -24), (torch.bfloat16, 0.0), (torch.bfloat16, 2.0 ** -110)])
+@pytest.mark.parametrize("rows", [1, 20, 200])
+@pytest.mark.parametrize("window,sinks", [(40, 0), (70, 1)])
+def test_windows_over_int8_caches_with_large_and_small_queries(dtype, size, rows, window, sinks):
+    from mindformers_amd import ops
+    rng = np.random.default_rng(rows)
+    lens, nh, nkv, d, block = [255, 254, 0, 255], 8, 2, 64, 16
+    q_lens = [rows, 1, 0, rows]
+    q = np.zeros((sum(q_lens), nh, d))
+    q[:, :, 5] = size
+    cache = rng.integers(-127, 128, (2, 64, block, nkv, d))
+    cache[0].reshape(4, 256, nkv, d)[..., 5] = 127 - np.minimum(np.arange(256), 254)[None, :, None]
+    tables = np.arange(64).reshape(4, 16)
+    keys, values = ([c.reshape(4, 256, nkv, d)[b, :n] / 128.0 for b, n in enumerate(lens)] for c in cache)
+    dq = torch.from_numpy(q.reshape(-1, nh * d)).to(dtype).cuda()
+    assert (_np(dq) == q.reshape(-1, nh * d)).all()
+    kc, vc = (torch.from_numpy(c).to(torch.int8).cuda() for c in cache)
+    got = ops.paged_attention_int8kv(dq, kc, vc, _i32(tables), _i32(lens), torch.full((2, nkv * d), 1 / 128.0, device="cuda"), None, nh, nkv,
+                                     0.125, q_starts=_i32(np.concatenate([[0], np.cumsum(q_lens)])), window=window, sinks=sinks)
+    _hold(_np(got), (q.reshape(-1, nh * d), keys, values, lens, q_lens, nh, nkv, 0.125, window, sinks), dtype, f"size {size}", "channel",
+          [np.full_like(v, 127.0) for v in values])
+
+
 @pytest.mark.parametrize("dtype", ACT)
 @pytest.mark.parametrize("window,sinks", [(100, 4), (1500, 300)])
 def test_a_few_rows_behind_a_long_context_are_cut_and_joined(dtype, window, sinks):
