@@ -183,8 +183,11 @@ __device__ __forceinline__ int list_cut(BeamList& l, int e, int n, float& bound)
 
 // A wave's list takes every logit above a bound that n logits of its piece are known to reach: first the n-th largest of
 // the lanes' maxima of a step (found bit by bit with ballots), later the n-th best entry, which is looked up only when the list has
-// grown by some tens (a look-up costs as much as two steps; done after every step that brought an entry, the kernel took 162 us
-// where it takes 68: 512 x 152064 float32).
+// grown by some tens (a look-up costs as much as two steps; done after every step that brought an entry, the kernel took more than
+// twice as long).
+// Bound: the vector unit, beside the stream: 512 x 152064 float32, 16 best of 8 beams, 76 us under the profiler (4.1 TB/s; bf16 logits, half the
+// bytes, take 8 us less), of about 7400 vector instructions a wave the exponentials are 4560.  A reference of 0 without its subtraction
+// won nothing, the waves of a row that share the best of their bounds through LDS lost 3 us.
 template <typename L>
 __global__ __launch_bounds__(BS_WAVES * 64) void beam_partial_kernel(const void* __restrict__ logits, int64_t row_stride,
                                                                      const float* __restrict__ run, int vocab, int cols, int chunks,
@@ -390,7 +393,8 @@ __global__ __launch_bounds__(BS_WAVES * 64) void beam_partial_kernel(const void*
 }
 
 // Joins the pieces of a group's beams and ranks their candidates.  What bounds it: a chain of dependent reads and reductions, a
-// workgroup a group.  HELD: the candidates fit the registers, and are read once, beside the pieces' sums.
+// workgroup a group (64 groups of 8 beams, 16 candidates: a call takes 84 us with the entries ranked by sixteen lanes each and a bound of 20
+// bits, 90 with a lane each and all 32).  HELD: the candidates fit the registers, and are read once, beside the pieces' sums.
 constexpr int BJ_THREADS = 1024;
 constexpr int BJ_WAVES = BJ_THREADS / 64;
 constexpr int BJ_HELD = 4;                                    // candidates a thread
@@ -476,7 +480,7 @@ __global__ __launch_bounds__(BJ_THREADS) void beam_join_kernel(const float* __re
         }
     }
     uint32_t t = 0;
-    for (int bit = 31; bit >= 0; --bit) {
+    for (int bit = 31; bit >= 12; --bit) {                    // a lower bound does as well: the last bits keep few candidates away
         const uint32_t trial = t | (1u << bit);
         if (__popcll(__ballot(key >= trial)) >= n) t = trial;
     }
@@ -507,12 +511,15 @@ __global__ __launch_bounds__(BJ_THREADS) void beam_join_kernel(const float* __re
     __syncthreads();
     const int count = s_count;
     if (count <= BJ_LIST) {
-        for (int i = tid; i < count; i += BJ_THREADS) {
+        for (int i0 = 0; i0 < count; i0 += BJ_THREADS / 16) { // sixteen lanes an entry
+            const int i = min(i0 + tid / 16, count - 1);
             const double s = l_score[i];
             const int at = l_at[i];
             int rank = 0;
-            for (int j = 0; j < count; ++j) rank += l_score[j] > s || (l_score[j] == s && l_at[j] < at);
-            if (rank < n) {
+            for (int j = tid & 15; j < count; j += 16) rank += l_score[j] > s || (l_score[j] == s && l_at[j] < at);
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) rank += __shfl_xor(rank, o, 64);
+            if (rank < n) {                                   // (lanes of one entry, and those past the last, write the same)
                 best_score[rank] = s;
                 best_at[rank] = at;
             }
