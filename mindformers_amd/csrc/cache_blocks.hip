@@ -3,7 +3,9 @@
 // an entry of a table names it, so that the tables are the only state and a step is a function of them.
 //
 // What bounds the two planning operators is launch latency and one workgroup's walk over the tables: their answer hangs
-// on a ranking of all free blocks, which one workgroup forms from a bitmap in LDS (one bit a block, 128 KB for a million).
+// on a ranking of all free blocks, which one workgroup forms from a bitmap in LDS (one bit a block, 128 KB for a million).  Under the
+// profiler 16 rows of 32 blocks in 1024 take 7.8 us in one launch, 512 rows of 256 in 131072 3.5 + 16.0, closing up 64 rows of
+// 32 in 1024 8.4 + 3.0.
 #include <algorithm>
 
 #include "common.h"
@@ -331,8 +333,8 @@ __global__ __launch_bounds__(256) void compact_remap_kernel(int32_t* __restrict_
 
 // Block copies within the cache tensors of all layers in one launch.  The list is on the device and may be longer than
 // what is used of it (it ends at the first negative source), so the workgroups look for its end and take (copy, tensor, piece) in
-// turn.  Bound: memory.  24 open blocks of 64 caches, 420 MB read and written: 87 us (4.8 TB/s; a plain copy of 200 MB reaches 5.4, the
-// library's), 96 through the caches with 32 KB pieces on 2048 workgroups; 192 whole blocks of 16 caches, 1.6 GB: 280 us.
+// turn.  Bound: memory.  24 open blocks of 64 caches, 420 MB read and written: 91 us (4.6 TB/s; the library's copy of 200 MiB reaches 5.4),
+// 96 through the caches with 32 KB pieces on 2048 workgroups; 192 whole blocks of 16 caches, 1.6 GB: 296 us (5.4 TB/s).
 constexpr int COPY_TENSORS = 128;
 constexpr int COPY_PIECE = 16384;                             // bytes of a block that a workgroup copies at a time
 constexpr int COPY_THREADS = 256;

@@ -47,7 +47,7 @@ struct PaQuantArgs {
 // workgroups on (a workgroup takes 8 us + 12.8 ns a token, a combine 4.5 us).  Measured, us with the plan of a full context | one partition |
 // this one | best: 64 sequences of 512 to 4096 tokens through 1024, 32/8 heads 55.7 | 46.1 | 46.1 | 46.1, over int8 40.5 | 32.3 | 32.3 |
 // 32.3; 32 through 512 19.8 | 17.4 | 17.4 | 17.3; 16 of 16 to 32 k through 4096, 64/8 heads 59.1 | 68.9 | 52.9 | 52.9, over int8 41.4 | 68.1 |
-// 36.8 | 36.8; 16 through 1024 21.8 | 22.8 | 20.9 | 20.0; 4 through 2048 16.1 | 34.4 | 16.0 | 15.0; one through 4096 13.2 | 61.1 | 13.6 | 13.2.
+// 36.6 | 36.6; 16 through 1024 21.8 | 22.8 | 20.9 | 20.0; 4 through 2048 16.1 | 34.4 | 16.0 | 15.0; one through 4096 13.2 | 61.1 | 13.6 | 13.2.
 struct PaWinPlan {
     int part_tokens, max_parts;
 };

@@ -776,10 +776,10 @@ static inline int64_t pf_win_walk(int64_t max_ctx, int cols, int n_rep, PaWindow
 // Plan of a step with a window on the 128-column kernel.  Walks are about equally long (no short causal ranges), so the time is priced
 // for every number of partitions: 8 us a round of 768 workgroups, and the tiles of one chain at 0.72 us or of a compute unit at
 // 0.54 us each (heads of 128), whichever is more; a cut adds 2.5 us and 0.33 us for every megabyte of partials written and read
-// back.  Measured, us with the plan of a full context | uncut | this one | best: chunks of 512 rows beside 24 decoding sequences through 1024,
-// 32/8 heads 68 | 48 | 44 | 44, one chunk of 64 through 2048 22.9 | 62.6 | 23.1 | 22.9, one of 32 beside 24 through 512, 28/4 heads, blocks of
-// 16 24.4 | 32.8 | 19.4 | 19.4, a prompt of 2048 rows through 1024, 8/1 heads 32.3 | 34.5 | 30.6 | 30.6, one of 4096 through 512, 8/8 30.5 |
-// 28.4 | 24.7 | 24.7 (the uncut ones here without the launch for rows of no sequence).
+// back.  Measured, us with the plan of a full context | uncut | this one | best of 1 to 6 partitions, heads of 128: chunks of 512 rows beside 24
+// decoding sequences through 1024, 32/8 heads, int8 64.7 | 43.7 | 43.7 | 43.7; a chunk of 64 through 2048 23.0 | 60.7 | 23.0 | 23.0; one of
+// 32 beside 24 through 512, 28/4, blocks of 16 24.1 | 30.8 | 19.8 | 19.8; a prompt of 2048 rows through 1024, 8/1 31.5 | 33.1 | 31.8 | 30.9; of
+// 4096 through 512, 8/8 37.3 | 26.2 | 26.2 | 26.2; 1024 rows in four through 256, 32/8 29.9 | 16.8 | 16.8 | 16.8.
 static inline PfPlan pf_win_plan(int batch, int64_t total_q, int n_heads, int n_kv, int head_dim, int64_t walk) {
     PfPlan best = pf_plan(batch, total_q, n_heads, n_kv, walk);
     const int64_t groups = std::max<int64_t>((total_q * (n_heads / n_kv) + PF_COLS - 1) / PF_COLS, std::min<int64_t>(batch, total_q));
@@ -787,7 +787,7 @@ static inline PfPlan pf_win_plan(int batch, int64_t total_q, int n_heads, int n_
     const float width = (0.012f + 0.000058f * head_dim) / 0.0194f, tiles = (float)(walk / PF_TOK);
     const float mb = 4e-6f * (head_dim + 2) * total_q * n_heads;
     float best_us = 0.f;
-    for (int64_t parts = 1; parts <= std::max<int64_t>(1, std::min<int64_t>(32, walk / PA_WAVE_TOKENS)); ++parts) {
+    for (int64_t parts = 1; parts <= std::min<int64_t>(32, (walk + PA_WAVE_TOKENS - 1) / PA_WAVE_TOKENS); ++parts) {
         PfPlan p = best;
         pf_cut(p, walk, parts);
         const int64_t n = wgs * p.max_parts;
