@@ -127,7 +127,7 @@ __device__ __forceinline__ uint32_t in_range(int w, int num_blocks) {
 // new tokens; request i gets the i-th lowest free block.  GATHER: the rows are gathered here too (small tables: one launch).
 struct ForkRequest {
     ForkRow r;
-    int open, wanted;                                         // block to copy (-1: none), blocks behind it
+    int open, wanted, over;                                   // block to copy (-1: none), blocks behind it, more for which the table has no place
 };
 template <bool GATHER>
 __global__ __launch_bounds__(CB_THREADS) void fork_assign_kernel(ForkArgs a) {
@@ -151,11 +151,13 @@ __global__ __launch_bounds__(CB_THREADS) void fork_assign_kernel(ForkArgs a) {
     __syncthreads();
 
     auto request = [&](int s) -> ForkRequest {
-        ForkRequest q = {{-1, 0, 0}, -1, 0};
+        ForkRequest q = {{-1, 0, 0}, -1, 0, 0};
         if (s >= a.rows) return q;
         q.r = fork_row(a, s);
         if (q.r.parent < 0) return q;
-        q.wanted = (int)(((int64_t)q.r.len + a.new_tokens + a.block_size - 1) / a.block_size) - q.r.used;
+        const int all = (int)(((int64_t)q.r.len + a.new_tokens + a.block_size - 1) / a.block_size) - q.r.used;
+        q.wanted = min(all, a.width - q.r.used);
+        q.over = all - q.wanted;
         if (q.r.len % a.block_size != 0 && eldest[q.r.parent] != s) q.open = a.tables_out[(int64_t)s * a.width + q.r.used - 1];
         return q;
     };
@@ -210,8 +212,8 @@ __global__ __launch_bounds__(CB_THREADS) void fork_assign_kernel(ForkArgs a) {
                     ++given;
                 }
             }
-            const int got = max(min(min(q.wanted, a.width - r.used), found - begin - split), 0);
-            given += got;
+            const int got = max(min(q.wanted, found - begin - split), 0);
+            given += got - q.over;
             const int cap = a.width * a.block_size;
             a.lens_out[s] = r.parent >= 0 ? (int)min((int64_t)r.len + a.new_tokens, (int64_t)cap) : 0;
             if (a.new_tokens > FORK_FILL) a.ranks[1 + s] = begin + split;

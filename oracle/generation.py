@@ -62,8 +62,8 @@ def fork_blocks(tables, lens, num_blocks, block_size, parents=None, new_tokens=0
         n = int(olens[r])
         want += [(j, -1, 0) for j in range(-(-n // block_size), -(-(n + new_tokens) // block_size))]
         for j, src, rows in want:
-            page = free.pop(0) if free else -1                      # a block is taken even where the table has no place for it
-            if page < 0 or j >= m:
+            page = free.pop(0) if free and j < m else -1            # no block is taken where the table has no place for it
+            if page < 0:
                 missing += 1
                 continue
             out[r, j] = page

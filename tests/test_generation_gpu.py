@@ -177,6 +177,15 @@ def test_fork_without_blocks_left_counts_what_is_missing():
     assert int(full.missing) == 12 and (full.slot_mapping == -1).all() and (full.context_lens == 48).all()
 
 
+@pytest.mark.parametrize("new", [5, 40])
+def test_a_row_as_long_as_its_table_takes_no_block_from_another(new):
+    tables = np.full((3, 8), -1)
+    tables[0], tables[1, 0], tables[2] = np.arange(8), 8, np.arange(9, 17)
+    need = -(-new // 8)
+    got = _fork(tables, np.array([64, 8, 64]), 17 + need, 8, new_tokens=new)       # the pool holds what row 1 needs
+    assert int(got.missing) == 2 * need and (_np(got.slot_mapping).reshape(3, new)[1] >= 0).all()
+
+
 def test_fork_ignores_entries_that_name_no_block():
     tables = np.array([[3, 99, -7, 2], [0, 1, -1, -1], [5, 6, 7, 8]])
     got = _fork(tables, np.array([7, 3, -4]), 10, 2, parents=np.array([0, 0, 2]), new_tokens=1)
@@ -422,6 +431,31 @@ def test_windows_over_int8_caches_with_large_and_small_queries(dtype, size, rows
                                      0.125, q_starts=_i32(np.concatenate([[0], np.cumsum(q_lens)])), window=window, sinks=sinks)
     _hold(_np(got), (q.reshape(-1, nh * d), keys, values, lens, q_lens, nh, nkv, 0.125, window, sinks), dtype, f"size {size}", "channel",
           [np.full_like(v, 127.0) for v in values])
+
+
+@pytest.mark.parametrize("kind", ["16", "channel", "token"])
+@pytest.mark.parametrize("dtype", ACT)
+@pytest.mark.parametrize("window,sinks", [(2000, 3), (40, 2 ** 31 - 1), (2 ** 31 - 1, 0), (20, 0)])
+def test_rows_of_no_sequence_are_zero_and_their_queries_unread(kind, dtype, window, sinks):
+    from mindformers_amd import ops
+    rng = np.random.default_rng(11)
+    lens, q_lens, nh, nkv, d, block = np.array([3000, 0, 700, 9]), np.array([4, 0, 5, 9]), 4, 2, 64, 16
+    q, cache, scales, tables, keys, values = _paged(rng, dtype, lens, q_lens, nh, nkv, d, block, window, sinks, kind)
+    wide = torch.full((27, nh * d), float("nan"), dtype=dtype, device="cuda")
+    wide[3:21] = torch.from_numpy(q).to(dtype)
+    out = torch.full_like(wide, float("nan"))
+    kc, vc = (torch.from_numpy(c).to(dtype if kind == "16" else torch.int8).cuda() for c in cache)
+    t, n, starts, scale = _i32(tables), _i32(lens), _i32([3, 7, 7, 12, 21]), 1 / np.sqrt(d)
+    view = dict(window=window, sinks=sinks, out=out)
+    if kind == "16":
+        ops.paged_attention_prefill(wide, kc, vc, t, n, starts, nh, nkv, scale, **view)
+    else:
+        s = torch.from_numpy(scales).float().cuda()
+        par = dict(token_scales=(s[0].contiguous(), s[1].contiguous())) if kind == "token" else {}
+        ops.paged_attention_int8kv(wide, kc, vc, t, n, None if par else s, None, nh, nkv, scale, q_starts=starts, **par, **view)
+    assert (out[:3] == 0).all() and (out[21:] == 0).all()
+    _hold(_np(out[3:21]), (q, keys, values, lens, q_lens, nh, nkv, scale, window, sinks), dtype, f"window {window}, sinks {sinks}", kind,
+          [np.full_like(v, 127.0) for v in values] if kind == "token" else None)
 
 
 @pytest.mark.parametrize("dtype", ACT)
