@@ -777,7 +777,7 @@ static inline int64_t pf_win_walk(int64_t max_ctx, int cols, int n_rep, PaWindow
 // for every number of partitions: 8 us a round of 768 workgroups, and the tiles of one chain at 0.72 us or of a compute unit at
 // 0.54 us each (heads of 128), whichever is more; a cut adds 2.5 us and 0.33 us for every megabyte of partials written and read
 // back.  Measured, us with the plan of a full context | uncut | this one | best of 1 to 6 partitions, heads of 128: chunks of 512 rows beside 24
-// decoding sequences through 1024, 32/8 heads, int8 64.7 | 43.7 | 43.7 | 43.7; a chunk of 64 through 2048 23.0 | 60.7 | 23.0 | 23.0; one of
+// decoding sequences through 1024, 32/8 heads 64.7 | 43.7 | 43.7 | 43.7; a chunk of 64 through 2048 23.0 | 60.7 | 23.0 | 23.0; one of
 // 32 beside 24 through 512, 28/4, blocks of 16 24.1 | 30.8 | 19.8 | 19.8; a prompt of 2048 rows through 1024, 8/1 31.5 | 33.1 | 31.8 | 30.9; of
 // 4096 through 512, 8/8 37.3 | 26.2 | 26.2 | 26.2; 1024 rows in four through 256, 32/8 29.9 | 16.8 | 16.8 | 16.8.
 static inline PfPlan pf_win_plan(int batch, int64_t total_q, int n_heads, int n_kv, int head_dim, int64_t walk) {

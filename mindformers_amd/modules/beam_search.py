@@ -60,8 +60,7 @@ class BeamSearch:
     def step(self, logits):
         """From the logits [B * K, vocab] of the beams' last tokens to the next tokens, int32 [B * K]; block_tables, context_lens and
         slot_mapping then describe the model's step that reads them."""
-        if self.scores is None:
-            raise RuntimeError("call start() first")
+        self._started()
         sel = ops.beam_search_select(logits, self.scores, eos_token_id=self.eos_token_id)
         parents = sel.next_rows.view(-1)
         if self._out is not None:
@@ -75,8 +74,13 @@ class BeamSearch:
         self._steps.append(sel)
         return sel.next_tokens.view(-1)
 
+    def _started(self):
+        if self.scores is None:
+            raise RuntimeError("call start() first")
+
     def release(self, groups):
         """Takes groups out of the search: their rows are empty from the next step on, and their blocks free."""
+        self._started()
         rows = torch.zeros(self.groups, dtype=torch.bool, device=self.scores.device)
         rows[torch.as_tensor(groups, device=rows.device)] = True
         self.scores = torch.where(rows[:, None], -torch.inf, self.scores)
@@ -86,6 +90,7 @@ class BeamSearch:
     def compact(self):
         """Closes up the cache's blocks; returns the number in use, int32 [1] on the device: blocks from there on that are not held by
         others are free."""
+        self._started()
         self.block_tables, copies, live = ops.compact_blocks(self.block_tables, self.num_blocks, self.block_size, held=self.held)
         ops.copy_blocks(self.caches, copies)
         if self.slot_mapping is not None:                     # the slots of the step to come, in the moved blocks
@@ -99,6 +104,7 @@ class BeamSearch:
         """The finished and the running continuations of every group, on the host: a list of (score / length ** length_penalty, tokens) per
         group, best first.  A continuation is finished where the end token is among a step's K best candidates; its end token
         counts.  Raises if a step found no block for a beam."""
+        self._started()
         if int(self._missing):
             raise RuntimeError(f"the cache of {self.num_blocks} blocks was short of {int(self._missing)} blocks for the beams")
         host = [[t.cpu().numpy() for t in sel] for sel in self._steps]

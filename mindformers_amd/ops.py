@@ -195,7 +195,7 @@ def check_window(window, sinks):
     if window is None:
         _need(sinks == 0, "sinks go with a window")
         return 0, 0
-    if not (int(window) == window and window > 0 and int(sinks) == sinks and sinks >= 0):
+    if not (0 < window < math.inf and int(window) == window and 0 <= sinks < math.inf and int(sinks) == sinks):
         raise ValueError(f"window must be a positive integer and sinks not negative, got {window!r} and {sinks!r}")
     return min(int(window), 0x7fffffff), min(int(sinks), 0x7fffffff)
 
@@ -774,9 +774,8 @@ def fork_blocks(block_tables, context_lens, num_blocks, block_size, parents=None
             if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.dim() == 1 and t.numel() == s and t.is_contiguous()):
                 raise ValueError(f"{name} must be a contiguous int32 [{s}]")
             _need(t.device == dev, "all tensors must be on the same device")
-    _need(block_size > 0 and new_tokens >= 0 and sinks >= 0, "block_size must be positive, new_tokens and sinks not negative")
-    _need(window is None or window > 0, "window must be positive (None: no window)")
-    _need(window is not None or sinks == 0, "sinks go with a window")
+    _need(block_size > 0 and new_tokens >= 0, "block_size must be positive, new_tokens not negative")
+    window, sinks = check_window(window, sinks)
     out = torch.empty(s * (m + new_tokens + 4) + 1, dtype=torch.int32, device=dev)
     a, b, c, d = s * m, s * (m + 1), s * (m + 4), s * (m + 4) + 1
     part = out.as_strided                                     # half the time of a slice and a view
@@ -787,8 +786,7 @@ def fork_blocks(block_tables, context_lens, num_blocks, block_size, parents=None
     at = out.data_ptr()
     with _on(dev):
         check(lib.mf_fork_blocks(at, at + 4 * a, at + 4 * d, at + 4 * b, at + 4 * c, ptr(block_tables), ptr(context_lens), ptr(parents),
-                                 ptr(held), s, m, num_blocks, block_size, new_tokens, min(window or 0, 0x7fffffff), min(sinks, 0x7fffffff),
-                                 ptr(ws), ws.numel(), stream_ptr(dev)), "mf_fork_blocks")
+                                 ptr(held), s, m, num_blocks, block_size, new_tokens, window, sinks, ptr(ws), ws.numel(), stream_ptr(dev)), "mf_fork_blocks")
     return res
 
 

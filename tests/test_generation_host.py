@@ -55,3 +55,79 @@ def test_ops_refuse_tensors_that_are_not_on_the_gpu():
                  lambda: ops.beam_search_select(torch.zeros(4, 9), torch.zeros(1, 4)), lambda: ops.copy_blocks([], [[0, 1]])):
         with pytest.raises(ValueError):
             call()
+
+
+def test_windowed_attention_is_refused_before_a_launch():
+    from mindformers_amd import _lib
+    lib = _lib.load()
+
+    def refused(name, args, word):
+        assert getattr(lib, name)(*args) == 1
+        assert word in lib.mf_last_error().decode(), lib.mf_last_error()
+
+    #        out  xq x_scale smooth layout q k v key_scale value_scale kv_quant tables lens b nh nkv d block width blocks
+    decode = [16, None, None, None, 0, 16, 16, 16, None, None, 0, 16, 16, 2, 8, 2, 64, 16, 200, 100, 0.125, 1000, 4, 0, 0, 16, 1 << 30, None]
+    need = lib.mf_window_attention_workspace_bytes(2, 8, 64, 3200, 1000, 4)
+    assert need > 0
+    for at, value, word in ((21, 0, "window"), (21, -3, "window"), (22, -1, "sinks"), (10, 3, "kv_quant"), (10, -1, "kv_quant"), (10, 1, "scales"),
+                            (14, 7, "multiple"), (16, 192, "head_dim"), (16, 48, "head_dim"), (17, 0, "geometry"), (18, 1 << 28, "overflows"),
+                            (24, 2, "dtype"), (5, None, "null"), (11, None, "null"), (7, 24, "aligned"), (23, 100, "stride"), (23, 516, "stride"),
+                            (26, need - 1, "workspace"), (25, None, "workspace"), (25, 24, "workspace")):
+        args = list(decode)
+        args[at] = value
+        refused("mf_window_attention_decode", args, word)
+    for xq, scale, smooth, layout, kvq, word in ((16, None, None, 0, 0, "quantised"), (16, 16, None, 2, 0, "quantised"), (16, 16, None, 0, 1, "quantised"),
+                                                 (20, 16, None, 0, 0, "aligned"), (16, 16, 24, 0, 0, "aligned")):
+        args = list(decode)
+        args[1:5], args[10] = [xq, scale, smooth, layout], kvq
+        refused("mf_window_attention_decode", args, word)
+    args = list(decode)
+    args[8:11] = [16, None, 2]
+    refused("mf_window_attention_decode", args, "per-token")
+    args[8:11], args[17] = [16, 16, 2], 6
+    refused("mf_window_attention_decode", args, "multiple of 4")
+    args = list(decode)
+    args[13] = 0
+    assert lib.mf_window_attention_decode(*args) == 0          # no sequence, nothing to do
+
+    #         out q k v key_scale value_scale kv_quant tables lens starts b rows nh nkv d block width blocks
+    prefill = [16, 16, 16, 16, None, None, 0, 16, 16, 16, 2, 40, 8, 2, 64, 16, 200, 100, 0.125, 1000, 4, 0, 0, 0, 16, 1 << 30, None]
+    need = lib.mf_window_attention_prefill_workspace_bytes(2, 40, 8, 2, 64, 3200, 1000, 4)
+    assert need > 0
+    for at, value, word in ((19, 0, "window"), (20, -1, "sinks"), (6, 3, "kv_quant"), (6, 1, "scales"), (12, 7, "multiple"), (14, 192, "32, 64 or 128"),
+                            (14, 48, "head_dim"), (23, 2, "dtype"), (1, None, "null"), (9, None, "null"), (3, 24, "aligned"), (21, 100, "stride"),
+                            (18, -1.0, "scale"), (25, need - 1, "workspace"), (24, None, "workspace"), (24, 24, "workspace")):
+        args = list(prefill)
+        args[at] = value
+        refused("mf_window_attention_prefill", args, word)
+    for sizes in ((0, 40, 8, 2, 64, 3200, 1000, 4), (2, 40, 8, 3, 64, 3200, 1000, 4), (2, 40, 8, 2, 64, 3200, 0, 4), (2, 40, 8, 2, 64, 3200, 1000, -1)):
+        assert lib.mf_window_attention_prefill_workspace_bytes(*sizes) == 0
+
+
+def test_windows_that_are_none():
+    from mindformers_amd import ops
+    from mindformers_amd.modules import BeamSearch, FlashAttention, PagedAttentionMgr
+    assert ops.check_window(None, 0) == (0, 0) and ops.check_window(7, 2) == (7, 2) and ops.check_window(7.0, 2) == (7, 2)
+    assert ops.check_window(1 << 40, 1 << 50) == (0x7fffffff, 0x7fffffff)
+    for window, sinks in ((0, 0), (-1, 0), (2.5, 0), (float("inf"), 0), (float("nan"), 0), (3, -1), (3, 0.5), (3, float("inf")), (None, 1)):
+        with pytest.raises(ValueError):
+            ops.check_window(window, sinks)
+        with pytest.raises(ValueError):
+            BeamSearch([torch.zeros(4, 2, 8)], 2, window=window, sinks=sinks)
+        with pytest.raises(ValueError):
+            PagedAttentionMgr(2, 32, 2, kv_shape=(4, 16, 2, 32), device="cpu", window=window, sinks=sinks)
+    with pytest.raises(NotImplementedError):
+        FlashAttention(2, head_dim=576, kv_head_num=1, pa_mla_v_dim=512, window=4)
+
+
+def test_a_beam_search_is_started_first():
+    from mindformers_amd.modules import BeamSearch
+    search = BeamSearch([torch.zeros(4, 2, 8)], 2)
+    for call in (lambda: search.step(torch.zeros(2, 9)), lambda: search.release([0]), search.compact, search.hypotheses):
+        with pytest.raises(RuntimeError, match="start"):
+            call()
+    for beams in (0, 33):
+        with pytest.raises(ValueError):
+            BeamSearch([torch.zeros(4, 2, 8)], beams)
+    with pytest.raises(ValueError):
+        BeamSearch([], 2)
