@@ -380,10 +380,10 @@ def read_layer_arrays(source, layer, model_config, prefix="model.layers."):
     return out
 
 
-def load_decode_layer(source, layer, model_config, act_quant=False, dtype=None, device="cuda", eps=None):
+def load_decode_layer(source, layer, model_config, act_quant=False, dtype=None, device="cuda", eps=None, window=None, sinks=0):
     """Build a ``QuantDecodeLayer`` for layer ``layer`` of a checkpoint (see read_layer_arrays for the accepted
     formats): float weights are quantized to int8 per output channel, int8 weights are taken with their scales; the
-    weights are then packed for the GEMM kernels."""
+    weights are then packed for the GEMM kernels.  ``window`` / ``sinks``: of the layer's attention."""
     import torch
     from .decode_layer import QuantDecodeLayer
     arrays = read_layer_arrays(source, layer, model_config)
@@ -395,7 +395,7 @@ def load_decode_layer(source, layer, model_config, act_quant=False, dtype=None, 
     dtype = dtype or torch.bfloat16
     eps = eps if eps is not None else (_cfg(model_config, "rms_norm_eps") or 1e-5)
     net = QuantDecodeLayer(hidden, num_heads, n_kv, head_dim, ffn, eps=eps, dtype=dtype, act_quant=act_quant,
-                           qkv_bias=arrays["qkv"][2] is not None, device=device)
+                           qkv_bias=arrays["qkv"][2] is not None, device=device, window=window, sinks=sinks)
     for name in QuantDecodeLayer.NAMES:
         w, scale, bias, smooth = arrays[name]
         if w.dtype != np.int8:

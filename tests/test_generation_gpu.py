@@ -710,6 +710,40 @@ def test_a_windowed_layer_is_a_full_one_on_the_tokens_that_it_sees(act_quant, ro
     assert torch.equal(got, want)
 
 
+def test_a_layer_from_a_checkpoint_has_its_window_over_16_bit_and_int8_caches():
+    from mindformers_amd import checkpoint, ops
+    rng = np.random.default_rng(5)
+    nh, nkv, d, ffn, bs, rows = 8, 2, 64, 512, 32, 5
+    cfg = dict(num_heads=nh, n_kv_heads=nkv, hidden_size=nh * d, intermediate_size=ffn, qkv_concat=False)
+    hf = {f"model.layers.0.{name}.weight": rng.normal(0, 0.03, shape).astype(np.float32) for name, shape in (
+        ("self_attn.q_proj", (512, 512)), ("self_attn.k_proj", (128, 512)), ("self_attn.v_proj", (128, 512)), ("self_attn.o_proj", (512, 512)),
+        ("mlp.gate_proj", (ffn, 512)), ("mlp.up_proj", (ffn, 512)), ("mlp.down_proj", (512, ffn)))}
+    hf.update({f"model.layers.0.{name}.weight": np.ones(512, np.float32) for name in ("input_layernorm", "post_attention_layernorm")})
+    layer, full = (checkpoint.load_decode_layer(hf, 0, cfg, dtype=torch.bfloat16, **view) for view in (dict(window=64, sinks=0), {}))
+    assert (layer.window, layer.sinks, full.window) == (64, 0, None)
+    tables = torch.randperm(rows * 8, device="cuda").int().view(rows, 8)
+    n = torch.full((rows,), 160, dtype=torch.int32, device="cuda")       # the window is tokens 96 to 159: blocks 3 and 4
+    x, slots = torch.randn(rows, 512, device="cuda").bfloat16(), tables[:, 4] * bs + 31
+    cos, sin = torch.ones(rows, d, device="cuda").bfloat16(), torch.zeros(rows, d, device="cuda").bfloat16()
+    caches = [torch.randn(rows * 8, bs, nkv, d, device="cuda").bfloat16() for _ in range(2)]
+    hidden = tables.clone()
+    hidden[:, :3] = -1
+    got = layer(x, *[c.clone() for c in caches], hidden, n, slots, cos, sin)
+    assert torch.equal(got, full(x, *[c.clone() for c in caches], tables[:, 3:].contiguous(), torch.full_like(n, 64), slots, cos, sin))
+    scale = torch.full((2, nkv * d), 2.0 ** -5, device="cuda")
+    layer.set_kv_quant(scale)
+    kc, vc = (torch.randint(-127, 128, (rows * 8, bs, nkv, d), device="cuda").to(torch.int8) for _ in range(2))
+    want = ops.paged_attention_int8kv(x, kc, vc, hidden, n, scale, None, nh, nkv, layer.scale_value, window=64)
+    assert torch.equal(layer.attend(x, kc, vc, hidden, n).view_as(want), want)
+    k2, v2 = kc.clone(), vc.clone()
+    out = layer(x, k2, v2, hidden, n, slots, cos, sin)
+    written = torch.zeros(rows * 8 * bs, dtype=torch.bool, device="cuda")
+    written[slots.long()] = True
+    assert torch.isfinite(out.float()).all()
+    for old, new in ((kc, k2), (vc, v2)):
+        assert torch.equal(old.view(-1, nkv * d)[~written], new.view(-1, nkv * d)[~written])
+
+
 def test_the_modules_pass_their_window_on():
     """InferAttention and FlashAttention in every form of their attention, a manager and its quantised successor."""
     from mindformers_amd import ops
