@@ -800,7 +800,8 @@ def compact_blocks(block_tables, num_blocks, block_size, held=None):
     s, m = block_tables.shape
     most = num_blocks // 2
     out = torch.empty(s * m + 3 * most + 1, dtype=torch.int32, device=dev)
-    tables, copies, live = out[:s * m].view(s, m), out[s * m:-1].view(most, 3), out[-1:]
+    part = out.as_strided
+    tables, copies, live = part((s, m), (m, 1), 0), part((most, 3), (3, 1), s * m), part((1,), (1,), s * m + 3 * most)
     ws = _scratch(lib.mf_compact_blocks_workspace_bytes(num_blocks), dev, "compact")
     with _on(dev):
         check(lib.mf_compact_blocks(ptr(tables), ptr(copies), ptr(live), ptr(block_tables), ptr(held), s, m, num_blocks, block_size,
@@ -817,14 +818,22 @@ def copy_blocks(caches, copies):
     lib = _lib.load()
     caches = list(caches)
     _need(len(caches) > 0, "caches must not be empty")
-    dev = _dev_ok(*caches)
-    first = caches[0].shape[:2]
-    nb, bs = first if len(first) == 2 else (0, 0)
-    _need(nb > 0 and bs > 0, "caches must be [num_blocks, block_size, ...]")
-    rows = []
-    for c in caches:
-        _need(c.shape[:2] == first and c.numel() > 0, "all caches must share num_blocks and block_size")
-        rows.append(c.numel() // (nb * bs) * c.element_size())
+    first = caches[0]
+    dev = _dev_ok(first)
+    index, shape, dtype = dev.index, first.shape, first.dtype
+    nb, bs = shape[:2] if len(shape) >= 2 else (0, 0)
+    _need(nb > 0 and bs > 0 and first.numel() > 0, "caches must be [num_blocks, block_size, ...]")
+    row = first.numel() // (nb * bs) * first.element_size()
+    at, rows = [], []
+    for c in caches:                                          # mostly alike: a few hundred nanoseconds each, of 64 or more
+        if not (isinstance(c, torch.Tensor) and c.get_device() == index and c.is_contiguous()):
+            _dev_ok(first, c)                                 # says what is wrong with it
+        if c.shape == shape and c.dtype == dtype:
+            rows.append(row)
+        else:
+            _need(c.shape[:2] == shape[:2] and c.numel() > 0, "all caches must share num_blocks and block_size")
+            rows.append(c.numel() // (nb * bs) * c.element_size())
+        at.append(c.data_ptr())
     if not (isinstance(copies, torch.Tensor) and copies.is_cuda):
         copies = _host_copies(copies, nb, bs)
         if copies.shape[0] == 0:
@@ -836,8 +845,8 @@ def copy_blocks(caches, copies):
           "copies must be a contiguous int32 [n, 3] on the caches' device, or host integers")
     n = len(caches)
     with _on(dev):
-        check(lib.mf_copy_blocks((ctypes.c_void_p * n)(*[c.data_ptr() for c in caches]), (ctypes.c_int32 * n)(*rows), n, ptr(copies),
-                                 copies.shape[0], nb, bs, stream_ptr(dev)), "mf_copy_blocks")
+        check(lib.mf_copy_blocks((ctypes.c_void_p * n)(*at), (ctypes.c_int32 * n)(*rows), n, ptr(copies), copies.shape[0], nb, bs,
+                                 stream_ptr(dev)), "mf_copy_blocks")
 
 
 def _host_copies(copies, nb, bs):
