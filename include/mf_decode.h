@@ -94,7 +94,7 @@ int mf_swap_blocks(void* host_cache, void* device_cache, const int64_t* pairs, i
  *     entries stay -1 and *missing counts them.
  * Distinct rows must not share an open block in `tables` unless one is copied from the other by this call.  num_blocks <= 2^20, rows <= 4096;
  * workspace: mf_fork_blocks_workspace_bytes. */
-size_t mf_fork_blocks_workspace_bytes(int rows, int block_size, int new_tokens);
+size_t mf_fork_blocks_workspace_bytes(int rows, int width, int num_blocks, int block_size, int new_tokens);
 int mf_fork_blocks(int32_t* tables_out, int32_t* lens_out, int32_t* slots, int32_t* copies, int32_t* missing,
                    const int32_t* tables, const int32_t* lens, const int32_t* parents, const uint8_t* held, int rows, int width,
                    int num_blocks, int block_size, int new_tokens, int window, int sinks, void* workspace,

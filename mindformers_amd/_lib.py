@@ -25,7 +25,7 @@ SIGNATURES = {
     "mf_rope_rows": (_I, [_P, _P, _P, _P, _I, _I, _I, _P]),
     "mf_rope_and_cache": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _L, _L, _L, _L, _I, _I, _P]),
     "mf_swap_blocks": (_I, [_P, _P, _P, _L, _L, _L, _L, _I, _P]),
-    "mf_fork_blocks_workspace_bytes": (_Z, [_I, _I, _I]),
+    "mf_fork_blocks_workspace_bytes": (_Z, [_I] * 5),
     "mf_fork_blocks": (_I, [_P] * 9 + [_I] * 7 + [_P, _Z, _P]),
     "mf_compact_blocks_workspace_bytes": (_Z, [_I]),
     "mf_compact_blocks": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _Z, _P]),

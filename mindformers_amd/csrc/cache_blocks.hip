@@ -4,7 +4,7 @@
 //
 // What bounds the two planning operators is launch latency and one workgroup's walk over the tables: their answer hangs
 // on a ranking of all free blocks, which one workgroup forms from a bitmap in LDS (one bit a block, 128 KB for a million).  Under the
-// profiler 16 rows of 32 blocks in 1024 take 7.8 us in one launch, 512 rows of 256 in 131072 3.5 + 16.0, closing up 64 rows of
+// profiler 16 rows of 32 blocks in 1024 take 8 us in one launch, 512 rows of 256 in 131072 6.0 + 10.6 in two, closing up 64 rows of
 // 32 in 1024 8.4 + 3.0.
 #include <algorithm>
 
@@ -17,6 +17,7 @@ constexpr int CB_WAVES = CB_THREADS / 64;
 constexpr int CB_MAX_BLOCKS = 1 << 20;                        // bits of the bitmap: 128 KB of LDS
 constexpr int FORK_FILL = 16;                                 // more new tokens than this a row are placed by a kernel of their own
 constexpr int CB_MAX_ROWS = 4096;                             // rows of a fork: 16 KB of LDS beside it
+constexpr int FORK_MARKERS = 16;                              // most workgroups that mark the blocks of large tables
 
 struct ForkArgs {
     int32_t *tables_out, *lens_out, *slots, *copies, *missing;
@@ -24,6 +25,8 @@ struct ForkArgs {
     const uint8_t* held;
     int32_t *fresh, *ranks;                                   // workspace: the blocks that are handed out; with FORK_FILL, [1 + rows]:
                                                               // how many, and the place of each row's first block behind its open one
+    uint32_t* marks;                                          // workspace: the markers' bitmaps, fork_words() each
+    int markers;                                              // workgroups of fork_mark_kernel, 0: none
     int rows, width, num_blocks, block_size, new_tokens, window, sinks;
 };
 
@@ -65,6 +68,42 @@ __device__ __forceinline__ void fork_gather_row(const ForkArgs& a, int s) {
 __global__ __launch_bounds__(256) void fork_gather_kernel(ForkArgs a) {
     const int s = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (s < a.rows) fork_gather_row(a, s);
+}
+
+// words of a bitmap with a bit for every block, as 16-byte pieces
+__host__ __device__ __forceinline__ int fork_words(int num_blocks) { return (num_blocks + 127) / 128 * 4; }
+
+// The rows gathered and their blocks marked, each workgroup in a bitmap of its own that the assigning one joins.  512 rows of 256
+// entries: 6.0 us and 10.6 for the assigning workgroup; 3.4 and 16.0 where that one marks all entries (an LDS operation each).
+__global__ __launch_bounds__(CB_THREADS) void fork_mark_kernel(ForkArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint32_t bits[];
+    const int words = fork_words(a.num_blocks), lane = threadIdx.x & 63;
+    for (int w = threadIdx.x; w < words; w += CB_THREADS) bits[w] = 0;
+    __syncthreads();
+    for (int s = blockIdx.x * CB_WAVES + (threadIdx.x >> 6); s < a.rows; s += gridDim.x * CB_WAVES) {
+        const ForkRow r = fork_row(a, s);
+        const int32_t* from = a.tables + (int64_t)max(r.parent, 0) * a.width;
+        int32_t* to = a.tables_out + (int64_t)s * a.width;
+        for (int j0 = 0; j0 < a.width; j0 += 256) {
+            int page[4];                                      // four reads on their way at a time
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int j = j0 + 64 * k + lane;
+                page[k] = j < r.used && j < a.width && fork_keeps(a, j, r.len) ? from[j] : -1;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int j = j0 + 64 * k + lane;
+                if (j >= a.width) continue;
+                const bool on = page[k] >= 0 && page[k] < a.num_blocks;
+                to[j] = on ? page[k] : -1;
+                if (on) atomicOr(&bits[page[k] >> 5], 1u << (page[k] & 31));
+            }
+        }
+    }
+    __syncthreads();
+    u32x4* mine = (u32x4*)(a.marks + (int64_t)blockIdx.x * words);
+    for (int i = threadIdx.x; i < words / 4; i += CB_THREADS) mine[i] = ((const u32x4*)bits)[i];
 }
 
 // Exclusive prefix sum over the workgroup's threads; `total` is the sum.  red: CB_WAVES ints of LDS.
@@ -131,12 +170,26 @@ struct ForkRequest {
 };
 template <bool GATHER>
 __global__ __launch_bounds__(CB_THREADS) void fork_assign_kernel(ForkArgs a) {
-    extern __shared__ uint32_t bits[];
+    extern __shared__ __attribute__((aligned(16))) uint32_t bits[];
     __shared__ int red[CB_WAVES];
     const int tid = threadIdx.x;
-    const int words = (a.num_blocks + 31) / 32;
+    const int words = fork_words(a.num_blocks);
     int* eldest = (int*)(bits + words);                       // lowest child of every row
-    for (int w = tid; w < words; w += CB_THREADS) bits[w] = held_word(a.held, w, a.num_blocks);
+    if (!GATHER && a.markers) {
+        for (int i = tid; i < words / 4; i += CB_THREADS) {
+            u32x4 m = {0u, 0u, 0u, 0u}, v[FORK_MARKERS];
+#pragma unroll
+            for (int g = 0; g < FORK_MARKERS; ++g) v[g] = ((const u32x4*)(a.marks + (int64_t)min(g, a.markers - 1) * words))[i];
+#pragma unroll
+            for (int g = 0; g < FORK_MARKERS; ++g) m |= v[g];
+            if (a.held)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) m[e] |= held_word(a.held, 4 * i + e, a.num_blocks);
+            ((u32x4*)bits)[i] = m;
+        }
+    } else {
+        for (int w = tid; w < words; w += CB_THREADS) bits[w] = held_word(a.held, w, a.num_blocks);
+    }
     for (int s = tid; s < a.rows; s += CB_THREADS) eldest[s] = a.rows;
     if constexpr (GATHER) {
         for (int s = tid >> 6; s < a.rows; s += CB_WAVES) fork_gather_row(a, s);
@@ -147,7 +200,7 @@ __global__ __launch_bounds__(CB_THREADS) void fork_assign_kernel(ForkArgs a) {
         const int p = a.parents ? a.parents[s] : s;
         if (p >= 0 && p < a.rows) atomicMin(&eldest[p], s);
     }
-    mark_table(bits, a.tables_out, (int64_t)a.rows * a.width, a.num_blocks);
+    if (GATHER || !a.markers) mark_table(bits, a.tables_out, (int64_t)a.rows * a.width, a.num_blocks);
     __syncthreads();
 
     auto request = [&](int s) -> ForkRequest {
@@ -403,10 +456,20 @@ int set_lds(K kern, size_t bytes, bool (&done)[MF_MAX_DEVICES]) {
 
 }  // namespace
 
-extern "C" size_t mf_fork_blocks_workspace_bytes(int rows, int block_size, int new_tokens) {
-    if (rows <= 0 || block_size <= 0 || new_tokens < 0) return 0;
-    // `ranks`; at most a copied block and the blocks of the new tokens for every row
-    return sizeof(int32_t) * (1 + (size_t)rows * (2 + ((size_t)new_tokens + block_size - 1) / block_size));
+// Markers of a fork: one for every 8192 entries from two on, as long as the assigning workgroup has no more than 256 KB of bitmaps
+// to read.
+static int fork_markers(int rows, int width, int num_blocks) {
+    const int64_t n = std::min<int64_t>((int64_t)rows * width / 8192, 65536 / fork_words(num_blocks));
+    return n < 2 ? 0 : (int)std::min<int64_t>(n, FORK_MARKERS);
+}
+// `ranks`; at most a copied block and the blocks of the new tokens for every row
+static size_t fork_list_words(int rows, int block_size, int new_tokens) {
+    return (1 + (size_t)rows * (2 + ((size_t)new_tokens + block_size - 1) / block_size) + 3) / 4 * 4;
+}
+extern "C" size_t mf_fork_blocks_workspace_bytes(int rows, int width, int num_blocks, int block_size, int new_tokens) {
+    if (rows <= 0 || width <= 0 || num_blocks <= 0 || num_blocks > CB_MAX_BLOCKS || block_size <= 0 || new_tokens < 0) return 0;
+    return sizeof(int32_t) * (fork_list_words(rows, block_size, new_tokens) +
+                              (size_t)fork_markers(rows, width, num_blocks) * fork_words(num_blocks));
 }
 
 extern "C" int mf_fork_blocks(int32_t* tables_out, int32_t* lens_out, int32_t* slots, int32_t* copies, int32_t* missing,
@@ -422,22 +485,28 @@ extern "C" int mf_fork_blocks(int32_t* tables_out, int32_t* lens_out, int32_t* s
     MF_REQUIRE(window > 0 || sinks == 0, "fork_blocks: sinks go with a window");
     MF_REQUIRE(tables_out && lens_out && copies && missing && tables && lens && (slots || new_tokens == 0), "fork_blocks: null argument");
     MF_REQUIRE(tables_out != tables && lens_out != lens, "fork_blocks: a row is read by all its children: the outputs need tensors of their own");
-    const size_t need = mf_fork_blocks_workspace_bytes(rows, block_size, new_tokens);
-    MF_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 3) == 0,
-               "fork_blocks: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    const size_t need = mf_fork_blocks_workspace_bytes(rows, width, num_blocks, block_size, new_tokens);
+    MF_REQUIRE(workspace && workspace_bytes >= need, "fork_blocks: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    MF_REQUIRE(((uintptr_t)workspace & 15) == 0, "fork_blocks: workspace must be 16-byte aligned");
     int32_t* ws = (int32_t*)workspace;
+    const int markers = fork_markers(rows, width, num_blocks);
     const ForkArgs a = {tables_out, lens_out, slots, copies, missing, tables, lens, parents, held, ws + 1 + rows, ws,
-                        rows, width, num_blocks, block_size, new_tokens, window, sinks};
+                        (uint32_t*)ws + fork_list_words(rows, block_size, new_tokens), markers, rows, width, num_blocks, block_size, new_tokens, window, sinks};
     hipStream_t st = (hipStream_t)stream;
-    const size_t lds = (((size_t)num_blocks + 31) / 32 + rows) * 4;
+    const size_t bitmap = (size_t)fork_words(num_blocks) * 4, lds = bitmap + 4 * (size_t)rows;
     const bool small = (int64_t)rows * width <= 8192;
-    static bool set[2][MF_MAX_DEVICES] = {};
+    static bool set[3][MF_MAX_DEVICES] = {};
     int rc;
     if (small) {
         if ((rc = set_lds(fork_assign_kernel<true>, lds, set[1]))) return rc;
         hipLaunchKernelGGL(fork_assign_kernel<true>, dim3(1), dim3(CB_THREADS), lds, st, a);
     } else {
-        hipLaunchKernelGGL(fork_gather_kernel, dim3((rows + 3) / 4), dim3(256), 0, st, a);
+        if (markers) {
+            if ((rc = set_lds(fork_mark_kernel, bitmap, set[2]))) return rc;
+            hipLaunchKernelGGL(fork_mark_kernel, dim3(markers), dim3(CB_THREADS), bitmap, st, a);
+        } else {
+            hipLaunchKernelGGL(fork_gather_kernel, dim3((rows + 3) / 4), dim3(256), 0, st, a);
+        }
         if ((rc = MF_LAUNCH_CHECK())) return rc;
         if ((rc = set_lds(fork_assign_kernel<false>, lds, set[0]))) return rc;
         hipLaunchKernelGGL(fork_assign_kernel<false>, dim3(1), dim3(CB_THREADS), lds, st, a);

@@ -781,7 +781,7 @@ def fork_blocks(block_tables, context_lens, num_blocks, block_size, parents=None
     part = out.as_strided                                     # half the time of a slice and a view
     res = ForkedBlocks(part((s, m), (m, 1), 0), part((s,), (1,), a), part((s * new_tokens,), (1,), d), part((s, 3), (3, 1), b),
                        part((1,), (1,), c))
-    need = lib.mf_fork_blocks_workspace_bytes(s, block_size, new_tokens)
+    need = lib.mf_fork_blocks_workspace_bytes(s, m, num_blocks, block_size, new_tokens)
     ws = _scratch(need, dev, "fork")
     at = out.data_ptr()
     with _on(dev):

@@ -52,7 +52,8 @@ def fork_blocks(tables, lens, num_blocks, block_size, parents=None, new_tokens=0
                 out[r, j] = -1
             else:
                 eldest[p] = r
-    free = [i for i in range(num_blocks) if i not in set(out[out >= 0].tolist()) and not (held is not None and held[i])]
+    named = set(out[out >= 0].tolist())
+    free = [i for i in range(num_blocks) if i not in named and not (held is not None and held[i])]
     copies, missing = [], 0
     slots = np.full((s, new_tokens), -1, np.int64)
     for r in range(s):

@@ -192,6 +192,20 @@ def test_fork_ignores_entries_that_name_no_block():
     assert got.block_tables[0, 1] == -1 and got.context_lens[2] == 1
 
 
+@pytest.mark.parametrize("rows,width,block,new,blocks", [(64, 257, 3, 1, 16500), (64, 256, 1, 2, 40001), (300, 100, 2, 20, 33001), (1030, 33, 2, 1, 70000),
+                                                         (70, 300, 2, 1, 1 << 20), (9, 16000, 1, 1, 150001)])
+def test_fork_of_large_tables_matches_the_oracle(rows, width, block, new, blocks):
+    rng = np.random.default_rng(width)
+    used = rows * width
+    tables, lens = _tables(rng, rows, width, block, min(blocks, used + 9) if blocks < (1 << 20) else used, groups=7) if blocks > used else (
+        rng.integers(-1, blocks + 2, (rows, width)), rng.integers(0, width * block + 1, rows))
+    if blocks == 1 << 20:
+        tables = np.where(tables >= 0, (1 << 20) - 1 - 37 * tables, -1)   # the upper end of the pool too
+    held = rng.random(blocks) < 0.5
+    for kw in (dict(), dict(parents=rng.integers(-1, rows, rows), held=held), dict(parents=rng.integers(0, rows, rows), window=width // 2, sinks=1)):
+        _fork(tables, lens, blocks, block, new_tokens=new, **kw)
+
+
 def test_fork_of_a_pool_of_a_million_blocks():
     """The largest bitmap: 128 KB of LDS; free blocks only at the far end."""
     blocks = 1 << 20
