@@ -42,22 +42,26 @@ struct PaQuantArgs {
 };
 
 // Tokens a partition and partitions of a decode step with a window, over contexts of up to max_ctx tokens.  Walks are mostly of one
-// length, so there is no ragged tail to fill: one partition, and no combine, where the sequences and kv heads alone give every
-// compute unit a workgroup; else as many partitions as fit the device at once (768 workgroups), of 256 tokens at least, 384 from 64
-// workgroups on (a workgroup takes 8 us + 12.8 ns a token, a combine 4.5 us).  Measured, us with the plan of a full context | one partition |
-// this one | best: 64 sequences of 512 to 4096 tokens through 1024, 32/8 heads 55.7 | 46.1 | 46.1 | 46.1, over int8 40.5 | 32.3 | 32.3 |
-// 32.3; 32 through 512 19.8 | 17.4 | 17.4 | 17.3; 16 of 16 to 32 k through 4096, 64/8 heads 59.1 | 68.9 | 52.9 | 52.9, over int8 41.4 | 68.1 |
-// 36.6 | 36.6; 16 through 1024 21.8 | 22.8 | 20.9 | 20.0; 4 through 2048 16.1 | 34.4 | 16.0 | 15.0; one through 4096 13.2 | 61.1 | 13.6 | 13.2.
+// length, so there is no ragged tail to fill, and what counts is that every compute unit has the same number of workgroups: one, so
+// 256 workgroups over the device, and no combine where the sequences and kv heads alone are that many; two for int8 caches, whose
+// tiles have more to compute, but for a few sequences, where a cut costs more than it brings.  Partitions of 128 tokens at least, 384 from 64
+// workgroups on (a workgroup takes 8 us + 12.8 ns a token, a combine 3 to 4.5 us).  us with 768 workgroups of 256 (384) tokens at least | with this
+// plan, bf16 and int8, sequences through a window, 32/8 heads: 1 through 1024 11.4 | 10.3, 11.6 | 10.2; 2 through 4096 16.6 | 14.9, 15.1 |
+// 13.8; 4 through 2048 16.1 | 14.5, 14.3 | 13.6; 6 through 4096 27.2 | 24.1; 8 through 4096 29.2 | 29.1, 23.2 | 21.4; 12 through 2048 27.2 |
+// 25.3, 21.0 | 19.2; 24 through 1024 27.0 | 23.5, 21.0 | 21.9; 64 of 512 to 4096 tokens through 1024 with the plan of a full context 55.7 | 46.1,
+// 40.5 | 32.3.
 struct PaWinPlan {
     int part_tokens, max_parts;
 };
-static inline int64_t pa_win_most_parts(int64_t walk) { return (walk + 2 * PA_WAVE_TOKENS - 1) / (2 * PA_WAVE_TOKENS); }
-static inline PaWinPlan pa_win_plan(int64_t max_ctx, int64_t batch_kv_groups, PaWindow win) {
+static inline int64_t pa_win_most_parts(int64_t walk, int batch) {
+    return std::min<int64_t>((walk + PA_WAVE_TOKENS - 1) / PA_WAVE_TOKENS, std::max(1, 512 / batch));
+}
+static inline PaWinPlan pa_win_plan(int64_t max_ctx, int64_t batch_kv_groups, PaWindow win, bool int8) {
     const int64_t walk = pa_win_tiles(max_ctx, 1, win) * PA_TILE;
-    const int64_t least = batch_kv_groups >= 64 ? 3 * PA_WAVE_TOKENS : 2 * PA_WAVE_TOKENS;
     int64_t part = walk;
     if (batch_kv_groups < 256) {
-        const int64_t parts = 768 / batch_kv_groups;
+        const int64_t parts = std::max<int64_t>(1, (int8 && batch_kv_groups > 32 ? 512 : 256) / batch_kv_groups);
+        const int64_t least = batch_kv_groups >= 64 ? 3 * PA_WAVE_TOKENS : PA_WAVE_TOKENS;
         part = std::max(least, (walk + parts - 1) / parts);
     }
     part = (part + PA_WAVE_TOKENS - 1) / PA_WAVE_TOKENS * PA_WAVE_TOKENS;
@@ -74,7 +78,7 @@ int launch_pa(void* out, const void* query, const void* key_cache, const void* v
     const int64_t max_ctx = (int64_t)max_blocks * block_size;
     const int tpw = WIN ? 0 : pa_launch_tiles_per_wave(max_ctx, KVQ, (int64_t)batch * n_kv * head_groups);
     PaWinPlan plan = {tpw * PA_WAVE_TOKENS, 0};
-    if constexpr (WIN) plan = pa_win_plan(max_ctx, (int64_t)batch * n_kv * head_groups, win);
+    if constexpr (WIN) plan = pa_win_plan(max_ctx, (int64_t)batch * n_kv * head_groups, win, KVQ != 0);
     const int part_tokens = plan.part_tokens;
     const int max_parts = WIN ? plan.max_parts : (int)((max_ctx + part_tokens - 1) / part_tokens);
     float* part_out = (float*)workspace;
@@ -260,7 +264,7 @@ extern "C" size_t mf_window_attention_workspace_bytes(int batch, int n_heads, in
     if (batch <= 0 || n_heads <= 0 || head_dim <= 0 || max_context <= 0 || window <= 0 || sinks < 0) return 0;
     // as many partitions as the launch rule may choose, which knows the kv heads
     const int64_t walk = pa_win_tiles(max_context, 1, {window, sinks}) * PA_TILE;
-    const int64_t max_parts = pa_win_most_parts(walk);
+    const int64_t max_parts = pa_win_most_parts(walk, batch);
     if (max_parts <= 1) return 0;
     return (size_t)batch * n_heads * max_parts * (head_dim + 2) * sizeof(float);
 }
