@@ -192,6 +192,8 @@ def rope_and_cache(query, key, value, cos, sin, key_cache, value_cache, slot_map
 def check_window(window, sinks):
     """(window, sinks) as the library takes them, window 0 = none.  A query at position p sees the tokens j <= p with
     j > p - window (``window`` tokens with its own) or j < sinks."""
+    if type(window) is int and type(sinks) is int and 0 < window <= 0x7fffffff and 0 <= sinks <= 0x7fffffff:
+        return window, sinks
     if window is None:
         _need(sinks == 0, "sinks go with a window")
         return 0, 0
@@ -891,9 +893,9 @@ def beam_search_select(logits, beam_scores, eos_token_id=-1, n_candidates=None):
     g, k = beam_scores.shape
     _need(logits.dtype in _ACT or logits.dtype == torch.float32, "logits must be bf16, fp16 or fp32")
     if logits.dim() == 3:
-        _need(logits.shape[:2] == (g, k) and (logits.stride(0) == k * logits.stride(1) or g == 1),
+        _need(logits.shape[:2] == (g, k) and (logits.stride(0) == k * logits.stride(1) or g == 1 or k == 1),
               "logits must be [groups, beams, vocab] with evenly spaced rows")
-        v, stride = logits.shape[2], logits.stride(1)
+        v, stride = logits.shape[2], logits.stride(0 if k == 1 else 1)
     else:
         _need(logits.dim() == 2 and logits.shape[0] == g * k, "logits must hold a row for every beam")
         v, stride = logits.shape[1], logits.stride(0)
@@ -904,21 +906,20 @@ def beam_search_select(logits, beam_scores, eos_token_id=-1, n_candidates=None):
     eos = -1 if eos_token_id is None else int(eos_token_id)
     if not (1 <= k <= 64 and k * (2 if eos >= 0 else 1) <= n <= min(64, k * v)):
         raise ValueError(f"{n} candidates of {k} beams and {v} tokens: one a beam at least (two with an end token), 64 or all at most")
-    scores = torch.empty((g * (n + k),), dtype=torch.float32, device=dev)
-    ids = torch.empty((2 * g * (n + k),), dtype=torch.int32, device=dev)
     gn, gk = g * n, g * k
-    val, num = scores.as_strided, ids.as_strided              # half the time of a slice and a view
-    res = BeamSelection(val((g, n), (n, 1), 0), num((g, n), (n, 1), 0), num((g, n), (n, 1), gn), val((g, k), (k, 1), gn),
-                        num((g, k), (k, 1), 2 * gn), num((g, k), (k, 1), 2 * gn + gk))
+    ids = torch.empty(3 * (gn + gk), dtype=torch.int32, device=dev)
+    val, num = ids.view(torch.float32).as_strided, ids.as_strided        # half the time of a slice and a view
+    all_n, all_k, row_n, row_k = (g, n), (g, k), (n, 1), (k, 1)
+    res = BeamSelection(val(all_n, row_n, 0), num(all_n, row_n, gn), num(all_n, row_n, 2 * gn), val(all_k, row_k, 3 * gn),
+                        num(all_k, row_k, 3 * gn + gk), num(all_k, row_k, 3 * gn + 2 * gk))
     if g == 0:
         return res
     code = dtype_code(logits.dtype)
     ws = _scratch(lib.mf_beam_search_workspace_bytes(g, k, v, n, code), dev, "beam")
-    a, i = scores.data_ptr(), ids.data_ptr()
+    a, b = ids.data_ptr(), ids.data_ptr() + 12 * gn
     with _on(dev):
-        check(lib.mf_beam_search_select(a, i, i + 4 * gn, a + 4 * gn, i + 8 * gn, i + 8 * gn + 4 * gk, ptr(logits), stride,
-                                        ptr(beam_scores), g, k, v, n, eos, code, ptr(ws), ws.numel(), stream_ptr(dev)),
-              "mf_beam_search_select")
+        check(lib.mf_beam_search_select(a, a + 4 * gn, a + 8 * gn, b, b + 4 * gk, b + 8 * gk, ptr(logits), stride, ptr(beam_scores), g, k,
+                                        v, n, eos, code, ptr(ws), ws.numel(), stream_ptr(dev)), "mf_beam_search_select")
     return res
 
 

@@ -96,6 +96,20 @@ def test_selection_reads_a_slice_of_wider_rows(dtype, off):
     _select(wide[:, off:off + 4000], -torch.rand(2, 3, generator=gen).cuda(), eos=7)
 
 
+def test_selection_of_the_last_rows_of_sequences():
+    """Logits [groups, beams, vocab] that are slices: one beam a group with the rows of a longer step between, and beams of one group."""
+    wide = torch.randn(5, 7, 301, device="cuda")
+    scores = torch.randn(5, 1, device="cuda")
+    from mindformers_amd import ops
+    for got, want in zip(ops.beam_search_select(wide[:, -1:], scores), ops.beam_search_select(wide[:, -1].contiguous(), scores)):
+        assert torch.equal(got, want)
+    for got, want in zip(ops.beam_search_select(wide[2:3, ::2], scores[:4].view(1, 4)), ops.beam_search_select(wide[2, ::2].contiguous(), scores[:4].view(1, 4))):
+        assert torch.equal(got, want)
+    for bad in (wide[:, ::3], wide.transpose(1, 2)[:, :1], wide[:1, :1].expand(5, 1, 301)):
+        with pytest.raises(ValueError):
+            ops.beam_search_select(bad, torch.zeros(5, bad.shape[1], device="cuda"))
+
+
 def test_selection_orders_candidates_that_float32_sums_would_not():
     """Two beams whose scores differ by 2e-8 only: the order hangs on the last bits of the logsums."""
     logits, _ = _beams(1, 2, 50001, torch.float32, seed=3, std=1.0)
