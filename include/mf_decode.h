@@ -93,7 +93,7 @@ int mf_swap_blocks(void* host_cache, void* device_cache, const int64_t* pairs, i
  *     not mark, handed out row by row: in a row the copied open block first.  Where they, or the table's width, do not suffice, the
  *     entries stay -1 and *missing counts them.
  * Distinct rows must not share an open block in `tables` unless one is copied from the other by this call.  num_blocks <= 2^20, rows <= 4096;
- * workspace: mf_fork_blocks_workspace_bytes. */
+ * workspace: mf_fork_blocks_workspace_bytes, 16-byte aligned. */
 size_t mf_fork_blocks_workspace_bytes(int rows, int width, int num_blocks, int block_size, int new_tokens);
 int mf_fork_blocks(int32_t* tables_out, int32_t* lens_out, int32_t* slots, int32_t* copies, int32_t* missing,
                    const int32_t* tables, const int32_t* lens, const int32_t* parents, const uint8_t* held, int rows, int width,
