@@ -387,60 +387,81 @@ __global__ __launch_bounds__(256) void compact_remap_kernel(int32_t* __restrict_
 }
 
 // Block copies within the cache tensors of all layers in one launch.  The list is on the device and may be longer than
-// what is used of it (it ends at the first negative source), so the workgroups look for its end and take (copy, tensor, piece) in
-// turn.  Bound: memory.  24 open blocks of 64 caches, 420 MB read and written: 91 us (4.6 TB/s; the library's copy of 200 MiB reaches 5.4),
-// 96 through the caches with 32 KB pieces on 2048 workgroups; 192 whole blocks of 16 caches, 1.6 GB: 296 us (5.4 TB/s).
+// what is used of it (it ends at the first negative source, whatever lies behind that).  The workgroups take (copy, tensor, piece) in
+// turn, stop at a negative source of their own, and store nothing before they have seen that none lies in front of their entry; those
+// reads go beside the block's.  Bound: memory.
 constexpr int COPY_TENSORS = 128;
 constexpr int COPY_PIECE = 16384;                             // bytes of a block that a workgroup copies at a time
 constexpr int COPY_THREADS = 256;
+// Lists of up to this many entries go to as many as 16384 workgroups, longer ones, of which every workgroup reads the entries in front of its
+// own, to 2048.  us on 2048 | 16384 | 65536, used of listed copies: 24 of 512 in 64 caches, blocks of 256 KB 152 | 146 | 163, 192 of 512 in 16
+// caches 312 | 299 | 299 (5.4 TB/s; the library's copy of 200 MiB reaches 5.4), 3000 of 4096 in 8 2513 | 2476 | 2423, 30000 of 60000 in 2, blocks of
+// 32 KB 803 | 797 | 1222, of 2 KB 112 | 247 | 437, 250000 of 500000 of these 892 | 2245 | 7080.
+constexpr int COPY_SHORT = 4096;
 struct CopyTensors {
     uint8_t* base[COPY_TENSORS];
     uint32_t row_bytes[COPY_TENSORS];
 };
+// Whether one of the entries [from, to), from < to, has a negative source.  Up to COPY_ALONE of them are read by every wave for itself,
+// without a barrier; more by the workgroup, a wave every fourth 64.  from and to are the workgroup's.
+constexpr int COPY_WAVES = COPY_THREADS / 64;
+constexpr int COPY_ALONE = 512;
+__device__ __forceinline__ bool copies_end(const int32_t* __restrict__ copies, int from, int to) {
+    const int lane = threadIdx.x & 63;
+    const bool alone = to - from <= COPY_ALONE;
+    const int64_t step = alone ? 64 : 64 * COPY_WAVES;
+    int any = 0;
+    for (int64_t n0 = from + lane + (alone ? 0 : 64 * (threadIdx.x >> 6)); n0 - lane < to; n0 += 4 * step) {
+        int src[4];                                           // four reads on their way at a time
+#pragma unroll
+        for (int k = 0; k < 4; ++k) src[k] = copies[3 * min(n0 + k * step, (int64_t)to - 1)];
+        any |= src[0] | src[1] | src[2] | src[3];
+    }
+    return alone ? __ballot(any < 0) != 0 : __syncthreads_or(any < 0);
+}
 __global__ __launch_bounds__(COPY_THREADS) void copy_blocks_kernel(CopyTensors t, const int32_t* __restrict__ copies, int most,
                                                                    int tensors, int pieces, int num_blocks, int block_size) {
-    const int lane = threadIdx.x & 63;
-    int n = 0, end = most;                                    // copies in use: the list's leading entries; between n and end of them
-    while (n < end) {
-        const int step = (end - n + 63) / 64;
-        const int64_t at = n + (int64_t)lane * step;
-        const int used = __popcll(__ballot(at < end && copies[3 * at] >= 0));      // of the probes, one a lane
-        if (!used) break;
-        n += (used - 1) * step + 1;
-        end = min(end, n - 1 + step);
-    }
-    const int64_t items = (int64_t)n * tensors * pieces;
+    int seen = 0;                                             // no negative source in front of this entry
+    const int64_t items = (int64_t)most * tensors * pieces;
     for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
         const int piece = (int)(it % pieces);
         const int64_t ct = it / pieces;
         const int x = (int)(ct % tensors);
         const int c = (int)(ct / tensors);
-        const int src = copies[3 * c], dst = copies[3 * c + 1];
-        const int rows = min(max(copies[3 * c + 2], 0), block_size);
+        const int32_t* e = copies + 3 * (int64_t)c;
+        const int src = e[0], dst = e[1];
+        if (src < 0) return;                                  // the end, or behind it: this workgroup's later entries are too
+        const int rows = min(max(e[2], 0), block_size);
         if (src >= num_blocks || dst < 0 || dst >= num_blocks || src == dst) continue;
         const int64_t block_bytes = (int64_t)block_size * t.row_bytes[x];
         const int64_t from = (int64_t)piece * COPY_PIECE;
         const int64_t to = min((int64_t)rows * t.row_bytes[x], from + COPY_PIECE);
         const uint8_t* s = t.base[x] + src * block_bytes;
         uint8_t* d = t.base[x] + dst * block_bytes;
-        int64_t i = from;
-        if ((((uintptr_t)s | (uintptr_t)d) & 15) == 0) {
-            const int64_t end = to & ~(int64_t)15;
-            constexpr int STEP = COPY_THREADS * 16;
-            i += threadIdx.x * 16;
-            for (; i + 3 * STEP < end; i += 4 * STEP) {
-                u32x4 v[4];                                   // past the caches: neither side is read again soon
+        const bool wide = (((uintptr_t)s | (uintptr_t)d) & 15) == 0;
+        const int64_t end = wide ? max(to & ~(int64_t)15, from) : from;        // 16 bytes at a time as far as there
+        constexpr int STEP = COPY_THREADS * 16;
+        int64_t i = from + threadIdx.x * 16;
+        u32x4 v[4];                                           // past the caches: neither side is read again soon
+        const bool ahead = i + 3 * STEP < end;
+        if (ahead) {                                          // on their way while the list is looked through
 #pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = __builtin_nontemporal_load((const u32x4*)(s + i + k * STEP));
-#pragma unroll
-                for (int k = 0; k < 4; ++k) __builtin_nontemporal_store(v[k], (u32x4*)(d + i + k * STEP));
-            }
-            for (; i < end; i += STEP) *(u32x4*)(d + i) = *(const u32x4*)(s + i);
-            i = max(end, from);
+            for (int k = 0; k < 4; ++k) v[k] = __builtin_nontemporal_load((const u32x4*)(s + i + k * STEP));
         }
-        for (i += threadIdx.x; i < to; i += COPY_THREADS) d[i] = s[i];
+        if (c > seen) {
+            if (copies_end(copies, seen, c)) return;
+            seen = c;
+        }
+        if (ahead) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) __builtin_nontemporal_store(v[k], (u32x4*)(d + i + k * STEP));
+            i += 4 * STEP;
+        }
+        for (; i < end; i += STEP) *(u32x4*)(d + i) = *(const u32x4*)(s + i);
+        for (i = end + threadIdx.x; i < to; i += COPY_THREADS) d[i] = s[i];
     }
 }
+static_assert(COPY_PIECE == 4 * 16 * COPY_THREADS, "a piece is what the workgroup reads at once");
 
 template <typename K>
 int set_lds(K kern, size_t bytes, bool (&done)[MF_MAX_DEVICES]) {
@@ -567,8 +588,9 @@ extern "C" int mf_copy_blocks(void* const* host_caches, const int32_t* host_row_
         }
         const int pieces = (int)((block + COPY_PIECE - 1) / COPY_PIECE);
         const int64_t items = (int64_t)n_copies * n * pieces;
-        hipLaunchKernelGGL(copy_blocks_kernel, dim3((unsigned)std::min<int64_t>(items, 65536)), dim3(COPY_THREADS), 0, st, t, copies,
-                           n_copies, n, pieces, num_blocks, block_size);
+        const int64_t grid = std::min<int64_t>(items, n_copies <= COPY_SHORT ? 16384 : 2048);
+        hipLaunchKernelGGL(copy_blocks_kernel, dim3((unsigned)grid), dim3(COPY_THREADS), 0, st, t, copies, n_copies, n, pieces,
+                           num_blocks, block_size);
         const int rc = MF_LAUNCH_CHECK();
         if (rc) return rc;
     }

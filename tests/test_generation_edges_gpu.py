@@ -1,0 +1,54 @@
+"""Calls of the generation-side operators at the edges of what their documentation allows."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _i32(a):
+    return torch.from_numpy(np.ascontiguousarray(a).astype(np.int32)).cuda()
+
+
+# --------------------------------------------------------------------------------------------- lists of copies
+def _copy(entries, blocks, block=8, row=(2, 32), dtype=torch.float16):
+    """Runs a device list and holds it to the list taken entry by entry up to the first negative source."""
+    from mindformers_amd import ops
+    caches = [torch.randint(-100, 100, (blocks, block) + row, device="cuda").to(dtype) for _ in range(3)]
+    want = [c.clone() for c in caches]
+    for s, d, r in np.asarray(entries).tolist():
+        if s < 0:
+            break
+        if s < blocks and 0 <= d < blocks:
+            for c in want:
+                c[d, :max(0, min(r, block))] = c[s, :max(0, min(r, block))]
+    ops.copy_blocks(caches, _i32(entries))
+    assert all(torch.equal(c, w) for c, w in zip(caches, want))
+
+
+@pytest.mark.parametrize("entries", [
+    [[5, 6, 8], [-1, 3, 8], [7, 9, 8]], [[5, 6, 8], [-1, -1, 0], [7, 9, 8], [8, 10, 8]], [[-1, 5, 8], [0, 1, 8]], [[-7, 5, 8]],
+    [[0, 1, 8], [2, 3, 8], [-1, 4, 8], [5, 6, 8]], [[0, 1, 8], [99, 3, 8], [4, 99, 8], [5, 6, 8], [-1, 7, 8]], [[0, 1, 8]] + [[-1, 2, 8], [3, 4, 8]] * 9])
+def test_a_list_of_copies_ends_at_its_first_negative_source(entries):
+    """Whatever lies behind it, a valid destination of its own included."""
+    _copy(entries, 12)
+    _copy(entries, 12, block=8, row=(3,), dtype=torch.int8)   # rows that are no multiple of 16 bytes
+
+
+@pytest.mark.parametrize("n", [64, 65, 200, 513, 2049, 4096, 5000, 9000])
+def test_long_lists_of_copies_with_holes(n):
+    """Several lists one behind the other, and single negative sources anywhere in a full one: at the ends of what a lane, a wave and a
+    workgroup read at a time, where 16384 workgroups take the entries and where 2048 do."""
+    rng = np.random.default_rng(n)
+    perm = rng.permutation(2 * n)
+    full = np.stack([perm[:n], perm[n:], rng.integers(1, 3, n)], axis=1)
+    _copy(full, 2 * n, block=2, row=(16,))
+    for hole in sorted({0, 1, 63, 64, 65, 255, 256, 511, 512, 513, 2047, 2048, 4095, n - 2, n - 1, int(rng.integers(n))}):
+        if hole < n:
+            entries = full.copy()
+            entries[hole, 0] = -1 - hole % 2                  # its destination stays
+            _copy(entries, 2 * n, block=2, row=(16,))
+    parts = full.copy()
+    parts[n // 3:n // 2] = (-1, -1, 0)
+    parts[2 * n // 3:] = (-1, -1, 0)
+    _copy(parts, 2 * n, block=2, row=(16,))
