@@ -48,21 +48,27 @@ class BeamSearch:
             raise ValueError(f"block_tables, context_lens and logits must hold a row for each of {b} prompts")
         self.groups = b
         self.block_tables = tables.repeat_interleave(k, dim=0)
-        # every beam starts as its prompt's row; only the first is in the search, and all children go on from it
+        # every beam starts as its prompt's row; only the first is in the search
         self.context_lens = lens.reshape(-1).repeat_interleave(k)
         self.scores = torch.full((b, k), -torch.inf, dtype=torch.float32, device=dev)
         self.scores[:, 0] = 0.0
         self._missing = torch.zeros(1, dtype=torch.int32, device=dev)
         self._out = None                                      # rows of groups that were released
         self._steps = []
-        return self.step(logits.repeat_interleave(k, dim=0))
+        # All rows go on from it, those too whose candidate is of a beam that is out (a vocabulary of no more than K words has no K others): the
+        # rows of a prompt share its open block, so that it has to have one lowest child.
+        first = torch.arange(0, b * k, k, dtype=torch.int32, device=dev).repeat_interleave(k)
+        return self._step(logits.repeat_interleave(k, dim=0), first)
 
     def step(self, logits):
         """From the logits [B * K, vocab] of the beams' last tokens to the next tokens, int32 [B * K]; block_tables, context_lens and
         slot_mapping then describe the model's step that reads them."""
         self._started()
+        return self._step(logits)
+
+    def _step(self, logits, parents=None):
         sel = ops.beam_search_select(logits, self.scores, eos_token_id=self.eos_token_id)
-        parents = sel.next_rows.view(-1)
+        parents = sel.next_rows.view(-1) if parents is None else parents
         if self._out is not None:
             parents = torch.where(self._out, -1, parents)
         fork = ops.fork_blocks(self.block_tables, self.context_lens, self.num_blocks, self.block_size, parents=parents, new_tokens=1,

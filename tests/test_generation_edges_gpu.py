@@ -52,3 +52,45 @@ def test_long_lists_of_copies_with_holes(n):
     parts[n // 3:n // 2] = (-1, -1, 0)
     parts[2 * n // 3:] = (-1, -1, 0)
     _copy(parts, 2 * n, block=2, row=(16,))
+
+
+# --------------------------------------------------------------------------------------------- beam search
+@pytest.mark.parametrize("vocab,beams,eos", [(2, 2, 1), (3, 4, -1), (4, 4, 2), (5, 4, 0), (2, 3, -1), (33, 32, 4)])
+def test_beams_of_a_small_vocabulary_share_no_open_block(vocab, beams, eos):
+    """No more words than beams: the first step goes on from beams that are out too.  Every row's cache holds the tokens of its own
+    line of beams, whatever the others write."""
+    from mindformers_amd.modules import BeamSearch
+    rng = np.random.default_rng(vocab)
+    lens, bs, width = [5, 8, 1], 4, 8
+    blocks = 3 * beams * width + 10
+    caches = [torch.zeros(blocks, bs, 1, 8, dtype=torch.int32, device="cuda") for _ in range(2)]
+    tables = np.full((3, width), -1)
+    perm = iter(rng.permutation(blocks).tolist())
+    hist = []
+    for g, n in enumerate(lens):
+        for j in range(-(-n // bs)):
+            tables[g, j] = next(perm)
+        for t in range(n):
+            for c in caches:
+                c[int(tables[g, t // bs]), t % bs] = -1 - 100 * g - t
+        hist += [[-1 - 100 * g - t for t in range(n)]] * beams
+    logits = lambda rows: torch.from_numpy(rng.normal(0, 1, (rows, vocab)).astype(np.float32)).cuda()  # noqa: E731
+    search = BeamSearch(caches, beams, eos_token_id=eos)
+    search.start(tables, np.array(lens), logits(3))
+    for step in range(6):
+        if step:
+            search.step(logits(3 * beams))
+            hist = [hist[p] for p in search._steps[-1].next_rows.view(-1).tolist()]
+        slots = search.slot_mapping.tolist()
+        assert min(slots) >= 0 and len(set(slots)) == len(slots), f"step {step}"
+        for r, s in enumerate(slots):
+            for c in caches:
+                c.view(-1, 8)[s] = 1000 * step + r + 1
+            hist[r] = hist[r] + [1000 * step + r + 1]
+        t, n = search.block_tables.tolist(), search.context_lens.tolist()
+        held = [c.view(-1, 8).cpu().numpy() for c in caches]
+        for r in range(3 * beams):
+            assert n[r] == len(hist[r])
+            for h in held:
+                got = h[[t[r][p // bs] * bs + p % bs for p in range(n[r])]]
+                assert (got == np.array(hist[r])[:, None]).all(), f"step {step}, row {r}"
