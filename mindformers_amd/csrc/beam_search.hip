@@ -275,8 +275,9 @@ __global__ __launch_bounds__(BS_WAVES * 64) void beam_partial_kernel(const void*
 #pragma unroll
             for (int k = 0; k < E / 4; ++k) mx4[k] = mx4[k] == INFINITY ? 3.402823466e38f : mx4[k];
         }
-        // ---- the sum: the reference of a lane moves when a logit would leave the range of a double
-        const bool moves = mx > -INFINITY && (!has || mx > ref + 600.f);
+        // ---- the sum: the reference of a lane moves when a logit would leave the range of a double.  (Their difference: the sum ref + 600
+        // may round up to a logit that is a step of 1024 away.)
+        const bool moves = mx > -INFINITY && (!has || mx - ref > 600.f);
         if (__ballot(moves)) {
             if (moves) {
                 sum = has ? sum * exp_sum((double)ref - (double)mx) : 0.0;

@@ -3,6 +3,8 @@ import numpy as np
 import pytest
 import torch
 
+from test_generation_gpu import _select
+
 pytestmark = pytest.mark.gpu
 
 
@@ -94,3 +96,21 @@ def test_beams_of_a_small_vocabulary_share_no_open_block(vocab, beams, eos):
             for h in held:
                 got = h[[t[r][p // bs] * bs + p % bs for p in range(n[r])]]
                 assert (got == np.array(hist[r])[:, None]).all(), f"step {step}, row {r}"
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("power", [24, 30, 32, 33, 34, 36, 60, 127])
+def test_selection_of_logits_whose_neighbours_are_far_apart(sign, power):
+    """Float32 logits a few of their steps apart, the larger one in a later step of the same lane: what lies between is more than
+    the reference's reach, less than it, or just at it."""
+    v, n = 70001, 8                                           # a wave walks 2048 columns, 1024 at a time
+    ulp = 2.0 ** (power - 23)
+    logits = torch.full((6, v), -3.0e38 if sign < 0 else 0.0, device="cuda")
+    base = sign * 2.0 ** power - (16 * ulp if sign < 0 else 0)
+    for r, k in enumerate((1, 2, 3)):
+        logits[r, 5] = base
+        logits[r, 1024 + 5] = base + k * ulp
+        logits[r, 2048 + 9] = base - 5 * ulp
+    logits[3:] = torch.randn(3, v, device="cuda") * 2.5
+    _select(logits, torch.tensor([[-1.0, -1.5], [-2.0, -1.0], [-0.5, -20.0]], device="cuda"), n=n, eos=5)
+    _select(logits[[0, 3, 1, 4, 2, 5]].contiguous(), torch.full((3, 2), -1.0, device="cuda"), n=n)
