@@ -776,7 +776,7 @@ def fork_blocks(block_tables, context_lens, num_blocks, block_size, parents=None
             if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.dim() == 1 and t.numel() == s and t.is_contiguous()):
                 raise ValueError(f"{name} must be a contiguous int32 [{s}]")
             _need(t.device == dev, "all tensors must be on the same device")
-    _need(block_size > 0 and new_tokens >= 0, "block_size must be positive, new_tokens not negative")
+    _need(0 < block_size <= 0x7fffffff and 0 <= new_tokens <= 0x7fffffff, "block_size must be positive, new_tokens not negative")
     window, sinks = check_window(window, sinks)
     out = torch.empty(s * (m + new_tokens + 4) + 1, dtype=torch.int32, device=dev)
     a, b, c, d = s * m, s * (m + 1), s * (m + 4), s * (m + 4) + 1
@@ -798,7 +798,7 @@ def compact_blocks(block_tables, num_blocks, block_size, held=None):
     copies are made; blocks that the new tables do not name are free, blocks held by others stay where they are."""
     lib = _lib.load()
     dev = _table_args(block_tables, num_blocks, held)
-    _need(block_size > 0, "block_size must be positive")
+    _need(0 < block_size <= 0x7fffffff, "block_size must be positive")
     s, m = block_tables.shape
     most = num_blocks // 2
     out = torch.empty(s * m + 3 * most + 1, dtype=torch.int32, device=dev)
@@ -903,7 +903,7 @@ def beam_search_select(logits, beam_scores, eos_token_id=-1, n_candidates=None):
         stride = v                                            # one row: whatever its stride says
     _need(v > 0 and (logits.stride(-1) == 1 or v == 1) and stride >= v, "logits rows must have a unit column stride and not overlap")
     n = 2 * k if n_candidates is None else int(n_candidates)
-    eos = -1 if eos_token_id is None else int(eos_token_id)
+    eos = -1 if eos_token_id is None else min(max(int(eos_token_id), -1), 0x7fffffff)      # no token is that large
     if not (1 <= k <= 64 and k * (2 if eos >= 0 else 1) <= n <= min(64, k * v)):
         raise ValueError(f"{n} candidates of {k} beams and {v} tokens: one a beam at least (two with an end token), 64 or all at most")
     gn, gk = g * n, g * k

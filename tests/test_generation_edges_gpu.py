@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_generation_gpu import _select
+from test_generation_gpu import _beams, _select
 
 pytestmark = pytest.mark.gpu
 
@@ -114,3 +114,21 @@ def test_selection_of_logits_whose_neighbours_are_far_apart(sign, power):
     logits[3:] = torch.randn(3, v, device="cuda") * 2.5
     _select(logits, torch.tensor([[-1.0, -1.5], [-2.0, -1.0], [-0.5, -20.0]], device="cuda"), n=n, eos=5)
     _select(logits[[0, 3, 1, 4, 2, 5]].contiguous(), torch.full((3, 2), -1.0, device="cuda"), n=n)
+
+
+def test_an_end_token_outside_the_vocabulary_ends_nothing():
+    from mindformers_amd import ops
+    logits, scores = _beams(2, 3, 50, torch.float32, seed=2)
+    want = ops.beam_search_select(logits, scores)
+    for eos in (50, 2 ** 31 - 1, 2 ** 31 + 5, 2 ** 32 + int(want.tokens[0, 0]), -1, -2 ** 32 + int(want.tokens[0, 0]), -2 ** 40):
+        for have, w in zip(ops.beam_search_select(logits, scores, eos_token_id=eos), want):
+            assert torch.equal(have, w), eos
+
+
+def test_sizes_that_pass_32_bits_are_refused():
+    from mindformers_amd import ops
+    t, n = _i32(np.zeros((2, 3))), _i32([4, 5])
+    for call in (lambda: ops.fork_blocks(t, n, 8, 2 ** 32 + 16), lambda: ops.fork_blocks(t, n, 8, 16, new_tokens=2 ** 32 + 1),
+                 lambda: ops.compact_blocks(t, 8, 2 ** 32 + 16), lambda: ops.fork_blocks(t, n, 2 ** 32 + 8, 16)):
+        with pytest.raises(ValueError):
+            call()
