@@ -80,10 +80,13 @@ def rows_of(x, width):
     return x if x.dim() == 2 and x.shape[1] == width else x.reshape(-1, width)
 
 
-def workspace(nbytes, device, tag="default"):
+def workspace(nbytes, device, tag="default", capturing=None):
     """A cached scratch buffer per (device, stream, purpose), grown on demand and never shrunk.  Two streams never
     share one (their kernels would race on the partial sums), and a buffer that is outgrown is kept alive rather than
-    freed: a captured HIP graph may still replay into its address."""
+    freed.  Inside a stream capture (``capturing``: what ``is_current_stream_capturing`` says, where the caller has asked) a
+    buffer of its own, in the graph's memory: two graphs are captured on one stream and may be replayed at once on others."""
+    if torch.cuda.is_current_stream_capturing() if capturing is None else capturing:
+        return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
     key = (device, stream_ptr(device), tag)
     buf = _workspaces.get(key)
     if buf is None or buf.numel() < nbytes:
@@ -93,14 +96,6 @@ def workspace(nbytes, device, tag="default"):
         buf = torch.empty(size, dtype=torch.uint8, device=device)
         _workspaces[key] = buf
     return buf
-
-
-def _scratch(nbytes, device, tag):
-    """``workspace``, but a buffer of its own inside a stream capture: graphs that are replayed at once must not share one, and this
-    one belongs to the graph's memory."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
-    return workspace(nbytes, device, tag)
 
 
 # --------------------------------------------------------------------------------------------- KV cache
@@ -259,7 +254,7 @@ def _window_decode(lib, dev, out, quant, query, key_cache, value_cache, key_scal
     nb, bs, _, d = key_cache.shape
     b, max_blocks = block_tables.shape
     need = lib.mf_window_attention_workspace_bytes(b, n_heads, d, max_blocks * bs, window, sinks)
-    ws = _scratch(need, dev, "pa") if need else None
+    ws = workspace(need, dev, "pa") if need else None
     smooth, tiled = quant if quant is not None else (None, False)
     xq = xs = None
     if quant is not None:
@@ -287,7 +282,7 @@ def _window_prefill(lib, dev, out, query, key, value, key_scale, value_scale, kv
     nb, bs, max_blocks = (key.shape[0], key.shape[1], block_tables.shape[1]) if block_tables is not None else (0, 0, 0)
     need = lib.mf_window_attention_prefill_workspace_bytes(b, total_q, n_heads, n_kv_heads, d,
                                                            max_blocks * bs if block_tables is not None else total_q, window, sinks)
-    ws = _scratch(need, dev, "pa_prefill") if need else None
+    ws = workspace(need, dev, "pa_prefill") if need else None
     with _on(dev):
         check(lib.mf_window_attention_prefill(
             ptr(out), ptr(query), ptr(key), ptr(value), ptr(key_scale), ptr(value_scale), kvq, ptr(block_tables), ptr(context_lens),
@@ -784,7 +779,7 @@ def fork_blocks(block_tables, context_lens, num_blocks, block_size, parents=None
     res = ForkedBlocks(part((s, m), (m, 1), 0), part((s,), (1,), a), part((s * new_tokens,), (1,), d), part((s, 3), (3, 1), b),
                        part((1,), (1,), c))
     need = lib.mf_fork_blocks_workspace_bytes(s, m, num_blocks, block_size, new_tokens)
-    ws = _scratch(need, dev, "fork")
+    ws = workspace(need, dev, "fork")
     at = out.data_ptr()
     with _on(dev):
         check(lib.mf_fork_blocks(at, at + 4 * a, at + 4 * d, at + 4 * b, at + 4 * c, ptr(block_tables), ptr(context_lens), ptr(parents),
@@ -804,7 +799,7 @@ def compact_blocks(block_tables, num_blocks, block_size, held=None):
     out = torch.empty(s * m + 3 * most + 1, dtype=torch.int32, device=dev)
     part = out.as_strided
     tables, copies, live = part((s, m), (m, 1), 0), part((most, 3), (3, 1), s * m), part((1,), (1,), s * m + 3 * most)
-    ws = _scratch(lib.mf_compact_blocks_workspace_bytes(num_blocks), dev, "compact")
+    ws = workspace(lib.mf_compact_blocks_workspace_bytes(num_blocks), dev, "compact")
     with _on(dev):
         check(lib.mf_compact_blocks(ptr(tables), ptr(copies), ptr(live), ptr(block_tables), ptr(held), s, m, num_blocks, block_size,
                                     ptr(ws), ws.numel(), stream_ptr(dev)), "mf_compact_blocks")
@@ -915,7 +910,7 @@ def beam_search_select(logits, beam_scores, eos_token_id=-1, n_candidates=None):
     if g == 0:
         return res
     code = dtype_code(logits.dtype)
-    ws = _scratch(lib.mf_beam_search_workspace_bytes(g, k, v, n, code), dev, "beam")
+    ws = workspace(lib.mf_beam_search_workspace_bytes(g, k, v, n, code), dev, "beam")
     a, b = ids.data_ptr(), ids.data_ptr() + 12 * gn
     with _on(dev):
         check(lib.mf_beam_search_select(a, a + 4 * gn, a + 8 * gn, b, b + 4 * gk, b + 8 * gk, ptr(logits), stride, ptr(beam_scores), g, k,
@@ -1682,11 +1677,12 @@ def decode_layer_step(x, normed, attn_norm, ffn_norm, next_norm, weights, qkv_bi
     device = x.device
     sizes = (rows, hidden, n_heads, n_kv, d, ffn)
     need = lib.mf_decode_layer_workspace_bytes(*sizes)
-    ws = workspace(need, device, "gemm") if need else None
+    capturing = torch.cuda.is_current_stream_capturing()
+    ws = workspace(need, device, "gemm", capturing) if need else None
     window, sinks = check_window(window, sinks)
     need = lib.mf_window_attention_workspace_bytes(rows, n_heads, d, tables.shape[1] * bs, window, sinks) if window else \
         lib.mf_paged_attention_workspace_bytes(rows, n_heads, d, tables.shape[1] * bs)
-    pws = workspace(need, device, "pa") if need else None
+    pws = workspace(need, device, "pa", capturing) if need else None
     scratch_bytes = lib.mf_decode_layer_scratch_bytes(*sizes)
     scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=device)
     out = torch.empty_like(x)

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_generation_gpu import _beams, _select
+from test_generation_gpu import _beams, _select, _stack
 
 pytestmark = pytest.mark.gpu
 
@@ -132,3 +132,55 @@ def test_sizes_that_pass_32_bits_are_refused():
                  lambda: ops.compact_blocks(t, 8, 2 ** 32 + 16), lambda: ops.fork_blocks(t, n, 2 ** 32 + 8, 16)):
         with pytest.raises(ValueError):
             call()
+
+# --------------------------------------------------------------------------------------------- captures
+def test_a_capture_takes_workspaces_of_its_own():
+    from mindformers_amd import ops
+    dev = torch.device("cuda", torch.cuda.current_device())
+    eager = ops.workspace(1 << 20, dev, "gemm")
+    graphs, got = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for g in graphs:
+        with torch.cuda.graph(g):
+            got.append([ops.workspace(1 << 20, dev, tag).fill_(1) for tag in ("gemm", "pa")])
+    places = [eager.data_ptr()] + [w.data_ptr() for ws in got for w in ws]
+    assert all(abs(a - b) >= 1 << 20 for i, a in enumerate(places) for b in places[:i])
+    assert ops.workspace(1 << 20, dev, "gemm") is eager
+
+
+@pytest.mark.parametrize("act_quant", [False, True])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (900, 4)])
+def test_steps_of_a_stack_replayed_at_once_share_no_workspace(window, sinks, act_quant):
+    """Two captured decode steps of the serving runner, whose attention and products are cut, replayed together on two streams."""
+    from mindformers_amd.runner import DecodeStackRunner
+    layers, bs, rows, width = _stack(window, sinks, act_quant), 16, 5, 100
+    runs = [DecodeStackRunner(layers, npu_mem_size=0.05, cpu_mem_size=0, block_size=bs) for _ in range(2)]
+    assert runs[0].npu_num_blocks >= rows * width
+    gen = torch.Generator(device="cuda")
+    steps = []
+    for i, run in enumerate(runs):
+        gen.manual_seed(i)
+        for c in run.caches():
+            c.normal_(generator=gen)
+        n = torch.randint(1000, width * bs, (rows,), generator=gen, device="cuda").int()
+        tables = torch.randperm(rows * width, generator=gen, device="cuda").int().view(rows, width)
+        slots = (torch.gather(tables, 1, ((n - 1) // bs)[:, None].long())[:, 0] * bs + (n - 1) % bs).int()
+        steps.append((torch.randn(rows, 512, generator=gen, device="cuda").bfloat16(), n, tables, slots))
+    want = [run.decode(*s).clone() for run, s in zip(runs, steps)]
+    torch.cuda.synchronize()
+    graphs, got = [], []
+    for run, s in zip(runs, steps):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            for _ in range(4):                                # the same step again: the token's row is written anew each time
+                out = run.decode(*s)
+        got.append(out)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(30):
+        for out in got:
+            out.zero_()
+        for g, st in zip(graphs, streams):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
