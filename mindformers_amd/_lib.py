@@ -114,6 +114,7 @@ SIGNATURES = {
     "mf_decode_layer_scratch_bytes": (_Z, [_I] * 6),
     "mf_decode_layer_workspace_bytes": (_Z, [_I] * 6),
     "mf_decode_layer_step": (_I, [ctypes.c_char_p]),
+    "mf_decode_layer_step_window": (_I, [ctypes.c_char_p, _I, _I]),
     "mf_moe_unpermute": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P]),
 }
 
@@ -124,7 +125,7 @@ DECODE_LAYER_FIELDS = {
           "context_lens", "out", "norm_out", "scratch", "workspace", "attn_workspace", "stream"),
     "q": ("rows", "hidden", "n_heads", "n_kv_heads", "head_dim", "ffn", "block_size", "num_blocks", "max_blocks", "dtype",
           "table_dtype", "attn_gamma_dtype", "ffn_gamma_dtype", "next_gamma_dtype", "scratch_bytes", "workspace_bytes",
-          "attn_workspace_bytes", "window", "sinks"),
+          "attn_workspace_bytes"),
     "d": ("eps", "next_eps", "scale"),
 }
 DECODE_LAYER_ARGS = struct.Struct("@" + "".join(f"{len(names)}{kind}" for kind, names in DECODE_LAYER_FIELDS.items()))

@@ -42,7 +42,13 @@ extern "C" size_t mf_decode_layer_workspace_bytes(int rows, int hidden, int n_he
     return need;
 }
 
-extern "C" int mf_decode_layer_step(const mf_decode_layer_args* a) {
+extern "C" int mf_decode_layer_step(const mf_decode_layer_args* a) { return mf_decode_layer_step_window(a, 0, 0); }
+
+extern "C" int mf_decode_layer_step_window(const mf_decode_layer_args* a, int window, int sinks) {
+    if (window < 0 || sinks < 0 || (window == 0 && sinks)) {
+        mf_set_error("decode_layer_step: window %d, sinks %d", window, sinks);
+        return 1;
+    }
     if (!a || !a->scratch || !a->out) {
         mf_set_error("decode_layer_step: null argument");
         return 1;
@@ -70,15 +76,11 @@ extern "C" int mf_decode_layer_step(const mf_decode_layer_args* a) {
                                           a->value_cache, a->slot_mapping, rows, nh, nkv, d, a->num_blocks * a->block_size, hidden,
                                           dtype, (int)a->table_dtype, ws, wsb, st)))
         return rc;
-    if (a->window < 0 || a->window > 0x7fffffff || a->sinks < 0 || a->sinks > 0x7fffffff) {
-        mf_set_error("decode_layer_step: window %lld, sinks %lld", (long long)a->window, (long long)a->sinks);
-        return 1;
-    }
-    if (a->window)
+    if (window)
         rc = mf_window_attention_decode(attn, nullptr, nullptr, nullptr, 0, qkv, a->key_cache, a->value_cache, nullptr, nullptr, 0,
                                         a->block_tables, a->context_lens, rows, nh, nkv, d, (int)a->block_size, (int)a->max_blocks,
-                                        (int)a->num_blocks, (float)a->scale, (int)a->window, (int)a->sinks,
-                                        (int64_t)(nh + 2 * nkv) * d, dtype, a->attn_workspace, (size_t)a->attn_workspace_bytes, st);
+                                        (int)a->num_blocks, (float)a->scale, window, sinks, (int64_t)(nh + 2 * nkv) * d, dtype,
+                                        a->attn_workspace, (size_t)a->attn_workspace_bytes, st);
     else
         rc = mf_paged_attention_decode(attn, qkv, a->key_cache, a->value_cache, a->block_tables, a->context_lens, rows, nh, nkv, d,
                                        (int)a->block_size, (int)a->max_blocks, (int)a->num_blocks, (float)a->scale,

@@ -1698,8 +1698,8 @@ def decode_layer_step(x, normed, attn_norm, ffn_norm, next_norm, weights, qkv_bi
         rows, hidden, n_heads, n_kv, d, ffn, bs, nb, tables.shape[1],
         dtype_code(dt), dtype_code(cos.dtype), dtype_code(attn_norm.dtype), dtype_code(ffn_norm.dtype),
         0 if gamma is None else dtype_code(gamma.dtype), scratch_bytes, 0 if ws is None else ws.numel(),
-        0 if pws is None else pws.numel(), window, sinks, float(eps), float(next_eps), float(scale))
-    check(lib.mf_decode_layer_step(args), "mf_decode_layer_step")
+        0 if pws is None else pws.numel(), float(eps), float(next_eps), float(scale))
+    check(lib.mf_decode_layer_step_window(args, window, sinks), "mf_decode_layer_step_window")
     return out, norm_out
 
 
