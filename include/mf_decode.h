@@ -187,9 +187,9 @@ int mf_paged_attention_decode_static(void* out, const void* query, const void* k
  * with its own) or j < sinks, at their own positions.  FlashAttentionScore's band (sparse_mode 4, pre_tokens = window - 1,
  * mindformers/parallel_core/inference/transformer/flash_attention.py:96-104) plus the first tokens, which keep the softmax's weight
  * where training put it.  Entries of the block table whose block holds no visible token are not read (-1 where the block was given
- * back), nor are the cache rows of hidden tokens.  kv_quant: 0 = 16-bit caches, 1 = int8 with key_scale = antiquant_scale
- * [2, n_kv * D] and value_scale = antiquant_offset (may be NULL), 2 = int8 with one key and one value scale per slot.  xq (may be
- * NULL; 16-bit caches), x_scale, smooth, xq_layout: as mf_paged_attention_decode_dynamic_quant. */
+ * back), nor are the cache rows of hidden tokens.  A table may name 2^30 tokens a sequence.  kv_quant: 0 = 16-bit caches, 1 = int8
+ * with key_scale = antiquant_scale [2, n_kv * D] and value_scale = antiquant_offset (may be NULL), 2 = int8 with one key and one
+ * value scale per slot.  xq (may be NULL; 16-bit caches), x_scale, smooth, xq_layout: as mf_paged_attention_decode_dynamic_quant. */
 size_t mf_window_attention_workspace_bytes(int batch, int n_heads, int head_dim, int max_context, int window, int sinks);
 int mf_window_attention_decode(void* out, int8_t* xq, float* x_scale, const float* smooth, int xq_layout, const void* query,
                                const void* key_cache, const void* value_cache, const float* key_scale,

@@ -162,6 +162,9 @@ static int pa_decode_entry(void* out, const void* query, const void* key_cache, 
                "paged_attention: head_dim %d not supported (32, 64, 128)", head_dim);
     MF_REQUIRE(block_size > 0 && max_blocks_per_seq > 0 && num_blocks > 0, "paged_attention: bad block geometry");
     MF_REQUIRE((int64_t)block_size * max_blocks_per_seq <= 0x7fffffffLL, "paged_attention: context capacity overflows int");
+    MF_REQUIRE(!win.window || (int64_t)block_size * max_blocks_per_seq <= PA_WIN_MAX_CTX,
+               "paged_attention: a block table of %lld tokens, with a window up to %lld are served",
+               (long long)block_size * max_blocks_per_seq, (long long)PA_WIN_MAX_CTX);
     if (q_row_stride <= 0) q_row_stride = (int64_t)n_heads * head_dim;
     MF_REQUIRE(q_row_stride >= (int64_t)n_heads * head_dim && q_row_stride % 8 == 0,
                "paged_attention: query row stride must be >= n_heads*head_dim and a multiple of 8 elements");

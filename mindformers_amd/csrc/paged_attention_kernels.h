@@ -53,6 +53,8 @@ struct PaSmem {
 struct PaWindow {
     int window, sinks;                                        // window 0: none
 };
+// Tokens that a block table may name with a window: a partition may be as long as the walk, and the two are added in 32 bits.
+constexpr int64_t PA_WIN_MAX_CTX = 1 << 30;
 struct PaWinRange {
     int lo, sv;                                               // first token of the first row's window; sinks in front of it
     int ns, w0, tiles;                                        // tiles with sinks, first tile of the windows, tiles of the walk

@@ -954,6 +954,9 @@ static int pa_prefill_entry(void* out, const void* query, const void* key_cache,
                "paged_attention_prefill: bad block geometry");
     MF_REQUIRE(contiguous || (int64_t)block_size * max_blocks_per_seq <= 0x7fffffffLL,
                "paged_attention_prefill: context capacity overflows int");
+    MF_REQUIRE(!win.window || (contiguous ? total_q : (int64_t)block_size * max_blocks_per_seq) <= PA_WIN_MAX_CTX,
+               "paged_attention_prefill: a context of %lld tokens, with a window up to %lld are served",
+               contiguous ? (long long)total_q : (long long)block_size * max_blocks_per_seq, (long long)PA_WIN_MAX_CTX);
     if (kv_row_stride <= 0) kv_row_stride = (int64_t)n_kv_heads * head_dim;
     MF_REQUIRE(kv_row_stride >= (int64_t)n_kv_heads * head_dim && kv_row_stride % 8 == 0,
                "paged_attention_prefill: key/value row stride must be >= n_kv_heads*head_dim and a multiple of 8");

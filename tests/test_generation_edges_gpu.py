@@ -184,3 +184,24 @@ def test_steps_of_a_stack_replayed_at_once_share_no_workspace(window, sinks, act
                 g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# --------------------------------------------------------------------------------------------- windowed attention
+def test_windows_over_the_widest_tables():
+    """Tables that name 2^30 tokens, walks of 40000: the same bits as behind tables that end with the context."""
+    from mindformers_amd import ops
+    bs, b, nh, nkv, d = 16384, 32, 8, 8, 32
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(1)
+    kc, vc = (torch.randn(3, bs, nkv, d, generator=gen, device="cuda").bfloat16() for _ in range(2))
+    narrow = torch.arange(3, dtype=torch.int32, device="cuda").repeat(b, 1)
+    wide = torch.full((b, (1 << 30) // bs), -1, dtype=torch.int32, device="cuda")
+    wide[:, :3] = narrow
+    n, starts = torch.randint(33000, 40001, (b,), generator=gen, device="cuda").int(), torch.arange(b + 1, device="cuda").int()
+    q = torch.randn(b, nh * d, generator=gen, device="cuda").bfloat16()
+    for window, sinks in ((2 ** 31 - 1, 0), (1 << 30, 3), (35000, 100)):
+        got, want = (ops.paged_attention(q, kc, vc, t, n, nh, nkv, 0.2, window=window, sinks=sinks) for t in (wide, narrow))
+        assert torch.equal(got, want) and got.float().abs().amax(1).min() > 0
+    rows = torch.randn(4 * b, nh * d, generator=gen, device="cuda").bfloat16()
+    got, want = (ops.paged_attention_prefill(rows, kc, vc, t, n, 4 * starts, nh, nkv, 0.2, window=300, sinks=3) for t in (wide, narrow))
+    assert torch.equal(got, want) and got.float().abs().amax(1).min() > 0

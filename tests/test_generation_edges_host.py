@@ -18,3 +18,18 @@ def test_the_decode_step_refuses_a_window_before_any_launch(window, sinks):
     assert lib.mf_decode_layer_step_window(args, window, sinks) == 1 and "window" in lib.mf_last_error().decode()
     for rc in (lib.mf_decode_layer_step_window(args, 4, 1), lib.mf_decode_layer_step(args)):
         assert rc == 1 and "null" in lib.mf_last_error().decode()
+
+
+def test_windows_over_tables_of_more_than_2_to_the_30_tokens_are_refused():
+    """The plan may take the whole walk as one partition, and walk and partition are added in 32 bits."""
+    from mindformers_amd import _lib
+    lib = _lib.load()
+    for block, width, ok in ((128, 1 << 23, True), (128, (1 << 23) + 1, False), (32768, 65535, False), (1, (1 << 30) + 1, False)):
+        # without a workspace: what is served is refused for that, further down
+        decode = [16, None, None, None, 0, 16, 16, 16, None, None, 0, 16, 16, 2, 8, 2, 64, block, width, 100, 0.125, 1 << 30, 4, 0, 0, None, 0, None]
+        prefill = [16, 16, 16, 16, None, None, 0, 16, 16, 16, 2, 40, 8, 2, 64, block, width, 100, 0.125, 1 << 30, 4, 0, 0, 0, None, 0, None]
+        for name, args in (("mf_window_attention_decode", decode), ("mf_window_attention_prefill", prefill)):
+            assert getattr(lib, name)(*args) == 1
+            assert ("workspace" if ok else "with a window") in lib.mf_last_error().decode(), lib.mf_last_error()
+    packed = [16, 16, 16, 16, None, None, 0, None, None, 16, 1, (1 << 30) + 1, 8, 2, 64, 0, 0, 0, 0.125, 1 << 30, 4, 0, 0, 0, None, 0, None]
+    assert lib.mf_window_attention_prefill(*packed) == 1 and "with a window" in lib.mf_last_error().decode()
