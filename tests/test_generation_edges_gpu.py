@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_generation_gpu import _beams, _select, _stack
+from test_generation_gpu import ACT, _beams, _hold, _np, _paged, _select, _stack
 
 pytestmark = pytest.mark.gpu
 
@@ -205,3 +205,159 @@ def test_windows_over_the_widest_tables():
     rows = torch.randn(4 * b, nh * d, generator=gen, device="cuda").bfloat16()
     got, want = (ops.paged_attention_prefill(rows, kc, vc, t, n, 4 * starts, nh, nkv, 0.2, window=300, sinks=3) for t in (wide, narrow))
     assert torch.equal(got, want) and got.float().abs().amax(1).min() > 0
+
+
+@pytest.mark.parametrize("dtype", ACT)
+@pytest.mark.parametrize("b,nh,nkv,hi,window", [(3, 8, 2, 40, 20), (5, 8, 2, 1500, 900), (70, 8, 2, 200, 64), (80, 4, 1, 1900, 1500), (131, 2, 1, 1900, 1500),
+                                                (16, 8, 2, 700, 513)])
+def test_tiled_codes_of_windowed_decode_equal_two_calls(dtype, b, nh, nkv, hi, window):
+    """The layout that the W8A8 layers take, of walks in one partition and in several, with whole 64 rows and without."""
+    from helpers import untile_int8
+    from mindformers_amd import ops
+    rng = np.random.default_rng(b)
+    lens = rng.integers(0, hi + 1, b)
+    q, cache, _, tables, _, _ = _paged(rng, dtype, lens, [1] * b, nh, nkv, 64, 16, window, 5)
+    dq, kc, vc = (torch.from_numpy(x).to(dtype).cuda() for x in (q, *cache))
+    k = nh * 64
+    for smooth in (None, torch.rand(k, device="cuda") + 0.5):
+        args = (dq, kc, vc, _i32(tables), _i32(lens), nh, nkv, 0.1)
+        want = ops.paged_attention(*args, window=window, sinks=5)
+        assert (want[torch.from_numpy(lens == 0).cuda()] == 0).all()
+        rows, scales = ops.dynamic_quant(want, smooth)
+        for tiled in (False, True):
+            out, xq, xs = ops.paged_attention(*args, quant=(smooth, tiled), window=window, sinks=5)
+            codes = untile_int8(xq.data.cpu().numpy(), b, k) if tiled else xq.cpu().numpy()
+            assert torch.equal(out, want) and torch.equal(xs, scales)
+            np.testing.assert_array_equal(codes, rows.cpu().numpy())
+
+
+@pytest.mark.parametrize("rows", [2, 5, 70])
+def test_a_w8a8_layer_behind_a_long_window_is_its_separate_operators(rows, monkeypatch):
+    """The walk is cut: the attention's partitions are joined by the kernel that quantises the row too."""
+    from mindformers_amd import ops
+    from mindformers_amd.decode_layer import QuantDecodeLayer
+    layer, = _stack(1500, 7, act_quant=True, n=1)
+    bs, width = 32, 60
+    kc, vc = (torch.randn(rows * width, bs, 2, 64, device="cuda").bfloat16() for _ in range(2))
+    tables = torch.randperm(rows * width, device="cuda").int().view(rows, width)
+    n = torch.randint(1, width * bs + 1, (rows,), device="cuda").int()
+    slots = (torch.gather(tables, 1, ((n - 1) // bs)[:, None].long())[:, 0] * bs + (n - 1) % bs).int()
+    x = torch.randn(rows, 512, device="cuda").bfloat16()
+    cos, sin = torch.ones(rows, 64, device="cuda").bfloat16(), torch.zeros(rows, 64, device="cuda").bfloat16()
+    got = layer(x, kc.clone(), vc.clone(), tables, n, slots, cos, sin)
+    calls, whole = [], ops.paged_attention
+
+    def in_two(*args, quant=None, **kw):
+        out = whole(*args, **kw)
+        calls.append(kw)
+        return out if quant is None else (out, *ops.dynamic_quant(out, quant[0], tiled=quant[1]))
+
+    monkeypatch.setattr(ops, "paged_attention", in_two)
+    want = QuantDecodeLayer.forward(layer, x, kc.clone(), vc.clone(), tables, n, slots, cos, sin)
+    assert calls == [dict(window=1500, sinks=7)]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype,size", [(torch.bfloat16, 2.0 ** 40), (torch.bfloat16, 2.0 ** -50), (torch.bfloat16, 2.0 ** 25), (torch.float16, 2.0 ** 15),
+                                        (torch.float16, 2.0 ** -24), (torch.bfloat16, 0.0), (torch.bfloat16, 2.0 ** -110)])
+@pytest.mark.parametrize("rows", [1, 20])
+@pytest.mark.parametrize("window,sinks", [(40, 0), (70, 1), (230, 3)])
+def test_int8_windows_with_large_and_small_queries_at_a_channels_own_tolerance(dtype, size, rows, window, sinks):
+    """One row a sequence in the decode form, more of them as chunks; the largest key of the queries' channel is the first token, which
+    the window leaves."""
+    from mindformers_amd import ops
+    rng = np.random.default_rng(rows)
+    lens, nh, nkv, d, block = [255, 254, 0, 255], 8, 2, 64, 16
+    q_lens = [rows, 1, rows if rows == 1 else 0, rows]
+    q = np.zeros((sum(q_lens), nh, d))
+    q[:, :, 5] = size
+    cache = rng.integers(-127, 128, (2, 64, block, nkv, d))
+    cache[0].reshape(4, 256, nkv, d)[..., 5] = 127 - np.minimum(np.arange(256), 254)[None, :, None]
+    keys, values = ([c.reshape(4, 256, nkv, d)[b, :n] / 128.0 for b, n in enumerate(lens)] for c in cache)
+    dq = torch.from_numpy(q.reshape(-1, nh * d)).to(dtype).cuda()
+    kc, vc = (torch.from_numpy(c).to(torch.int8).cuda() for c in cache)
+    starts = None if rows == 1 else _i32(np.concatenate([[0], np.cumsum(q_lens)]))
+    got = ops.paged_attention_int8kv(dq, kc, vc, _i32(np.arange(64).reshape(4, 16)), _i32(lens), torch.full((2, nkv * d), 1 / 128.0, device="cuda"),
+                                     None, nh, nkv, 0.125, q_starts=starts, window=window, sinks=sinks)
+    _hold(_np(got), (q.reshape(-1, nh * d), keys, values, lens, q_lens, nh, nkv, 0.125, window, sinks), dtype, f"size {size}", "channel")
+
+
+# Tolerance: as in the form without offsets, of the int8 values and of the offset, which is taken off their sum.
+@pytest.mark.parametrize("dtype", ACT)
+@pytest.mark.parametrize("q_lens", [[1, 1, 1, 1, 1], [1, 40, 7, 0, 200]])
+@pytest.mark.parametrize("nh,nkv,d,block", [(8, 2, 64, 16), (7, 1, 128, 128), (4, 4, 32, 12)])
+@pytest.mark.parametrize("window,sinks", [(5, 3), (300, 20)])
+def test_windows_over_int8_caches_with_offsets(dtype, q_lens, nh, nkv, d, block, window, sinks):
+    from helpers import assert_within
+    from mindformers_amd import ops
+    from oracle import generation as G
+    rng = np.random.default_rng(d)
+    lens = [1, 97, 300, 0, 1100]
+    q, cache, scales, tables, _, _ = _paged(rng, dtype, lens, q_lens, nh, nkv, d, block, window, sinks, "channel")
+    offset = rng.integers(-30, 31, (2, nkv * d)).astype(np.float32)
+    need = [-(-n // block) for n in lens]
+    raw, keys, values = [], [], []
+    for b, n in enumerate(lens):
+        k8, v8 = (c[np.maximum(tables[b, :need[b]], 0)].astype(np.float64).reshape(-1, nkv, d)[:n] for c in cache)
+        s, o = scales.reshape(2, nkv, d), offset.reshape(2, nkv, d)
+        keys.append((k8 - o[0]) * s[0])
+        values.append((v8 - o[1]) * s[1])
+        raw.append((np.abs(v8) + np.abs(o[1])) * s[1])
+    s, o = torch.from_numpy(scales).float().cuda(), torch.from_numpy(offset).cuda()
+    starts = None if max(q_lens) == 1 else _i32(np.concatenate([[0], np.cumsum(q_lens)]))
+    dq, (kc, vc) = torch.from_numpy(q).to(dtype).cuda(), (torch.from_numpy(c).to(torch.int8).cuda() for c in cache)
+    got = ops.paged_attention_int8kv(dq, kc, vc, _i32(tables), _i32(lens), s, o, nh, nkv, 1 / np.sqrt(d), q_starts=starts, window=window, sinks=sinks)
+    rest = (lens, q_lens, nh, nkv, 1 / np.sqrt(d), window, sinks)
+    extra = 2.0 ** -25 * G.window_attention(q, keys, raw, *rest, of="sum") + (2.0 ** -25 if dtype == torch.float16 else 0)
+    want = G.window_attention(q, keys, values, *rest)
+    assert_within(_np(got), want, G.window_attention(q, keys, raw, *rest, of="magnitude"), dtype, ulps=3.0, extra=extra, what="offsets")
+    if max(q_lens) == 1:
+        assert (got[3] == 0).all()
+
+
+@pytest.mark.parametrize("kind", ["16", "channel", "token"])
+def test_windowed_attention_repeats_itself_bit_for_bit(kind):
+    """Walks in one and in several partitions: the order in which waves arrive changes no sum."""
+    from mindformers_amd import ops
+    rng = np.random.default_rng(2)
+    lens = rng.integers(1, 2600, 20)
+    q, cache, scales, tables, _, _ = _paged(rng, torch.bfloat16, lens, [1] * 20, 8, 2, 128, 32, 1200, 4, kind, poison=False)
+    dq, (kc, vc) = torch.from_numpy(q).bfloat16().cuda(), (torch.from_numpy(c).to(torch.bfloat16 if kind == "16" else torch.int8).cuda() for c in cache)
+    t = _i32(tables)
+    few = torch.randn(int(min(lens[0], 9)) + 30, 1024, device="cuda").bfloat16()
+    lens[1] = max(lens[1], 30)
+    n, starts = _i32(lens), _i32(np.concatenate([[0, few.shape[0] - 30], np.full(19, few.shape[0])]))
+    s = None if scales is None else torch.from_numpy(scales).float().cuda()
+    par = dict(token_scales=(s[0].contiguous(), s[1].contiguous())) if kind == "token" else {}
+    view = dict(window=1200, sinks=4)
+
+    def calls():
+        if kind == "16":
+            return [ops.paged_attention(dq, kc, vc, t, n, 8, 2, 0.1, **view), ops.paged_attention_prefill(few, kc, vc, t, n, starts, 8, 2, 0.1, **view)]
+        return [ops.paged_attention_int8kv(x, kc, vc, t, n, None if par else s, None, 8, 2, 0.1, q_starts=st, **par, **view)
+                for x, st in ((dq, None), (few, starts))]
+
+    want = calls()
+    for _ in range(20):
+        for have, w in zip(calls(), want):
+            assert torch.equal(have, w)
+
+
+@pytest.mark.parametrize("blocks,rows", [(1 << 19, 3), ((1 << 19) - 128, 3), ((1 << 19) - 128 * 8, 248), ((1 << 19) + 1, 5)])
+def test_pools_whose_bitmap_is_64_kb(blocks, rows):
+    from mindformers_amd import ops
+    from oracle import generation as G
+    rng = np.random.default_rng(rows)
+    tables = rng.choice(blocks, (rows, 40), replace=False)
+    tables[0, :3] = (blocks - 1, 0, blocks - 2)
+    lens = rng.integers(1, 161, rows)
+    got = ops.fork_blocks(_i32(tables), _i32(lens), blocks, 4, new_tokens=3)
+    for have, w in zip(got, G.fork_blocks(tables, lens, blocks, 4, new_tokens=3)):
+        np.testing.assert_array_equal(have.cpu().numpy().reshape(np.shape(w)), w)
+    named = np.sort(np.unique(tables))
+    to = dict(zip(named[named >= len(named)].tolist(), np.setdiff1d(np.arange(len(named)), named).tolist()))
+    out, copies, live = ops.compact_blocks(_i32(tables), blocks, 4)
+    assert int(live) == len(named)
+    np.testing.assert_array_equal(out.cpu().numpy(), np.vectorize(lambda p: to.get(p, p))(tables))
+    np.testing.assert_array_equal(copies[:len(to)].cpu().numpy(), [(a, b, 4) for a, b in to.items()])
+    assert (copies[len(to):] == torch.tensor([-1, -1, 0], device="cuda")).all()
