@@ -11,9 +11,9 @@ class FlashAttention(nn.Module):
     """ReshapeAndCache, then FlashAttentionScore (prefill) or PagedAttention (decode; with q_seq_lens: several new
     tokens per sequence; with pa_mla_v_dim > 0: multi-latent decode over the single latent cache, whose prefill runs as
     ordinary attention on the up-projected keys and values).  Masks are causal: `attn_mask` is accepted for signature parity and taken to be the lower
-    triangle the reference's models build; sparse modes other than the causal default are not built.  ``window`` (None: the
-    whole context) / ``sinks``: a query sees its own and the window - 1 tokens in front of it, and the first ``sinks`` tokens
-    (not with multi-latent attention)."""
+    triangle the reference's models build; sparse modes other than the causal default are not built, and
+    `pre_tokens` is not read (a band asked for by them is warned of).  ``window`` (None: the whole context) / ``sinks``: a query sees its
+    own and the window - 1 tokens in front of it, and the first ``sinks`` tokens (not with multi-latent attention)."""
 
     window, sinks = None, 0
 
@@ -22,6 +22,7 @@ class FlashAttention(nn.Module):
                  pa_kv_head_num=None, pa_mla_v_dim=0, window=None, sinks=0):
         super().__init__()
         ops.check_window(window, sinks)
+        ops.check_band(pre_tokens, sparse_mode, window)
         if window is not None and pa_mla_v_dim > 0:
             raise NotImplementedError("a window over a latent cache is not built")
         self.window, self.sinks = window, sinks

@@ -39,8 +39,8 @@ class InferAttention(nn.Module):
     context length including the token written by this call.  Prefill (`is_first_iteration`): causal attention over
     this call's own keys; in the TH layout `batch_valid_length` (the lengths of the packed sequences, or their
     increasing row ends) is what the reference hands to FlashAttentionScore (infer_attention.py:459-461), in BSH
-    every batch row is a full sequence of S tokens.  Masks are causal; `attn_mask` is not read.  ``window`` / ``sinks``: as in
-    PagedAttentionMgr, for every form of the attention."""
+    every batch row is a full sequence of S tokens.  Masks are causal; `attn_mask`, `pre_tokens` and `sparse_mode` are not read (a band
+    asked for by them is warned of).  ``window`` / ``sinks``: as in PagedAttentionMgr, for every form of the attention."""
 
     def __init__(self, n_head, head_dim, n_kv_head, pa_n_head_split=None, pa_n_kv_head_split=None, keep_prob=1.0,
                  scale_value=1.0, pre_tokens=2147483647, next_tokens=2147483647, sparse_mode=0, block_size=16,
@@ -50,6 +50,7 @@ class InferAttention(nn.Module):
         super().__init__()
         if use_alibi_mask:
             raise NotImplementedError("alibi attention is not built")
+        ops.check_band(pre_tokens, sparse_mode, window)
         if keep_prob != 1.0:
             raise ValueError("keep_prob must be 1.0 for inference")
         self.n_head = n_head

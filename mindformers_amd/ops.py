@@ -7,6 +7,7 @@ the kernel on torch's current stream.  Nothing is computed in Python.
 import contextlib
 import ctypes
 import math
+import warnings
 from typing import NamedTuple
 
 import torch
@@ -195,6 +196,13 @@ def check_window(window, sinks):
     if not (0 < window < math.inf and int(window) == window and 0 <= sinks < math.inf and int(sinks) == sinks):
         raise ValueError(f"window must be a positive integer and sinks not negative, got {window!r} and {sinks!r}")
     return min(int(window), 0x7fffffff), min(int(sinks), 0x7fffffff)
+
+
+def check_band(pre_tokens, sparse_mode, window):
+    """Says so where a cell is asked for a band by the reference's arguments, which it does not read, and has no window."""
+    if window is None and sparse_mode in (0, 4) and (pre_tokens < 2147483647 or sparse_mode == 4):
+        warnings.warn(f"sparse_mode {sparse_mode} with pre_tokens {pre_tokens}: the attention is causal over the whole context; a band is "
+                      f"window=pre_tokens + 1", stacklevel=3)
 
 
 def paged_attention(query, key_cache, value_cache, block_tables, context_lens, n_heads, n_kv_heads, scale, out=None,

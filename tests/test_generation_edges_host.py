@@ -33,3 +33,18 @@ def test_windows_over_tables_of_more_than_2_to_the_30_tokens_are_refused():
             assert ("workspace" if ok else "with a window") in lib.mf_last_error().decode(), lib.mf_last_error()
     packed = [16, 16, 16, 16, None, None, 0, None, None, 16, 1, (1 << 30) + 1, 8, 2, 64, 0, 0, 0, 0.125, 1 << 30, 4, 0, 0, 0, None, 0, None]
     assert lib.mf_window_attention_prefill(*packed) == 1 and "with a window" in lib.mf_last_error().decode()
+
+
+def test_a_band_asked_for_by_the_reference_s_arguments_is_warned_of():
+    import warnings
+    from mindformers_amd.modules import FlashAttention, InferAttention
+    flash = lambda **kw: FlashAttention(2, 32, 2, **kw)  # noqa: E731
+    infer = lambda **kw: InferAttention(2, 32, 2, num_blocks=2, device="cpu", **kw)  # noqa: E731
+    for make in (flash, infer):
+        for band in (dict(sparse_mode=4), dict(pre_tokens=511), dict(pre_tokens=511, sparse_mode=4)):
+            with pytest.warns(UserWarning, match="window=pre_tokens"):
+                assert make(**band) is not None
+        with warnings.catch_warnings():
+            warnings.simplefilter("error")
+            for quiet in ({}, dict(window=512, pre_tokens=511, sparse_mode=4), dict(pre_tokens=511, sparse_mode=2), dict(sparse_mode=3)):
+                make(**quiet)
