@@ -4,7 +4,9 @@
 //
 // One pass over the logits: a wave walks a piece of one beam's row and keeps its n best logits (order within a beam needs no
 // normalisation) beside the row's running sum of exponentials; a second kernel, a workgroup a group of beams, joins the
-// sums, scores what the waves kept and ranks it.  Ties go to the lowest (beam, token).
+// sums, scores what the waves kept and ranks it.  Ties go to the lowest (beam, token), but tokens of one beam are told apart by
+// their logits throughout: where a logit is so large that the scores of the others are one number in float64, the waves could not
+// keep the lowest of these.
 //
 // The order of candidates of different beams hangs on the difference of two logsums, so sums and scores are held in 64
 // bits: with sums in float32 two candidates a few 1e-7 apart change places.  The vector unit runs float64 at the rate of
@@ -411,11 +413,13 @@ __global__ __launch_bounds__(BJ_THREADS) void beam_join_kernel(const float* __re
     __shared__ float s_run[BS_MAX_N];
     __shared__ double l_score[BJ_LIST];
     __shared__ int l_at[BJ_LIST];
+    __shared__ float l_x[BJ_LIST];
     __shared__ double best_score[BS_MAX_N];
     __shared__ int best_at[BS_MAX_N];
     __shared__ uint64_t w_key[BJ_WAVES];
     __shared__ uint32_t w_bound[BJ_WAVES];
     __shared__ int w_at[BJ_WAVES];
+    __shared__ float w_x[BJ_WAVES];
     __shared__ int s_count;
     const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int per_beam = chunks * n, all = beams * per_beam;
@@ -489,24 +493,25 @@ __global__ __launch_bounds__(BJ_THREADS) void beam_join_kernel(const float* __re
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < BJ_WAVES; ++i) t = max(t, w_bound[i]);
-    auto keep = [&](double s, int at) {
+    auto keep = [&](double s, float x, int at) {
         if (order32((float)s + 0.f) >= t) {
             const int p = atomicAdd(&s_count, 1);
             if (p < BJ_LIST) {
                 l_score[p] = s;
                 l_at[p] = at;
+                l_x[p] = x;
             }
         }
     };
     if constexpr (HELD) {
 #pragma unroll
         for (int c = 0; c < BJ_HELD; ++c)
-            if (ha[c] >= 0) keep(hs[c], ha[c]);
+            if (ha[c] >= 0) keep(hs[c], hx[c], ha[c]);
     } else {
         for (int i = tid; i < all; i += BJ_THREADS) {
             double s;
             const int at = candidate(i, s);
-            if (at >= 0) keep(s, at);
+            if (at >= 0) keep(s, cand_x[first + i], at);
         }
     }
     __syncthreads();
@@ -517,7 +522,14 @@ __global__ __launch_bounds__(BJ_THREADS) void beam_join_kernel(const float* __re
             const double s = l_score[i];
             const int at = l_at[i];
             int rank = 0;
-            for (int j = tid & 15; j < count; j += 16) rank += l_score[j] > s || (l_score[j] == s && l_at[j] < at);
+            for (int j = tid & 15; j < count; j += 16) {
+                rank += l_score[j] > s;
+                if (l_score[j] == s && j != i) {              // rare
+                    const int aj = l_at[j], bi = at / vocab, bj = aj / vocab;
+                    const float x = l_x[i], xj = l_x[j];
+                    rank += bj < bi || (bj == bi && (xj > x || (xj == x && aj < at)));
+                }
+            }
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) rank += __shfl_xor(rank, o, 64);
             if (rank < n) {                                   // (lanes of one entry, and those past the last, write the same)
@@ -527,47 +539,46 @@ __global__ __launch_bounds__(BJ_THREADS) void beam_join_kernel(const float* __re
         }
         __syncthreads();
     } else {                                                  // more ties than the list holds: one after the other
-        uint64_t last = ~0ull;
-        int last_at = -1;
+        struct Entry {
+            uint64_t k;
+            float x;
+            int at;
+        };
+        auto before = [&](const Entry& a, const Entry& b) -> bool {
+            if (a.k != b.k) return a.k > b.k;
+            const int ba = a.at / vocab, bb = b.at / vocab;
+            return ba != bb ? ba < bb : (a.x != b.x ? a.x > b.x : a.at < b.at);
+        };
+        Entry last = {~0ull, 0.f, 0};                         // no score has this key
         for (int r = 0; r < n; ++r) {
-            uint64_t k = 0;
-            int at = 0x7fffffff;
+            Entry top = {0, 0.f, 0x7fffffff};
             for (int i = tid; i < all; i += BJ_THREADS) {
                 double s;
                 const int c = candidate(i, s);
                 if (c < 0) continue;
-                const uint64_t ks = order64(s);
-                const bool after = ks < last || (ks == last && c > last_at);
-                if (after && (ks > k || (ks == k && c < at))) {
-                    k = ks;
-                    at = c;
-                }
+                const Entry e = {order64(s), cand_x[first + i], c};
+                if (before(last, e) && before(e, top)) top = e;
             }
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) {
-                const uint64_t ok = __shfl_xor((unsigned long long)k, o, 64);
-                const int oa = __shfl_xor(at, o, 64);
-                if (ok > k || (ok == k && oa < at)) {
-                    k = ok;
-                    at = oa;
-                }
+                const Entry e = {__shfl_xor((unsigned long long)top.k, o, 64), __shfl_xor(top.x, o, 64), __shfl_xor(top.at, o, 64)};
+                if (before(e, top)) top = e;
             }
             __syncthreads();
             if (lane == 0) {
-                w_key[w] = k;
-                w_at[w] = at;
+                w_key[w] = top.k;
+                w_x[w] = top.x;
+                w_at[w] = top.at;
             }
             __syncthreads();
-            for (int i = 0; i < BJ_WAVES; ++i)
-                if (w_key[i] > k || (w_key[i] == k && w_at[i] < at)) {
-                    k = w_key[i];
-                    at = w_at[i];
-                }
-            last = k;
-            last_at = at;
+            for (int i = 0; i < BJ_WAVES; ++i) {
+                const Entry e = {w_key[i], w_x[i], w_at[i]};
+                if (before(e, top)) top = e;
+            }
+            last = top;
             if (tid == 0) {
-                best_score[r] = __longlong_as_double((long long)((k >> 63) ? k ^ 0x8000000000000000ull : ~k));
-                best_at[r] = at;
+                best_score[r] = __longlong_as_double((long long)((top.k >> 63) ? top.k ^ 0x8000000000000000ull : ~top.k));
+                best_at[r] = top.at;
             }
         }
         __syncthreads();

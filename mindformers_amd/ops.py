@@ -885,10 +885,11 @@ class BeamSelection(NamedTuple):
 
 def beam_search_select(logits, beam_scores, eos_token_id=-1, n_candidates=None):
     """One step of beam search over B groups of K beams: the ``n_candidates`` (default 2 K) best of
-    beam_scores[b, k] + log_softmax(logits[b * K + k])[v] over (k, v), ties to the lowest k * vocab + v, and the first K of them
-    whose token is not ``eos_token_id`` (negative: no such token).  logits [B * K, vocab] or [B, K, vocab], bf16, fp16 or fp32,
-    may be a slice of wider rows; beam_scores fp32 [B, K].  NaN logits count as -inf; a beam whose score is -inf, NaN or beyond
-    +-1e30 is out of the search: its candidates score -inf."""
+    beam_scores[b, k] + log_softmax(logits[b * K + k])[v] over (k, v), ties to the lowest k * vocab + v (tokens of one beam by
+    their logits, where float64 tells their scores apart no longer), and the first K of them whose token is not ``eos_token_id``
+    (negative: no such token).  logits [B * K, vocab] or [B, K, vocab], bf16, fp16 or fp32, may be a slice of wider rows; beam_scores
+    fp32 [B, K].  NaN logits count as -inf, +inf as the largest float; a beam whose score is -inf, NaN or beyond +-1e30 is out of the
+    search: its candidates score -inf."""
     lib = _lib.load()
     dev = _dev_of(logits, beam_scores)
     _need(beam_scores.dtype == torch.float32 and beam_scores.dim() == 2 and beam_scores.is_contiguous(),

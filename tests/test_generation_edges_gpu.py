@@ -116,6 +116,33 @@ def test_selection_of_logits_whose_neighbours_are_far_apart(sign, power):
     _select(logits[[0, 3, 1, 4, 2, 5]].contiguous(), torch.full((3, 2), -1.0, device="cuda"), n=n)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("b,k,v,n", [(2, 1, 16, 8), (1, 1, 25, 25), (3, 2, 39, 24), (2, 2, 5003, 20), (1, 1, 70001, 64), (1, 2, 70001, 64), (2, 40, 3001, 64)])
+def test_tokens_of_one_beam_whose_scores_are_one_number_go_by_their_logits(b, k, v, n, dtype):
+    """Beside +inf, and logits that vanish beside the largest one: equal scores in float64, up to more of them than the join's list
+    holds.  Order: score, beam, logit, token."""
+    from mindformers_amd import ops
+    logits, scores = _beams(b, k, v, dtype, seed=v)
+    if dtype == torch.float32:
+        logits[::2] *= 1e-25                                  # beside their largest, 3: one number
+        logits[::2, v // 2] = 3.0
+    else:
+        logits[0, v // 3] = float("inf")
+    logits[-1, v - 2] = float("inf")
+    logits[:, 3] = logits[:, 1]                               # equal logits too
+    got = ops.beam_search_select(logits, scores, n_candidates=n)
+    x = np.minimum(_np(logits).astype(np.float64), np.finfo(np.float32).max).reshape(b, k, v)
+    d = x - x.max(-1, keepdims=True)
+    total = _np(scores)[..., None] + (d - np.log(np.exp(d).sum(-1, keepdims=True)))
+    beam, token = (a.reshape(-1) for a in np.meshgrid(np.arange(k), np.arange(v), indexing="ij"))
+    for g in range(b):
+        order = np.lexsort((token, -x[g].reshape(-1), beam, -total[g].reshape(-1)))[:n]
+        np.testing.assert_array_equal(_np(got.beams[g]), beam[order])
+        np.testing.assert_array_equal(_np(got.tokens[g]), token[order])
+        want = total[g].reshape(-1)[order]
+        assert (np.abs(_np(got.scores[g]) - want) <= 2.0 ** -24 * np.abs(want) + 1.4e-10).all()
+
+
 def test_an_end_token_outside_the_vocabulary_ends_nothing():
     from mindformers_amd import ops
     logits, scores = _beams(2, 3, 50, torch.float32, seed=2)
