@@ -41,28 +41,39 @@ struct PaQuantArgs {
     int layout;
 };
 
-// Tokens a partition and partitions of a decode step with a window, over contexts of up to max_ctx tokens.  Walks are mostly of one
-// length, so there is no ragged tail to fill, and what counts is that every compute unit has the same number of workgroups: one, so
-// 256 workgroups over the device, and no combine where the sequences and kv heads alone are that many; two for int8 caches, whose
-// tiles have more to compute, but for a few sequences, where a cut costs more than it brings.  Partitions of 128 tokens at least, 384 from 64
-// workgroups on (a workgroup takes 8 us + 12.8 ns a token, a combine 3 to 4.5 us).  us with 768 workgroups of 256 (384) tokens at least | with this
-// plan, bf16 and int8, sequences through a window, 32/8 heads: 1 through 1024 11.4 | 10.3, 11.6 | 10.2; 2 through 4096 16.6 | 14.9, 15.1 |
-// 13.8; 4 through 2048 16.1 | 14.5, 14.3 | 13.6; 6 through 4096 27.2 | 24.1; 8 through 4096 29.2 | 29.1, 23.2 | 21.4; 12 through 2048 27.2 |
-// 25.3, 21.0 | 19.2; 24 through 1024 27.0 | 23.5, 21.0 | 21.9; 64 of 512 to 4096 tokens through 1024 with the plan of a full context 55.7 | 46.1,
-// 40.5 | 32.3.
+// Tokens a partition and partitions of a decode step with a window, over contexts of up to max_ctx tokens.  Walks through a window that
+// most contexts exceed are of one length: there is no ragged tail to fill, and what counts is that every compute unit has the same number of
+// workgroups: one, so 256 workgroups over the device, and no combine where the sequences and kv heads alone are that many; two for int8
+// caches, whose tiles have more to compute, but for a few sequences, where a cut costs more than it brings.  Partitions of 128 tokens at
+// least, 384 from 64 workgroups on (a workgroup takes 8 us + 12.8 ns a token, a combine 3 to 4.5 us).  us with 768 workgroups of 256 (384)
+// tokens at least | with this plan, bf16 and int8, sequences through a window, 32/8 heads: 1 through 1024 11.4 | 10.3, 11.6 | 10.2; 2 through
+// 4096 16.6 | 14.9, 15.1 | 13.8; 4 through 2048 16.1 | 14.5, 14.3 | 13.6; 6 through 4096 27.2 | 24.1; 8 through 4096 29.2 | 29.1, 23.2 |
+// 21.4; 12 through 2048 27.2 | 25.3, 21.0 | 19.2; 24 through 1024 27.0 | 23.5, 21.0 | 21.9 (the one that loses); 64 of 512 to 4096 tokens
+// through 1024 with the plan of a full context 55.7 | 46.1, 40.5 | 32.3.
+// A window that most contexts do not reach has walks as ragged as they are, and the longest would be walked alone: walks that may pass
+// PA_WIN_WHOLE tokens are cut into PA_WIN_CUT at most.  us uncut (256 workgroups) | cut, and without a window: one context of 32000 tokens
+// beside 31 of 500, window 32768, 354 | 43, 42, int8 387 | 36, 32; one of 8000 beside 31 of 500 through 8192 96 | 39, 24, int8 102 | 35, 18; 64
+// of 500 to 32000 539 | 319, 319, int8 398 | 178, 175.  Of one length: 64 through 8192 336 | 338, int8 191 | 187; 32 through 32768 650 |
+// 673, int8 439 | 367; 16 through 16384 163 | 178, int8 103 | 108; cut from 2048 on, 64 through 2048 89 | 101, int8 53 | 65.
 struct PaWinPlan {
     int part_tokens, max_parts;
 };
-static inline int64_t pa_win_most_parts(int64_t walk, int batch) {
-    return std::min<int64_t>((walk + PA_WAVE_TOKENS - 1) / PA_WAVE_TOKENS, std::max(1, 512 / batch));
+constexpr int64_t PA_WIN_WHOLE = 6144, PA_WIN_CUT = 2048;
+// ... and no more of them than 8192 (sequence, partition) pairs: what a table may hold sizes the workspace and the grid.
+static inline int64_t pa_win_cuts(int64_t walk, int batch) {
+    return walk <= PA_WIN_WHOLE ? 1 : std::min<int64_t>((walk + PA_WIN_CUT - 1) / PA_WIN_CUT, std::max(1, 8192 / batch));
 }
-static inline PaWinPlan pa_win_plan(int64_t max_ctx, int64_t batch_kv_groups, PaWindow win, bool int8) {
+static inline int64_t pa_win_most_parts(int64_t walk, int batch) {
+    return std::min<int64_t>((walk + PA_WAVE_TOKENS - 1) / PA_WAVE_TOKENS, std::max<int64_t>(pa_win_cuts(walk, batch), 512 / batch));
+}
+static inline PaWinPlan pa_win_plan(int64_t max_ctx, int batch, int64_t batch_kv_groups, PaWindow win, bool int8) {
     const int64_t walk = pa_win_tiles(max_ctx, 1, win) * PA_TILE;
-    int64_t part = walk;
+    const int64_t cuts = pa_win_cuts(walk, batch);
+    int64_t part = (walk + cuts - 1) / cuts;
     if (batch_kv_groups < 256) {
         const int64_t parts = std::max<int64_t>(1, (int8 && batch_kv_groups > 32 ? 512 : 256) / batch_kv_groups);
         const int64_t least = batch_kv_groups >= 64 ? 3 * PA_WAVE_TOKENS : PA_WAVE_TOKENS;
-        part = std::max(least, (walk + parts - 1) / parts);
+        part = std::min(part, std::max(least, (walk + parts - 1) / parts));
     }
     part = (part + PA_WAVE_TOKENS - 1) / PA_WAVE_TOKENS * PA_WAVE_TOKENS;
     return {(int)part, (int)((walk + part - 1) / part)};
@@ -78,7 +89,7 @@ int launch_pa(void* out, const void* query, const void* key_cache, const void* v
     const int64_t max_ctx = (int64_t)max_blocks * block_size;
     const int tpw = WIN ? 0 : pa_launch_tiles_per_wave(max_ctx, KVQ, (int64_t)batch * n_kv * head_groups);
     PaWinPlan plan = {tpw * PA_WAVE_TOKENS, 0};
-    if constexpr (WIN) plan = pa_win_plan(max_ctx, (int64_t)batch * n_kv * head_groups, win, KVQ != 0);
+    if constexpr (WIN) plan = pa_win_plan(max_ctx, batch, (int64_t)batch * n_kv * head_groups, win, KVQ != 0);
     const int part_tokens = plan.part_tokens;
     const int max_parts = WIN ? plan.max_parts : (int)((max_ctx + part_tokens - 1) / part_tokens);
     float* part_out = (float*)workspace;

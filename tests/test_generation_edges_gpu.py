@@ -215,23 +215,34 @@ def test_steps_of_a_stack_replayed_at_once_share_no_workspace(window, sinks, act
 
 # --------------------------------------------------------------------------------------------- windowed attention
 def test_windows_over_the_widest_tables():
-    """Tables that name 2^30 tokens, walks of 40000: the same bits as behind tables that end with the context."""
+    """Tables that name 2^30 tokens, walks of 40000, cut in other places than behind tables that end with the context: every query
+    finds its one key, whose probability is 1 in either."""
     from mindformers_amd import ops
-    bs, b, nh, nkv, d = 16384, 32, 8, 8, 32
+    bs, b, nh, d = 16384, 32, 8, 32
     gen = torch.Generator(device="cuda")
     gen.manual_seed(1)
-    kc, vc = (torch.randn(3, bs, nkv, d, generator=gen, device="cuda").bfloat16() for _ in range(2))
+    kc, vc = (torch.randn(3, bs, nh, d, generator=gen, device="cuda").bfloat16() for _ in range(2))
     narrow = torch.arange(3, dtype=torch.int32, device="cuda").repeat(b, 1)
     wide = torch.full((b, (1 << 30) // bs), -1, dtype=torch.int32, device="cuda")
     wide[:, :3] = narrow
     n, starts = torch.randint(33000, 40001, (b,), generator=gen, device="cuda").int(), torch.arange(b + 1, device="cuda").int()
-    q = torch.randn(b, nh * d, generator=gen, device="cuda").bfloat16()
-    for window, sinks in ((2 ** 31 - 1, 0), (1 << 30, 3), (35000, 100)):
-        got, want = (ops.paged_attention(q, kc, vc, t, n, nh, nkv, 0.2, window=window, sinks=sinks) for t in (wide, narrow))
-        assert torch.equal(got, want) and got.float().abs().amax(1).min() > 0
-    rows = torch.randn(4 * b, nh * d, generator=gen, device="cuda").bfloat16()
-    got, want = (ops.paged_attention_prefill(rows, kc, vc, t, n, 4 * starts, nh, nkv, 0.2, window=300, sinks=3) for t in (wide, narrow))
-    assert torch.equal(got, want) and got.float().abs().amax(1).min() > 0
+    q = torch.randn(4 * b, nh, d, generator=gen, device="cuda").bfloat16()
+    kc.mul_(0.01)
+
+    def plant(row, token):                                    # a score of about 0.2 * 32 * 32, the others' are below 2
+        kc.view(-1, nh, d)[token] = 32 * q[row]
+        return vc.view(-1, nh, d)[token].reshape(-1).clone()
+
+    for window, sinks in ((2 ** 31 - 1, 0), (1 << 30, 3), (35000, 5100)):
+        keep = kc.clone()
+        want = torch.stack([plant(i, int(n[i]) - 1 - 1031 * i) for i in range(b)])
+        for t in (wide, narrow):
+            assert torch.equal(ops.paged_attention(q[:b].reshape(b, -1), kc, vc, t, n, nh, nh, 0.2, window=window, sinks=sinks), want)
+        kc.copy_(keep)
+    n = torch.arange(33000, 33000 + 220 * b, 220, device="cuda").int()
+    want = torch.stack([plant(4 * i + j, int(n[i]) - 4 + j - 50 * j) for i in range(b) for j in range(4)])
+    for t in (wide, narrow):
+        assert torch.equal(ops.paged_attention_prefill(q.reshape(4 * b, -1), kc, vc, t, n, 4 * starts, nh, nh, 0.2, window=200, sinks=3), want)
 
 
 @pytest.mark.parametrize("dtype", ACT)
@@ -388,3 +399,39 @@ def test_pools_whose_bitmap_is_64_kb(blocks, rows):
     np.testing.assert_array_equal(out.cpu().numpy(), np.vectorize(lambda p: to.get(p, p))(tables))
     np.testing.assert_array_equal(copies[:len(to)].cpu().numpy(), [(a, b, 4) for a, b in to.items()])
     assert (copies[len(to):] == torch.tensor([-1, -1, 0], device="cuda")).all()
+
+
+@pytest.mark.parametrize("kind", ["16", "channel", "token"])
+@pytest.mark.parametrize("lens,window,sinks", [([9000, 7, 0, 2049] + [40] * 30, 8192, 5), ([6200, 6143, 6300], 6100, 40), ([9000] + [300] * 9, 2 ** 31 - 1, 0)])
+def test_long_windows_over_ragged_contexts_match_the_oracle(kind, lens, window, sinks):
+    """Walks that are cut however many sequences there are, and walks next to that length."""
+    from test_generation_gpu import _windowed
+    _windowed(torch.bfloat16, lens, [1] * len(lens), 8, 8, 32, 32, window, sinks, kind)
+
+
+@pytest.mark.parametrize("longest", [9000, 36000])
+def test_long_windows_with_quantised_output_equal_two_calls(longest):
+    """Five partitions, joined by the kernel that quantises, and eighteen, which it does not take; a workspace smaller than they need is
+    refused."""
+    from mindformers_amd import _lib, ops
+    bs, b, nh, nkv, d = 128, 40, 8, 8, 32
+    width = -(-longest // bs)
+    kc, vc = (torch.randn(width, bs, nkv, d, device="cuda").bfloat16() for _ in range(2))
+    tables = torch.stack([torch.randperm(width, device="cuda").int() for _ in range(b)])
+    n = torch.randint(1, 1000, (b,), device="cuda").int()
+    n[7] = longest
+    q = torch.randn(b, nh * d, device="cuda").bfloat16()
+    want = ops.paged_attention(q, kc, vc, tables, n, nh, nkv, 0.2, window=longest)
+    full = ops.paged_attention(q, kc, vc, tables, n, nh, nkv, 0.2)
+    assert (want.float() - full.float()).abs().max() <= 2 * 2.0 ** -8 * vc.float().abs().max()
+    for tiled in (False, True):
+        out, xq, xs = ops.paged_attention(q, kc, vc, tables, n, nh, nkv, 0.2, quant=(None, tiled), window=longest)
+        wq, ws = ops.dynamic_quant(want, None, tiled=tiled)
+        assert torch.equal(out, want) and torch.equal(xs, ws)
+        from helpers import untile_int8
+        codes = [untile_int8(x.data.cpu().numpy(), b, nh * d) if tiled else x.cpu().numpy() for x in (xq, wq)]
+        np.testing.assert_array_equal(*codes)
+    lib = _lib.load()
+    need = lib.mf_window_attention_workspace_bytes(b, nh, d, width * bs, longest, 0)
+    parts = -(-(width * bs) // 2048)
+    assert need >= b * nh * parts * (d + 2) * 4
