@@ -813,7 +813,10 @@ int launch_pf(void* out, const void* query, const void* key_cache, const void* v
     const bool contiguous = block_tables == nullptr;
     const int64_t max_ctx = contiguous ? total_q : (int64_t)max_blocks * block_size;
     const bool tib_tok = contiguous || block_size % PF_TOK == 0;       // a staged tile never straddles two blocks
-    // int8 caches with per-channel scales and a window take the 128-column kernel at any number of rows
+    // int8 caches with per-channel scales and a window have the 128-column kernel alone, at any number of rows: it wins from a few hundred
+    // rows on and loses below.  us of it | of the 16-column one, 32/8 heads behind 5000 tokens, windows of 512, 1024 and 4096: 8 rows 18 |
+    // 15, 18 | 15, 23 | 19; 64 rows 25 | 20, 27 | 24, 47 | 59; 128 rows 28 | 23, 42 | 38, 54 | 82; 300 rows 34 | 47, 38 | 74, 73 | 144; 64
+    // rows beside 24 decoding ones 44 | 28, 55 | 35, 106 | 60.  Per-token scales have the 16-column kernel, on the plan of full contexts.
     const bool cols16 = KVQ == 2 || (KVQ == 1 && !WIN && pf_cols16(pf_plan(batch, total_q, n_heads, n_kv, max_ctx), batch, n_kv, D, max_ctx));
     const int64_t walk = WIN ? pf_win_walk(max_ctx, cols16 ? 16 : PF_COLS, n_rep, win) : max_ctx;
     const PfPlan plan = WIN && KVQ != 2 ? pf_win_plan(batch, total_q, n_heads, n_kv, D, walk)
