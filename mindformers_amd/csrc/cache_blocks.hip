@@ -4,8 +4,8 @@
 //
 // What bounds the two planning operators is launch latency and one workgroup's walk over the tables: their answer hangs
 // on a ranking of all free blocks, which one workgroup forms from a bitmap in LDS (one bit a block, 128 KB for a million).  Under the
-// profiler 16 rows of 32 blocks in 1024 take 8 us in one launch, 512 rows of 256 in 131072 6.0 + 10.6 in two, closing up 64 rows of
-// 32 in 1024 8.4 + 3.0.
+// profiler 16 rows of 32 blocks in 1024 take 8 us in one launch, 512 rows of 256 in 131072 6.7 + 10.3 in two, closing up 64 rows of
+// 32 in 1024 9.3 + 4.5.
 #include <algorithm>
 
 #include "common.h"
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(256) void fork_gather_kernel(ForkArgs a) {
 __host__ __device__ __forceinline__ int fork_words(int num_blocks) { return (num_blocks + 127) / 128 * 4; }
 
 // The rows gathered and their blocks marked, each workgroup in a bitmap of its own that the assigning one joins.  512 rows of 256
-// entries: 6.0 us and 10.6 for the assigning workgroup; 3.4 and 16.0 where that one marks all entries (an LDS operation each).
+// entries: 6.7 us and 10.3 for the assigning workgroup; 3.4 and 16.0 where that one marks all entries (an LDS operation each).
 __global__ __launch_bounds__(CB_THREADS) void fork_mark_kernel(ForkArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint32_t bits[];
     const int words = fork_words(a.num_blocks), lane = threadIdx.x & 63;
@@ -393,10 +393,10 @@ __global__ __launch_bounds__(256) void compact_remap_kernel(int32_t* __restrict_
 constexpr int COPY_TENSORS = 128;
 constexpr int COPY_PIECE = 16384;                             // bytes of a block that a workgroup copies at a time
 constexpr int COPY_THREADS = 256;
-// Lists of up to this many entries go to as many as 16384 workgroups, longer ones, of which every workgroup reads the entries in front of its
-// own, to 2048.  us on 2048 | 16384 | 65536, used of listed copies: 24 of 512 in 64 caches, blocks of 256 KB 152 | 146 | 163, 192 of 512 in 16
-// caches 312 | 299 | 299 (5.4 TB/s; the library's copy of 200 MiB reaches 5.4), 3000 of 4096 in 8 2513 | 2476 | 2423, 30000 of 60000 in 2, blocks of
-// 32 KB 803 | 797 | 1222, of 2 KB 112 | 247 | 437, 250000 of 500000 of these 892 | 2245 | 7080.
+// Lists of up to this many entries go to as many as 32768 workgroups, longer ones, of which every workgroup reads the entries in front of its
+// own, to 2048.  us on 2048 | 16384 | 32768 | 65536, used of listed copies: 24 of 512 in 64 caches, blocks of 256 KB 152 | 143 | 144 | 161, 192 of
+// 512 in 16 caches 312 | 296 | 288 (5.6 TB/s; the library's copy of 200 MiB reaches 5.4) | 297, 3000 of 4096 in 8 2513 | 2472 | 2397 | 2443; on
+// 2048 | 16384 | 65536 30000 of 60000 in 2, blocks of 32 KB 809 | 797 | 1222, of 2 KB 116 | 247 | 437, 250000 of 500000 of these 926 | 2245 | 7080.
 constexpr int COPY_SHORT = 4096;
 struct CopyTensors {
     uint8_t* base[COPY_TENSORS];
@@ -411,11 +411,11 @@ __device__ __forceinline__ bool copies_end(const int32_t* __restrict__ copies, i
     const bool alone = to - from <= COPY_ALONE;
     const int64_t step = alone ? 64 : 64 * COPY_WAVES;
     int any = 0;
-    for (int64_t n0 = from + lane + (alone ? 0 : 64 * (threadIdx.x >> 6)); n0 - lane < to; n0 += 4 * step) {
-        int src[4];                                           // four reads on their way at a time
+    for (int64_t n0 = from + lane + (alone ? 0 : 64 * (threadIdx.x >> 6)); n0 - lane < to; n0 += 2 * step) {
+        int src[2];                                           // two reads on their way at a time: most entries have few in front
 #pragma unroll
-        for (int k = 0; k < 4; ++k) src[k] = copies[3 * min(n0 + k * step, (int64_t)to - 1)];
-        any |= src[0] | src[1] | src[2] | src[3];
+        for (int k = 0; k < 2; ++k) src[k] = copies[3 * min(n0 + k * step, (int64_t)to - 1)];
+        any |= src[0] | src[1];
     }
     return alone ? __ballot(any < 0) != 0 : __syncthreads_or(any < 0);
 }
@@ -588,7 +588,7 @@ extern "C" int mf_copy_blocks(void* const* host_caches, const int32_t* host_row_
         }
         const int pieces = (int)((block + COPY_PIECE - 1) / COPY_PIECE);
         const int64_t items = (int64_t)n_copies * n * pieces;
-        const int64_t grid = std::min<int64_t>(items, n_copies <= COPY_SHORT ? 16384 : 2048);
+        const int64_t grid = std::min<int64_t>(items, n_copies <= COPY_SHORT ? 32768 : 2048);
         hipLaunchKernelGGL(copy_blocks_kernel, dim3((unsigned)grid), dim3(COPY_THREADS), 0, st, t, copies, n_copies, n, pieces,
                            num_blocks, block_size);
         const int rc = MF_LAUNCH_CHECK();
