@@ -4,8 +4,8 @@
 //
 // What bounds the two planning operators is launch latency and one workgroup's walk over the tables: their answer hangs
 // on a ranking of all free blocks, which one workgroup forms from a bitmap in LDS (one bit a block, 128 KB for a million).  Under the
-// profiler 16 rows of 32 blocks in 1024 take 8 us in one launch, 512 rows of 256 in 131072 6.7 + 10.3 in two, closing up 64 rows of
-// 32 in 1024 9.3 + 4.5.
+// profiler 16 rows of 32 blocks in 1024 take 8 us in one launch, 512 rows of 256 in 131072 5.9 + 10.6 in two, closing up 64 rows of
+// 32 in 1024 9.0 + 4.5.
 #include <algorithm>
 
 #include "common.h"
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(256) void fork_gather_kernel(ForkArgs a) {
 __host__ __device__ __forceinline__ int fork_words(int num_blocks) { return (num_blocks + 127) / 128 * 4; }
 
 // The rows gathered and their blocks marked, each workgroup in a bitmap of its own that the assigning one joins.  512 rows of 256
-// entries: 6.7 us and 10.3 for the assigning workgroup; 3.4 and 16.0 where that one marks all entries (an LDS operation each).
+// entries: 5.9 us and 10.6 for the assigning workgroup; 3.4 and 16.0 where that one marks all entries (an LDS operation each).
 __global__ __launch_bounds__(CB_THREADS) void fork_mark_kernel(ForkArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint32_t bits[];
     const int words = fork_words(a.num_blocks), lane = threadIdx.x & 63;
