@@ -200,7 +200,8 @@ def check_window(window, sinks):
 
 def check_band(pre_tokens, sparse_mode, window):
     """Says so where a cell is asked for a band by the reference's arguments, which it does not read, and has no window."""
-    if window is None and sparse_mode in (0, 4) and (pre_tokens < 2147483647 or sparse_mode == 4):
+    short = pre_tokens is not None and pre_tokens < 2147483647
+    if window is None and sparse_mode in (0, 4) and (short or sparse_mode == 4):
         warnings.warn(f"sparse_mode {sparse_mode} with pre_tokens {pre_tokens}: the attention is causal over the whole context; a band is "
                       f"window=pre_tokens + 1", stacklevel=3)
 

@@ -46,5 +46,6 @@ def test_a_band_asked_for_by_the_reference_s_arguments_is_warned_of():
                 assert make(**band) is not None
         with warnings.catch_warnings():
             warnings.simplefilter("error")
-            for quiet in ({}, dict(window=512, pre_tokens=511, sparse_mode=4), dict(pre_tokens=511, sparse_mode=2), dict(sparse_mode=3)):
+            for quiet in ({}, dict(window=512, pre_tokens=511, sparse_mode=4), dict(pre_tokens=511, sparse_mode=2), dict(sparse_mode=3),
+                          dict(pre_tokens=None, sparse_mode=None), dict(pre_tokens=None)):
                 make(**quiet)
