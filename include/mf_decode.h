@@ -125,7 +125,7 @@ int mf_copy_blocks(void* const* host_caches, const int32_t* host_row_bytes, int 
  * next_tokens [groups, beams]: the first `beams` of them whose token is not eos (eos < 0: the first ones).  Scores are compared in
  * float64 (tokens of one beam by their logits) and rounded once.  A NaN logit counts as -inf, +inf as the largest float; a
  * beam whose running score is not in (-1e30, 1e30) is out: its candidates score -inf.  beams, n <= 64; n >= beams, with
- * eos >= 0 n >= 2 beams. */
+ * eos >= 0 n >= 2 beams; beams * vocab <= 0x7c000000 (2080374784). */
 size_t mf_beam_search_workspace_bytes(int groups, int beams, int vocab, int n, int dtype);
 int mf_beam_search_select(float* scores, int32_t* beam_ids, int32_t* tokens, float* next_scores, int32_t* next_rows,
                           int32_t* next_tokens, const void* logits, int64_t row_stride, const float* beam_scores, int groups,

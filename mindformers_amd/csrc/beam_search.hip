@@ -19,6 +19,7 @@ namespace {
 
 constexpr int BS_WAVES = 4;
 constexpr int BS_MAX_N = 64;                                  // candidates a group, beams a group
+constexpr int64_t BS_MAX_PLACES = 0x7c000000;                 // beams x vocabulary: a place, and a column a piece behind it, in 32 bits
 constexpr int BS_TAKE = 128;                                  // entries that a wave takes from a step
 constexpr int BS_GROW = 40;                                   // entries beyond the n best that a list may hold between two steps
 constexpr int BS_LIST = 256;                                  // entries of a wave's list: 64 + BS_GROW + BS_TAKE fit
@@ -649,7 +650,7 @@ extern "C" int mf_beam_search_select(float* scores, int32_t* beam_ids, int32_t* 
     MF_REQUIRE(n >= (eos >= 0 ? 2 : 1) * beams && (int64_t)n <= (int64_t)beams * vocab,
                "beam_search_select: %d candidates of %d beams x %d tokens: at least one a beam (two with an end token) and no more than there are",
                n, beams, vocab);
-    MF_REQUIRE((int64_t)groups * beams <= 65535 && (int64_t)beams * vocab <= 0x7fffffffLL, "beam_search_select: %d x %d beams of %d tokens",
+    MF_REQUIRE((int64_t)groups * beams <= 65535 && (int64_t)beams * vocab <= BS_MAX_PLACES, "beam_search_select: %d x %d beams of %d tokens",
                groups, beams, vocab);
     if (row_stride <= 0) row_stride = vocab;
     MF_REQUIRE(row_stride >= vocab, "beam_search_select: row stride %lld below the vocabulary's %d", (long long)row_stride, vocab);

@@ -906,6 +906,7 @@ def beam_search_select(logits, beam_scores, eos_token_id=-1, n_candidates=None):
         v, stride = logits.shape[1], logits.stride(0)
     if g * k == 1:
         stride = v                                            # one row: whatever its stride says
+    _need(v <= 0x7c000000, "a vocabulary of more than 0x7c000000 tokens")
     _need(v > 0 and (logits.stride(-1) == 1 or v == 1) and stride >= v, "logits rows must have a unit column stride and not overlap")
     n = 2 * k if n_candidates is None else int(n_candidates)
     eos = -1 if eos_token_id is None else min(max(int(eos_token_id), -1), 0x7fffffff)      # no token is that large

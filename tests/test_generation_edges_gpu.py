@@ -152,6 +152,22 @@ def test_an_end_token_outside_the_vocabulary_ends_nothing():
             assert torch.equal(have, w), eos
 
 
+def test_selection_from_the_longest_row():
+    """0x7c000000 logits of one beam: columns next to 2^31.  Zeros but for a few, so that the sum is a whole number of ones and these:
+    2^-24 for the result's rounding, 5.6e-11 of the exponential and 2^-53 an addition of a lane's 508000."""
+    from mindformers_amd import ops
+    v = 0x7c000000
+    logits = torch.zeros(1, v, dtype=torch.bfloat16, device="cuda")
+    places, values = [v - 1, 5, v - 70001, v // 2 + 1], [9.0, 8.0, 7.5, 7.0]
+    logits[0, torch.tensor(places, device="cuda")] = torch.tensor(values, device="cuda").bfloat16()
+    got = ops.beam_search_select(logits, torch.zeros(1, 1, device="cuda"), n_candidates=6)
+    assert got.tokens[0].tolist() == places + [0, 1]
+    want = np.array(values + [0.0, 0.0]) - np.log((v - 4) + np.exp(values).sum())
+    assert (np.abs(got.scores[0].cpu().numpy() - want) <= 2.0 ** -24 * np.abs(want) + 5.6e-11 + 508000 * 2.0 ** -53).all()
+    with pytest.raises(ValueError):
+        ops.beam_search_select(torch.empty(1, device="cuda").expand(1, v + 1), torch.zeros(1, 1, device="cuda"))
+
+
 def test_sizes_that_pass_32_bits_are_refused():
     from mindformers_amd import ops
     t, n = _i32(np.zeros((2, 3))), _i32([4, 5])

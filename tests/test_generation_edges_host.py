@@ -49,3 +49,13 @@ def test_a_band_asked_for_by_the_reference_s_arguments_is_warned_of():
             for quiet in ({}, dict(window=512, pre_tokens=511, sparse_mode=4), dict(pre_tokens=511, sparse_mode=2), dict(sparse_mode=3),
                           dict(pre_tokens=None, sparse_mode=None), dict(pre_tokens=None)):
                 make(**quiet)
+
+
+def test_vocabularies_whose_columns_pass_32_bits_are_refused():
+    """A wave's piece may end a 64th behind the row's end, and its next step behind that."""
+    from mindformers_amd import _lib
+    lib = _lib.load()
+    for beams, vocab, word in ((1, 0x7c000000, "workspace"), (1, 0x7c000001, "tokens"), (1, 0x7fffffff, "tokens"), (2, 0x3e000001, "tokens"),
+                               (62, 33554432, "workspace")):
+        args = [8] * 7 + [0, 8, 1, beams, vocab, beams, -1, 0, None, 0, None]
+        assert lib.mf_beam_search_select(*args) == 1 and word in lib.mf_last_error().decode(), lib.mf_last_error()
