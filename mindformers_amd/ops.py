@@ -828,8 +828,14 @@ def copy_blocks(caches, copies):
     dev = _dev_ok(first)
     index, shape, dtype = dev.index, first.shape, first.dtype
     nb, bs = shape[:2] if len(shape) >= 2 else (0, 0)
-    _need(nb > 0 and bs > 0 and first.numel() > 0, "caches must be [num_blocks, block_size, ...]")
-    row = first.numel() // (nb * bs) * first.element_size()
+    _need(0 < nb <= 0x7fffffff and bs > 0 and first.numel() > 0, "caches must be [num_blocks, block_size, ...]")
+
+    def row_bytes(c):
+        r = c.numel() // (nb * bs) * c.element_size()
+        _need(r * bs <= 0x7fffffff, "a block of 2 GiB or more")
+        return r
+
+    row = row_bytes(first)
     at, rows = [], []
     for c in caches:                                          # mostly alike: a few hundred nanoseconds each, of 64 or more
         if not (isinstance(c, torch.Tensor) and c.get_device() == index and c.is_contiguous()):
@@ -838,7 +844,7 @@ def copy_blocks(caches, copies):
             rows.append(row)
         else:
             _need(c.shape[:2] == shape[:2] and c.numel() > 0, "all caches must share num_blocks and block_size")
-            rows.append(c.numel() // (nb * bs) * c.element_size())
+            rows.append(row_bytes(c))
         at.append(c.data_ptr())
     if not (isinstance(copies, torch.Tensor) and copies.is_cuda):
         copies = _host_copies(copies, nb, bs)

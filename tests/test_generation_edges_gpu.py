@@ -176,6 +176,16 @@ def test_sizes_that_pass_32_bits_are_refused():
         with pytest.raises(ValueError):
             call()
 
+
+def test_copies_within_blocks_of_2_gib_and_more_are_refused():
+    from mindformers_amd import ops
+    small = torch.zeros(2, 1, 8, dtype=torch.int8, device="cuda")
+    for row in (2 ** 31, 2 ** 32 + 8):                        # the latter is 8 bytes in 32 bits
+        big = torch.empty(2, 1, row, dtype=torch.int8, device="cuda")
+        for caches in ([big], [small, big]):
+            with pytest.raises(ValueError, match="2 GiB"):
+                ops.copy_blocks(caches, [[0, 1]])
+
 # --------------------------------------------------------------------------------------------- captures
 def test_a_capture_takes_workspaces_of_its_own():
     from mindformers_amd import ops
