@@ -59,6 +59,19 @@ int mf_rope_half(void* query, void* key, const void* cos, const void* sin, int n
 int mf_rope_rows(void* cos, void* sin, const int32_t* positions, const float* inv_freq, int num_tokens, int head_dim,
                  int dtype, void* stream);
 
+/* Rotary positions of any layout and scaling, from the positions themselves: pairs (a, b) of the 2 n_pairs columns of every head from
+ * column `offset` on become scale * (a cos t - b sin t, b cos t + a sin t), t = positions[token] * inv_freq[pair] (radians, float64
+ * [n_pairs]); the other columns pass.  interleaved 0: a pair is columns (i, i + n_pairs) of the part, otherwise (2i, 2i + 1).  Angles
+ * in 64 bits, products in fp32, rounded once.  query, key, value: rows of n_heads / n_kv_heads / n_kv_heads x head_dim, *_row_stride
+ * elements apart (0 = dense).  query_out, key_out: where they go, the inputs themselves (in place) or memory of their own; key_out may
+ * be NULL, and without a key (n_kv_heads 0) so is key.  With caches (and value and slot_mapping) the key's and the value's rows also go
+ * to the cache rows slot_mapping names, as in mf_reshape_and_cache; slots outside [0, num_slots) are skipped. */
+int mf_rotary_embedding(void* query_out, void* key_out, const void* query, const void* key, const void* value, void* key_cache,
+                        void* value_cache, const int32_t* positions, const double* inv_freq, const int32_t* slot_mapping,
+                        int num_tokens, int n_heads, int n_kv_heads, int head_dim, int n_pairs, int offset, int interleaved,
+                        float scale, int64_t num_slots, int64_t q_row_stride, int64_t k_row_stride, int64_t v_row_stride,
+                        int64_t q_out_row_stride, int64_t k_out_row_stride, int dtype, void* stream);
+
 /* RoPE on q and k followed by the cache scatter of rotated k and of v, one launch (the sequence
  * infer_attention.py:445,453 performs).  q and k are rotated in place. */
 int mf_rope_and_cache(void* query, void* key, const void* value, const void* cos, const void* sin,
@@ -131,6 +144,40 @@ int mf_beam_search_select(float* scores, int32_t* beam_ids, int32_t* tokens, flo
                           int32_t* next_tokens, const void* logits, int64_t row_stride, const float* beam_scores, int groups,
                           int beams, int vocab, int n, int eos, int dtype, void* workspace, size_t workspace_bytes,
                           void* stream);
+
+/* ---- log probabilities ----------------------------------------------------------------------------------- */
+
+/* For every row of logits [rows, vocab] (dtype MF_BF16 / MF_FP16 / MF_FP32, rows row_stride elements apart, 0 = dense): the log
+ * probability of token tokens[row] under softmax, its rank (tokens with a larger logit, or the same and a lower place; 0: the most
+ * likely), the distribution's entropy (nats), and with n_top > 0 the n_top most likely tokens [rows, n_top] in that order with their
+ * log probabilities.  A NaN logit counts as -inf, +inf as the largest float; a token outside [0, vocab) gets -inf and rank -1; a row
+ * without a finite logit has entropy 0 and log probabilities -inf.  n_top <= 64, vocab <= 0x7c000000, rows < 2^24. */
+size_t mf_token_logprobs_workspace_bytes(int rows, int vocab, int n_top, int dtype);
+int mf_token_logprobs(float* logprobs, int32_t* ranks, float* entropy, int32_t* top_tokens, float* top_logprobs, const void* logits,
+                      int64_t row_stride, const int32_t* tokens, int rows, int vocab, int n_top, int dtype, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* ---- low-rank adapters ------------------------------------------------------------------------------------ */
+
+/* The S-LoRA cells (mindformers/pet/tuners/slora_adapter.py) beside a quantized projection.
+ * A step's rows sorted by the adapter that each has chosen, once for all projections of the step: plan int32
+ * [mf_adapter_rows_ints], 16-byte aligned, from adapter_ids int32 [tokens] (outside [0, adapters): none).  tile 16 or 64: rows of one
+ * adapter that are computed together.  Up to 1024 adapters, 2^20 rows. */
+int64_t mf_adapter_rows_ints(int tokens, int adapters, int tile);
+int mf_adapter_rows(int32_t* plan, const int32_t* adapter_ids, int tokens, int adapters, int tile, void* stream);
+
+/* out[t, s] = base[t, s] + scales[a] * lora_b[a, s] . (lora_a[a, s] . x[t]) for the rows of adapter a and the slices s of a fused
+ * projection; rows without an adapter are base.  x [tokens, k]; lora_a [adapters, slices, rank, k]; lora_b [adapters, n, rank], its
+ * n = sum(host_widths) rows slice after slice (host_widths: HOST array [slices]); base and out [tokens, n], may be the same; rows
+ * *_row_stride elements apart (0 = dense).  ranks int32 [adapters] (NULL: all `rank`): what lies behind an adapter's rank is not used.
+ * scales fp32 [adapters] (NULL: 1).  plan, tokens, adapters and tile as given to mf_adapter_rows.  Sums in fp32, one rounding of the
+ * result, and lora_a . x enters the second product with at least 16 bits.  k and rank multiples of 8, rank <= 128, up to 8 slices;
+ * x and its rows, lora_a and lora_b on 16-byte borders. */
+size_t mf_adapter_workspace_bytes(int tokens, int adapters, int tile, int k, int slices, int rank);
+int mf_adapter_linear(void* out, const void* x, const void* lora_a, const void* lora_b, const void* base, const int32_t* plan,
+                      const int32_t* ranks, const float* scales, const int32_t* host_widths, int slices, int tokens, int adapters,
+                      int tile, int k, int rank, int64_t x_row_stride, int64_t base_row_stride, int64_t out_row_stride, int dtype,
+                      void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- paged attention (decode) --------------------------------------------------------------------- */
 

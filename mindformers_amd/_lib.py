@@ -32,6 +32,13 @@ SIGNATURES = {
     "mf_copy_blocks": (_I, [_P, _P, _I, _P, _I, _I, _I, _P]),
     "mf_beam_search_workspace_bytes": (_Z, [_I, _I, _I, _I, _I]),
     "mf_beam_search_select": (_I, [_P] * 7 + [_L, _P] + [_I] * 6 + [_P, _Z, _P]),
+    "mf_token_logprobs_workspace_bytes": (_Z, [_I] * 4),
+    "mf_token_logprobs": (_I, [_P] * 6 + [_L, _P] + [_I] * 4 + [_P, _Z, _P]),
+    "mf_rotary_embedding": (_I, [_P] * 10 + [_I] * 7 + [_F] + [_L] * 6 + [_I, _P]),
+    "mf_adapter_rows_ints": (_L, [_I] * 3),
+    "mf_adapter_rows": (_I, [_P, _P, _I, _I, _I, _P]),
+    "mf_adapter_workspace_bytes": (_Z, [_I] * 6),
+    "mf_adapter_linear": (_I, [_P] * 9 + [_I] * 6 + [_L] * 3 + [_I, _P, _Z, _P]),
     "mf_paged_attention_workspace_bytes": (_Z, [_I, _I, _I, _I]),
     "mf_paged_attention_decode_dynamic_quant": (_I, [_P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I,
                                                      _F, _L, _I, _P, _Z, _P]),

@@ -1,0 +1,237 @@
+// Rotary positions: pairs (a, b) of a head's columns turned by an angle that grows with the token's position,
+//
+//   a' = s (a cos t - b sin t),   b' = s (b cos t + a sin t),   t = position * inv_freq[i]
+//
+// with a, b = columns (i, i + p/2) or (2i, 2i + 1) of the p columns from `offset` on; the others pass as they are.  The turned key and
+// the value go to their cache rows in the same launch.
+//
+// Angles in 64 bits: at position 10^6 a float32 product is off by up to 0.03 radians.  Turns (t / 2 pi) lose their whole part, the rest,
+// within half a turn, goes on in float32 (an error below 2e-7 radians).  A workgroup computes the cosines and sines of its rows once, for
+// all heads, into LDS: one double product and one sincospi a pair and row.  Sums in float32, rounded once.
+#include <algorithm>
+
+#include "common.h"
+
+namespace {
+
+constexpr int RO_THREADS = 256;
+constexpr int RO_ROWS = 4;                                    // rows of a workgroup, at most
+constexpr int RO_MAX_PAIRS = 512;
+
+struct RotaryArgs {
+    uint16_t *q_out, *k_out, *k_cache, *v_cache;              // k_out, caches: may be null
+    const uint16_t *q, *k, *v;
+    const int32_t *positions, *slots;
+    const double* inv_freq;
+    int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride, num_slots;
+    int tokens, heads, kv_heads, dim, pairs, offset, rows;    // rows: of a workgroup
+    int units, v_units;                                       // of a head; of a row's values
+    uint32_t unit_magic;                                      // 2^32 / units, rounded up
+    float scale;
+};
+
+// N 16-bit elements moved at once
+template <int N>
+struct Piece {
+    typedef __attribute__((ext_vector_type(N / 2))) uint32_t vec;
+    vec v;
+    __device__ __forceinline__ void load(const uint16_t* p) { v = *(const vec*)p; }
+    __device__ __forceinline__ void store(uint16_t* p) const { *(vec*)p = v; }
+    __device__ __forceinline__ uint16_t at(int i) const { return (uint16_t)(v[i >> 1] >> (16 * (i & 1))); }
+    template <typename T>
+    __device__ __forceinline__ void set2(int i, float lo, float hi) { v[i >> 1] = pack2<T>(lo, hi); }
+};
+template <>
+struct Piece<2> {
+    uint32_t v;
+    __device__ __forceinline__ void load(const uint16_t* p) { v = *(const uint32_t*)p; }
+    __device__ __forceinline__ void store(uint16_t* p) const { *(uint32_t*)p = v; }
+    __device__ __forceinline__ uint16_t at(int i) const { return (uint16_t)(v >> (16 * (i & 1))); }
+    template <typename T>
+    __device__ __forceinline__ void set2(int, float lo, float hi) { v = pack2<T>(lo, hi); }
+};
+template <>
+struct Piece<1> {
+    uint16_t v;
+    __device__ __forceinline__ void load(const uint16_t* p) { v = *p; }
+    __device__ __forceinline__ void store(uint16_t* p) const { *p = v; }
+    __device__ __forceinline__ uint16_t at(int) const { return v; }
+    template <typename T>
+    __device__ __forceinline__ void set2(int, float lo, float) { v = T::from_float(lo); }
+};
+
+__device__ __forceinline__ void turn(float a, float b, float2 cs, float& oa, float& ob) {
+    oa = fmaf(a, cs.x, -(b * cs.y));
+    ob = fmaf(b, cs.x, a * cs.y);
+}
+
+// One unit of a head.  NEAR (neighbours in pairs, VEC >= 2): VEC columns, of which those inside the turned part are turned.  Otherwise a
+// piece of the first members with the piece of their partners, or, behind those units, VEC columns that pass; with VEC 1 the partner
+// may be the neighbour.  out1 and out2 (null: none) get the result; `copied` says whether what passes has to be written to out1.
+template <typename T, int VEC, bool NEAR>
+__device__ __forceinline__ void rotary_unit(const RotaryArgs& A, int u, const uint16_t* in, uint16_t* out1, bool copied, uint16_t* out2,
+                                            const float2* cs) {
+    if constexpr (NEAR && VEC >= 2) {
+        const int c = u * VEC, p0 = (c - A.offset) >> 1;      // offset is even
+        const bool inside = p0 + VEC / 2 > 0 && p0 < A.pairs;
+        if (!inside && !copied && !out2) return;
+        Piece<VEC> x;
+        x.load(in + c);
+        if (inside) {
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) {
+                const int p = p0 + i;
+                float a, b;
+                turn(T::to_float(x.at(2 * i)), T::to_float(x.at(2 * i + 1)), cs[min(max(p, 0), A.pairs - 1)], a, b);
+                Piece<2> two;
+                two.template set2<T>(0, a, b);
+                if constexpr (VEC == 2) x.v = p >= 0 && p < A.pairs ? two.v : x.v;
+                else x.v[i] = p >= 0 && p < A.pairs ? two.v : x.v[i];
+            }
+        }
+        if (out1 && (inside || copied)) x.store(out1 + c);
+        if (out2) x.store(out2 + c);
+    } else {
+        const int turned = A.pairs / VEC;
+        if (u < turned) {
+            const int c = A.offset + (NEAR ? 2 * u : u * VEC), d = NEAR ? c + 1 : c + A.pairs;
+            Piece<VEC> x, y;
+            x.load(in + c);
+            y.load(in + d);
+            float a[VEC], b[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) turn(T::to_float(x.at(i)), T::to_float(y.at(i)), cs[u * VEC + i], a[i], b[i]);
+#pragma unroll
+            for (int i = 0; i < VEC; i += 2) {
+                x.template set2<T>(i, a[i], VEC > 1 ? a[i + (VEC > 1)] : 0.f);
+                y.template set2<T>(i, b[i], VEC > 1 ? b[i + (VEC > 1)] : 0.f);
+            }
+            if (out1) { x.store(out1 + c); y.store(out1 + d); }
+            if (out2) { x.store(out2 + c); y.store(out2 + d); }
+        } else {
+            if (!copied && !out2) return;
+            int c = (u - turned) * VEC;
+            c = c < A.offset ? c : c + 2 * A.pairs;
+            Piece<VEC> x;
+            x.load(in + c);
+            if (out1 && copied) x.store(out1 + c);
+            if (out2) x.store(out2 + c);
+        }
+    }
+}
+
+template <typename T, int VEC, bool NEAR>
+__global__ __launch_bounds__(RO_THREADS) void rotary_kernel(const RotaryArgs A) {
+    extern __shared__ float2 table[];                         // [rows][pairs]: s cos, s sin
+    const int64_t row0 = (int64_t)blockIdx.x * A.rows;
+    const int rows = (int)min((int64_t)A.rows, A.tokens - row0);
+    for (int i = threadIdx.x; i < rows * A.pairs; i += RO_THREADS) {
+        const int r = i / A.pairs, p = i - r * A.pairs;
+        const double turns = (double)A.positions[row0 + r] * (A.inv_freq[p] * 0.15915494309189535);
+        float sn, cn;
+        sincospif(2.f * (float)(turns - rint(turns)), &sn, &cn);
+        table[i] = make_float2(A.scale * cn, A.scale * sn);
+    }
+    __syncthreads();
+    const int n_q = A.heads * A.units, n_qk = n_q + A.kv_heads * A.units;
+    for (int r = 0; r < rows; ++r) {
+        const int64_t row = row0 + r;
+        const int64_t slot = A.slots ? A.slots[row] : -1;
+        const bool cached = slot >= 0 && slot < A.num_slots;
+        const int64_t at = cached ? slot * A.kv_heads * A.dim : 0;
+        const float2* cs = table + r * A.pairs;
+        const int all = n_qk + (cached ? A.v_units : 0);
+        for (int i = threadIdx.x; i < all; i += RO_THREADS) {
+            if (i < n_qk) {
+                const bool is_q = i < n_q;
+                const int j = is_q ? i : i - n_q;
+                const int head = A.units == 1 ? j : (int)__umulhi((uint32_t)j, A.unit_magic), u = j - head * A.units;
+                const int c = head * A.dim;
+                const uint16_t* in = is_q ? A.q + row * A.q_stride + c : A.k + row * A.k_stride + c;
+                uint16_t* out = is_q ? A.q_out + row * A.q_out_stride + c : A.k_out ? A.k_out + row * A.k_out_stride + c : nullptr;
+                rotary_unit<T, VEC, NEAR>(A, u, in, out, out && out != in, !is_q && cached ? A.k_cache + at + c : nullptr, cs);
+            } else {
+                const int c = (i - n_qk) * VEC;
+                Piece<VEC> x;
+                x.load(A.v + row * A.v_stride + c);
+                x.store(A.v_cache + at + c);
+            }
+        }
+    }
+}
+
+// The widest access that every piece's start and length allows.  With partners half the part away both pieces begin VEC columns apart,
+// with neighbours a pair must not lie across two.
+int rotary_vec(const RotaryArgs& A, bool near) {
+    uint64_t bits = (uint64_t)A.dim | A.q_stride | A.q_out_stride;
+    uint64_t at = (uintptr_t)A.q | (uintptr_t)A.q_out;
+    if (A.k) bits |= A.k_stride, at |= (uintptr_t)A.k;
+    if (A.k_out) bits |= A.k_out_stride, at |= (uintptr_t)A.k_out;
+    if (A.k_cache) bits |= A.v_stride, at |= (uintptr_t)A.k_cache | (uintptr_t)A.v_cache | (uintptr_t)A.v;
+    if (near) bits |= (A.offset & 1);
+    else bits |= A.offset | A.pairs;
+    bits |= at >> 1;
+    return bits & 1 ? 1 : bits & 2 ? 2 : bits & 4 ? 4 : 8;
+}
+
+}  // namespace
+
+extern "C" int mf_rotary_embedding(void* query_out, void* key_out, const void* query, const void* key, const void* value, void* key_cache,
+                                   void* value_cache, const int32_t* positions, const double* inv_freq, const int32_t* slot_mapping,
+                                   int num_tokens, int n_heads, int n_kv_heads, int head_dim, int n_pairs, int offset, int interleaved,
+                                   float scale, int64_t num_slots, int64_t q_row_stride, int64_t k_row_stride, int64_t v_row_stride,
+                                   int64_t q_out_row_stride, int64_t k_out_row_stride, int dtype, void* stream) {
+    MF_REQUIRE(dtype == MF_BF16 || dtype == MF_FP16, "rotary_embedding: dtype must be bf16 or fp16");
+    MF_REQUIRE(num_tokens >= 0 && num_tokens < (1 << 24) && n_heads > 0 && n_kv_heads >= 0 && head_dim > 0 && n_heads <= 4096 && n_kv_heads <= 4096,
+               "rotary_embedding: bad sizes");
+    MF_REQUIRE(n_pairs > 0 && n_pairs <= RO_MAX_PAIRS && offset >= 0 && offset + 2 * n_pairs <= head_dim && head_dim <= 2 * RO_MAX_PAIRS,
+               "rotary_embedding: %d pairs from column %d do not fit heads of %d (up to %d)", n_pairs, offset, head_dim, 2 * RO_MAX_PAIRS);
+    if (num_tokens == 0) return 0;
+    MF_REQUIRE(query && query_out && positions && inv_freq, "rotary_embedding: null argument");
+    MF_REQUIRE((key != nullptr) == (n_kv_heads > 0) && (key || !key_out), "rotary_embedding: a key goes with its heads and its output");
+    MF_REQUIRE((key_cache != nullptr) == (value_cache != nullptr) && (key_cache != nullptr) == (value != nullptr) &&
+               (key_cache != nullptr) == (slot_mapping != nullptr) && (!key_cache || key),
+               "rotary_embedding: caches go with a key, a value and slots");
+    MF_REQUIRE(!key_cache || num_slots > 0, "rotary_embedding: caches without slots");
+    MF_REQUIRE((((uintptr_t)query | (uintptr_t)query_out | (uintptr_t)key | (uintptr_t)key_out | (uintptr_t)value) & 1) == 0 &&
+               ((uintptr_t)inv_freq & 7) == 0, "rotary_embedding: tensors must be aligned to their type");
+    RotaryArgs A = {};
+    A.q_out = (uint16_t*)query_out, A.k_out = (uint16_t*)key_out, A.k_cache = (uint16_t*)key_cache, A.v_cache = (uint16_t*)value_cache;
+    A.q = (const uint16_t*)query, A.k = (const uint16_t*)key, A.v = (const uint16_t*)value;
+    A.positions = positions, A.slots = slot_mapping, A.inv_freq = inv_freq;
+    const int64_t qw = (int64_t)n_heads * head_dim, kw = (int64_t)n_kv_heads * head_dim;
+    A.q_stride = q_row_stride > 0 ? q_row_stride : qw;
+    A.q_out_stride = q_out_row_stride > 0 ? q_out_row_stride : qw;
+    A.k_stride = k_row_stride > 0 ? k_row_stride : kw;
+    A.k_out_stride = k_out_row_stride > 0 ? k_out_row_stride : kw;
+    A.v_stride = v_row_stride > 0 ? v_row_stride : kw;
+    MF_REQUIRE(A.q_stride >= qw && A.q_out_stride >= qw && A.k_stride >= kw && A.k_out_stride >= kw && A.v_stride >= kw,
+               "rotary_embedding: rows overlap");
+    A.num_slots = num_slots, A.tokens = num_tokens, A.heads = n_heads, A.kv_heads = n_kv_heads, A.dim = head_dim, A.pairs = n_pairs;
+    A.offset = offset, A.scale = scale;
+    const int vec = rotary_vec(A, interleaved != 0);
+    A.units = interleaved && vec > 1 ? head_dim / vec : n_pairs / vec + (head_dim - 2 * n_pairs) / vec;
+    A.unit_magic = (uint32_t)((0x100000000ull + A.units - 1) / A.units);   // exact for up to 2^32 / units units; not used for one
+    A.v_units = (int)(kw / vec);
+    // several rows a workgroup where there are enough to fill the device: their angles take its threads at once
+    A.rows = num_tokens >= 2048 ? std::max(1, std::min(RO_ROWS, RO_THREADS / n_pairs)) : 1;
+    const dim3 grid((unsigned)((num_tokens + A.rows - 1) / A.rows));
+    const size_t lds = (size_t)A.rows * n_pairs * sizeof(float2);
+    hipStream_t st = (hipStream_t)stream;
+#define RO_LAUNCH(T, N)                                                                                      \
+    do {                                                                                                     \
+        if (vec == 8) hipLaunchKernelGGL((rotary_kernel<T, 8, N>), grid, dim3(RO_THREADS), lds, st, A);      \
+        else if (vec == 4) hipLaunchKernelGGL((rotary_kernel<T, 4, N>), grid, dim3(RO_THREADS), lds, st, A); \
+        else if (vec == 2) hipLaunchKernelGGL((rotary_kernel<T, 2, N>), grid, dim3(RO_THREADS), lds, st, A); \
+        else hipLaunchKernelGGL((rotary_kernel<T, 1, N>), grid, dim3(RO_THREADS), lds, st, A);               \
+    } while (0)
+    if (dtype == MF_BF16) {
+        if (interleaved) RO_LAUNCH(BF16, true);
+        else RO_LAUNCH(BF16, false);
+    } else {
+        if (interleaved) RO_LAUNCH(FP16, true);
+        else RO_LAUNCH(FP16, false);
+    }
+#undef RO_LAUNCH
+    return MF_LAUNCH_CHECK();
+}

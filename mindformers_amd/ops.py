@@ -161,6 +161,63 @@ def rope_rows(positions, inv_freq, dtype):
     return cos, sin
 
 
+def rotary_embedding(query, key, positions, inv_freq, head_dim, interleaved=False, scale=1.0, offset=0, value=None, key_cache=None,
+                     value_cache=None, slot_mapping=None, out=None):
+    """Rotary positions of any layout and scaling, angles from the positions in 64 bits: of every head of ``query`` [T, n_heads * D] and
+    ``key`` [T, n_kv * D] (or None) the 2 * len(inv_freq) columns from ``offset`` on are turned in pairs by positions[t] * inv_freq[i]
+    radians and multiplied with ``scale``; the others pass.  A pair is columns (i, i + len(inv_freq)) of that part, or (2 i, 2 i + 1) with
+    ``interleaved``.  positions int32 [T], inv_freq float64.  In place, or into ``out`` = (query_out, key_out or None), which share no
+    memory with the inputs.  With ``key_cache`` / ``value_cache`` [num_blocks, block_size, n_kv, D] the turned key and ``value`` go to
+    the rows that ``slot_mapping`` names as well (a negative slot: to none).  Returns (query, key) where they went."""
+    lib = _lib.load()
+    dev = _dev_of(query, key, value)
+    _need(_dev_ok(positions, inv_freq, key_cache, value_cache, slot_mapping) == dev, "all tensors must be on the same device")
+    d = int(head_dim)
+    _need(d > 0 and query.dim() >= 1 and query.shape[-1] % d == 0 and query.shape[-1] > 0, "query must be [T, n_heads * head_dim]")
+    _need(positions.dtype == torch.int32 and positions.dim() == 1 and inv_freq.dtype == torch.float64 and inv_freq.dim() == 1,
+          "positions must be int32 [T], inv_freq float64 [pairs]")
+    t, pairs, qw = positions.numel(), inv_freq.numel(), query.shape[-1]
+    if not (0 < pairs and 0 <= offset and offset + 2 * pairs <= d <= 1024):
+        raise ValueError(f"{pairs} pairs from column {offset} do not fit heads of {d} (up to 1024)")
+    query, qs = _rows(query, qw, "query")
+    _need(query.dtype in _ACT and query.numel() == t * qw, "query must be bf16/fp16 and hold a row for each position")
+    kw, ks, vs, slots = 0, 0, 0, 0
+    if key is not None:
+        _need(key.dim() >= 1 and key.shape[-1] % d == 0 and key.shape[-1] > 0, "key must be [T, n_kv_heads * head_dim]")
+        kw = key.shape[-1]
+        key, ks = _rows(key, kw, "key")
+        _need(key.dtype == query.dtype and key.numel() == t * kw, "key must have query's type and a row for each position")
+    if key_cache is not None or value_cache is not None or value is not None or slot_mapping is not None:
+        _need(key is not None and key_cache is not None and value_cache is not None and value is not None and slot_mapping is not None,
+              "key, value, both caches and slot_mapping go together")
+        _need(key_cache.dim() == 4 and value_cache.shape == key_cache.shape and key_cache.shape[2] * key_cache.shape[3] == kw
+              and key_cache.shape[3] == d, "caches must be [num_blocks, block_size, n_kv_heads, head_dim]")
+        _need(key_cache.dtype == query.dtype and value_cache.dtype == query.dtype and value.dtype == query.dtype, "dtype mismatch")
+        value, vs = _rows(value, kw, "value")
+        _need(value.numel() == t * kw and slot_mapping.dtype == torch.int32 and slot_mapping.numel() == t and slot_mapping.dim() == 1,
+              "value and int32 slot_mapping must hold a row for each position")
+        slots = key_cache.shape[0] * key_cache.shape[1]
+        _need(slots > 0, "caches without a block")
+    q_out, k_out = (query, key) if out is None else out
+    qos, kos = qs, ks
+    if out is not None:
+        _need(_dev_of(q_out, k_out) == dev, "out must be on the inputs' device")
+        q_out, qos = _rows(q_out, qw, "query_out")
+        _need(q_out.dtype == query.dtype and q_out.numel() == t * qw, "query_out must have query's rows and type")
+        if k_out is not None:
+            _need(key is not None, "key_out without a key")
+            k_out, kos = _rows(k_out, kw, "key_out")
+            _need(k_out.dtype == query.dtype and k_out.numel() == t * kw, "key_out must have key's rows and type")
+        else:
+            _need(key is None or key_cache is not None, "a key that goes neither to key_out nor into a cache")
+    with _on(dev):
+        check(lib.mf_rotary_embedding(ptr(q_out), ptr(k_out), ptr(query), ptr(key), ptr(value), ptr(key_cache), ptr(value_cache),
+                                      ptr(positions), ptr(inv_freq), ptr(slot_mapping), t, qw // d, kw // d, d, pairs, int(offset),
+                                      1 if interleaved else 0, float(scale), slots, qs, ks, vs, qos, kos, dtype_code(query.dtype),
+                                      stream_ptr(dev)), "mf_rotary_embedding")
+    return q_out, k_out
+
+
 def rope_and_cache(query, key, value, cos, sin, key_cache, value_cache, slot_mapping, n_heads):
     """RoPE on q/k (in place) then scatter of rotated k and v into the caches, one launch."""
     lib = _lib.load()
@@ -933,6 +990,122 @@ def beam_search_select(logits, beam_scores, eos_token_id=-1, n_candidates=None):
         check(lib.mf_beam_search_select(a, a + 4 * gn, a + 8 * gn, b, b + 4 * gk, b + 8 * gk, ptr(logits), stride, ptr(beam_scores), g, k,
                                         v, n, eos, code, ptr(ws), ws.numel(), stream_ptr(dev)), "mf_beam_search_select")
     return res
+
+
+# --------------------------------------------------------------------------------------------- log probabilities
+class TokenLogprobs(NamedTuple):
+    """What ``token_logprobs`` returns: of the given tokens logprobs fp32 [T] and ranks int32 [T] (0: the most likely), of their rows
+    entropy fp32 [T] (nats), and the n most likely tokens [T, n], int32 and fp32, best first."""
+    logprobs: torch.Tensor
+    ranks: torch.Tensor
+    entropy: torch.Tensor
+    top_tokens: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+def token_logprobs(logits, tokens, n_top=0):
+    """Log probabilities of ``tokens`` int32 [T] under softmax(logits[t]), their ranks, the entropy of every row and its ``n_top`` (up to
+    64) most likely tokens; ties go to the lowest token.  logits [T, vocab], bf16, fp16 or fp32, may be a slice of wider rows.  A NaN logit
+    counts as -inf, +inf as the largest float; a token outside the vocabulary (-1: a row of padding) gets -inf and rank -1."""
+    lib = _lib.load()
+    dev = _dev_of(logits, tokens)
+    _need(logits.dtype in _ACT or logits.dtype == torch.float32, "logits must be bf16, fp16 or fp32")
+    _need(logits.dim() == 2, "logits must be [T, vocab]")
+    t, v = logits.shape
+    _need(tokens.dtype == torch.int32 and tokens.dim() == 1 and tokens.numel() == t and tokens.is_contiguous(),
+          "tokens must be a contiguous int32 [T]")
+    _need(0 < v <= 0x7c000000 and t < 1 << 24, "1 to 0x7c000000 tokens of vocabulary and fewer than 2^24 rows")
+    stride = logits.stride(0) if t > 1 else v                 # one row: whatever its stride says
+    _need((logits.stride(1) == 1 or v == 1) and stride >= v, "logits rows must have a unit column stride and not overlap")
+    n = int(n_top)
+    if not 0 <= n <= min(64, v):
+        raise ValueError(f"n_top must be 0 to 64 and no more than the {v} tokens, got {n_top}")
+    buf = torch.empty(t * (3 + 2 * n), dtype=torch.int32, device=dev)
+    val, num = buf.view(torch.float32).as_strided, buf.as_strided
+    res = TokenLogprobs(val((t,), (1,), 0), num((t,), (1,), t), val((t,), (1,), 2 * t), num((t, n), (n, 1), 3 * t),
+                        val((t, n), (n, 1), (3 + n) * t))
+    if t == 0:
+        return res
+    code = dtype_code(logits.dtype)
+    need = lib.mf_token_logprobs_workspace_bytes(t, v, n, code)
+    ws = workspace(need, dev, "logprobs") if need else None
+    a = buf.data_ptr()
+    with _on(dev):
+        check(lib.mf_token_logprobs(a, a + 4 * t, a + 8 * t, a + 12 * t, a + 4 * (3 + n) * t, ptr(logits), stride, ptr(tokens), t, v, n, code,
+                                    ptr(ws), ws.numel() if ws is not None else 0, stream_ptr(dev)), "mf_token_logprobs")
+    return res
+
+
+# --------------------------------------------------------------------------------------------- low-rank adapters
+class AdapterRows(NamedTuple):
+    """What ``adapter_rows`` returns: the rows of a step sorted by adapter, for every projection of the step."""
+    plan: torch.Tensor
+    tokens: int
+    adapters: int
+    tile: int
+
+
+def adapter_rows(adapter_ids, n_adapters):
+    """Sorts the rows of a step by the adapter that each has chosen: ``adapter_ids`` int32 [T], outside [0, n_adapters) none (-1).  Once a
+    step; ``adapter_linear`` of every projection takes the result.  Up to 1024 adapters and 2^20 rows."""
+    lib = _lib.load()
+    dev = _dev_ok(adapter_ids)
+    _need(adapter_ids.dtype == torch.int32 and adapter_ids.dim() == 1, "adapter_ids must be int32 [T]")
+    t, n = adapter_ids.numel(), int(n_adapters)
+    if not (0 < n <= 1024 and t <= 1 << 20):
+        raise ValueError(f"1 to 1024 adapters and up to 2^20 rows, got {n_adapters} and {t}")
+    tile = 16 if t <= 1024 else 64                            # prompts share weights and rows among 64, decode rows are of many adapters
+    plan = torch.empty(lib.mf_adapter_rows_ints(t, n, tile), dtype=torch.int32, device=dev)
+    with _on(dev):
+        check(lib.mf_adapter_rows(ptr(plan), ptr(adapter_ids), t, n, tile, stream_ptr(dev)), "mf_adapter_rows")
+    return AdapterRows(plan, t, n, tile)
+
+
+def adapter_linear(x, lora_a, lora_b, rows, base, widths=None, ranks=None, scales=None, out=None):
+    """base + scales[a] * lora_b[a] (lora_a[a] x) for the rows of every adapter a; rows without one are base.  ``x`` [T, K] what went into the
+    shared projection and ``base`` [T, N] what came out of it (either may be a column slice of wider rows); ``rows``: the step's
+    ``adapter_rows``.  ``widths`` (default (N,)): the slices of a fused projection, each with a matrix of its own in ``lora_a``
+    [n, slices, R, K] (one slice: [n, R, K] too); ``lora_b`` [n, N, R] holds them one after the other.  ``ranks`` int32 [n]: each adapter's
+    own, up to R (None: R); ``scales`` fp32 [n] (None: 1).  ``out``: base itself (in place) or memory of its own.  K and R multiples
+    of 8, R up to 128, 8 slices."""
+    lib = _lib.load()
+    dev = _dev_of(x, base, out)
+    _need(_dev_ok(lora_a, lora_b, rows.plan, ranks, scales) == dev, "all tensors must be on the same device")
+    t, n = rows.tokens, rows.adapters
+    _need(lora_a.dim() in (3, 4) and lora_b.dim() == 3 and lora_a.shape[0] == n and lora_b.shape[0] == n,
+          "lora_a must be [n, slices, R, K] and lora_b [n, N, R] for the adapters of rows")
+    k, r, cols = lora_a.shape[-1], lora_a.shape[-2], lora_b.shape[1]
+    widths = (cols,) if widths is None else tuple(widths)
+    slices = len(widths)
+    if sum(widths) != cols or not 1 <= slices <= 8 or min(widths) < 1:
+        raise ValueError(f"1 to 8 slices that make up lora_b's {cols} columns, got widths {widths}")
+    _need(lora_b.shape[2] == r and (lora_a.shape[1] == slices if lora_a.dim() == 4 else slices == 1), "lora_a and lora_b do not match")
+    if k % 8 or r % 8 or not 0 < r <= 128 or not k:
+        raise ValueError(f"input width {k} and rank {r} must be multiples of 8, the rank up to 128")
+    _need(x.dtype in _ACT and base.dtype == x.dtype and lora_a.dtype == x.dtype and lora_b.dtype == x.dtype, "dtype mismatch")
+    _need(x.dim() >= 1 and x.shape[-1] == k and base.dim() >= 1 and base.shape[-1] == cols, "x must be [T, K], base [T, N]")
+    if ranks is not None:
+        _need(ranks.dtype == torch.int32 and ranks.numel() == n, "ranks must be int32 [n]")
+    if scales is not None:
+        _need(scales.dtype == torch.float32 and scales.numel() == n, "scales must be fp32 [n]")
+    x, xs = _rows(x, k, "x")
+    if x.data_ptr() % 16 or xs % 8:                           # a slice whose rows are not on 16-byte borders
+        x, xs = x.reshape(-1, k).clone(memory_format=torch.contiguous_format), k
+    if out is None:
+        out = torch.empty(base.shape, dtype=base.dtype, device=dev)
+    base, bs = _rows(base, cols, "base")
+    got, os = _rows(out, cols, "out")
+    if not (x.numel() == t * k and base.numel() == t * cols and got.numel() == t * cols and got.dtype == x.dtype):
+        raise ValueError(f"x, base and out must hold the {t} rows that adapter_rows was given")
+    if t == 0:
+        return out
+    _need(lora_a.data_ptr() % 16 == 0 and lora_b.data_ptr() % 16 == 0, "lora_a and lora_b must lie on 16-byte borders")
+    ws = workspace(lib.mf_adapter_workspace_bytes(t, n, rows.tile, k, slices, r), dev, "adapter")
+    with _on(dev):
+        check(lib.mf_adapter_linear(ptr(got), ptr(x), ptr(lora_a), ptr(lora_b), ptr(base), ptr(rows.plan), ptr(ranks), ptr(scales),
+                                    (ctypes.c_int32 * slices)(*widths), slices, t, n, rows.tile, k, r, xs, bs, os,
+                                    dtype_code(x.dtype), ptr(ws), ws.numel(), stream_ptr(dev)), "mf_adapter_linear")
+    return out
 
 
 # --------------------------------------------------------------------------------------------- norm / activation
