@@ -18,8 +18,11 @@
 namespace {
 
 constexpr int BS_WAVES = 4;
-constexpr int BS_MAX_N = LIST_MAX_N;                                  // candidates a group, beams a group
+constexpr int BS_MAX_N = 64;                                  // candidates a group, beams a group
 constexpr int64_t BS_MAX_PLACES = 0x7c000000;                 // beams x vocabulary: a place, and a column a piece behind it, in 32 bits
+constexpr int BS_TAKE = 128;                                  // entries that a wave takes from a step
+constexpr int BS_GROW = 40;                                   // entries beyond the n best that a list may hold between two steps
+constexpr int BS_LIST = 256;                                  // entries of a wave's list: 64 + BS_GROW + BS_TAKE fit
 
 __device__ __forceinline__ uint64_t order64(double f) {
     const uint64_t u = (uint64_t)__double_as_longlong(f);
@@ -46,8 +49,118 @@ __device__ __forceinline__ double exp_sum(double d) {
     return __hiloint2double(__double2hiint(p) + (__double2loint(z) << 20), __double2loint(p));
 }
 
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+// c + set bits of m below this lane's
+__device__ __forceinline__ int lanes_before(uint64_t m, int c) {
+    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, (uint32_t)c));
+}
+__device__ __forceinline__ int wave_scan_excl(int v, int& total) {
+    const int lane = threadIdx.x & 63;
+    int incl = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int t = __shfl_up(incl, o, 64);
+        if (lane >= o) incl += t;
+    }
+    total = __shfl(incl, 63, 64);
+    return incl - v;
+}
+
 // A beam that is out of the search: its running score is no finite log probability
 __device__ __forceinline__ bool dead_beam(float run) { return !(fabsf(run) < 1e30f); }
+
+struct BeamList {
+    float x[BS_LIST];
+    int i[BS_LIST];
+};
+
+// The n best of a wave's list (entries [0, e), e >= 1) to its front, best first; returns how many there are.  Entries are held one a
+// lane (and a second, third, fourth round of them) and compared with every other, which goes round as a scalar.
+__device__ __forceinline__ int list_prune(BeamList& l, int e, int n) {
+    constexpr int R = BS_LIST / 64;
+    const int lane = threadIdx.x & 63;
+    wave_fence();
+    float x[R];
+    int id[R], rank[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        const int at = min(lane + 64 * k, e - 1);
+        x[k] = l.x[at];
+        id[k] = l.i[at];
+        rank[k] = lane + 64 * k < e ? 0 : BS_LIST;
+    }
+#pragma unroll
+    for (int jr = 0; jr < R; ++jr) {
+        const int last = min(64, e - 64 * jr);
+        for (int j = 0; j < last; ++j) {
+            const float xj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x[jr]), j));
+            const int ij = __builtin_amdgcn_readlane(id[jr], j);
+            rank[0] += xj > x[0] || (xj == x[0] && ij < id[0]);
+            if (e > 64) {
+#pragma unroll
+                for (int k = 1; k < R; ++k) rank[k] += xj > x[k] || (xj == x[k] && ij < id[k]);
+            }
+        }
+    }
+    wave_fence();
+#pragma unroll
+    for (int k = 0; k < R; ++k)
+        if (rank[k] < n) {
+            l.x[rank[k]] = x[k];
+            l.i[rank[k]] = id[k];
+        }
+    wave_fence();
+    return min(e, n);
+}
+
+// The list cut to the entries that reach its n-th best (e >= n), in any order; `bound` is that entry.  Found bit by bit with ballots,
+// a third of the instructions that ranking takes.  Where more than BS_GROW / 2 entries are alike there they are ranked.
+template <int R>
+__device__ __forceinline__ int list_cut(BeamList& l, int e, int n, float& bound) {
+    const int lane = threadIdx.x & 63;
+    wave_fence();
+    float x[R];
+    int id[R];
+    uint32_t key[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        const int at = min(lane + 64 * k, e - 1);
+        x[k] = l.x[at] + 0.f;
+        id[k] = l.i[at];
+        key[k] = lane + 64 * k < e ? order32(x[k]) : 0u;
+    }
+    uint32_t t = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t trial = t | (1u << bit);
+        int c = 0;
+#pragma unroll
+        for (int k = 0; k < R; ++k) c += __popcll(__ballot(key[k] >= trial));
+        if (c >= n) t = trial;
+    }
+    bound = order32_back(t);
+    int c = 0;
+#pragma unroll
+    for (int k = 0; k < R; ++k) c += __popcll(__ballot(key[k] >= t));
+    if (c > n + BS_GROW / 2) return list_prune(l, e, n);
+    wave_fence();
+    c = 0;
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        const bool keep = key[k] >= t;
+        const uint64_t m = __ballot(keep);
+        if (keep) {
+            const int at = lanes_before(m, c);
+            l.x[at] = x[k];
+            l.i[at] = id[k];
+        }
+        c += __popcll(m);
+    }
+    wave_fence();
+    return c;
+}
 
 // A wave's list takes every logit above a bound that n logits of its piece are known to reach: first the n-th largest of
 // the lanes' maxima of a step (found bit by bit with ballots), later the n-th best entry, which is looked up only when the list has
@@ -63,11 +176,11 @@ __global__ __launch_bounds__(BS_WAVES * 64) void beam_partial_kernel(const void*
                                                                      double* __restrict__ part_sum, float* __restrict__ cand_x,
                                                                      int* __restrict__ cand_tok) {
     constexpr int VEC = L::VEC, BS_VECS = L::VECS, E = BS_VECS * VEC, STEP = 64 * E;
-    __shared__ LogitList lists[BS_WAVES];
+    __shared__ BeamList lists[BS_WAVES];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int chunk = blockIdx.x * BS_WAVES + w, row = blockIdx.y;
     if (chunk >= chunks) return;                              // no workgroup barrier below
-    LogitList& list = lists[w];
+    BeamList& list = lists[w];
     const uint8_t* base = (const uint8_t*)logits + row * row_stride * L::BYTES;
     // columns are counted from the 16-byte boundary at or before the row's start, `mis` elements in front of it
     const int mis = (int)(((uintptr_t)base & 15) / L::BYTES);
@@ -157,7 +270,91 @@ __global__ __launch_bounds__(BS_WAVES * 64) void beam_partial_kernel(const void*
 #pragma unroll
         for (int k = 0; k < E; ++k) sum += exp_sum((double)f[k] - r);
 
-        list_step<L>(list, f, mx4, mx, n, v0, mis, c1, full, thr, count);
+        // ---- the list
+        if (!full || __ballot(mx > thr)) {
+            auto at_least = [&](float x) {                    // logits of the step that reach x
+                int c = 0;
+#pragma unroll
+                for (int k = 0; k < E; ++k) c += __popcll(__ballot(f[k] >= x));
+                return c;
+            };
+            if (!full) {
+                const uint32_t key = order32(mx);
+                uint32_t t = 0;
+                for (int bit = 31; bit >= 0; --bit) {
+                    const uint32_t trial = t | (1u << bit);
+                    if (__popcll(__ballot(key >= trial)) >= n) t = trial;
+                }
+                thr = order32_back(t) + 0.f;                  // (no negative zero: the values next to thr are found by its key)
+            }
+            // The lowest logit that is taken: above thr, at it while fewer than n are known, and no masked one.
+            float low = full || thr == -INFINITY ? order32_back(order32(thr) + 1) : thr;
+            // (a few lanes cannot hold too many)
+            int reach = E * __popcll(__ballot(mx >= low));
+            if (!full || reach > BS_TAKE) reach = at_least(low);
+            int ties = full || thr > -INFINITY ? 0 : max(n - reach, 0);        // masked ones, the lowest tokens first
+            if (reach > BS_TAKE) {                            // the step's own n-th largest logit
+                uint32_t t = 0;
+                for (int bit = 31; bit >= 0; --bit) {
+                    const uint32_t trial = t | (1u << bit);
+                    if (at_least(order32_back(trial)) >= n) t = trial;
+                }
+                thr = low = order32_back(t) + 0.f;
+                if (at_least(low) > BS_TAKE) {                // many alike: the lowest tokens of them too
+                    low = order32_back(order32(thr) + 1);
+                    ties = n - at_least(low);
+                }
+            }
+            full = ties == 0 || thr > -INFINITY;
+#pragma unroll
+            for (int k4 = 0; k4 < E; k4 += 4) {
+                if (!__ballot(mx4[k4 / 4] >= low)) continue;
+#pragma unroll
+                for (int k = k4; k < k4 + 4; ++k) {
+                    const uint64_t m = __ballot(f[k] >= low);
+                    if (!m) continue;
+                    if (f[k] >= low) {
+                        const int at = lanes_before(m, count);
+                        list.x[at] = f[k];
+                        list.i[at] = lane * VEC - mis + (v0 + (k / VEC) * 64 * VEC + k % VEC);
+                    }
+                    count += __popcll(m);
+                }
+            }
+            // logits at thr in the order of the tokens; of masked ones, -inf and NaN, which counts as it
+            for (int u = 0; u < BS_VECS && ties > 0; ++u) {
+                const int v = v0 + (u * 64 + lane) * VEC;
+                int c = 0;
+                bool tie[VEC];
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) {
+                    float fq = f[q];
+#pragma unroll
+                    for (int uu = 1; uu < BS_VECS; ++uu) fq = u == uu ? f[uu * VEC + q] : fq;
+                    tie[q] = v + q >= mis && v + q < c1 && (thr == -INFINITY ? !(fq > thr) : fq == thr);
+                    c += tie[q];
+                }
+                int all;
+                int pos = wave_scan_excl(c, all);
+#pragma unroll
+                for (int q = 0; q < VEC; ++q)
+                    if (tie[q]) {
+                        if (pos < ties) {
+                            list.x[count + pos] = thr;
+                            list.i[count + pos] = v + q - mis;
+                        }
+                        ++pos;
+                    }
+                all = min(all, ties);
+                count += all;
+                ties -= all;
+            }
+            full = full || ties == 0;                         // masked logits may have filled it
+        }
+        if (count > n + BS_GROW) {
+            count = count <= 128 ? list_cut<2>(list, count, n, thr) : list_cut<BS_LIST / 64>(list, count, n, thr);
+            full = true;
+        }
     }
     if (count > n) count = list_cut<2>(list, count, n, thr);  // no more than n + BS_GROW here
     if (count) count = list_prune(list, count, n);

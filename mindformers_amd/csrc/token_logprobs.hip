@@ -3,10 +3,12 @@
 //   lp(v) = x[v] - m - log Z,   Z = sum_u exp(x[u] - m),   H = log Z - (1 / Z) sum_u (x[u] - m) exp(x[u] - m)
 //   rank(v) = number of tokens u with x[u] > x[v], or x[u] = x[v] and u < v
 //
-// One pass over the logits.  A wave walks a piece of a row and keeps the two sums about a reference m of each lane's own (moved when a
-// logit passes it by more than 8: the sums stay in range and H loses no more than that), the count of the rank and, where asked for, a
-// list of its best logits.  The waves of a workgroup join in LDS; a row of one workgroup is done then, others take a second kernel.
-// Sums in float32: their errors are of the size of the rounding of what comes out.
+// One pass over the logits for the sums, the rank and every lane's largest logit; the best ones are looked for behind it, in the columns
+// of the lanes whose largest is among the n largest of the workgroup's 256 (n / 256 of the columns, read once more; a list kept on the
+// way took 90 us of 345 for 4137 x 152064 bf16 with 20 alternatives, 260 in 545 with 64).  The waves of a workgroup take the steps of a
+// piece of a row in turn; each lane's sums are about a reference m of its own (moved when a logit passes it by more than 8: the sums stay
+// in range and H loses no more than that).  A row of one workgroup is done then, others are joined by a second kernel.  Sums in
+// float32: their errors are of the size of the rounding of what comes out.
 #include <algorithm>
 
 #include "logit_rows.h"
@@ -15,6 +17,8 @@ namespace {
 
 constexpr int TL_WAVES = 4;
 constexpr int TL_MAX_GROUPS = 64;                             // workgroups of a row
+constexpr int TL_MAX_N = 64;                                  // alternatives
+constexpr int TL_LIST = 512;                                  // logits that a workgroup ranks at a time
 constexpr int64_t TL_MAX_VOCAB = 0x7c000000;                  // a column a piece behind the last in 32 bits
 
 struct RowSums {
@@ -29,7 +33,9 @@ struct LogprobOut {
     float* top_logprobs;
 };
 
-__device__ __forceinline__ float exp_neg(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896341f); }      // d >= -104
+constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
+constexpr float FAR = 65536.f;                                // references whose product with LOG2E is rounded by 2^-8 at most
+__device__ __forceinline__ float exp_neg(float d) { return __builtin_amdgcn_exp2f(d * LOG2E); }      // d >= -104
 
 // the sums moved to a reference m at or above their own
 __device__ __forceinline__ void sums_to(RowSums& s, float m) {
@@ -39,6 +45,28 @@ __device__ __forceinline__ void sums_to(RowSums& s, float m) {
     s.z *= e;
     s.m = m;
 }
+
+// A lane's sums while it walks, in units of log 2: an exponent is x LOG2E - refl, one operation, with the product ref LOG2E rounded
+// once, to refl; `rest` is what that left out, which the sums make good when they are taken out.
+struct LaneSums {
+    float ref = 0.f, refl = 0.f, rest = 0.f, z = 0.f, w = 0.f;
+    bool has = false;                                         // a finite logit was seen: ref is one
+    __device__ __forceinline__ RowSums out(int above) const {
+        const float e = __builtin_amdgcn_exp2f(-rest);
+        return {has ? ref : -INFINITY, z * e, (w - rest * z) * e * LN2, above};
+    }
+    __device__ __forceinline__ void move(float to) {
+        RowSums s = out(0);
+        sums_to(s, to);
+        has = true;
+        ref = to;
+        refl = fabsf(to) < FAR ? to * LOG2E : 0.f;            // far: not used
+        rest = fabsf(to) < FAR ? fmaf(to, LOG2E, -refl) : 0.f;
+        const float e = __builtin_amdgcn_exp2f(rest);         // out(), backwards
+        z = s.z * e;
+        w = s.w * e * LOG2E + rest * z;
+    }
+};
 
 struct TokenGiven {
     int token;                                                // -1: none
@@ -65,17 +93,140 @@ __device__ __forceinline__ TokenGiven given(const uint8_t* base, int token, int 
     return t;
 }
 
+// the float below x; of zeros of both signs, the one below them
+__device__ __forceinline__ float below(float x) { return order32_back(order32(x == 0.f ? -0.f : x) - 1); }
+
 __device__ u32x4 tl_nothing;                                  // what a row without a whole vector loads in its place
 
-// How many of a list, best first and `n` long, come in front of x; of equals those of lists in front
-__device__ __forceinline__ int in_front(const float* l, int n, float x, bool lower) {
-    int lo = 0, hi = n;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (l[mid] > x || (lower && l[mid] == x)) lo = mid + 1;
+// The columns of a row that a workgroup has, and how its lanes take them: lane l of wave w has, of step k, vectors u at columns
+// c0 + (k TL_WAVES + w) STEP + (64 u + l) VEC.  Columns are counted from the 16-byte boundary at or before the row's start, `mis` elements in
+// front of it.
+struct RowPiece {
+    const uint8_t* base;
+    int mis, vocab, c0, c1, in0, in1;                         // in0 .. in1: whole vectors inside the row
+};
+
+// logits of one vector, those outside the row or the piece as -inf
+template <typename L>
+__device__ __forceinline__ void edge_vector(const RowPiece& p, int v, float* f) {
+    if ((v < p.in0 || v > p.in1) && v < p.c1)                 // not wholly inside the row: element by element
+#pragma unroll
+        for (int e = 0; e < L::VEC; ++e) f[e] = L::at(p.base, min(max(v + e - p.mis, 0), p.vocab - 1));
+#pragma unroll
+    for (int e = 0; e < L::VEC; ++e) f[e] = v + e >= p.mis && v + e < p.c1 ? f[e] : -INFINITY;
+}
+
+struct TopShared {
+    uint32_t key[TL_WAVES * 64];                              // of the lanes' largest logits (0: no column)
+    int hit[TL_WAVES * 64];                                   // lanes in question
+    float x[TL_LIST];                                         // logits in question, their tokens
+    int tok[TL_LIST];
+    int hits, count, ties;
+};
+
+// Calls what(x, token) for the logits of the lanes in question, a vector a thread at a time.
+template <typename L, typename F>
+__device__ __forceinline__ void for_hits(const RowPiece& p, const TopShared& sh, F&& what) {
+    constexpr int VEC = L::VEC, VECS = L::VECS, STEP = 64 * VEC * VECS;
+    const int turns = (p.c1 - p.c0 + TL_WAVES * STEP - 1) / (TL_WAVES * STEP), per = turns * VECS, items = sh.hits * per;
+    for (int i = threadIdx.x; i < items; i += TL_WAVES * 64) {
+        const int h = i / per, r = i - h * per, lane = sh.hit[h];
+        const int v = p.c0 + (r / VECS * TL_WAVES + (lane >> 6)) * STEP + (r % VECS * 64 + (lane & 63)) * VEC;
+        if (v >= p.c1) continue;
+        float f[VEC];
+        if (v >= p.in0 && v <= p.in1) {
+            const u32x4 raw = *(const u32x4*)(p.base + (int64_t)(v - p.mis) * L::BYTES);
+            L::unpack(raw, f);
+        }
+        edge_vector<L>(p, v, f);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+            if (v + e >= p.mis && v + e < p.c1) what(counted(f[e]), v + e - p.mis);
+    }
+}
+
+// The n best logits of the piece, or all, in sh.x and sh.tok, with others beside them; returns how many there are.
+template <typename L>
+__device__ int best_of_piece(const RowPiece& p, TopShared& sh, uint32_t key, int n) {
+    const int lane = threadIdx.x & 63;
+    sh.key[threadIdx.x] = key;
+    if (threadIdx.x == 0) sh.hits = sh.count = 0;
+    __syncthreads();
+    // the n-th largest of the lanes' keys, bit by bit; fewer lanes with a column than that: the lowest key
+    uint32_t k4[TL_WAVES], bound = 0;
+#pragma unroll
+    for (int i = 0; i < TL_WAVES; ++i) k4[i] = sh.key[lane + 64 * i];
+    auto lanes_at = [&](uint32_t k) {
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < TL_WAVES; ++i) c += __popcll(__ballot(k4[i] >= k));
+        return c;
+    };
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t trial = bound | (1u << bit);
+        const int c = lanes_at(trial);
+        if (c >= n) bound = trial;
+        if (c == n) break;                                    // no bit below changes which lanes these are
+    }
+    bound = max(bound, 1u);
+    const uint64_t m = __ballot(key >= bound);
+    int at = 0;
+    if (lane == 0 && m) at = atomicAdd(&sh.hits, __popcll(m));
+    at = __builtin_amdgcn_readfirstlane(at);
+    if (key >= bound) sh.hit[at + __popcll(m & ((1ull << lane) - 1ull))] = threadIdx.x;
+    __syncthreads();
+    auto count_from = [&](uint32_t k) {                       // how many reach key k; the first TL_LIST of them go into the list
+        __syncthreads();
+        if (threadIdx.x == 0) sh.count = 0;
+        __syncthreads();
+        for_hits<L>(p, sh, [&](float x, int tok) {
+            if (order32(x + 0.f) >= k) {
+                const int i = atomicAdd(&sh.count, 1);
+                if (i < TL_LIST) {
+                    sh.x[i] = x;
+                    sh.tok[i] = tok;
+                }
+            }
+        });
+        __syncthreads();
+        return sh.count;
+    };
+    int c = count_from(bound);
+    if (c <= TL_LIST) return c;
+    // More than fit: a higher bound that at least n reach, between `bound` and the largest key; the same in every thread.
+    uint32_t lo = bound, hi = 0xff800001u;                    // (no key is above that of +inf)
+    while (hi - lo > 1) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        c = count_from(mid);
+        if (c >= n && c <= TL_LIST) return c;
+        if (c > TL_LIST) lo = mid;
         else hi = mid;
     }
-    return lo;
+    // Fewer than n above the logits of key `lo`, and more of those than fit: the lowest tokens of them, looked for in order.
+    c = count_from(hi);
+    const float level = order32_back(lo);
+    for (int v0 = p.c0 / L::VEC * L::VEC; v0 < p.c1 && c < n; v0 += TL_WAVES * 64) {
+        const int v = v0 + (int)threadIdx.x;
+        const bool in = v >= p.mis && v >= p.c0 && v < p.c1;
+        const bool tie = in && counted(L::at(p.base, min(max(v - p.mis, 0), p.vocab - 1))) == level;
+        const uint64_t t = __ballot(tie);
+        if (lane == 0) sh.hit[threadIdx.x >> 6] = __popcll(t);
+        __syncthreads();
+        int before = c, all = 0;
+#pragma unroll
+        for (int i = 0; i < TL_WAVES; ++i) {
+            if (i < (int)(threadIdx.x >> 6)) before += sh.hit[i];
+            all += sh.hit[i];
+        }
+        before += __popcll(t & ((1ull << lane) - 1ull));
+        if (tie && before < n) {
+            sh.x[before] = level;
+            sh.tok[before] = v - p.mis;
+        }
+        c = min(c + all, n);
+        __syncthreads();
+    }
+    return c;
 }
 
 template <typename L, bool TOP>
@@ -84,27 +235,28 @@ __global__ __launch_bounds__(TL_WAVES * 64) void logprob_kernel(const void* __re
                                                                 const LogprobOut out, RowSums* __restrict__ part,
                                                                 float* __restrict__ cand_x, int* __restrict__ cand_tok) {
     constexpr int VEC = L::VEC, VECS = L::VECS, E = VECS * VEC, STEP = 64 * E;
-    __shared__ LogitList lists[TOP ? TL_WAVES : 1];
+    __shared__ TopShared sh;                                  // (without TOP: not used, no LDS)
     __shared__ RowSums w_sums[TL_WAVES];
-    __shared__ int w_count[TL_WAVES];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t row = blockIdx.x / groups;
     const int group = (int)(blockIdx.x - row * groups);
-    const uint8_t* base = (const uint8_t*)logits + row * row_stride * L::BYTES;
-    // columns are counted from the 16-byte boundary at or before the row's start, `mis` elements in front of it
-    const int mis = (int)(((uintptr_t)base & 15) / L::BYTES);
-    const int v_end = vocab + mis;
-    const int64_t piece = (int64_t)(group * TL_WAVES + w) * cols;
-    const int c0 = (int)min(piece, (int64_t)v_end), c1 = (int)min(piece + cols, (int64_t)v_end);
+    RowPiece p;
+    p.base = (const uint8_t*)logits + row * row_stride * L::BYTES;
+    p.mis = (int)(((uintptr_t)p.base & 15) / L::BYTES);
+    p.vocab = vocab;
+    const int v_end = vocab + p.mis;
+    p.c0 = (int)min((int64_t)group * cols, (int64_t)v_end);
+    p.c1 = (int)min((int64_t)p.c0 + cols, (int64_t)v_end);
+    p.in0 = p.mis ? VEC : 0;
+    p.in1 = v_end / VEC * VEC - VEC;
 
-    u32x4 raw[VECS];                                          // a step's logits as stored, loaded one step ahead
-    const int in0 = mis ? VEC : 0, in1 = v_end / VEC * VEC - VEC;
-    const uint8_t* vec0 = in1 >= in0 ? base - (int64_t)mis * L::BYTES : (const uint8_t*)&tl_nothing;
-    const int lo = in1 >= in0 ? in0 : 0, hi = in1 >= in0 ? in1 : 0;
-    auto whole = [&](int v0) { return v0 >= mis && v0 + STEP <= c1; };
+    u32x4 raw[VECS];                                          // a step's logits as stored, loaded one step ahead, from whole vectors
+    const uint8_t* vec0 = p.in1 >= p.in0 ? p.base - (int64_t)p.mis * L::BYTES : (const uint8_t*)&tl_nothing;
+    const int lo = p.in1 >= p.in0 ? p.in0 : 0, hi = p.in1 >= p.in0 ? p.in1 : 0;
+    auto whole = [&](int v0) { return v0 >= p.mis && v0 + STEP <= p.c1; };
     auto load = [&](int v0) {
         if (whole(v0)) {
-            const uint8_t* at = base + (int64_t)(v0 - mis) * L::BYTES;
+            const uint8_t* at = p.base + (int64_t)(v0 - p.mis) * L::BYTES;
 #pragma unroll
             for (int u = 0; u < VECS; ++u) raw[u] = __builtin_nontemporal_load((const u32x4*)(at + (uint32_t)(1024 * u + 16 * lane)));
         } else {
@@ -115,73 +267,66 @@ __global__ __launch_bounds__(TL_WAVES * 64) void logprob_kernel(const void* __re
             }
         }
     };
-    load(c0);
-    const int token = tokens[row];
-    const TokenGiven tok = given<L>(base, token, vocab);
+    const int v_first = p.c0 + w * STEP;
+    load(v_first);
+    const TokenGiven tok = given<L>(p.base, tokens[row], vocab);
     // Logits above `after` count for the rank, in vectors that end in front of the token those at it too: above `before`.  (A masked
     // token: all in front of it count, which is added in the end.)
     const float after = tok.x;
-    const float before = !(tok.x > -INFINITY) || tok.token < 0 ? INFINITY : order32_back(order32(tok.x == 0.f ? -0.f : tok.x) - 1);
-    const int tok_v = tok.token < 0 ? -1 : tok.token + mis;   // its column
+    const float before = !(tok.x > -INFINITY) || tok.token < 0 ? INFINITY : below(tok.x);
+    const float counts = fminf(before, after);
+    const int tok_v = tok.token < 0 ? -1 : tok.token + p.mis; // its column
     int above = 0;
-    if (tok_v >= c0 && tok_v < c1) {                          // of the token's own vector, those in front of it: the equal ones, or, of
+    if (w == 0 && tok_v >= p.c0 && tok_v < p.c1) {            // of the token's own vector, those in front of it: the equal ones, or, of
         const int v = tok_v / VEC * VEC + lane;               // a masked token, those that would count twice
-        if (lane < VEC && v >= mis && v < tok_v) {
-            const float x = counted(L::at(base, v - mis));
+        if (lane < VEC && v >= p.mis && v < tok_v) {
+            const float x = counted(L::at(p.base, v - p.mis));
             above = tok.x > -INFINITY ? x == tok.x : -(int)(x > -INFINITY);
         }
     }
 
-    float thr = -INFINITY;
-    bool full = false;
-    int count = 0;
-    bool has = false;                                         // a finite logit was seen: ref is one
-    float ref = 0.f, z = 0.f, ws = 0.f;
-    for (int v0 = c0; v0 < c1; v0 += STEP) {
+    LaneSums sum;
+    float most = -INFINITY;
+    for (int v0 = v_first; v0 < p.c1; v0 += TL_WAVES * STEP) {
         float f[E];
 #pragma unroll
         for (int u = 0; u < VECS; ++u) L::unpack(raw[u], f + u * VEC);
-        if (!whole(v0)) {
+        if (!whole(v0)) {                                     // the row's and the piece's ends
 #pragma unroll
-            for (int u = 0; u < VECS; ++u) {
-                const int v = v0 + (u * 64 + lane) * VEC;
-                if (!(v >= mis && v + VEC <= c1))
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e)
-                        f[u * VEC + e] = v + e >= mis && v + e < c1 ? L::at(base, v + e - mis) : -INFINITY;
-            }
+            for (int u = 0; u < VECS; ++u) edge_vector<L>(p, v0 + (u * 64 + lane) * VEC, f + u * VEC);
         }
-        load(v0 + STEP);                                      // on its way behind this step's work
-        float mx4[E / 4], mx = -INFINITY;                     // of four logits, of all
+        load(v0 + TL_WAVES * STEP);                           // on its way behind this step's work
+        float mx = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < E / 4; ++k) {
-            mx4[k] = fmaxf(fmaxf(f[4 * k], f[4 * k + 1]), fmaxf(f[4 * k + 2], f[4 * k + 3]));
-            mx = fmaxf(mx, mx4[k]);
-        }
+        for (int k = 0; k < E; k += 2) mx = fmaxf(fmaxf(f[k], f[k + 1]), mx);
         if (__ballot(mx == INFINITY)) {                       // +inf counts as the largest finite value
 #pragma unroll
             for (int k = 0; k < E; ++k) f[k] = f[k] == INFINITY ? 3.402823466e38f : f[k];
             mx = mx == INFINITY ? 3.402823466e38f : mx;
-#pragma unroll
-            for (int k = 0; k < E / 4; ++k) mx4[k] = mx4[k] == INFINITY ? 3.402823466e38f : mx4[k];
         }
-        const bool moves = mx > -INFINITY && (!has || mx - ref > 8.f);
+        most = fmaxf(most, mx);
+        const bool moves = mx > -INFINITY && (!sum.has || mx - sum.ref > 8.f);
         if (__ballot(moves)) {
-            if (moves) {
-                RowSums s = {has ? ref : -INFINITY, z, ws, 0};
-                sums_to(s, mx);
-                ref = mx, z = s.z, ws = s.w;
-                has = true;
+            if (moves) sum.move(mx);
+        }
+        // 2^-150 is no float32 any more; -inf and NaN end there too
+        if (!__ballot(!(fabsf(sum.ref) < FAR))) {
+#pragma unroll
+            for (int k = 0; k < E; ++k) {
+                const float d = fmaxf(fmaf(f[k], LOG2E, -sum.refl), -150.f), e = __builtin_amdgcn_exp2f(d);
+                sum.z += e;
+                sum.w = fmaf(d, e, sum.w);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < E; ++k) {
+                const float x = fabsf(sum.ref) < FAR ? fmaf(f[k], LOG2E, -sum.refl) : (f[k] - sum.ref) * LOG2E;
+                const float d = fmaxf(x, -150.f), e = __builtin_amdgcn_exp2f(d);
+                sum.z += e;
+                sum.w = fmaf(d, e, sum.w);
             }
         }
-#pragma unroll
-        for (int k = 0; k < E; ++k) {
-            const float d = fmaxf(f[k] - ref, -104.f);        // e^-104 is no float32 any more; -inf and NaN end there too
-            const float e = exp_neg(d);
-            z += e;
-            ws = fmaf(d, e, ws);
-        }
-        if (__ballot(mx > fminf(before, after))) {
+        if (__ballot(mx > counts)) {
 #pragma unroll
             for (int u = 0; u < VECS; ++u) {
                 const float t = v0 + (u * 64 + lane) * VEC + VEC <= tok_v ? before : after;
@@ -189,24 +334,18 @@ __global__ __launch_bounds__(TL_WAVES * 64) void logprob_kernel(const void* __re
                 for (int e = 0; e < VEC; ++e) above += f[u * VEC + e] > t;
             }
         }
-        if constexpr (TOP) list_step<L>(lists[w], f, mx4, mx, n, v0, mis, c1, full, thr, count);
-    }
-    if constexpr (TOP) {
-        if (count > n) count = list_cut<2>(lists[w], count, n, thr);
-        if (count) count = list_prune(lists[w], count, n);
     }
     // ---- the wave's sums, the workgroup's
-    RowSums s = {has ? ref : -INFINITY, z, ws, above};
+    RowSums s = sum.out(above);
     sums_to(s, wave_max(s.m));
     s.z = wave_sum(s.z);
     s.w = wave_sum(s.w);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s.above += __shfl_xor(s.above, o, 64);
-    if (lane == 0) {
-        w_sums[w] = s;
-        w_count[w] = count;
-    }
-    __syncthreads();
+    if (lane == 0) w_sums[w] = s;
+    int kept = 0;
+    if constexpr (TOP) kept = best_of_piece<L>(p, sh, v_first + lane * VEC < p.c1 ? order32(most + 0.f) : 0u, n);
+    else __syncthreads();
     float m = w_sums[0].m;
 #pragma unroll
     for (int i = 1; i < TL_WAVES; ++i) m = fmaxf(m, w_sums[i].m);
@@ -225,74 +364,63 @@ __global__ __launch_bounds__(TL_WAVES * 64) void logprob_kernel(const void* __re
         else part[blockIdx.x] = all;
     }
     if constexpr (TOP) {
-        int have = 0;
-#pragma unroll
-        for (int i = 0; i < TL_WAVES; ++i) have += w_count[i];
-        const int e_w = threadIdx.x / n, e_i = threadIdx.x - e_w * n;         // an entry a thread: 4 n of them at most
-        int rank = 2 * LIST_MAX_N, id = -1;
-        float x = -INFINITY;
-        if (e_w < TL_WAVES && e_i < w_count[e_w]) {
-            x = lists[e_w].x[e_i];
-            id = lists[e_w].i[e_i];
-            rank = e_i;
-            for (int i = 0; i < TL_WAVES; ++i)
-                if (i != e_w) rank += in_front(lists[i].x, w_count[i], x, i < e_w);
-        }
-        if (groups == 1) {
-            if (rank < n) {
+        const int64_t at = (int64_t)blockIdx.x * n;
+        for (int i = threadIdx.x; i < kept; i += TL_WAVES * 64) {
+            const float x = sh.x[i];
+            const int id = sh.tok[i];
+            int rank = 0;
+            for (int j = 0; j < kept; ++j) rank += sh.x[j] > x || (sh.x[j] == x && sh.tok[j] < id);
+            if (rank >= n) continue;
+            if (groups == 1) {
                 out.top_tokens[row * n + rank] = id;
                 out.top_logprobs[row * n + rank] = log_prob(x, all, log_z);
-            }
-        } else {
-            const int64_t at = (int64_t)blockIdx.x * n;
-            if (rank < n) {
-                cand_x[at + rank] = x;
+            } else {
+                cand_x[at + rank] = x + 0.f;                  // no negative zero: the join goes by keys
                 cand_tok[at + rank] = id;
             }
-            if ((int)threadIdx.x >= have && (int)threadIdx.x < n) {           // fewer tokens than that in the group
-                cand_x[at + threadIdx.x] = -INFINITY;
-                cand_tok[at + threadIdx.x] = -1;
-            }
+        }
+        if (groups > 1 && (int)threadIdx.x >= kept && (int)threadIdx.x < n) { // fewer tokens than that in the piece
+            cand_x[at + threadIdx.x] = -INFINITY;
+            cand_tok[at + threadIdx.x] = -1;
         }
     }
 }
 
-// Joins the workgroups of a row.  Every group's list is in order, so an entry's rank is its place and a search in each other list; only
-// entries at or above the best of the lists' last ones can be among the n.
+// the largest of a wave's values, in every lane
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+#define TL_DPP(ctrl) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xf, 0xf, false))
+    TL_DPP(0x111);                                            // from 1, 2, 4, 8 lanes below within sixteen
+    TL_DPP(0x112);
+    TL_DPP(0x114);
+    TL_DPP(0x118);
+    TL_DPP(0x142);                                            // the last lane of sixteen to the next sixteen, of 32 to the next 32
+    TL_DPP(0x143);
+#undef TL_DPP
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+// Joins the workgroups of a row: their sums, and their lists, which are in order, by taking the best head n times (a lane a list; equal
+// heads: the lower list, whose tokens are the lower ones).
 constexpr int TJ_THREADS = 256;
 template <typename L, bool TOP>
 __global__ __launch_bounds__(TJ_THREADS) void logprob_join_kernel(const void* __restrict__ logits, int64_t row_stride,
                                                                   const int* __restrict__ tokens, int vocab, int groups, int n,
                                                                   const LogprobOut out, const RowSums* __restrict__ part,
                                                                   const float* __restrict__ cand_x, const int* __restrict__ cand_tok) {
-    extern __shared__ float l_x[];                            // [groups x n] logits, tokens behind them, then the entries in question
-    __shared__ int l_count[TL_MAX_GROUPS], s_count;
-    __shared__ float s_bound[TJ_THREADS / 64];
+    extern __shared__ uint32_t l_key[];                       // [groups x n] keys (0: no entry), tokens behind them
     const int64_t row = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, entries = groups * n;
-    int* l_tok = (int*)(l_x + entries);
-    uint16_t* l_at = (uint16_t*)(l_tok + entries);
-    const TokenGiven tok = given<L>((const uint8_t*)logits + row * row_stride * L::BYTES, tokens[row], vocab);
+    int* l_tok = (int*)(l_key + entries);
     if constexpr (TOP) {
-        for (int i = tid; i < groups; i += TJ_THREADS) l_count[i] = 0;
-        if (tid == 0) s_count = 0;
-        __syncthreads();
-        float bound = -INFINITY;
         for (int i = tid; i < entries; i += TJ_THREADS) {
-            const float x = cand_x[row * entries + i];
-            const int t = cand_tok[row * entries + i], g = i / n;
-            l_x[i] = x;
+            const int t = cand_tok[row * entries + i];
+            l_key[i] = t >= 0 ? order32(cand_x[row * entries + i]) : 0u;
             l_tok[i] = t;
-            if (t >= 0) {
-                atomicAdd(&l_count[g], 1);
-                if (i - g * n == n - 1) bound = fmaxf(bound, x);
-            }
         }
-        bound = wave_max(bound);
-        if (lane == 0) s_bound[tid >> 6] = bound;
     }
     RowSums s = {-INFINITY, 0.f, 0.f, 0};
     if (lane < groups) s = part[row * groups + lane];
+    const TokenGiven tok = given<L>((const uint8_t*)logits + row * row_stride * L::BYTES, tokens[row], vocab);
     sums_to(s, wave_max(s.m));
     s.z = wave_sum(s.z);
     s.w = wave_sum(s.w);
@@ -302,27 +430,28 @@ __global__ __launch_bounds__(TJ_THREADS) void logprob_join_kernel(const void* __
     if (tid == 0) write_row(out, row, tok, s, log_z);
     if constexpr (TOP) {
         __syncthreads();
-        float bound = s_bound[0];
-#pragma unroll
-        for (int i = 1; i < TJ_THREADS / 64; ++i) bound = fmaxf(bound, s_bound[i]);
-        for (int i = tid; i < entries; i += TJ_THREADS)
-            if (l_tok[i] >= 0 && l_x[i] >= bound) l_at[atomicAdd(&s_count, 1)] = (uint16_t)i;
-        __syncthreads();
-        const int count = s_count;
-        for (int c0 = 0; c0 < count; c0 += TJ_THREADS / 16) { // sixteen lanes an entry
-            const int c = c0 + tid / 16;
-            const int i = l_at[min(c, count - 1)], g = i / n;
-            const float x = l_x[i];
-            int rank = 0;
-            for (int o = tid & 15; o < groups; o += 16)
-                if (o != g) rank += in_front(l_x + o * n, l_count[o], x, o < g);
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) rank += __shfl_xor(rank, o, 64);
-            rank += i - g * n;
-            if (c < count && (tid & 15) == 0 && rank < n) {
-                out.top_tokens[row * n + rank] = l_tok[i];
-                out.top_logprobs[row * n + rank] = log_prob(x, s, log_z);
+        if (tid >= 64) return;
+        int at = lane * n;
+        const int end = lane < groups ? at + n : at;
+        uint32_t key = at < end ? l_key[at] : 0u, best = 0;
+        int head = at < end ? l_tok[at] : 0, id = 0;
+        for (int i = 0; i < n; ++i) {
+            const uint32_t m = wave_max_u32(key);
+            const int from = (int)__builtin_ctzll(__ballot(key == m));
+            const int t = __builtin_amdgcn_readlane(head, from);
+            if (lane == i) {
+                best = m;
+                id = t;
             }
+            if (lane == from) {
+                ++at;
+                key = at < end ? l_key[at] : 0u;
+                head = at < end ? l_tok[at] : 0;
+            }
+        }
+        if (lane < n) {
+            out.top_tokens[row * n + lane] = id;
+            out.top_logprobs[row * n + lane] = log_prob(order32_back(best), s, log_z);
         }
     }
 }
@@ -332,14 +461,14 @@ struct LogprobPlan {
     size_t x, tok, bytes;
 };
 LogprobPlan logprob_plan(int64_t rows, int64_t vocab, int n, int dtype) {
-    constexpr int64_t STEP = 64 * 16;                         // logits of a wave's step, of either width
+    constexpr int64_t STEP = TL_WAVES * 64 * 16;              // logits of a workgroup's step, of either width
     const int64_t span = vocab + (dtype == MF_FP32 ? 3 : 7);
-    int64_t cols = std::max<int64_t>(STEP, rows * span / 8192);
-    cols = std::max(cols, (span + TL_MAX_GROUPS * TL_WAVES - 1) / (TL_MAX_GROUPS * TL_WAVES));
+    int64_t cols = std::max<int64_t>(STEP, rows * span / 2048);
+    cols = std::max(cols, (span + TL_MAX_GROUPS - 1) / TL_MAX_GROUPS);
     cols = std::min((cols + STEP - 1) / STEP * STEP, (span + STEP - 1) / STEP * STEP);
     LogprobPlan p;
     p.cols = (int)cols;
-    p.groups = (int)((span + cols * TL_WAVES - 1) / (cols * TL_WAVES));
+    p.groups = (int)((span + cols - 1) / cols);
     const size_t parts = p.groups == 1 ? 0 : (size_t)rows * p.groups;
     p.x = parts * sizeof(RowSums);
     p.tok = p.x + parts * n * 4;
@@ -350,7 +479,7 @@ LogprobPlan logprob_plan(int64_t rows, int64_t vocab, int n, int dtype) {
 }  // namespace
 
 extern "C" size_t mf_token_logprobs_workspace_bytes(int rows, int vocab, int n_top, int dtype) {
-    if (rows <= 0 || vocab <= 0 || n_top < 0 || n_top > LIST_MAX_N || dtype < 0 || dtype > MF_FP32) return 0;
+    if (rows <= 0 || vocab <= 0 || n_top < 0 || n_top > TL_MAX_N || dtype < 0 || dtype > MF_FP32) return 0;
     return logprob_plan(rows, vocab, n_top, dtype).bytes;
 }
 
@@ -359,8 +488,8 @@ extern "C" int mf_token_logprobs(float* logprobs, int32_t* ranks, float* entropy
                                  void* workspace, size_t workspace_bytes, void* stream) {
     MF_REQUIRE(dtype == MF_BF16 || dtype == MF_FP16 || dtype == MF_FP32, "token_logprobs: dtype must be bf16, fp16 or fp32");
     MF_REQUIRE(rows >= 0 && rows < (1 << 24) && vocab > 0 && vocab <= TL_MAX_VOCAB, "token_logprobs: %d rows of %d tokens", rows, vocab);
-    MF_REQUIRE(n_top >= 0 && n_top <= LIST_MAX_N && n_top <= vocab, "token_logprobs: %d alternatives of %d tokens, up to %d", n_top, vocab,
-               LIST_MAX_N);
+    MF_REQUIRE(n_top >= 0 && n_top <= TL_MAX_N && n_top <= vocab, "token_logprobs: %d alternatives of %d tokens, up to %d", n_top, vocab,
+               TL_MAX_N);
     if (rows == 0) return 0;
     if (row_stride <= 0) row_stride = vocab;
     MF_REQUIRE(row_stride >= vocab, "token_logprobs: row stride %lld below the vocabulary's %d", (long long)row_stride, vocab);
@@ -376,7 +505,7 @@ extern "C" int mf_token_logprobs(float* logprobs, int32_t* ranks, float* entropy
     const LogprobOut out = {logprobs, ranks, entropy, top_tokens, top_logprobs};
     hipStream_t st = (hipStream_t)stream;
     const dim3 grid((unsigned)rows * (unsigned)p.groups);
-    const size_t lds = (size_t)p.groups * n_top * 10;
+    const size_t lds = (size_t)p.groups * n_top * 8;
 #define TL_LAUNCH2(L, TOP)                                                                                                              \
     do {                                                                                                                                \
         hipLaunchKernelGGL((logprob_kernel<L, TOP>), grid, dim3(TL_WAVES * 64), 0, st, logits, row_stride, tokens, vocab, p.cols, p.groups, \
