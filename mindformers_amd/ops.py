@@ -1037,6 +1037,9 @@ def token_logprobs(logits, tokens, n_top=0):
 
 
 # --------------------------------------------------------------------------------------------- low-rank adapters
+_INTS = [ctypes.c_int32 * n for n in range(9)]                # host arrays of slices
+
+
 class AdapterRows(NamedTuple):
     """What ``adapter_rows`` returns: the rows of a step sorted by adapter, for every projection of the step."""
     plan: torch.Tensor
@@ -1068,43 +1071,56 @@ def adapter_linear(x, lora_a, lora_b, rows, base, widths=None, ranks=None, scale
     [n, slices, R, K] (one slice: [n, R, K] too); ``lora_b`` [n, N, R] holds them one after the other.  ``ranks`` int32 [n]: each adapter's
     own, up to R (None: R); ``scales`` fp32 [n] (None: 1).  ``out``: base itself (in place) or memory of its own.  K and R multiples
     of 8, R up to 128, 8 slices."""
-    lib = _lib.load()
-    dev = _dev_of(x, base, out)
-    _need(_dev_ok(lora_a, lora_b, rows.plan, ranks, scales) == dev, "all tensors must be on the same device")
-    t, n = rows.tokens, rows.adapters
-    _need(lora_a.dim() in (3, 4) and lora_b.dim() == 3 and lora_a.shape[0] == n and lora_b.shape[0] == n,
-          "lora_a must be [n, slices, R, K] and lora_b [n, N, R] for the adapters of rows")
-    k, r, cols = lora_a.shape[-1], lora_a.shape[-2], lora_b.shape[1]
+    plan, t, n, tile = rows
+    ashape, bshape, dtype = lora_a.shape, lora_b.shape, lora_a.dtype
+    if not (len(ashape) in (3, 4) and len(bshape) == 3 and ashape[0] == n and bshape[0] == n):
+        raise ValueError("lora_a must be [n, slices, R, K] and lora_b [n, N, R] for the adapters of rows")
+    r, k, cols = ashape[-2], ashape[-1], bshape[1]
     widths = (cols,) if widths is None else tuple(widths)
     slices = len(widths)
     if sum(widths) != cols or not 1 <= slices <= 8 or min(widths) < 1:
         raise ValueError(f"1 to 8 slices that make up lora_b's {cols} columns, got widths {widths}")
-    _need(lora_b.shape[2] == r and (lora_a.shape[1] == slices if lora_a.dim() == 4 else slices == 1), "lora_a and lora_b do not match")
+    if bshape[2] != r or (ashape[1] if len(ashape) == 4 else 1) != slices:
+        raise ValueError("lora_a and lora_b do not match")
     if k % 8 or r % 8 or not 0 < r <= 128 or not k:
         raise ValueError(f"input width {k} and rank {r} must be multiples of 8, the rank up to 128")
-    _need(x.dtype in _ACT and base.dtype == x.dtype and lora_a.dtype == x.dtype and lora_b.dtype == x.dtype, "dtype mismatch")
-    _need(x.dim() >= 1 and x.shape[-1] == k and base.dim() >= 1 and base.shape[-1] == cols, "x must be [T, K], base [T, N]")
-    if ranks is not None:
-        _need(ranks.dtype == torch.int32 and ranks.numel() == n, "ranks must be int32 [n]")
-    if scales is not None:
-        _need(scales.dtype == torch.float32 and scales.numel() == n, "scales must be fp32 [n]")
+    index = lora_a.get_device()                               # -1: not a GPU
+    if not (index >= 0 and lora_b.get_device() == index and plan.get_device() == index and x.get_device() == index
+            and base.get_device() == index and (out is None or out.get_device() == index)
+            and lora_a.is_contiguous() and lora_b.is_contiguous() and plan.is_contiguous()):
+        _dev_ok(lora_a, lora_b, plan)                         # says what is wrong
+        _dev_of(lora_a, x, base, out)
+    if not (dtype in _ACT and x.dtype is dtype and base.dtype is dtype and lora_b.dtype is dtype):
+        raise ValueError("x, base, lora_a and lora_b must share a bf16/fp16 dtype")
+    if ranks is not None and not (ranks.dtype is torch.int32 and ranks.numel() == n and ranks.get_device() == index and ranks.is_contiguous()):
+        raise ValueError("ranks must be a contiguous int32 [n] on the adapters' device")
+    if scales is not None and not (scales.dtype is torch.float32 and scales.numel() == n and scales.get_device() == index and scales.is_contiguous()):
+        raise ValueError("scales must be a contiguous fp32 [n] on the adapters' device")
+    if x.shape[-1:] != (k,) or base.shape[-1:] != (cols,):
+        raise ValueError(f"x must be [T, {k}], base [T, {cols}]")
     x, xs = _rows(x, k, "x")
-    if x.data_ptr() % 16 or xs % 8:                           # a slice whose rows are not on 16-byte borders
+    at = x.data_ptr()
+    if at % 16 or xs % 8:                                     # a slice whose rows are not on 16-byte borders
         x, xs = x.reshape(-1, k).clone(memory_format=torch.contiguous_format), k
-    if out is None:
-        out = torch.empty(base.shape, dtype=base.dtype, device=dev)
+        at = x.data_ptr()
     base, bs = _rows(base, cols, "base")
-    got, os = _rows(out, cols, "out")
-    if not (x.numel() == t * k and base.numel() == t * cols and got.numel() == t * cols and got.dtype == x.dtype):
-        raise ValueError(f"x, base and out must hold the {t} rows that adapter_rows was given")
+    if out is None:
+        out = torch.empty_like(base) if base.is_contiguous() else base.new_empty(base.shape)
+        got, os = out, cols
+    else:
+        got, os = _rows(out, cols, "out")
+    if not (x.numel() == t * k and base.numel() == t * cols and got.numel() == t * cols and got.dtype is dtype):
+        raise ValueError(f"x, base and out must hold the {t} rows that adapter_rows was given, of one type")
     if t == 0:
         return out
-    _need(lora_a.data_ptr() % 16 == 0 and lora_b.data_ptr() % 16 == 0, "lora_a and lora_b must lie on 16-byte borders")
-    ws = workspace(lib.mf_adapter_workspace_bytes(t, n, rows.tile, k, slices, r), dev, "adapter")
+    pa, pb = lora_a.data_ptr(), lora_b.data_ptr()
+    _need((pa | pb) % 16 == 0, "lora_a and lora_b must lie on 16-byte borders")
+    lib, dev = _lib.load(), lora_a.device
+    ws = workspace(lib.mf_adapter_workspace_bytes(t, n, tile, k, slices, r), dev, "adapter")
     with _on(dev):
-        check(lib.mf_adapter_linear(ptr(got), ptr(x), ptr(lora_a), ptr(lora_b), ptr(base), ptr(rows.plan), ptr(ranks), ptr(scales),
-                                    (ctypes.c_int32 * slices)(*widths), slices, t, n, rows.tile, k, r, xs, bs, os,
-                                    dtype_code(x.dtype), ptr(ws), ws.numel(), stream_ptr(dev)), "mf_adapter_linear")
+        check(lib.mf_adapter_linear(got.data_ptr(), at, pa, pb, base.data_ptr(), plan.data_ptr(), ptr(ranks), ptr(scales),
+                                    _INTS[slices](*widths), slices, t, n, tile, k, r, xs, bs, os, dtype_code(dtype), ws.data_ptr(),
+                                    ws.numel(), stream_ptr(dev)), "mf_adapter_linear")
     return out
 
 
