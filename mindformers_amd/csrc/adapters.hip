@@ -164,7 +164,7 @@ struct AdapterArgs {
     float* h;                                                 // [cuts][tokens][slices x rank]
     int64_t x_stride, base_stride, out_stride;
     int tokens, k, rank, cuts, cut_units, blocks;             // cut_units: of 64 columns of x; blocks: of rank tiles
-    int max_tiles;
+    int max_tiles, subs;                                      // subs: pieces of a tile that the second product takes
     int groups_each;                                          // column groups of a wave
     int pitch;                                                // 16-bit values of a row of h in LDS
     int vec_io;                                               // base and out rows on 16-byte borders
@@ -173,14 +173,16 @@ struct AdapterArgs {
 
 __device__ __forceinline__ int adapter_rank(const AdapterArgs& A, int a) { return A.ranks ? min(max(A.ranks[a], 0), A.rank) : A.rank; }
 
-// h of RT x 16 rows and up to CT tiles of 16 ranks (of whatever slices), over one cut of K.  Lane l of a fragment holds rank or row
-// l & 15 and 8 values from 8 (l >> 4) on, as both operands lie in memory.  The waves take units of 64 columns in turn, half a unit's
-// loads on their way behind the products of the other half, and meet in LDS.  The workgroups that share x (of one tile and cut) run next
-// to each other on one XCD.
+// h of RT x 16 rows and up to CT tiles of 16 ranks (of whatever slices), over one cut of K.  The waves take units of 64 columns in turn
+// and meet in LDS.  A wave's unit goes through LDS of its own: it is loaded 8 lanes a row, as it lies in memory, and read back as the
+// matrix instruction wants it, a row a lane (loaded that way, every four lanes name four cache lines, and the vector memory unit takes
+// as many turns: 16 bytes a clock and compute unit).  The next unit is on its way meanwhile.  The workgroups that share x (of one tile
+// and cut) run next to each other on one XCD.
 template <typename T, int RT, int CT>
 __global__ __launch_bounds__(AD_WAVES * 64) void adapter_shrink_kernel(const AdapterArgs A) {
-    constexpr int N = RT * CT, SENT = N % 4 == 0 ? N / 2 : N;
-    __shared__ f32x4 red[AD_WAVES][SENT][64];
+    constexpr int N = RT * CT, ROWS = (RT + CT) * 16, SENT = N % 4 == 0 ? N / 2 : N;
+    static_assert(SENT * 64 <= ROWS * 8, "the waves' sums go where their units were");
+    __shared__ u32x4 stage[AD_WAVES][ROWS * 8];               // rows of 8 pieces of 16 bytes, piece p of row r at p ^ (r & 7)
     const int id = blockIdx.x, turn = id >> 3, item = turn / A.blocks * 8 + (id & 7), z = turn % A.blocks;
     const int cut = item / A.max_tiles;
     if (cut >= A.cuts) return;
@@ -190,51 +192,57 @@ __global__ __launch_bounds__(AD_WAVES * 64) void adapter_shrink_kernel(const Ada
     const int per = (rank + 15) >> 4, units = per * A.s.n, c0 = z * CT;
     if (c0 >= units) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, i16 = lane & 15;
-    const uint16_t* xr[RT];
+    const int r8 = lane >> 3, p8 = lane & 7;
+    const uint16_t* xr[2 * RT];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) xr[r] = A.x + (int64_t)A.order[tile.first + min(r * 16 + i16, tile.count - 1)] * A.x_stride + 8 * q;
-    const uint16_t* ar[CT];
+    for (int r = 0; r < 2 * RT; ++r) xr[r] = A.x + (int64_t)A.order[tile.first + min(r * 8 + r8, tile.count - 1)] * A.x_stride;
+    const uint16_t* a0 = A.a + (int64_t)tile.adapter * A.s.n * A.rank * A.k;
+    int64_t ar[2 * CT];
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {                            // tiles past the last one, ranks past the adapter's: others once more
-        const int u = min(c0 + c, units - 1), s = u / per, row = min((u - s * per) * 16 + i16, rank - 1);
-        ar[c] = A.a + ((int64_t)(tile.adapter * A.s.n + s) * A.rank + row) * A.k + 8 * q;
+    for (int c = 0; c < 2 * CT; ++c) {                        // tiles past the last one, ranks past the adapter's: others once more
+        const int u = min(c0 + c / 2, units - 1), s = u / per, row = min((u - s * per) * 16 + (c & 1) * 8 + r8, rank - 1);
+        ar[c] = (int64_t)(s * A.rank + row) * A.k;
     }
     f32x4 acc[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
     const int u_end = min((cut + 1) * A.cut_units, (A.k + 63) >> 6);
-    const int last = A.k - 8 - 8 * q;                         // where this lane's last whole piece starts
-    constexpr int NB = RT == 1 ? 4 : 2;                       // half units on their way
-    u32x4 xv[NB][RT], av[NB][CT];
-    auto load = [&](int b, int u) {
-        const int k = u * 64 + (b & 1) * 32, at = min(k, last);       // last may be negative: then this lane's piece starts in front
+    u32x4 in[2 * (RT + CT)];
+    auto load = [&](int u) {
+        const int k = u * 64 + 8 * p8, at = min(k, A.k - 8);
 #pragma unroll
-        for (int r = 0; r < RT; ++r) xv[b][r] = *(const u32x4*)(xr[r] + at);
+        for (int c = 0; c < 2 * CT; ++c) in[2 * RT + c] = *(const u32x4*)(a0 + ar[c] + at);
 #pragma unroll
-        for (int c = 0; c < CT; ++c) av[b][c] = *(const u32x4*)(ar[c] + at);
+        for (int r = 0; r < 2 * RT; ++r) in[r] = *(const u32x4*)(xr[r] + at);
+        if (k != at)                                          // behind the row's end: nothing
+#pragma unroll
+            for (int r = 0; r < 2 * RT; ++r) in[r] = (u32x4){0, 0, 0, 0};
     };
-    auto product = [&](int b, int u) {
-        if (u * 64 + (b & 1) * 32 > last)                     // behind the row's end: nothing
+    u32x4* mine = stage[w];
+    int u = cut * A.cut_units + w;
+    if (u < u_end) load(u);
+    for (; u < u_end; u += AD_WAVES) {
+        sort_fence();                                         // (a wave's LDS operations take place in order)
 #pragma unroll
-            for (int r = 0; r < RT; ++r) xv[b][r] = (u32x4){0, 0, 0, 0};
+        for (int i = 0; i < 2 * (RT + CT); ++i) mine[(i * 8 + r8) * 8 + (p8 ^ r8)] = in[i];
+        sort_fence();
+        if (u + AD_WAVES < u_end) load(u + AD_WAVES);
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
+        for (int half = 0; half < 2; ++half) {
+            u32x4 xv[RT];
 #pragma unroll
-            for (int c = 0; c < CT; ++c)
-                acc[r * CT + c] = T::mfma16(bitcast<typename T::vec8>(av[b][c]), bitcast<typename T::vec8>(xv[b][r]), acc[r * CT + c]);
-    };
-    const int u0 = cut * A.cut_units + w;
+            for (int r = 0; r < RT; ++r) xv[r] = mine[(r * 16 + i16) * 8 + ((4 * half + q) ^ (i16 & 7))];
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-        if (u0 + b / 2 * AD_WAVES < u_end) load(b, u0 + b / 2 * AD_WAVES);
-    for (int u = u0; u < u_end; u += NB / 2 * AD_WAVES)
+            for (int c = 0; c < CT; ++c) {
+                const u32x4 av = mine[((RT + c) * 16 + i16) * 8 + ((4 * half + q) ^ (i16 & 7))];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const int now = u + b / 2 * AD_WAVES, next = now + NB / 2 * AD_WAVES;
-            if (now >= u_end) break;
-            product(b, now);
-            if (next < u_end) load(b, next);
+                for (int r = 0; r < RT; ++r)
+                    acc[r * CT + c] = T::mfma16(bitcast<typename T::vec8>(av), bitcast<typename T::vec8>(xv[r]), acc[r * CT + c]);
+            }
         }
+    }
+    __syncthreads();
+    u32x4(*red)[ROWS * 8] = stage;                            // float32 from here on
     const int width = A.s.n * A.rank;
     auto store = [&](int t, const f32x4& v) {
         const int r = t / CT, c = t - r * CT, u = c0 + c;
@@ -243,151 +251,39 @@ __global__ __launch_bounds__(AD_WAVES * 64) void adapter_shrink_kernel(const Ada
         if (row < tile.count && j < A.rank) *(f32x4*)(A.h + ((int64_t)cut * A.tokens + tile.first + row) * width + s * A.rank + j) = v;
     };
     if constexpr (N % 4 == 0) {                               // halves exchanged with wave w ^ 2, halves of those with wave w ^ 1
-        f32x4 mine[N / 2], last4[N / 4];
+        f32x4 half[N / 2], quarter[N / 4];
         // (branches, not selections: those would put the accumulators into memory)
         auto exchange = [&](auto n, bool up, const f32x4* v, f32x4* kept, int other) {
             constexpr int H = decltype(n)::value;
             if (up) {
 #pragma unroll
-                for (int i = 0; i < H; ++i) { red[w][i][lane] = v[i]; kept[i] = v[H + i]; }
+                for (int i = 0; i < H; ++i) { red[w][i * 64 + lane] = bitcast<u32x4>(v[i]); kept[i] = v[H + i]; }
             } else {
 #pragma unroll
-                for (int i = 0; i < H; ++i) { red[w][i][lane] = v[H + i]; kept[i] = v[i]; }
+                for (int i = 0; i < H; ++i) { red[w][i * 64 + lane] = bitcast<u32x4>(v[H + i]); kept[i] = v[i]; }
             }
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < H; ++i) kept[i] += red[other][i][lane];
+            for (int i = 0; i < H; ++i) kept[i] += bitcast<f32x4>(red[other][i * 64 + lane]);
             __syncthreads();
         };
-        exchange(std::integral_constant<int, N / 2>{}, w & 2, acc, mine, w ^ 2);
-        exchange(std::integral_constant<int, N / 4>{}, w & 1, mine, last4, w ^ 1);
+        exchange(std::integral_constant<int, N / 2>{}, w & 2, acc, half, w ^ 2);
+        exchange(std::integral_constant<int, N / 4>{}, w & 1, half, quarter, w ^ 1);
         const int t0 = (w & 2 ? N / 2 : 0) + (w & 1 ? N / 4 : 0);
 #pragma unroll
-        for (int i = 0; i < N / 4; ++i) store(t0 + i, last4[i]);
+        for (int i = 0; i < N / 4; ++i) store(t0 + i, quarter[i]);
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) red[w][i][lane] = acc[i];
+        for (int i = 0; i < N; ++i) red[w][i * 64 + lane] = bitcast<u32x4>(acc[i]);
         __syncthreads();
         for (int t = w; t < N; t += AD_WAVES) {
-            f32x4 v = red[0][t][lane];
+            f32x4 v = bitcast<f32x4>(red[0][t * 64 + lane]);
 #pragma unroll
-            for (int o = 1; o < AD_WAVES; ++o) v += red[o][t][lane];
+            for (int o = 1; o < AD_WAVES; ++o) v += bitcast<f32x4>(red[o][t * 64 + lane]);
             store(t, v);
         }
     }
 }
-
-// out = base + (B h) for groups of 64 columns of one slice and RT x 16 rows, h in LDS as hi and lo planes [2][RT x 16][pitch].  The product
-// is taken with the columns as the matrix instruction's rows, in an order that leaves a lane twice 8 columns side by side of one
-// row: base and out move in 16 bytes a lane, 64 a row and instruction.  A group's base rows and first two rank tiles are loaded
-// behind the group before it.
-template <typename T, int RT>
-struct ColumnGroups {
-    const AdapterArgs& A;
-    int adapter, count, rank, per, first, cols, q, i16;
-    int rows[RT];
-    u32x4 bv[2][4], raw[RT][2];
-
-    __device__ __forceinline__ ColumnGroups(const AdapterArgs& args, const AdapterTile& tile, int rk, int s)
-        : A(args), adapter(tile.adapter), count(tile.count), rank(rk), per((rk + 15) >> 4), first(args.s.first[s]), cols(args.s.width[s]),
-          q((threadIdx.x & 63) >> 4), i16(threadIdx.x & 15) {
-#pragma unroll
-        for (int r = 0; r < RT; ++r) rows[r] = A.order[tile.first + min(r * 16 + i16, count - 1)];
-    }
-    __device__ __forceinline__ bool whole(int c0) const { return A.vec_io && c0 + AD_GROUP <= cols && (first & 7) == 0; }
-    __device__ __forceinline__ void load_b(int b, int c0, int t) {    // rank tile t of the group's columns, 8 ranks a lane
-        const int k = min(t * 16 + 8 * (q & 1), A.rank - 8);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int n = min(c0 + (j >> 1) * 32 + (i16 >> 2) * 8 + (j & 1) * 4 + (i16 & 3), cols - 1);
-            bv[b][j] = *(const u32x4*)(A.b + ((int64_t)adapter * A.s.total + first + n) * A.rank + k);
-        }
-    }
-    __device__ __forceinline__ void load(int c0) {
-        if (rank) {
-            load_b(0, c0, 0);
-            if (per > 1) load_b(1, c0, 1);
-        }
-        if (whole(c0))
-#pragma unroll
-            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                for (int p = 0; p < 2; ++p)
-                    raw[r][p] = *(const u32x4*)(A.base + (int64_t)rows[r] * A.base_stride + first + c0 + 32 * p + 8 * q);
-    }
-    // groups from column c0 on, `step` columns apart, up to `end`; load(c0) has been called
-    __device__ __forceinline__ void run(int c0, int step, int end, const uint16_t* planes, int pitch, const float* factor) {
-        const uint16_t* mine = planes + (((threadIdx.x & 63) >> 5) * RT * 16 + i16) * pitch + 8 * (q & 1);
-        float f[RT];
-#pragma unroll
-        for (int r = 0; r < RT; ++r) f[r] = rank ? factor[r * 16 + i16] : 0.f;
-        for (; c0 < end; c0 += step) {
-            f32x4 acc[RT][4];
-#pragma unroll
-            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[r][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-            auto product = [&](int b, int t) {
-                const int left = rank - (t * 16 + 8 * (q & 1));
-                if (t == per - 1 && (rank & 15)) {            // behind the adapter's rank, whatever lies there
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) bv[b][j][e] &= left >= 2 * e + 2 ? 0xffffffffu : left == 2 * e + 1 ? 0xffffu : 0u;
-                }
-#pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    const u32x4 hv = *(const u32x4*)(mine + r * 16 * pitch + t * 16);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        acc[r][j] = T::mfma16(bitcast<typename T::vec8>(bv[b][j]), bitcast<typename T::vec8>(hv), acc[r][j]);
-                }
-            };
-            for (int t = 0; t < per; t += 2) {
-                product(0, t);
-                if (t + 2 < per) load_b(0, c0, t + 2);
-                if (t + 1 < per) {
-                    product(1, t + 1);
-                    if (t + 3 < per) load_b(1, c0, t + 3);
-                }
-            }
-            const bool vec = whole(c0);
-            u32x4 had[RT][2];
-#pragma unroll
-            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                for (int p = 0; p < 2; ++p) had[r][p] = raw[r][p];
-            if (c0 + step < end) load(c0 + step);
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                if (r * 16 + i16 >= count) continue;
-                uint16_t* out = A.out + (int64_t)rows[r] * A.out_stride + first + c0 + 8 * q;
-                if (vec) {
-#pragma unroll
-                    for (int p = 0; p < 2; ++p) {
-                        float x[8];
-                        unpack8<T>(had[r][p], x);
-                        u32x4 o = had[r][p];
-                        if (rank)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                o[e] = pack2<T>(fmaf(acc[r][2 * p + (e >> 1)][2 * (e & 1)], f[r], x[2 * e]),
-                                                fmaf(acc[r][2 * p + (e >> 1)][2 * (e & 1) + 1], f[r], x[2 * e + 1]));
-                        *(u32x4*)(out + 32 * p) = o;
-                    }
-                } else {
-                    const uint16_t* base = A.base + (int64_t)rows[r] * A.base_stride + first + c0 + 8 * q;
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int at = (e >> 3) * 32 + (e & 7);
-                        if (c0 + 8 * q + at < cols)
-                            out[at] = rank ? T::from_float(fmaf(acc[r][e >> 2][e & 3], f[r], T::to_float(base[at]))) : base[at];
-                    }
-                }
-            }
-        }
-    }
-};
 
 // A row of h, scaled, to the planes: sixteen lanes a row, v[i] the ranks 64 i + 4 (lane & 15) .. + 3 of it; what lies at or behind the
 // adapter's rank becomes zero.  `factor` gets what the products of the row are to be multiplied with.
@@ -417,7 +313,7 @@ __device__ __forceinline__ void row_to_planes(f32x4* v, float scale, int rank, i
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int j = 64 * i + 4 * i16;
-        if (j >= (rank + 15) / 16 * 16) continue;
+        if (j >= (rank + 31) / 32 * 32) continue;
         uint32_t hi[2], lo[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -441,24 +337,52 @@ __device__ __forceinline__ int slice_of(const AdapterArgs& A, int& block, int bl
     }
 }
 
-// The second product by itself: a workgroup adds up the cuts of its rows' h and computes 4 x groups_each groups of columns.  The first
-// group's loads are in front of those of h.
+// out = base + (B h): a workgroup adds up the cuts of RT x 16 rows' h, puts them into LDS as hi and lo, and computes 4 x groups_each groups
+// of 64 columns of one slice.  The product is taken with the columns as the matrix instruction's rows, 32 ranks at a time, once with hi
+// and once with lo; its results go through LDS (of the wave's own) into rows of 128 bytes, eight lanes each, as base and out are moved.  A
+// group's base rows and its first 64 ranks of B are loaded behind the group before it, the first one's in front of the sums of h.
+constexpr int AD_PITCH = AD_GROUP + 4;                        // floats of a row of results
 template <typename T, int RT>
 __global__ __launch_bounds__(AD_WAVES * 64) void adapter_expand_kernel(const AdapterArgs A) {
     constexpr int ROWS = RT * 16, NV = AD_MAX_RANK / 64;
-    extern __shared__ __align__(16) uint16_t planes[];
-    __shared__ float factor[ROWS];
-    const AdapterTile tile = A.tiles[blockIdx.x];
+    extern __shared__ __align__(16) uint16_t planes[];        // [2][ROWS][pitch]
+    __shared__ __align__(16) float turned[AD_WAVES][16 * AD_PITCH];
+    __shared__ float factor[ROWS];                            // what a row's products are to be multiplied with
+    AdapterTile tile = A.tiles[blockIdx.x / A.subs];
+    tile.first += blockIdx.x % A.subs * ROWS;
+    tile.count = min(tile.count - (int)(blockIdx.x % A.subs) * ROWS, ROWS);
     if (tile.count <= 0) return;
     const int rank = tile.adapter < 0 ? 0 : adapter_rank(A, tile.adapter);
     if (rank == 0 && A.out == A.base) return;
+    const int block_cols = AD_GROUP * AD_WAVES * A.groups_each;
     int block = blockIdx.y;
-    const int block_cols = AD_GROUP * AD_WAVES * A.groups_each, s = slice_of(A, block, block_cols);
+    const int s = slice_of(A, block, block_cols);
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, i16 = lane & 15;
-    const int width = A.s.n * A.rank;
-    ColumnGroups<T, RT> groups(A, tile, rank, s);
-    const int c0 = block * block_cols + w * AD_GROUP, end = min((block + 1) * block_cols, groups.cols);
-    if (c0 < end) groups.load(c0);
+    const int r8 = lane >> 3, p8 = lane & 7;
+    const int per = (rank + 31) >> 5, width = A.s.n * A.rank, first = A.s.first[s], cols = A.s.width[s];
+    const int start = block * block_cols + w * AD_GROUP;
+    const int end = min((block + 1) * block_cols, cols);
+    int rows[2 * RT];
+#pragma unroll
+    for (int r = 0; r < 2 * RT; ++r) rows[r] = A.order[tile.first + min(r * 8 + r8, tile.count - 1)];
+    u32x4 bv[2][4], raw[2 * RT];
+    const uint16_t* b0 = A.b + ((int64_t)max(tile.adapter, 0) * A.s.total + first) * A.rank;
+    auto load_b = [&](int c0, int b, int t) {                 // 32 ranks of the group's columns
+        const int k = min(t * 32 + 8 * q, A.rank - 8);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bv[b][j] = *(const u32x4*)(b0 + (int64_t)min(c0 + 16 * j + i16, cols - 1) * A.rank + k);
+    };
+    auto whole = [&](int c0) { return A.vec_io && (first & 7) == 0 && c0 + 8 * p8 + 8 <= cols; };
+    auto load = [&](int c0) {
+        if (rank) {
+            load_b(c0, 0, 0);
+            if (per > 1) load_b(c0, 1, 1);
+        }
+        if (whole(c0))
+#pragma unroll
+            for (int r = 0; r < 2 * RT; ++r) raw[r] = *(const u32x4*)(A.base + (int64_t)rows[r] * A.base_stride + first + c0 + 8 * p8);
+    };
+    if (start < end) load(start);
     if (rank) {
         const float scale = A.scales ? A.scales[tile.adapter] : 1.f;
         f32x4 v[RT][NV];
@@ -488,27 +412,98 @@ __global__ __launch_bounds__(AD_WAVES * 64) void adapter_expand_kernel(const Ada
         for (int r = 0; r < RT; ++r) row_to_planes<T>(v[r], scale, rank, (r * AD_WAVES + w) * 4 + q, ROWS, planes, A.pitch, factor);
     }
     __syncthreads();
-    groups.run(c0, AD_GROUP * AD_WAVES, end, planes, A.pitch, factor);
+    const uint16_t* hi = planes + i16 * A.pitch + 8 * q;
+    const uint16_t* lo = hi + ROWS * A.pitch;
+    float* mine = turned[w];
+    float f[2 * RT];
+#pragma unroll
+    for (int r = 0; r < 2 * RT; ++r) f[r] = rank ? factor[r * 8 + r8] : 0.f;
+    for (int c0 = start; c0 < end; c0 += AD_GROUP * AD_WAVES) {
+        f32x4 acc[RT][4];
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[r][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        auto product = [&](int b, int t) {
+            if (t == per - 1 && (rank & 31)) {                // behind the adapter's rank, whatever lies there
+                const int left = rank - (t * 32 + 8 * q);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) bv[b][j][e] &= left >= 2 * e + 2 ? 0xffffffffu : left == 2 * e + 1 ? 0xffffu : 0u;
+            }
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const u32x4 h = *(const u32x4*)(hi + r * 16 * A.pitch + t * 32), l = *(const u32x4*)(lo + r * 16 * A.pitch + t * 32);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[r][j] = T::mfma16(bitcast<typename T::vec8>(bv[b][j]), bitcast<typename T::vec8>(h), acc[r][j]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[r][j] = T::mfma16(bitcast<typename T::vec8>(bv[b][j]), bitcast<typename T::vec8>(l), acc[r][j]);
+            }
+        };
+        for (int t = 0; t < per; t += 2) {
+            product(0, t);
+            if (t + 2 < per) load_b(c0, 0, t + 2);
+            if (t + 1 < per) {
+                product(1, t + 1);
+                if (t + 3 < per) load_b(c0, 1, t + 3);
+            }
+        }
+        const bool vec = whole(c0);
+        const int col = c0 + 8 * p8;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            sort_fence();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) *(f32x4*)(mine + i16 * AD_PITCH + 16 * j + 4 * q) = acc[r][j];
+            sort_fence();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int at = 2 * r + h;
+                const f32x4 d0 = *(const f32x4*)(mine + (8 * h + r8) * AD_PITCH + 8 * p8), d1 = *(const f32x4*)(mine + (8 * h + r8) * AD_PITCH + 8 * p8 + 4);
+                if (at * 8 + r8 >= tile.count) continue;
+                uint16_t* out = A.out + (int64_t)rows[at] * A.out_stride + first + col;
+                if (vec) {
+                    float x[8];
+                    unpack8<T>(raw[at], x);
+                    u32x4 o = raw[at];
+                    if (rank)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const f32x4& d = e < 2 ? d0 : d1;
+                            o[e] = pack2<T>(fmaf(d[2 * (e & 1)], f[at], x[2 * e]), fmaf(d[2 * (e & 1) + 1], f[at], x[2 * e + 1]));
+                        }
+                    *(u32x4*)out = o;
+                } else {
+                    const uint16_t* base = A.base + (int64_t)rows[at] * A.base_stride + first + col;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (col + e < cols) out[e] = rank ? T::from_float(fmaf(e < 4 ? d0[e & 3] : d1[e & 3], f[at], T::to_float(base[e]))) : base[e];
+                }
+            }
+        }
+        if (c0 + AD_GROUP * AD_WAVES < end) load(c0 + AD_GROUP * AD_WAVES);
+    }
 }
 
 // How the products are cut.  Tiles of ranks a workgroup: as few workgroups that share x as the registers of RT x CT accumulators allow, evenly
 // filled.  Cuts of K: 1024 workgroups where there is that much, four units a wave and cut at least; a cut is another float32 copy of h.
 // Groups of columns a wave: more than one, so that the sums of h are shared, while 512 workgroups are left.
 struct AdapterPlan {
-    int cuts, cut_units, blocks, ct, groups_each;
+    int cuts, cut_units, blocks, ct, ert, groups_each;
 };
 AdapterPlan adapter_plan(int tokens, int adapters, int tile, int k, int slices, int rank, const int32_t* widths) {
     AdapterPlan p;
-    const int units = slices * ((rank + 15) / 16), most = tile == 16 ? 4 : 6;
+    const int units = slices * ((rank + 15) / 16), most = 4;
     p.blocks = (units + most - 1) / most;
     p.ct = (units + p.blocks - 1) / p.blocks;
-    if (p.ct == 5) p.ct = 6;
     const int k_units = (k + 63) / 64;
     const int64_t tiles = std::min<int64_t>(adapter_max_tiles(tokens, adapters, tile), tokens);
     const int64_t want = (1024 + tiles * p.blocks - 1) / (tiles * p.blocks);
     const int cuts = (int)std::min<int64_t>(std::min<int64_t>(want, 8), std::max(1, k_units / (4 * AD_WAVES)));
     p.cut_units = (k_units + cuts - 1) / cuts;
     p.cuts = (k_units + p.cut_units - 1) / p.cut_units;
+    p.ert = tile == 16 ? 1 : 2;
     p.groups_each = 1;
     for (; widths && p.groups_each < 4; p.groups_each *= 2) {
         int64_t blocks = 0;
@@ -588,12 +583,11 @@ extern "C" int mf_adapter_linear(void* out, const void* x, const void* lora_a, c
     A.vec_io = ((((uintptr_t)out | (uintptr_t)base) & 15) == 0 && A.base_stride % 8 == 0 && A.out_stride % 8 == 0) ? 1 : 0;
     hipStream_t st = (hipStream_t)stream;
     const int tiles = adapter_max_tiles(tokens, adapters, tile);
-    const size_t lds = (size_t)2 * tile * ((rank + 15) / 16 * 16 + 8) * 2;
     const int block_cols = AD_GROUP * AD_WAVES * p.groups_each;
     int64_t col_blocks = 0;
     for (int i = 0; i < slices; ++i) col_blocks += (A.s.width[i] + block_cols - 1) / block_cols;
     MF_REQUIRE(col_blocks <= 65535, "adapter_linear: %lld columns", (long long)columns);
-    A.max_tiles = tiles, A.blocks = p.blocks, A.pitch = (rank + 15) / 16 * 16 + 8;
+    A.max_tiles = tiles, A.blocks = p.blocks, A.pitch = (rank + 31) / 32 * 32 + 8;
     const int64_t shrinks = ((int64_t)tiles * p.cuts + 7) / 8 * 8 * p.blocks;
     MF_REQUIRE(shrinks < (1 << 24), "adapter_linear: %lld workgroups", (long long)shrinks);
     const dim3 g1((unsigned)shrinks);
@@ -609,8 +603,7 @@ extern "C" int mf_adapter_linear(void* out, const void* x, const void* lora_a, c
             if (p.ct == 1) AD_SHRINK(T, 4, 1);        \
             else if (p.ct == 2) AD_SHRINK(T, 4, 2);   \
             else if (p.ct == 3) AD_SHRINK(T, 4, 3);   \
-            else if (p.ct == 4) AD_SHRINK(T, 4, 4);   \
-            else AD_SHRINK(T, 4, 6);                  \
+            else AD_SHRINK(T, 4, 4);                  \
         }                                             \
     } while (0)
     if (dtype == MF_BF16) AD_SHRINK_T(BF16);
@@ -619,13 +612,18 @@ extern "C" int mf_adapter_linear(void* out, const void* x, const void* lora_a, c
 #undef AD_SHRINK
     const int rc = MF_LAUNCH_CHECK();
     if (rc) return rc;
-    const dim3 g2((unsigned)tiles, (unsigned)col_blocks);
+    const int ert = p.ert;
+    A.subs = tile / 16 / ert;
+    const dim3 g2((unsigned)(tiles * A.subs), (unsigned)col_blocks);
+    const size_t lds = (size_t)2 * ert * 16 * A.pitch * 2;
 #define AD_EXPAND(T, RT) hipLaunchKernelGGL((adapter_expand_kernel<T, RT>), g2, dim3(AD_WAVES * 64), lds, st, A)
     if (dtype == MF_BF16) {
-        if (tile == 16) AD_EXPAND(BF16, 1);
+        if (ert == 1) AD_EXPAND(BF16, 1);
+        else if (ert == 2) AD_EXPAND(BF16, 2);
         else AD_EXPAND(BF16, 4);
     } else {
-        if (tile == 16) AD_EXPAND(FP16, 1);
+        if (ert == 1) AD_EXPAND(FP16, 1);
+        else if (ert == 2) AD_EXPAND(FP16, 2);
         else AD_EXPAND(FP16, 4);
     }
 #undef AD_EXPAND
