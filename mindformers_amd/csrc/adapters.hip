@@ -16,7 +16,6 @@ namespace {
 constexpr int AD_MAX_ADAPTERS = 1024;
 constexpr int AD_MAX_RANK = 128;
 constexpr int AD_MAX_SLICES = 8;
-constexpr int AD_SORT_THREADS = 512, AD_SORT_WAVES = AD_SORT_THREADS / 64;
 constexpr int AD_WAVES = 4;
 constexpr int AD_GROUP = 64;                                  // columns that a wave computes at a time
 
@@ -51,17 +50,19 @@ __device__ __forceinline__ uint64_t same_key(int key, int bits, bool on) {
 // Bound by latency, ids, two scans and the placing one behind the other: ids are read 8 x 64 at a time, rows of one adapter among 64
 // found by a ballot a bit (one by one, behind atomics of LDS: 5.8 us for 64 rows and 15.6 us for 8191, 4.4 and 7.7 so).
 constexpr int AD_BATCH = 8;
-__global__ __launch_bounds__(AD_SORT_THREADS) void adapter_rows_kernel(int* __restrict__ order, AdapterTile* __restrict__ tiles,
+template <int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void adapter_rows_kernel(int* __restrict__ order, AdapterTile* __restrict__ tiles,
                                                                        const int* __restrict__ ids, int tokens, int adapters, int tile,
                                                                        int max_tiles, int bits) {
+    constexpr int THREADS = WAVES * 64;
     extern __shared__ int lds[];
     const int n = adapters + 1;                               // the last: rows without an adapter
     int* hist = lds;                                          // [waves][n]
-    int* start = hist + AD_SORT_WAVES * n;                    // [n + 1]
+    int* start = hist + WAVES * n;                    // [n + 1]
     int* tstart = start + n + 1;
-    __shared__ int w_rows[AD_SORT_WAVES], w_tiles[AD_SORT_WAVES];
+    __shared__ int w_rows[WAVES], w_tiles[WAVES];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int piece = ((tokens + AD_SORT_WAVES - 1) / AD_SORT_WAVES + 63) / 64 * 64;
+    const int piece = ((tokens + WAVES - 1) / WAVES + 63) / 64 * 64;
     const int r0 = min(w * piece, tokens), r1 = min(r0 + piece, tokens);
     int key[AD_BATCH];
     auto load = [&](int rb) {
@@ -72,7 +73,7 @@ __global__ __launch_bounds__(AD_SORT_THREADS) void adapter_rows_kernel(int* __re
         }
     };
     load(r0);
-    for (int i = tid; i < AD_SORT_WAVES * n; i += AD_SORT_THREADS) hist[i] = 0;
+    for (int i = tid; i < WAVES * n; i += THREADS) hist[i] = 0;
     __syncthreads();
     for (int rb = r0; rb < r1; rb += 64 * AD_BATCH) {
         if (rb != r0) load(rb);
@@ -88,12 +89,12 @@ __global__ __launch_bounds__(AD_SORT_THREADS) void adapter_rows_kernel(int* __re
     }
     __syncthreads();
     // each thread: a run of adapters, the waves' counts turned into places within the adapter
-    const int each = (n + AD_SORT_THREADS - 1) / AD_SORT_THREADS;
+    const int each = (n + THREADS - 1) / THREADS;
     const int a0 = min(tid * each, n), a1 = min(a0 + each, n);
     int rows = 0, tls = 0;
     for (int a = a0; a < a1; ++a) {
         int c = 0;
-        for (int v = 0; v < AD_SORT_WAVES; ++v) {
+        for (int v = 0; v < WAVES; ++v) {
             const int t = hist[v * n + a];
             hist[v * n + a] = c;
             c += t;
@@ -114,7 +115,7 @@ __global__ __launch_bounds__(AD_SORT_THREADS) void adapter_rows_kernel(int* __re
     pr -= rows;
     pt -= tls;
     int all_tiles = 0;
-    for (int v = 0; v < AD_SORT_WAVES; ++v) {
+    for (int v = 0; v < WAVES; ++v) {
         if (v < w) { pr += w_rows[v]; pt += w_tiles[v]; }
         all_tiles += w_tiles[v];
     }
@@ -136,7 +137,7 @@ __global__ __launch_bounds__(AD_SORT_THREADS) void adapter_rows_kernel(int* __re
             sort_fence();
         }
     }
-    for (int i = tid; i < max_tiles; i += AD_SORT_THREADS) {
+    for (int i = tid; i < max_tiles; i += THREADS) {
         AdapterTile t = {-1, 0, 0, 0};
         if (i < all_tiles) {
             int lo = 0, hi = n - 1;                           // the last adapter whose tiles start at or before i
@@ -288,7 +289,7 @@ __global__ __launch_bounds__(AD_WAVES * 64) void adapter_shrink_kernel(const Ada
 // A row of h, scaled, to the planes: sixteen lanes a row, v[i] the ranks 64 i + 4 (lane & 15) .. + 3 of it; what lies at or behind the
 // adapter's rank becomes zero.  `factor` gets what the products of the row are to be multiplied with.
 template <typename T>
-__device__ __forceinline__ void row_to_planes(f32x4* v, float scale, int rank, int row, int rows, uint16_t* planes, int pitch, float* factor) {
+__device__ __forceinline__ void row_to_planes(f32x4* v, float scale, int rank, int row, uint16_t* planes, int pitch, float* factor) {
     constexpr int NV = AD_MAX_RANK / 64;
     const int i16 = threadIdx.x & 15;
     float most = 0.f;
@@ -323,7 +324,7 @@ __device__ __forceinline__ void row_to_planes(f32x4* v, float scale, int rank, i
             lo[e] = pack2<T>(fabsf(ra) < INFINITY ? ra : 0.f, fabsf(rb) < INFINITY ? rb : 0.f);      // infinite: hi says it
         }
         *(u32x2*)(planes + row * pitch + j) = (u32x2){hi[0], hi[1]};
-        *(u32x2*)(planes + (rows + row) * pitch + j) = (u32x2){lo[0], lo[1]};
+        *(u32x2*)(planes + (16 + row) * pitch + j) = (u32x2){lo[0], lo[1]};
     }
 }
 
@@ -337,14 +338,14 @@ __device__ __forceinline__ int slice_of(const AdapterArgs& A, int& block, int bl
     }
 }
 
-// out = base + (B h): a workgroup adds up the cuts of RT x 16 rows' h, puts them into LDS as hi and lo, and computes 4 x groups_each groups
+// out = base + (B h): a workgroup adds up the cuts of 16 rows' h, puts them into LDS as hi and lo, and computes 4 x groups_each groups
 // of 64 columns of one slice.  The product is taken with the columns as the matrix instruction's rows, 32 ranks at a time, once with hi
 // and once with lo; its results go through LDS (of the wave's own) into rows of 128 bytes, eight lanes each, as base and out are moved.  A
 // group's base rows and its first 64 ranks of B are loaded behind the group before it, the first one's in front of the sums of h.
 constexpr int AD_PITCH = AD_GROUP + 4;                        // floats of a row of results
-template <typename T, int RT>
+template <typename T>
 __global__ __launch_bounds__(AD_WAVES * 64) void adapter_expand_kernel(const AdapterArgs A) {
-    constexpr int ROWS = RT * 16, NV = AD_MAX_RANK / 64;
+    constexpr int ROWS = 16, NV = AD_MAX_RANK / 64;
     extern __shared__ __align__(16) uint16_t planes[];        // [2][ROWS][pitch]
     __shared__ __align__(16) float turned[AD_WAVES][16 * AD_PITCH];
     __shared__ float factor[ROWS];                            // what a row's products are to be multiplied with
@@ -362,10 +363,10 @@ __global__ __launch_bounds__(AD_WAVES * 64) void adapter_expand_kernel(const Ada
     const int per = (rank + 31) >> 5, width = A.s.n * A.rank, first = A.s.first[s], cols = A.s.width[s];
     const int start = block * block_cols + w * AD_GROUP;
     const int end = min((block + 1) * block_cols, cols);
-    int rows[2 * RT];
+    int rows[2];
 #pragma unroll
-    for (int r = 0; r < 2 * RT; ++r) rows[r] = A.order[tile.first + min(r * 8 + r8, tile.count - 1)];
-    u32x4 bv[2][4], raw[2 * RT];
+    for (int r = 0; r < 2; ++r) rows[r] = A.order[tile.first + min(r * 8 + r8, tile.count - 1)];
+    u32x4 bv[2][4], raw[2];
     const uint16_t* b0 = A.b + ((int64_t)max(tile.adapter, 0) * A.s.total + first) * A.rank;
     auto load_b = [&](int c0, int b, int t) {                 // 32 ranks of the group's columns
         const int k = min(t * 32 + 8 * q, A.rank - 8);
@@ -380,50 +381,41 @@ __global__ __launch_bounds__(AD_WAVES * 64) void adapter_expand_kernel(const Ada
         }
         if (whole(c0))
 #pragma unroll
-            for (int r = 0; r < 2 * RT; ++r) raw[r] = *(const u32x4*)(A.base + (int64_t)rows[r] * A.base_stride + first + c0 + 8 * p8);
+            for (int r = 0; r < 2; ++r) raw[r] = *(const u32x4*)(A.base + (int64_t)rows[r] * A.base_stride + first + c0 + 8 * p8);
     };
     if (start < end) load(start);
     if (rank) {
         const float scale = A.scales ? A.scales[tile.adapter] : 1.f;
-        f32x4 v[RT][NV];
+        f32x4 v[NV];
         const int64_t cut = (int64_t)A.tokens * width;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {                        // sixteen lanes a row, four ranks a lane
             const int j = 64 * i + 4 * i16;
-#pragma unroll
-            for (int r = 0; r < RT; ++r) v[r][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            v[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
             if (j >= rank) continue;
-            const float* h = A.h + (int64_t)tile.first * width + s * A.rank + j;
+            const float* h = A.h + (int64_t)(tile.first + min(w * 4 + q, tile.count - 1)) * width + s * A.rank + j;
             for (int c = 0; c < A.cuts; c += 4) {
-                f32x4 part[RT][4];
+                f32x4 part[4];
 #pragma unroll
-                for (int r = 0; r < RT; ++r)
+                for (int o = 0; o < 4; ++o) part[o] = *(const f32x4*)(h + min(c + o, A.cuts - 1) * cut);
 #pragma unroll
-                    for (int o = 0; o < 4; ++o)
-                        part[r][o] = *(const f32x4*)(h + min((r * AD_WAVES + w) * 4 + q, tile.count - 1) * (int64_t)width + min(c + o, A.cuts - 1) * cut);
-#pragma unroll
-                for (int r = 0; r < RT; ++r)
-#pragma unroll
-                    for (int o = 0; o < 4; ++o)
-                        if (c + o < A.cuts) v[r][i] += part[r][o];
+                for (int o = 0; o < 4; ++o)
+                    if (c + o < A.cuts) v[i] += part[o];
             }
         }
-#pragma unroll
-        for (int r = 0; r < RT; ++r) row_to_planes<T>(v[r], scale, rank, (r * AD_WAVES + w) * 4 + q, ROWS, planes, A.pitch, factor);
+        row_to_planes<T>(v, scale, rank, w * 4 + q, planes, A.pitch, factor);
     }
     __syncthreads();
     const uint16_t* hi = planes + i16 * A.pitch + 8 * q;
     const uint16_t* lo = hi + ROWS * A.pitch;
     float* mine = turned[w];
-    float f[2 * RT];
+    float f[2];
 #pragma unroll
-    for (int r = 0; r < 2 * RT; ++r) f[r] = rank ? factor[r * 8 + r8] : 0.f;
+    for (int r = 0; r < 2; ++r) f[r] = rank ? factor[r * 8 + r8] : 0.f;
     for (int c0 = start; c0 < end; c0 += AD_GROUP * AD_WAVES) {
-        f32x4 acc[RT][4];
+        f32x4 acc[4];
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[r][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < 4; ++j) acc[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
         auto product = [&](int b, int t) {
             if (t == per - 1 && (rank & 31)) {                // behind the adapter's rank, whatever lies there
                 const int left = rank - (t * 32 + 8 * q);
@@ -432,14 +424,11 @@ __global__ __launch_bounds__(AD_WAVES * 64) void adapter_expand_kernel(const Ada
 #pragma unroll
                     for (int e = 0; e < 4; ++e) bv[b][j][e] &= left >= 2 * e + 2 ? 0xffffffffu : left == 2 * e + 1 ? 0xffffu : 0u;
             }
+            const u32x4 h = *(const u32x4*)(hi + t * 32), l = *(const u32x4*)(lo + t * 32);
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                const u32x4 h = *(const u32x4*)(hi + r * 16 * A.pitch + t * 32), l = *(const u32x4*)(lo + r * 16 * A.pitch + t * 32);
+            for (int j = 0; j < 4; ++j) acc[j] = T::mfma16(bitcast<typename T::vec8>(bv[b][j]), bitcast<typename T::vec8>(h), acc[j]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[r][j] = T::mfma16(bitcast<typename T::vec8>(bv[b][j]), bitcast<typename T::vec8>(h), acc[r][j]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[r][j] = T::mfma16(bitcast<typename T::vec8>(bv[b][j]), bitcast<typename T::vec8>(l), acc[r][j]);
-            }
+            for (int j = 0; j < 4; ++j) acc[j] = T::mfma16(bitcast<typename T::vec8>(bv[b][j]), bitcast<typename T::vec8>(l), acc[j]);
         };
         for (int t = 0; t < per; t += 2) {
             product(0, t);
@@ -451,59 +440,58 @@ __global__ __launch_bounds__(AD_WAVES * 64) void adapter_expand_kernel(const Ada
         }
         const bool vec = whole(c0);
         const int col = c0 + 8 * p8;
+        sort_fence();
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            sort_fence();
+        for (int j = 0; j < 4; ++j) *(f32x4*)(mine + i16 * AD_PITCH + 16 * j + 4 * q) = acc[j];
+        sort_fence();
 #pragma unroll
-            for (int j = 0; j < 4; ++j) *(f32x4*)(mine + i16 * AD_PITCH + 16 * j + 4 * q) = acc[r][j];
-            sort_fence();
+        for (int h = 0; h < 2; ++h) {
+            const float* at = mine + (8 * h + r8) * AD_PITCH + 8 * p8;
+            const f32x4 d0 = *(const f32x4*)at, d1 = *(const f32x4*)(at + 4);
+            if (8 * h + r8 >= tile.count) continue;
+            uint16_t* out = A.out + (int64_t)rows[h] * A.out_stride + first + col;
+            if (vec) {
+                float x[8];
+                unpack8<T>(raw[h], x);
+                u32x4 o = raw[h];
+                if (rank)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int at = 2 * r + h;
-                const f32x4 d0 = *(const f32x4*)(mine + (8 * h + r8) * AD_PITCH + 8 * p8), d1 = *(const f32x4*)(mine + (8 * h + r8) * AD_PITCH + 8 * p8 + 4);
-                if (at * 8 + r8 >= tile.count) continue;
-                uint16_t* out = A.out + (int64_t)rows[at] * A.out_stride + first + col;
-                if (vec) {
-                    float x[8];
-                    unpack8<T>(raw[at], x);
-                    u32x4 o = raw[at];
-                    if (rank)
+                    for (int e = 0; e < 4; ++e) {
+                        const f32x4& d = e < 2 ? d0 : d1;
+                        o[e] = pack2<T>(fmaf(d[2 * (e & 1)], f[h], x[2 * e]), fmaf(d[2 * (e & 1) + 1], f[h], x[2 * e + 1]));
+                    }
+                *(u32x4*)out = o;
+            } else {
+                const uint16_t* base = A.base + (int64_t)rows[h] * A.base_stride + first + col;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const f32x4& d = e < 2 ? d0 : d1;
-                            o[e] = pack2<T>(fmaf(d[2 * (e & 1)], f[at], x[2 * e]), fmaf(d[2 * (e & 1) + 1], f[at], x[2 * e + 1]));
-                        }
-                    *(u32x4*)out = o;
-                } else {
-                    const uint16_t* base = A.base + (int64_t)rows[at] * A.base_stride + first + col;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (col + e < cols) out[e] = rank ? T::from_float(fmaf(e < 4 ? d0[e & 3] : d1[e & 3], f[at], T::to_float(base[e]))) : base[e];
-                }
+                for (int e = 0; e < 8; ++e)
+                    if (col + e < cols) out[e] = rank ? T::from_float(fmaf(e < 4 ? d0[e & 3] : d1[e & 3], f[h], T::to_float(base[e]))) : base[e];
             }
         }
         if (c0 + AD_GROUP * AD_WAVES < end) load(c0 + AD_GROUP * AD_WAVES);
     }
 }
 
-// How the products are cut.  Tiles of ranks a workgroup: as few workgroups that share x as the registers of RT x CT accumulators allow, evenly
-// filled.  Cuts of K: 1024 workgroups where there is that much, four units a wave and cut at least; a cut is another float32 copy of h.
-// Groups of columns a wave: more than one, so that the sums of h are shared, while 512 workgroups are left.
+// How the products are cut.  Two tiles of ranks a workgroup (three of 64 rows: x is read by fewer).  Cuts of K: 1024 workgroups where there
+// is that much, four units a wave and cut at least (eight where there are 128 tiles), 8 cuts at most: a cut is another float32 copy
+// of h.  Groups of columns a wave: up to four behind one sum of h, while 512 workgroups are left.  (us, of both kernels.  8191 rows, K 4096,
+// 4096 + 2 x 1024 columns, rank 32: 72 in one cut, 68 in two, 78 in four; four tiles a workgroup 75; one group a wave 88.  64 rows of 24
+// adapters of up to 64 ranks, K 14336: 21 in two cuts, 16.5 in four, 15.3 in eight; K 4096, 2 x 14336 columns: one group a wave
+// 27, two 25.)
 struct AdapterPlan {
-    int cuts, cut_units, blocks, ct, ert, groups_each;
+    int cuts, cut_units, blocks, ct, groups_each;
 };
 AdapterPlan adapter_plan(int tokens, int adapters, int tile, int k, int slices, int rank, const int32_t* widths) {
     AdapterPlan p;
-    const int units = slices * ((rank + 15) / 16), most = 4;
+    const int units = slices * ((rank + 15) / 16), most = tile == 16 ? 2 : 3;
     p.blocks = (units + most - 1) / most;
     p.ct = (units + p.blocks - 1) / p.blocks;
     const int k_units = (k + 63) / 64;
     const int64_t tiles = std::min<int64_t>(adapter_max_tiles(tokens, adapters, tile), tokens);
     const int64_t want = (1024 + tiles * p.blocks - 1) / (tiles * p.blocks);
-    const int cuts = (int)std::min<int64_t>(std::min<int64_t>(want, 8), std::max(1, k_units / (4 * AD_WAVES)));
+    const int cuts = (int)std::min<int64_t>(std::min<int64_t>(want, 8), std::max(1, k_units / ((tiles < 128 ? 4 : 8) * AD_WAVES)));
     p.cut_units = (k_units + cuts - 1) / cuts;
     p.cuts = (k_units + p.cut_units - 1) / p.cut_units;
-    p.ert = tile == 16 ? 1 : 2;
     p.groups_each = 1;
     for (; widths && p.groups_each < 4; p.groups_each *= 2) {
         int64_t blocks = 0;
@@ -526,10 +514,14 @@ extern "C" int mf_adapter_rows(int32_t* plan, const int32_t* adapter_ids, int to
     MF_REQUIRE(tile == 16 || tile == 64, "adapter_rows: tiles of 16 or 64 rows, got %d", tile);
     if (tokens == 0) return 0;
     MF_REQUIRE(plan && adapter_ids && ((uintptr_t)plan & 15) == 0, "adapter_rows: null or unaligned argument");
-    const size_t lds = sizeof(int) * (size_t)((AD_SORT_WAVES + 2) * (adapters + 1) + 2);
-    hipLaunchKernelGGL(adapter_rows_kernel, dim3(1), dim3(AD_SORT_THREADS), lds, (hipStream_t)stream, plan,
-                       (AdapterTile*)(plan + adapter_order_ints(tokens)), adapter_ids, tokens, adapters, tile,
-                       adapter_max_tiles(tokens, adapters, tile), 32 - __builtin_clz((unsigned)adapters | 1u));
+    // 16 waves where their counts fit 64 KB of LDS
+#define AD_ROWS(WAVES)                                                                                                              \
+    hipLaunchKernelGGL(adapter_rows_kernel<WAVES>, dim3(1), dim3(WAVES * 64), sizeof(int) * (size_t)((WAVES + 2) * (adapters + 1) + 2), \
+                       (hipStream_t)stream, plan, (AdapterTile*)(plan + adapter_order_ints(tokens)), adapter_ids, tokens, adapters, tile, \
+                       adapter_max_tiles(tokens, adapters, tile), 32 - __builtin_clz((unsigned)adapters | 1u))
+    if (adapters <= 512) AD_ROWS(16);
+    else AD_ROWS(8);
+#undef AD_ROWS
     return MF_LAUNCH_CHECK();
 }
 
@@ -596,14 +588,11 @@ extern "C" int mf_adapter_linear(void* out, const void* x, const void* lora_a, c
     do {                                              \
         if (tile == 16) {                             \
             if (p.ct == 1) AD_SHRINK(T, 1, 1);        \
-            else if (p.ct == 2) AD_SHRINK(T, 1, 2);   \
-            else if (p.ct == 3) AD_SHRINK(T, 1, 3);   \
-            else AD_SHRINK(T, 1, 4);                  \
+            else AD_SHRINK(T, 1, 2);                  \
         } else {                                      \
             if (p.ct == 1) AD_SHRINK(T, 4, 1);        \
             else if (p.ct == 2) AD_SHRINK(T, 4, 2);   \
-            else if (p.ct == 3) AD_SHRINK(T, 4, 3);   \
-            else AD_SHRINK(T, 4, 4);                  \
+            else AD_SHRINK(T, 4, 3);                  \
         }                                             \
     } while (0)
     if (dtype == MF_BF16) AD_SHRINK_T(BF16);
@@ -612,20 +601,10 @@ extern "C" int mf_adapter_linear(void* out, const void* x, const void* lora_a, c
 #undef AD_SHRINK
     const int rc = MF_LAUNCH_CHECK();
     if (rc) return rc;
-    const int ert = p.ert;
-    A.subs = tile / 16 / ert;
+    A.subs = tile / 16;
     const dim3 g2((unsigned)(tiles * A.subs), (unsigned)col_blocks);
-    const size_t lds = (size_t)2 * ert * 16 * A.pitch * 2;
-#define AD_EXPAND(T, RT) hipLaunchKernelGGL((adapter_expand_kernel<T, RT>), g2, dim3(AD_WAVES * 64), lds, st, A)
-    if (dtype == MF_BF16) {
-        if (ert == 1) AD_EXPAND(BF16, 1);
-        else if (ert == 2) AD_EXPAND(BF16, 2);
-        else AD_EXPAND(BF16, 4);
-    } else {
-        if (ert == 1) AD_EXPAND(FP16, 1);
-        else if (ert == 2) AD_EXPAND(FP16, 2);
-        else AD_EXPAND(FP16, 4);
-    }
-#undef AD_EXPAND
+    const size_t lds = (size_t)2 * 16 * A.pitch * 2;
+    if (dtype == MF_BF16) hipLaunchKernelGGL(adapter_expand_kernel<BF16>, g2, dim3(AD_WAVES * 64), lds, st, A);
+    else hipLaunchKernelGGL(adapter_expand_kernel<FP16>, g2, dim3(AD_WAVES * 64), lds, st, A);
     return MF_LAUNCH_CHECK();
 }
