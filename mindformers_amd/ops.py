@@ -169,53 +169,69 @@ def rotary_embedding(query, key, positions, inv_freq, head_dim, interleaved=Fals
     ``interleaved``.  positions int32 [T], inv_freq float64.  In place, or into ``out`` = (query_out, key_out or None), which share no
     memory with the inputs.  With ``key_cache`` / ``value_cache`` [num_blocks, block_size, n_kv, D] the turned key and ``value`` go to
     the rows that ``slot_mapping`` names as well (a negative slot: to none).  Returns (query, key) where they went."""
-    lib = _lib.load()
-    dev = _dev_of(query, key, value)
-    _need(_dev_ok(positions, inv_freq, key_cache, value_cache, slot_mapping) == dev, "all tensors must be on the same device")
-    d = int(head_dim)
-    _need(d > 0 and query.dim() >= 1 and query.shape[-1] % d == 0 and query.shape[-1] > 0, "query must be [T, n_heads * head_dim]")
-    _need(positions.dtype == torch.int32 and positions.dim() == 1 and inv_freq.dtype == torch.float64 and inv_freq.dim() == 1,
-          "positions must be int32 [T], inv_freq float64 [pairs]")
-    t, pairs, qw = positions.numel(), inv_freq.numel(), query.shape[-1]
-    if not (0 < pairs and 0 <= offset and offset + 2 * pairs <= d <= 1024):
-        raise ValueError(f"{pairs} pairs from column {offset} do not fit heads of {d} (up to 1024)")
+    index, dtype, d, t, pairs = query.get_device(), query.dtype, int(head_dim), positions.numel(), inv_freq.numel()
+    if not (index >= 0 and positions.get_device() == index and inv_freq.get_device() == index and positions.is_contiguous()
+            and inv_freq.is_contiguous()):
+        _need(_dev_of(query) == _dev_ok(positions, inv_freq), "all tensors must be on the same device")
+    if not (positions.dtype is torch.int32 and positions.dim() == 1 and inv_freq.dtype is torch.float64 and inv_freq.dim() == 1):
+        raise ValueError("positions must be int32 [T], inv_freq float64 [pairs]")
+    if not (dtype in _ACT and query.dim() > 0):
+        raise ValueError("query must be bf16/fp16 [T, n_heads * head_dim]")
+    qw = query.shape[-1]
+    if not (0 < d <= 1024 and qw > 0 and qw % d == 0 and 0 < pairs and 0 <= offset and offset + 2 * pairs <= d):
+        raise ValueError(f"rows of {qw}, {pairs} pairs from column {offset} of heads of {d}: whole heads of up to 1024, and the pairs inside")
     query, qs = _rows(query, qw, "query")
-    _need(query.dtype in _ACT and query.numel() == t * qw, "query must be bf16/fp16 and hold a row for each position")
-    kw, ks, vs, slots = 0, 0, 0, 0
+    kw = ks = vs = slots = 0
+    if query.numel() != t * qw:
+        raise ValueError(f"query must hold a row for each of {t} positions")
     if key is not None:
-        _need(key.dim() >= 1 and key.shape[-1] % d == 0 and key.shape[-1] > 0, "key must be [T, n_kv_heads * head_dim]")
-        kw = key.shape[-1]
+        kw = _head_rows(key, t, d, dtype, index, "key")
         key, ks = _rows(key, kw, "key")
-        _need(key.dtype == query.dtype and key.numel() == t * kw, "key must have query's type and a row for each position")
-    if key_cache is not None or value_cache is not None or value is not None or slot_mapping is not None:
-        _need(key is not None and key_cache is not None and value_cache is not None and value is not None and slot_mapping is not None,
-              "key, value, both caches and slot_mapping go together")
-        _need(key_cache.dim() == 4 and value_cache.shape == key_cache.shape and key_cache.shape[2] * key_cache.shape[3] == kw
-              and key_cache.shape[3] == d, "caches must be [num_blocks, block_size, n_kv_heads, head_dim]")
-        _need(key_cache.dtype == query.dtype and value_cache.dtype == query.dtype and value.dtype == query.dtype, "dtype mismatch")
+    cached = key_cache is not None
+    if cached or value_cache is not None or value is not None or slot_mapping is not None:
+        if key is None or not cached or value_cache is None or value is None or slot_mapping is None:
+            raise ValueError("key, value, both caches and slot_mapping go together")
+        shape = key_cache.shape
+        if not (len(shape) == 4 and value_cache.shape == shape and shape[3] == d and shape[2] * d == kw and shape[0] * shape[1] > 0):
+            raise ValueError("caches must be [num_blocks, block_size, n_kv_heads, head_dim]")
+        if not (key_cache.dtype is dtype and value_cache.dtype is dtype and key_cache.get_device() == index
+                and value_cache.get_device() == index and key_cache.is_contiguous() and value_cache.is_contiguous()):
+            raise ValueError("caches must be contiguous, of query's type and on its device")
+        if not (slot_mapping.dtype is torch.int32 and slot_mapping.dim() == 1 and slot_mapping.numel() == t
+                and slot_mapping.get_device() == index and slot_mapping.is_contiguous()):
+            raise ValueError("slot_mapping must be a contiguous int32 [T] on query's device")
+        _need(_head_rows(value, t, d, dtype, index, "value") == kw, "value must have key's rows")
         value, vs = _rows(value, kw, "value")
-        _need(value.numel() == t * kw and slot_mapping.dtype == torch.int32 and slot_mapping.numel() == t and slot_mapping.dim() == 1,
-              "value and int32 slot_mapping must hold a row for each position")
-        slots = key_cache.shape[0] * key_cache.shape[1]
-        _need(slots > 0, "caches without a block")
-    q_out, k_out = (query, key) if out is None else out
-    qos, kos = qs, ks
-    if out is not None:
-        _need(_dev_of(q_out, k_out) == dev, "out must be on the inputs' device")
+        slots = shape[0] * shape[1]
+    if out is None:
+        q_out, k_out, qos, kos = query, key, qs, ks
+    else:
+        q_out, k_out = out
+        _need(_head_rows(q_out, t, d, dtype, index, "query_out") == qw, "query_out must have query's rows")
         q_out, qos = _rows(q_out, qw, "query_out")
-        _need(q_out.dtype == query.dtype and q_out.numel() == t * qw, "query_out must have query's rows and type")
+        kos = 0
         if k_out is not None:
-            _need(key is not None, "key_out without a key")
+            _need(key is not None and _head_rows(k_out, t, d, dtype, index, "key_out") == kw, "key_out must have key's rows")
             k_out, kos = _rows(k_out, kw, "key_out")
-            _need(k_out.dtype == query.dtype and k_out.numel() == t * kw, "key_out must have key's rows and type")
-        else:
-            _need(key is None or key_cache is not None, "a key that goes neither to key_out nor into a cache")
+        elif not (key is None or cached):
+            raise ValueError("a key that goes neither to key_out nor into a cache")
+    lib, dev = _lib.load(), query.device
     with _on(dev):
-        check(lib.mf_rotary_embedding(ptr(q_out), ptr(k_out), ptr(query), ptr(key), ptr(value), ptr(key_cache), ptr(value_cache),
-                                      ptr(positions), ptr(inv_freq), ptr(slot_mapping), t, qw // d, kw // d, d, pairs, int(offset),
-                                      1 if interleaved else 0, float(scale), slots, qs, ks, vs, qos, kos, dtype_code(query.dtype),
+        check(lib.mf_rotary_embedding(q_out.data_ptr(), ptr(k_out), query.data_ptr(), ptr(key), ptr(value), ptr(key_cache), ptr(value_cache),
+                                      positions.data_ptr(), inv_freq.data_ptr(), ptr(slot_mapping), t, qw // d, kw // d, d, pairs, int(offset),
+                                      1 if interleaved else 0, float(scale), slots, qs, ks, vs, qos, kos, dtype_code(dtype),
                                       stream_ptr(dev)), "mf_rotary_embedding")
     return q_out, k_out
+
+
+def _head_rows(x, t, d, dtype, index, what):
+    """Width of a row of heads beside query, checked."""
+    if not (x.dtype is dtype and x.get_device() == index and x.dim() > 0):
+        raise ValueError(f"{what} must have query's type and be on its device")
+    width = x.shape[-1]
+    if not (width > 0 and width % d == 0 and x.numel() == t * width):
+        raise ValueError(f"{what} must hold a row of heads of {d} for each of {t} positions")
+    return width
 
 
 def rope_and_cache(query, key, value, cos, sin, key_cache, value_cache, slot_mapping, n_heads):
