@@ -26,7 +26,7 @@ struct RotaryArgs {
     int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride, num_slots;
     int tokens, heads, kv_heads, dim, pairs, offset, rows;    // rows: of a workgroup
     int units, v_units;                                       // of a head; of a row's values
-    uint32_t unit_magic;                                      // 2^32 / units, rounded up
+    uint32_t unit_magic, row_magic;                           // 2^32 / units, and / units of a row, rounded up
     float scale;
 };
 
@@ -80,7 +80,7 @@ template <int VEC, bool NEAR>
 __device__ __forceinline__ void rotary_take(const RotaryArgs& A, RotaryUnit<VEC>& U, int i, int n_q, int n_qk, int64_t row, int64_t at, bool cached) {
     U.in = nullptr;
     if (i >= n_qk) {
-        U.in = A.v + row * A.v_stride;
+        if (cached) U.in = A.v + row * A.v_stride;
         U.out = nullptr, U.cache = A.v_cache + at;
         U.c = (i - n_qk) * VEC, U.d = -1, U.first = A.pairs;
         return;
@@ -162,29 +162,26 @@ __global__ __launch_bounds__(RO_THREADS) void rotary_kernel(const RotaryArgs A) 
         table[i] = make_float2(A.scale * cn, A.scale * sn);
     }
     __syncthreads();
-    const int n_q = A.heads * A.units, n_qk = n_q + A.kv_heads * A.units;
-    for (int r = 0; r < rows; ++r) {
-        const int64_t row = row0 + r;
-        const int64_t slot = A.slots ? A.slots[row] : -1;
-        const bool cached = slot >= 0 && slot < A.num_slots;
-        const int64_t at = cached ? slot * A.kv_heads * A.dim : 0;
-        const float2* cs = table + r * A.pairs;
-        const int all = n_qk + (cached ? A.v_units : 0);
-        for (int i = threadIdx.x; i < all; i += 2 * RO_THREADS) {
-            RotaryUnit<VEC> U[2];
+    const int n_q = A.heads * A.units, n_qk = n_q + A.kv_heads * A.units, each = n_qk + A.v_units, all = rows * each;
+    for (int i = threadIdx.x; i < all; i += 2 * RO_THREADS) {
+        RotaryUnit<VEC> U[2];
+        int r[2];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                U[k].in = nullptr;
-                if (i + k * RO_THREADS < all) rotary_take<VEC, NEAR>(A, U[k], i + k * RO_THREADS, n_q, n_qk, row, at, cached);
-                if (U[k].in) {
-                    U[k].x.load(U[k].in + U[k].c);
-                    if (U[k].d >= 0) U[k].y.load(U[k].in + U[k].d);
-                }
+        for (int k = 0; k < 2; ++k) {
+            const int j = min(i + k * RO_THREADS, all - 1);
+            r[k] = A.rows == 1 ? 0 : each == 1 ? j : (int)__umulhi((uint32_t)j, A.row_magic);
+            const int64_t row = row0 + r[k], slot = A.slots ? A.slots[row] : -1;
+            const bool cached = slot >= 0 && slot < A.num_slots;
+            rotary_take<VEC, NEAR>(A, U[k], j - r[k] * each, n_q, n_qk, row, cached ? slot * A.kv_heads * A.dim : 0, cached);
+            if (i + k * RO_THREADS >= all) U[k].in = nullptr;
+            if (U[k].in) {
+                U[k].x.load(U[k].in + U[k].c);
+                if (U[k].d >= 0) U[k].y.load(U[k].in + U[k].d);
             }
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-                if (U[k].in) rotary_finish<T, VEC, NEAR>(A, U[k], cs);
         }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (U[k].in) rotary_finish<T, VEC, NEAR>(A, U[k], table + r[k] * A.pairs);
     }
 }
 
@@ -239,10 +236,14 @@ extern "C" int mf_rotary_embedding(void* query_out, void* key_out, const void* q
     A.offset = offset, A.scale = scale;
     const int vec = rotary_vec(A, interleaved != 0);
     A.units = interleaved && vec > 1 ? head_dim / vec : n_pairs / vec + (head_dim - 2 * n_pairs) / vec;
-    A.unit_magic = (uint32_t)((0x100000000ull + A.units - 1) / A.units);   // exact for up to 2^32 / units units; not used for one
-    A.v_units = (int)(kw / vec);
+    A.v_units = key_cache ? (int)(kw / vec) : 0;
+    // exact for up to 2^32 / units units; not used for one
+    auto magic = [](int64_t units) { return (uint32_t)((0x100000000ll + units - 1) / units); };
+    const int64_t each = (int64_t)(n_heads + n_kv_heads) * A.units + A.v_units;
+    A.unit_magic = magic(A.units), A.row_magic = magic(each);
     // several rows a workgroup where there are enough to fill the device: their angles take its threads at once
     A.rows = num_tokens >= 2048 ? std::max(1, std::min(RO_ROWS, RO_THREADS / n_pairs)) : 1;
+    if (each > (1 << 14)) A.rows = 1;                         // the division by them is exact up to 2^32 / each
     const dim3 grid((unsigned)((num_tokens + A.rows - 1) / A.rows));
     const size_t lds = (size_t)A.rows * n_pairs * sizeof(float2);
     hipStream_t st = (hipStream_t)stream;
