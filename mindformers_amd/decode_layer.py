@@ -36,6 +36,7 @@ class QuantDecodeLayer(nn.Module):
         super().__init__()
         ops.check_window(window, sinks)
         self.window, self.sinks = window, sinks
+        self.banks = nn.ModuleDict()                          # adapters (set_adapters)
         self.hidden, self.n_head, self.n_kv_head, self.head_dim, self.ffn = hidden, n_head, n_kv_head, head_dim, ffn
         self.eps, self.dtype, self.act_quant = eps, dtype, act_quant
         self.scale_value = 1.0 / math.sqrt(head_dim)
@@ -73,15 +74,36 @@ class QuantDecodeLayer(nn.Module):
         row-major ``*_w`` tensors leave the module's buffers for host copies kept as plain attributes (``raw_weights``,
         still readable, e.g. for export), so that the device holds every weight once and a later ``.to(device)`` does
         not bring a second copy back; the ``*_w`` names then resolve to those host copies."""
-        dev = self.attn_norm.device
         for name in self.NAMES:
-            w, s = getattr(self, f"{name}_w").to(dev), getattr(self, f"{name}_s")
-            # W8A16: the gate/up projection runs fused with SiLU * mul, which wants gate/up rows interleaved
-            gated = name == "fc1" and not self.act_quant and getattr(self, "fc1_b") is None
-            self._packed[name] = ops.pack_w8a16_gated(w, s, "halves") if gated else ops.pack_w8a16(w, s)
+            w = self._pack(name)
             if release_raw:
                 self._buffers.pop(f"{name}_w", None)
                 self.raw_weights[f"{name}_w"] = w.cpu()
+        return self
+
+    def _pack(self, name):
+        w, s = getattr(self, f"{name}_w").to(self.attn_norm.device), getattr(self, f"{name}_s")
+        # W8A16: the gate/up projection runs fused with SiLU * mul, which wants gate/up rows interleaved; adapters come in between
+        gated = name == "fc1" and not self.act_quant and getattr(self, "fc1_b") is None and "fc1" not in self.banks
+        self._packed[name] = ops.pack_w8a16_gated(w, s, "halves") if gated else ops.pack_w8a16(w, s)
+        return w
+
+    def set_adapters(self, banks):
+        """Low-rank adapters beside this layer's projections: ``banks`` maps names out of NAMES to ``AdapterBank``s of as many slots each
+        (slices, where a bank has them: q, k and v of "qkv", gate and up of "fc1").  A step that brings ``adapters`` (``ops.adapter_rows``)
+        adds every row's; one without is the layer's own."""
+        for name, bank in banks.items():
+            if name not in self.NAMES:
+                raise ValueError(f"no projection {name!r}: {self.NAMES}")
+            shape = tuple(getattr(self, f"{name}_w").shape)
+            if (bank.out_features, bank.in_features) != shape or bank.dtype != self.dtype:
+                raise ValueError(f"{name}: {shape} in {self.dtype}, the bank is {(bank.out_features, bank.in_features)} in {bank.dtype}")
+        if len({bank.n_adapters for bank in banks.values()}) > 1:
+            raise ValueError("the banks of a layer must have as many slots each")
+        had = "fc1" in self.banks
+        self.banks = nn.ModuleDict(banks)
+        if had != ("fc1" in banks) and "fc1" in self._packed:
+            self._pack("fc1")                                 # packed for the other path
         return self
 
     def __getattr__(self, name):
@@ -92,6 +114,8 @@ class QuantDecodeLayer(nn.Module):
         buffers = d.get("_buffers")                            # nearly all that a step asks for
         if buffers is not None and name in buffers:
             return buffers[name]
+        if name == "banks" and name not in d.get("_modules", ()):   # a layer built before there were adapters
+            return {}
         return super().__getattr__(name)
 
     def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):
@@ -128,7 +152,7 @@ class QuantDecodeLayer(nn.Module):
                                            self.n_head, self.n_kv_head, self.scale_value, **self._view())
 
     def forward(self, x, key_cache, value_cache, block_tables, batch_valid_length, slot_mapping, cos, sin,
-                q_starts=None, normed=None, next_norm=None):
+                q_starts=None, normed=None, next_norm=None, adapters=None, rotary=None):
         """x [T, hidden]; caches [num_blocks, block_size, n_kv, D]; cos/sin [T, D] rows for this step's
         positions; batch_valid_length counts the tokens written by this step.  Decode: one token per sequence.
         Prefill / chunked prefill: ``q_starts`` int32 [B + 1] gives the row range of every sequence in x, its new
@@ -139,7 +163,13 @@ class QuantDecodeLayer(nn.Module):
         takes that second tensor as ``normed`` in place of computing its attention norm.  The norm then runs inside
         the kernel that finishes this layer's last projection (same bits, one launch fewer).  A W8A8 layer takes
         ``next_norm`` = (gamma, eps, smooth) with the next layer's QKV smoothing vector and hands over the quantised
-        norm output (xq, scale), which is what a W8A8 layer accepts as ``normed``."""
+        norm output (xq, scale), which is what a W8A8 layer accepts as ``normed``.
+
+        ``adapters``: the step's ``ops.adapter_rows``, for the banks of ``set_adapters``.  ``rotary`` = (positions int32 [T], RotaryPositions):
+        rotary positions of another layout or scaling in the place of the rows cos / sin, which are not read then."""
+        if rotary is not None or (adapters is not None and self.banks):
+            return self._step_of_requests(x, key_cache, value_cache, block_tables, batch_valid_length, slot_mapping, cos, sin, q_starts,
+                                          normed, next_norm, adapters if self.banks else None, rotary)
         # (int8 caches: asked first, so that a step which waits for the host does not pay for checks that end in the operators)
         if q_starts is None and not self.act_quant and key_cache.dtype is x.dtype and self._plain():
             packed, buffers = self._packed, self._buffers
@@ -225,6 +255,39 @@ class QuantDecodeLayer(nn.Module):
         if next_norm is not None and self.fc2_b is None and self._packed.get("fc2") is not None:
             return ops.w8a16_linear_add_rmsnorm(self.gate_up(n2), self._packed["fc2"], h, next_norm[0], next_norm[1])
         return self._chain(self._linear(self.gate_up(n2), "fc2", residual=h), next_norm)
+
+    def _step_of_requests(self, x, key_cache, value_cache, block_tables, batch_valid_length, slot_mapping, cos, sin, q_starts, normed,
+                          next_norm, adapters, rotary):
+        """A step whose rows bring adapters or rotary positions of their own: the projections by themselves, the adapters between them
+        and what follows."""
+        def project(inp, name, residual=None):
+            y = self._linear(inp, name, residual=residual)
+            return y if adapters is None or name not in self.banks else self.banks[name](inp, y, adapters, out=y)
+
+        nq, nkv = self.n_head * self.head_dim, self.n_kv_head * self.head_dim
+        n1 = normed if isinstance(normed, torch.Tensor) else ops.rms_norm(x, self.attn_norm, self.eps)
+        qkv = project(n1, "qkv")
+        q, k, v = qkv[:, :nq], qkv[:, nq:nq + nkv], qkv[:, nq + nkv:]
+        if key_cache.dtype == torch.int8:                     # rotate, then quantize into the int8 caches
+            if self.kv_scale is None:
+                raise RuntimeError("int8 caches need set_kv_quant(scale, offset)")
+            if rotary is None:
+                ops.apply_rotary_pos_emb(q, k, cos, sin, self.n_head, self.n_kv_head, self.head_dim)
+            else:
+                rotary[1](q, k, rotary[0])
+            ops.quant_reshape_and_cache(k, v, key_cache, value_cache, slot_mapping, self.kv_scale, self.kv_offset)
+        elif rotary is None:
+            ops.rope_and_cache(q, k, v, cos, sin, key_cache, value_cache, slot_mapping, self.n_head)
+        else:
+            rotary[1](q, k, rotary[0], v, key_cache, value_cache, slot_mapping)
+        h = project(self.attend(q, key_cache, value_cache, block_tables, batch_valid_length, q_starts), "wo", residual=x)
+        n2 = ops.rms_norm(h, self.ffn_norm, self.eps)
+        act = self.gate_up(n2) if adapters is None or "fc1" not in self.banks else ops.silu_mul(project(n2, "fc1"))
+        out = project(act, "fc2", residual=h)
+        if next_norm is not None and len(next_norm) == 3:     # the next W8A8 layer's quantised input
+            gamma, eps, smooth = next_norm
+            return out, ops.rms_norm_dynamic_quant(out, gamma, eps, smooth, tiled=True)
+        return self._chain(out, next_norm)
 
     @staticmethod
     def _chain(out, next_norm):

@@ -1,4 +1,5 @@
 """Drop-in modules of the decode path (same constructor / call surface as the reference's cells)."""
+from .adapters import AdapterBank, AdapterLinear
 from .beam_search import BeamSearch
 from .block_tables import BlockMemPool, BlockTables, CacheEngine
 from .flash_attention import FlashAttention
@@ -10,4 +11,4 @@ from .moe import GroupedMLP, MoELayer, QuantGroupedMLP, SharedExpertMLP, TopKRou
 from .multi_latent_attention import MLASelfAttention, MLASelfAttentionSubmodules, MLATransformerConfig
 from .norm import LlamaRMSNorm, RMSNorm
 from .paged_attention_mgr import PagedAttentionMgr, QuantPagedAttentionMgr
-from .rotary import FreqsMgr, Llama3RotaryEmbedding, RotaryEmbedding, YaRNScalingRotaryEmbedding
+from .rotary import FreqsMgr, Llama3RotaryEmbedding, RotaryEmbedding, RotaryPositions, YaRNScalingRotaryEmbedding

@@ -170,6 +170,66 @@ class YaRNScalingRotaryEmbedding(RotaryEmbedding):
         return self.mscale
 
 
+class RotaryPositions(nn.Module):
+    """Rotary positions without tables: any layout and scaling, angles from the positions in float64 (``ops.rotary_embedding``).
+
+    Of heads of ``head_dim`` columns the ``rotary_percent`` from column ``offset`` on are turned, in pairs (i, i + half) or, ``interleaved``,
+    (2 i, 2 i + 1).  ``scaling``, with its ``scaling_config``:
+      None; "linear" factor; "ntk" factor (of the base); "llama3" factor, low_freq_factor, high_freq_factor,
+      original_max_position_embeddings; "yarn" factor, original_max_position_embeddings, beta_fast, beta_slow, mscale, mscale_all_dim.
+    The formulas are those of the classes above, in float64.  Buffers: ``inv_freq`` float64 [pairs]; ``scale``: the factor on the result."""
+
+    def __init__(self, head_dim, rotary_percent=1.0, interleaved=False, base=10000.0, scaling=None, scaling_config=None, offset=0,
+                 device="cuda"):
+        super().__init__()
+        dim = int(head_dim * rotary_percent)
+        if dim % 2 or not 0 < dim or offset < 0 or offset + dim > head_dim:
+            raise ValueError(f"{dim} columns from column {offset} of heads of {head_dim}: an even number inside the head")
+        self.head_dim, self.dim, self.interleaved, self.offset = int(head_dim), dim, bool(interleaved), int(offset)
+        c, base, self.scale = dict(scaling_config or {}), float(base), 1.0
+        kind = None if scaling is None else str(scaling).lower()
+        known = {None: (), "linear": ("factor",), "ntk": ("factor",),
+                 "llama3": ("factor", "low_freq_factor", "high_freq_factor", "original_max_position_embeddings"),
+                 "yarn": ("factor", "original_max_position_embeddings", "beta_fast", "beta_slow", "mscale", "mscale_all_dim")}
+        if kind not in known:
+            raise ValueError(f"scaling {scaling!r}: None, linear, ntk, llama3 or yarn")
+        if set(c) - set(known[kind]) or not {k for k in known[kind] if k not in ("beta_fast", "beta_slow", "mscale", "mscale_all_dim")} <= set(c):
+            raise ValueError(f"scaling_config of {kind}: {known[kind]}, got {sorted(c)}")
+        factor = float(c.get("factor", 1.0))
+        if kind == "ntk":
+            base *= factor
+        inv = base ** (-np.arange(0, dim, 2, dtype=np.float64) / dim)
+        if kind == "linear":
+            inv = inv / factor
+        elif kind == "llama3":
+            lo, hi, old = float(c["low_freq_factor"]), float(c["high_freq_factor"]), float(c["original_max_position_embeddings"])
+            turns = old * inv / (2 * math.pi)                 # of a pair over the original context
+            mix = np.clip((turns - lo) / (hi - lo), 0.0, 1.0) if hi != lo else (turns > hi).astype(np.float64)
+            inv = (1 - mix) * inv / factor + mix * inv
+        elif kind == "yarn":
+            low, high = _yarn_find_correction_range(float(c.get("beta_fast", 32.0)), float(c.get("beta_slow", 1.0)), dim, base,
+                                                    c["original_max_position_embeddings"])
+            ramp = np.clip((np.arange(dim // 2) - low) / ((high - low) or 0.001), 0.0, 1.0)
+            inv = inv / factor * ramp + inv * (1 - ramp)
+            self.scale = _yarn_get_mscale(factor, float(c.get("mscale", 1.0))) / _yarn_get_mscale(factor, float(c.get("mscale_all_dim", 0.0)))
+        self.register_buffer("inv_freq", torch.from_numpy(inv).to(device), persistent=False)
+
+    def forward(self, query, key, positions, value=None, key_cache=None, value_cache=None, slot_mapping=None, out=None):
+        """query [T, n_heads * D] and key [T, n_kv * D] (or None) turned by ``positions`` int32 [T], in place or into ``out``, and with caches
+        key and value written to their slots."""
+        return ops.rotary_embedding(query, key, positions, self.inv_freq, self.head_dim, interleaved=self.interleaved, scale=self.scale,
+                                    offset=self.offset, value=value, key_cache=key_cache, value_cache=value_cache, slot_mapping=slot_mapping,
+                                    out=out)
+
+    construct = forward
+
+    def _apply(self, fn, *args, **kw):
+        super()._apply(fn, *args, **kw)
+        if self.inv_freq.dtype != torch.float64:              # .half() and the like are for weights
+            raise TypeError("the frequencies of RotaryPositions stay float64")
+        return self
+
+
 class FreqsMgr(nn.Module):
     """Legacy table owner (layers.py:1171-1333): ``increment(batch_valid_length)`` returns the rows for position
     batch_valid_length - 1 as (cos, sin, swap_mask); swap_mask is kept for signature parity (the rotate-half

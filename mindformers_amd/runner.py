@@ -30,10 +30,11 @@ class DecodeStackRunner:
     """Owns the layers' paged caches (device) and their swap space (pinned host) and runs scheduler steps.
 
     ``layers``: prepared ``QuantDecodeLayer``s.  ``npu_mem_size`` / ``cpu_mem_size`` are GiB, as in the reference;
-    ``rope_theta`` builds the rotary rows from the positions of each step."""
+    ``rope_theta`` builds the rotary rows from the positions of each step; ``rotary`` (a ``RotaryPositions``) takes their place:
+    another layout, part of the heads, or scaled for long contexts."""
 
     def __init__(self, layers, npu_mem_size, cpu_mem_size, block_size, rope_theta=10000.0, device="cuda",
-                 quantization_config=None):
+                 quantization_config=None, rotary=None):
         if not layers or not all(isinstance(l, QuantDecodeLayer) for l in layers):
             raise TypeError("layers must be a non-empty list of QuantDecodeLayer")
         first = layers[0]
@@ -43,6 +44,9 @@ class DecodeStackRunner:
         self.block_size = int(block_size)
         self.device = torch.device(device)
         self.rope_theta = rope_theta
+        if rotary is not None and rotary.head_dim != self.head_size:
+            raise ValueError(f"rotary is for heads of {rotary.head_dim}, the layers have {self.head_size}")
+        self.rotary = rotary
         # the cache dtype follows the quantization config when it names one (model_runner.py:364-368); int8 caches
         # need every layer's dequantisation parameters (QuantDecodeLayer.set_kv_quant)
         kv_name = getattr(quantization_config, "kvcache_quant_dtype", None) if quantization_config is not None else None
@@ -120,13 +124,14 @@ class DecodeStackRunner:
         return [dev[o:o + a.size].view(a.shape) if a.ndim != 1 else dev[o:o + a.size] for a, o in zip(arrays, at)]
 
     def forward(self, hidden_states, valid_length_each_example, block_tables, slot_mapping, prefill=True,
-                position_ids=None, q_seq_lens=None):
+                position_ids=None, q_seq_lens=None, adapter_ids=None):
         """One scheduler step over packed rows ``hidden_states`` [T, hidden].
 
         prefill=True: sequence b brings valid_length_each_example[b] prompt tokens (rows packed sequence after
         sequence), positions 0 .. len-1.  prefill=False: one new token per sequence at position len-1, or, with
         ``q_seq_lens``, q_seq_lens[b] new tokens ending at position len-1 (chunked prefill, parallel decoding).
-        ``position_ids`` overrides the positions.  Returns the last layer's output rows."""
+        ``position_ids`` overrides the positions.  ``adapter_ids`` (an integer a sequence, -1: none): the slot of the layers' adapter banks
+        that each has chosen.  Returns the last layer's output rows."""
         lens = np.asarray(valid_length_each_example, dtype=np.int64).reshape(-1)
         self.add_flags_custom(is_first_iteration=bool(prefill))
         if prefill:
@@ -156,32 +161,56 @@ class DecodeStackRunner:
         for name, a in (("tables", block_tables), ("slots", slot_mapping)):
             if isinstance(a, np.ndarray) and a.dtype.kind in "iu":
                 host[name] = a
+        ids_t = None
+        if adapter_ids is not None:
+            if isinstance(adapter_ids, torch.Tensor) and adapter_ids.is_cuda:
+                ids_t = adapter_ids.reshape(-1).to(torch.int32)
+                if ids_t.numel() == lens.size and q_lens is not None:
+                    ids_t = torch.repeat_interleave(ids_t, torch.as_tensor(q_lens, device=self.device), output_size=t)
+            else:
+                ids = np.asarray(adapter_ids, dtype=np.int64).reshape(-1)
+                if ids.size != lens.size:
+                    raise ValueError(f"{ids.size} adapter_ids for {lens.size} sequences")
+                host["ids"] = np.clip(ids if q_lens is None else np.repeat(ids, q_lens), -1, 2 ** 31 - 1)
         there = dict(zip(host, self._to_device(list(host.values()))))
         lens_t, q_starts = there["lens"], there.get("starts")
         tables = there["tables"] if "tables" in there else torch.as_tensor(block_tables, dtype=torch.int32,
                                                                             device=self.device)
         slots = there["slots"] if "slots" in there else torch.as_tensor(slot_mapping, dtype=torch.int32, device=self.device)
         pos_t = there["pos"] if "pos" in there else torch.as_tensor(position_ids, device=self.device).reshape(-1)
-        cos, sin = self._rope_rows(pos_t, there["freq"].view(torch.float32))
-        h = self._run_layers(hidden_states, tables, lens_t, slots, cos, sin, q_starts)
+        cos, sin = self._rope_rows(pos_t, there["freq"].view(torch.float32)) if self.rotary is None else (None, None)
+        h = self._run_layers(hidden_states, tables, lens_t, slots, cos, sin, q_starts, pos_t, there.get("ids", ids_t))
         if prefill:
             self.add_flags_custom(is_first_iteration=False)
         return h
 
-    def decode(self, hidden_states, context_lens, block_tables, slot_mapping):
+    def decode(self, hidden_states, context_lens, block_tables, slot_mapping, adapter_ids=None):
         """One decode step whose arrays are on the device, int32: what a loop that never comes back to the host has (``BeamSearch``).  Row i
-        brings the token at position context_lens[i] - 1; empty rows have length 0 and slot -1.  No host synchronisation; can be
-        captured into a graph."""
-        for t, n, name in ((context_lens, 1, "context_lens"), (slot_mapping, 1, "slot_mapping"), (block_tables, 2, "block_tables")):
+        brings the token at position context_lens[i] - 1; empty rows have length 0 and slot -1.  ``adapter_ids``: as in ``forward``, a row
+        each.  No host synchronisation; can be captured into a graph."""
+        for t, n, name in ((context_lens, 1, "context_lens"), (slot_mapping, 1, "slot_mapping"), (block_tables, 2, "block_tables"),
+                           (adapter_ids, 1, "adapter_ids")):
+            if t is None and name == "adapter_ids":
+                continue
             if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.int32 and t.dim() == n and t.is_contiguous()
                     and t.shape[0] == hidden_states.shape[0]):
                 raise ValueError(f"{name} must be a contiguous int32 device tensor with a row for each of {hidden_states.shape[0]} tokens")
         self.add_flags_custom(is_first_iteration=False)
-        cos, sin = self._rope_rows(torch.clamp(context_lens - 1, min=0), self._freq_dev)
-        return self._run_layers(hidden_states, block_tables, context_lens, slot_mapping, cos, sin, None)
+        pos = torch.clamp(context_lens - 1, min=0)
+        cos, sin = self._rope_rows(pos, self._freq_dev) if self.rotary is None else (None, None)
+        return self._run_layers(hidden_states, block_tables, context_lens, slot_mapping, cos, sin, None, pos, adapter_ids)
 
-    def _run_layers(self, h, tables, lens_t, slots, cos, sin, q_starts):
-        normed = None
+    def _run_layers(self, h, tables, lens_t, slots, cos, sin, q_starts, positions=None, adapter_ids=None):
+        normed, more = None, {}
+        if self.rotary is not None:
+            more["rotary"] = (positions.to(torch.int32).contiguous(), self.rotary)
+        if adapter_ids is not None:
+            counts = {bank.n_adapters for layer in self.layers for bank in layer.banks.values()}
+            if len(counts) != 1:
+                raise ValueError(f"adapter_ids need layers with adapter banks of one size, these have {sorted(counts)} slots")
+            if adapter_ids.numel() != h.shape[0]:
+                raise ValueError(f"{adapter_ids.numel()} adapter_ids for {h.shape[0]} rows")
+            more["adapters"] = ops.adapter_rows(adapter_ids.contiguous(), counts.pop())
         for i, layer in enumerate(self.layers):
             # layer i also computes layer i + 1's attention norm (W8A8: and its quantisation), in the kernel that
             # finishes its own last projection
@@ -191,7 +220,7 @@ class DecodeStackRunner:
             if chain:
                 nn = (nxt.attn_norm, nxt.eps, nxt.qkv_smooth) if nxt.act_quant else (nxt.attn_norm, nxt.eps)
             out = layer(h, self.key_cache[i], self.value_cache[i], tables, lens_t, slots, cos, sin, q_starts=q_starts,
-                        normed=normed, next_norm=nn)
+                        normed=normed, next_norm=nn, **more)
             h, normed = out if chain else (out, None)
         return h
 

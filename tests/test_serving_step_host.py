@@ -96,3 +96,79 @@ def test_sizes_of_plans_and_workspaces():
     assert lib.mf_adapter_workspace_bytes(4, 2, 16, 64, 1, 136) == 0
     assert lib.mf_token_logprobs_workspace_bytes(5000, 1000, 64, 0) == 0  # a workgroup a row
     assert lib.mf_token_logprobs_workspace_bytes(1, 152064, 65, 0) == 0
+
+
+# ------------------------------------------------------------------------------------------------ modules, on the CPU
+def test_a_bank_takes_and_refuses_adapters():
+    from mindformers_amd.modules import AdapterBank
+    bank = AdapterBank(3, 16, (8, 24), 8, device="cpu")
+    a, b = [torch.ones(4, 16), torch.full((2, 16), 2.0)], [torch.ones(8, 4), torch.full((24, 2), 3.0)]
+    bank.load(1, a, b, scale=0.5)
+    assert bank.ranks.tolist() == [0, 4, 0] and bank.scales[1] == 0.5
+    assert (bank.lora_a[1, 0, :4] == 1).all() and (bank.lora_a[1, 1, :2] == 2).all() and (bank.lora_a[1, 1, 2:] == 0).all()
+    assert (bank.lora_b[1, :8, :4] == 1).all() and (bank.lora_b[1, 8:, :2] == 3).all() and (bank.lora_b[1, 8:, 2:] == 0).all()
+    bank.load(1, [None, a[1]], [None, b[1]])                  # what was there before leaves
+    assert (bank.lora_a[1, 0] == 0).all() and (bank.lora_b[1, :8] == 0).all() and bank.ranks[1] == 2
+    for slot, x, y in ((3, a, b), (-1, a, b), (0, a[:1], b[:1]), (0, [a[0], None], b), (0, [torch.ones(9, 16), a[1]], [torch.ones(8, 9), b[1]]),
+                       (0, [torch.ones(4, 15), a[1]], b), (0, a, [torch.ones(8, 3), b[1]])):
+        with pytest.raises(ValueError):
+            bank.load(slot, x, y)
+    assert bank.unload(1).ranks.tolist() == [0, 0, 0]
+    for args in ((0, 16, 8, 8), (1025, 16, 8, 8), (2, 12, 8, 8), (2, 16, 8, 12), (2, 16, 8, 136), (2, 16, (), 8), (2, 16, (8, 0), 8), (2, 16, (8,) * 9, 8)):
+        with pytest.raises(ValueError):
+            AdapterBank(*args, device="cpu")
+    with pytest.raises(TypeError):
+        AdapterBank(2, 16, 8, 8, dtype=torch.float32, device="cpu")
+
+
+def test_a_layer_and_a_cell_refuse_banks_that_do_not_fit():
+    from mindformers_amd.decode_layer import QuantDecodeLayer
+    from mindformers_amd.modules import AdapterBank, AdapterLinear, Linear
+    layer = QuantDecodeLayer(64, 4, 2, 16, 128, device="cpu")
+    fits = AdapterBank(2, 64, (64, 32, 32), 8, device="cpu")
+    layer.set_adapters({"qkv": fits})
+    assert layer.banks["qkv"] is fits and any(k.startswith("banks.qkv") for k in layer.state_dict())
+    for banks in ({"gate": fits}, {"wo": fits}, {"qkv": AdapterBank(2, 64, 128, 8, FP, device="cpu")},
+                  {"qkv": fits, "wo": AdapterBank(3, 64, 64, 8, device="cpu")}):
+        with pytest.raises(ValueError):
+            layer.set_adapters(banks)
+    layer.set_adapters({})
+    assert not layer.banks
+    with pytest.raises(ValueError):
+        AdapterLinear(Linear(64, 128, device="cpu"), AdapterBank(2, 64, 64, 8, device="cpu"))
+    with pytest.raises(NotImplementedError):
+        AdapterLinear(Linear(64, 64, activation="silu", device="cpu"), AdapterBank(2, 64, 64, 8, device="cpu"))
+
+
+def test_rotary_positions_have_the_frequencies_of_the_tables():
+    """Against the tables of the float32 classes: the same formulas, so cosines at the first positions agree to float32."""
+    import numpy as np
+    from mindformers_amd.modules import FreqsMgr, Llama3RotaryEmbedding, RotaryEmbedding, RotaryPositions, YaRNScalingRotaryEmbedding
+    d, pos = 32, np.arange(40)
+
+    def near(rot, cos):
+        got = np.cos(pos[:, None] * rot.inv_freq.numpy()) * rot.scale
+        assert np.abs(got - cos[:40, :d // 2].numpy()).max() < 2e-5
+
+    common = dict(rotary_cos_format=2, rotary_dtype=F32, device="cpu")
+    near(RotaryPositions(d, device="cpu"), RotaryEmbedding(d, max_position_embeddings=64, **common).cos_cache)
+    near(RotaryPositions(d, base=5e5, device="cpu"), RotaryEmbedding(d, rotary_base=500000, max_position_embeddings=64, **common).cos_cache)
+    llama3 = dict(factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0, original_max_position_embeddings=64)
+    near(RotaryPositions(d, scaling="llama3", scaling_config=llama3, device="cpu"),
+         Llama3RotaryEmbedding(d, max_position_embeddings=64, scaling_factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0, orig_max_position=64,
+                               **common).cos_cache)
+    yarn = dict(factor=4.0, original_max_position_embeddings=64, beta_fast=32, beta_slow=1, mscale=1.0, mscale_all_dim=0.5)
+    near(RotaryPositions(d, scaling="YARN", scaling_config=yarn, device="cpu"),
+         YaRNScalingRotaryEmbedding(d, scaling_factor=4.0, original_max_position_embeddings=64, mscale=1.0, mscale_all_dim=0.5, **common).cos_cache)
+    near(RotaryPositions(d, scaling="linear", scaling_config=dict(factor=2.0), device="cpu"),
+         FreqsMgr(d, max_position_embedding=64, rotary_dtype=F32, extend_method="LINEAR", scaling_factor=dict(factor=2.0), device="cpu").freqs_cos)
+    near(RotaryPositions(d, scaling="ntk", scaling_config=dict(factor=2.0), device="cpu"),
+         FreqsMgr(d, max_position_embedding=64, rotary_dtype=F32, extend_method="NTK", scaling_factor=2.0, device="cpu").freqs_cos)
+    part = RotaryPositions(128, rotary_percent=0.25, interleaved=True, offset=96, device="cpu")
+    assert part.inv_freq.shape == (16,) and part.inv_freq.dtype == F64 and not part.state_dict()
+    for args, kw in (((32,), dict(rotary_percent=0.1)), ((32,), dict(offset=2)), ((32,), dict(scaling="su")), ((32,), dict(scaling="linear")),
+                     ((32,), dict(scaling="linear", scaling_config=dict(factor=2, beta_fast=1))), ((32,), dict(scaling_config=dict(factor=2.0)))):
+        with pytest.raises(ValueError):
+            RotaryPositions(*args, device="cpu", **kw)
+    with pytest.raises(TypeError):
+        RotaryPositions(32, device="cpu").half()
