@@ -341,7 +341,8 @@ __device__ __forceinline__ int slice_of(const AdapterArgs& A, int& block, int bl
 // out = base + (B h): a workgroup adds up the cuts of 16 rows' h, puts them into LDS as hi and lo, and computes 4 x groups_each groups
 // of 64 columns of one slice.  The product is taken with the columns as the matrix instruction's rows, 32 ranks at a time, once with hi
 // and once with lo; its results go through LDS (of the wave's own) into rows of 128 bytes, eight lanes each, as base and out are moved.  A
-// group's base rows and its first 64 ranks of B are loaded behind the group before it, the first one's in front of the sums of h.
+// group's first 64 ranks of B and its base rows are loaded behind the products and the results of the group before it, the first one's
+// in front of the sums of h.
 constexpr int AD_PITCH = AD_GROUP + 4;                        // floats of a row of results
 template <typename T>
 __global__ __launch_bounds__(AD_WAVES * 64) void adapter_expand_kernel(const AdapterArgs A) {
@@ -374,16 +375,19 @@ __global__ __launch_bounds__(AD_WAVES * 64) void adapter_expand_kernel(const Ada
         for (int j = 0; j < 4; ++j) bv[b][j] = *(const u32x4*)(b0 + (int64_t)min(c0 + 16 * j + i16, cols - 1) * A.rank + k);
     };
     auto whole = [&](int c0) { return A.vec_io && (first & 7) == 0 && c0 + 8 * p8 + 8 <= cols; };
-    auto load = [&](int c0) {
-        if (rank) {
-            load_b(c0, 0, 0);
-            if (per > 1) load_b(c0, 1, 1);
-        }
+    auto load_first_b = [&](int c0) {
+        if (rank) load_b(c0, 0, 0);
+        if (per > 1) load_b(c0, 1, 1);
+    };
+    auto load_base = [&](int c0) {
         if (whole(c0))
 #pragma unroll
             for (int r = 0; r < 2; ++r) raw[r] = *(const u32x4*)(A.base + (int64_t)rows[r] * A.base_stride + first + c0 + 8 * p8);
     };
-    if (start < end) load(start);
+    if (start < end) {
+        load_first_b(start);
+        load_base(start);
+    }
     if (rank) {
         const float scale = A.scales ? A.scales[tile.adapter] : 1.f;
         f32x4 v[NV];
@@ -438,6 +442,8 @@ __global__ __launch_bounds__(AD_WAVES * 64) void adapter_expand_kernel(const Ada
                 if (t + 3 < per) load_b(c0, 1, t + 3);
             }
         }
+        const int next = c0 + AD_GROUP * AD_WAVES;
+        if (next < end) load_first_b(next);
         const bool vec = whole(c0);
         const int col = c0 + 8 * p8;
         sort_fence();
@@ -468,7 +474,7 @@ __global__ __launch_bounds__(AD_WAVES * 64) void adapter_expand_kernel(const Ada
                     if (col + e < cols) out[e] = rank ? T::from_float(fmaf(e < 4 ? d0[e & 3] : d1[e & 3], f[h], T::to_float(base[e]))) : base[e];
             }
         }
-        if (c0 + AD_GROUP * AD_WAVES < end) load(c0 + AD_GROUP * AD_WAVES);
+        if (next < end) load_base(next);
     }
 }
 

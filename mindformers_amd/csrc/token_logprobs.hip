@@ -3,10 +3,11 @@
 //   lp(v) = x[v] - m - log Z,   Z = sum_u exp(x[u] - m),   H = log Z - (1 / Z) sum_u (x[u] - m) exp(x[u] - m)
 //   rank(v) = number of tokens u with x[u] > x[v], or x[u] = x[v] and u < v
 //
-// One pass over the logits for the sums, the rank and every lane's largest logit; the best ones are looked for behind it, in the columns
-// of the lanes whose largest is among the n largest of the workgroup's 256 (n / 256 of the columns, read once more; a list kept on the
-// way took 90 us of 345 for 4137 x 152064 bf16 with 20 alternatives, 260 in 545 with 64).  The waves of a workgroup take the steps of a
-// piece of a row in turn; each lane's sums are about a reference m of its own (moved when a logit passes it by more than 8: the sums stay
+// One pass over the logits for the sums, the rank and the largest logit of every lane's steps; the best ones are looked for behind it, in
+// those steps of lanes whose largest reaches the n-th largest of the workgroup's 256 lanes: some more than n times 16 logits, read once
+// more.  (4137 x 152064 bf16 with 5, 20 and 64 alternatives: 211, 215 and 228 us; whole lanes read again, of whose 16 bytes a step
+// memory gives 128, 220, 297 and 403; a list kept on the way 280, 347 and 545; without alternatives 215.)  The waves of a workgroup take the steps of a piece of a
+// row in turn; each lane's sums are about a reference m of its own (moved when a logit passes it by more than 8: the sums stay
 // in range and H loses no more than that).  A row of one workgroup is done then, others are joined by a second kernel.  Sums in
 // float32: their errors are of the size of the rounding of what comes out.
 #include <algorithm>
@@ -19,6 +20,8 @@ constexpr int TL_WAVES = 4;
 constexpr int TL_MAX_GROUPS = 64;                             // workgroups of a row
 constexpr int TL_MAX_N = 64;                                  // alternatives
 constexpr int TL_LIST = 512;                                  // logits that a workgroup ranks at a time
+constexpr int TL_TURNS = 24;                                  // groups of steps that lanes' largest logits are kept of
+constexpr int TL_HITS = 1024;                                 // (lane, group)s that are looked into at once
 constexpr int64_t TL_MAX_VOCAB = 0x7c000000;                  // a column a piece behind the last in 32 bits
 
 struct RowSums {
@@ -116,70 +119,98 @@ __device__ __forceinline__ void edge_vector(const RowPiece& p, int v, float* f) 
     for (int e = 0; e < L::VEC; ++e) f[e] = v + e >= p.mis && v + e < p.c1 ? f[e] : -INFINITY;
 }
 
+// the lowest bit of a key that two logits of the type differ in
+template <typename L> struct LowBit { static constexpr int value = 0; };
+template <> struct LowBit<Logit16<BF16>> { static constexpr int value = 16; };
+template <> struct LowBit<Logit16<FP16>> { static constexpr int value = 13; };
+
 struct TopShared {
     uint32_t key[TL_WAVES * 64];                              // of the lanes' largest logits (0: no column)
-    int hit[TL_WAVES * 64];                                   // lanes in question
-    float x[TL_LIST];                                         // logits in question, their tokens
-    int tok[TL_LIST];
-    int hits, count, ties;
+    uint16_t most[TL_TURNS][TL_WAVES * 64];                   // upper halves of those of a lane and group of steps
+    uint16_t hit[TL_HITS];                                    // group x 256 + lane: those in question
+    __align__(16) float x[TL_LIST];                           // logits in question, their tokens
+    __align__(16) int tok[TL_LIST];
+    int hits, count;
 };
+// the upper half of a key, of that of a float
+__device__ __forceinline__ uint32_t order_high(uint16_t h) { return (uint16_t)(h ^ ((int16_t)h < 0 ? 0xffffu : 0x8000u)); }
 
-// Calls what(x, token) for the logits of the lanes in question, a vector a thread at a time.
+// Calls what(x, token) for the logits of the lanes and groups whose largest may reach key k: from a list, a vector a thread (four at a time),
+// or, where they are more than it takes, each lane for itself.  `per`: steps of a group.
 template <typename L, typename F>
-__device__ __forceinline__ void for_hits(const RowPiece& p, const TopShared& sh, F&& what) {
-    constexpr int VEC = L::VEC, VECS = L::VECS, STEP = 64 * VEC * VECS;
-    const int turns = (p.c1 - p.c0 + TL_WAVES * STEP - 1) / (TL_WAVES * STEP), per = turns * VECS, items = sh.hits * per;
-    for (int i = threadIdx.x; i < items; i += TL_WAVES * 64) {
-        const int h = i / per, r = i - h * per, lane = sh.hit[h];
-        const int v = p.c0 + (r / VECS * TL_WAVES + (lane >> 6)) * STEP + (r % VECS * 64 + (lane & 63)) * VEC;
-        if (v >= p.c1) continue;
+__device__ __forceinline__ void for_hits(const RowPiece& p, TopShared& sh, int per, uint32_t k, F&& what) {
+    constexpr int VEC = L::VEC, VECS = L::VECS, STEP = 64 * VEC * VECS, AT_ONCE = 4;
+    const int turns = (p.c1 - p.c0 + TL_WAVES * STEP - 1) / (TL_WAVES * STEP), groups = (turns + per - 1) / per;
+    auto vector = [&](int g, int lane, int r) {               // column of vector r of a lane and group
+        return p.c0 + ((g * per + r / VECS) * TL_WAVES + (lane >> 6)) * STEP + (r % VECS * 64 + (lane & 63)) * VEC;
+    };
+    auto use = [&](int v, const u32x4& raw) {
         float f[VEC];
-        if (v >= p.in0 && v <= p.in1) {
-            const u32x4 raw = *(const u32x4*)(p.base + (int64_t)(v - p.mis) * L::BYTES);
-            L::unpack(raw, f);
-        }
+        L::unpack(raw, f);
         edge_vector<L>(p, v, f);
 #pragma unroll
         for (int e = 0; e < VEC; ++e)
             if (v + e >= p.mis && v + e < p.c1) what(counted(f[e]), v + e - p.mis);
+    };
+    auto load = [&](int v) { return v >= p.in0 && v <= p.in1 ? *(const u32x4*)(p.base + (int64_t)(v - p.mis) * L::BYTES) : (u32x4){0, 0, 0, 0}; };
+    __syncthreads();
+    if (threadIdx.x == 0) sh.hits = 0;
+    __syncthreads();
+    for (int g = 0; g < groups; ++g)
+        if (order_high(sh.most[g][threadIdx.x]) >= k >> 16) {
+            const int i = atomicAdd(&sh.hits, 1);
+            if (i < TL_HITS) sh.hit[i] = (uint16_t)(g * TL_WAVES * 64 + threadIdx.x);
+        }
+    __syncthreads();
+    const int hits = sh.hits, each = per * VECS, items = hits * each;
+    if (hits <= TL_HITS) {
+        for (int i0 = threadIdx.x; i0 < items; i0 += AT_ONCE * TL_WAVES * 64) {
+            u32x4 raw[AT_ONCE];
+            int at[AT_ONCE];
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j) {
+                const int i = min(i0 + j * TL_WAVES * 64, items - 1), h = i / each;
+                at[j] = vector(sh.hit[h] / (TL_WAVES * 64), sh.hit[h] % (TL_WAVES * 64), i - h * each);
+                raw[j] = load(at[j]);
+                if (i0 + j * TL_WAVES * 64 >= items) at[j] = p.c1;
+            }
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j)
+                if (at[j] < p.c1) use(at[j], raw[j]);
+        }
+    } else {
+        for (int g = 0; g < groups; ++g)
+            if (order_high(sh.most[g][threadIdx.x]) >= k >> 16)
+                for (int r = 0; r < each; ++r) {
+                    const int v = vector(g, threadIdx.x, r);
+                    if (v < p.c1) use(v, load(v));
+                }
     }
+    __syncthreads();
 }
 
 // The n best logits of the piece, or all, in sh.x and sh.tok, with others beside them; returns how many there are.
 template <typename L>
-__device__ int best_of_piece(const RowPiece& p, TopShared& sh, uint32_t key, int n) {
+__device__ int best_of_piece(const RowPiece& p, TopShared& sh, int per, uint32_t key, int n) {
     const int lane = threadIdx.x & 63;
     sh.key[threadIdx.x] = key;
-    if (threadIdx.x == 0) sh.hits = sh.count = 0;
     __syncthreads();
     // the n-th largest of the lanes' keys, bit by bit; fewer lanes with a column than that: the lowest key
     uint32_t k4[TL_WAVES], bound = 0;
 #pragma unroll
     for (int i = 0; i < TL_WAVES; ++i) k4[i] = sh.key[lane + 64 * i];
-    auto lanes_at = [&](uint32_t k) {
+    for (int bit = 31; bit >= LowBit<L>::value; --bit) {
+        const uint32_t trial = bound | (1u << bit);
         int c = 0;
 #pragma unroll
-        for (int i = 0; i < TL_WAVES; ++i) c += __popcll(__ballot(k4[i] >= k));
-        return c;
-    };
-    for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t trial = bound | (1u << bit);
-        const int c = lanes_at(trial);
+        for (int i = 0; i < TL_WAVES; ++i) c += __popcll(__ballot(k4[i] >= trial));
         if (c >= n) bound = trial;
         if (c == n) break;                                    // no bit below changes which lanes these are
     }
-    bound = max(bound, 1u);
-    const uint64_t m = __ballot(key >= bound);
-    int at = 0;
-    if (lane == 0 && m) at = atomicAdd(&sh.hits, __popcll(m));
-    at = __builtin_amdgcn_readfirstlane(at);
-    if (key >= bound) sh.hit[at + __popcll(m & ((1ull << lane) - 1ull))] = threadIdx.x;
-    __syncthreads();
     auto count_from = [&](uint32_t k) {                       // how many reach key k; the first TL_LIST of them go into the list
         __syncthreads();
         if (threadIdx.x == 0) sh.count = 0;
-        __syncthreads();
-        for_hits<L>(p, sh, [&](float x, int tok) {
+        for_hits<L>(p, sh, per, k, [&](float x, int tok) {
             if (order32(x + 0.f) >= k) {
                 const int i = atomicAdd(&sh.count, 1);
                 if (i < TL_LIST) {
@@ -188,7 +219,6 @@ __device__ int best_of_piece(const RowPiece& p, TopShared& sh, uint32_t key, int
                 }
             }
         });
-        __syncthreads();
         return sh.count;
     };
     int c = count_from(bound);
@@ -210,13 +240,13 @@ __device__ int best_of_piece(const RowPiece& p, TopShared& sh, uint32_t key, int
         const bool in = v >= p.mis && v >= p.c0 && v < p.c1;
         const bool tie = in && counted(L::at(p.base, min(max(v - p.mis, 0), p.vocab - 1))) == level;
         const uint64_t t = __ballot(tie);
-        if (lane == 0) sh.hit[threadIdx.x >> 6] = __popcll(t);
+        if (lane == 0) sh.key[threadIdx.x >> 6] = __popcll(t);
         __syncthreads();
         int before = c, all = 0;
 #pragma unroll
         for (int i = 0; i < TL_WAVES; ++i) {
-            if (i < (int)(threadIdx.x >> 6)) before += sh.hit[i];
-            all += sh.hit[i];
+            if (i < (int)(threadIdx.x >> 6)) before += sh.key[i];
+            all += sh.key[i];
         }
         before += __popcll(t & ((1ull << lane) - 1ull));
         if (tie && before < n) {
@@ -227,6 +257,25 @@ __device__ int best_of_piece(const RowPiece& p, TopShared& sh, uint32_t key, int
         __syncthreads();
     }
     return c;
+}
+
+// how many entries of a list come in front of (x, token); read four at a time, so that entries behind its end are to be list_end's
+__device__ __forceinline__ int rank_in(const float* l_x, const int* l_tok, int count, float x, int token) {
+    int rank = 0;
+#pragma unroll 2
+    for (int j = 0; j < count; j += 4) {
+        const f32x4 v = *(const f32x4*)(l_x + j);
+        const i32x4 t = *(const i32x4*)(l_tok + j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) rank += v[e] > x || (v[e] == x && t[e] < token);
+    }
+    return rank;
+}
+__device__ __forceinline__ void list_end(float* l_x, int* l_tok, int count, int i) {
+    if (count + i < (count + 3) / 4 * 4) {
+        l_x[count + i] = -INFINITY;
+        l_tok[count + i] = 0x7fffffff;
+    }
 }
 
 template <typename L, bool TOP>
@@ -286,7 +335,16 @@ __global__ __launch_bounds__(TL_WAVES * 64) void logprob_kernel(const void* __re
     }
 
     LaneSums sum;
-    float most = -INFINITY;
+    // a lane's largest logit, and that of the steps that make a group (`per` of them) with their count and the group's number
+    const int turns = (p.c1 - p.c0 + TL_WAVES * STEP - 1) / (TL_WAVES * STEP), per = (turns + TL_TURNS - 1) / TL_TURNS;
+    float most = -INFINITY, group_most = -INFINITY;
+    int steps = 0, step_group = 0;
+    auto keep_group = [&] {
+        sh.most[step_group++][threadIdx.x] = (uint16_t)(__float_as_uint(group_most + 0.f) >> 16);
+        most = fmaxf(most, group_most);
+        group_most = -INFINITY;
+        steps = 0;
+    };
     for (int v0 = v_first; v0 < p.c1; v0 += TL_WAVES * STEP) {
         float f[E];
 #pragma unroll
@@ -304,7 +362,10 @@ __global__ __launch_bounds__(TL_WAVES * 64) void logprob_kernel(const void* __re
             for (int k = 0; k < E; ++k) f[k] = f[k] == INFINITY ? 3.402823466e38f : f[k];
             mx = mx == INFINITY ? 3.402823466e38f : mx;
         }
-        most = fmaxf(most, mx);
+        if constexpr (TOP) {
+            group_most = fmaxf(group_most, mx);
+            if (++steps == per) keep_group();
+        }
         const bool moves = mx > -INFINITY && (!sum.has || mx - sum.ref > 8.f);
         if (__ballot(moves)) {
             if (moves) sum.move(mx);
@@ -344,7 +405,11 @@ __global__ __launch_bounds__(TL_WAVES * 64) void logprob_kernel(const void* __re
     for (int o = 32; o > 0; o >>= 1) s.above += __shfl_xor(s.above, o, 64);
     if (lane == 0) w_sums[w] = s;
     int kept = 0;
-    if constexpr (TOP) kept = best_of_piece<L>(p, sh, v_first + lane * VEC < p.c1 ? order32(most + 0.f) : 0u, n);
+    if constexpr (TOP) {
+        if (steps) keep_group();
+        for (; step_group < (turns + per - 1) / per; ++step_group) sh.most[step_group][threadIdx.x] = 0xffffu;      // below every logit
+    }
+    if constexpr (TOP) kept = best_of_piece<L>(p, sh, per, v_first + lane * VEC < p.c1 ? order32(most + 0.f) : 0u, n);
     else __syncthreads();
     float m = w_sums[0].m;
 #pragma unroll
@@ -365,11 +430,11 @@ __global__ __launch_bounds__(TL_WAVES * 64) void logprob_kernel(const void* __re
     }
     if constexpr (TOP) {
         const int64_t at = (int64_t)blockIdx.x * n;
+        if (threadIdx.x < 3) list_end(sh.x, sh.tok, kept, threadIdx.x);       // TL_LIST is a multiple of four
+        __syncthreads();
         for (int i = threadIdx.x; i < kept; i += TL_WAVES * 64) {
             const float x = sh.x[i];
-            const int id = sh.tok[i];
-            int rank = 0;
-            for (int j = 0; j < kept; ++j) rank += sh.x[j] > x || (sh.x[j] == x && sh.tok[j] < id);
+            const int id = sh.tok[i], rank = rank_in(sh.x, sh.tok, kept, x, id);
             if (rank >= n) continue;
             if (groups == 1) {
                 out.top_tokens[row * n + rank] = id;
@@ -431,10 +496,11 @@ __global__ __launch_bounds__(TJ_THREADS) void logprob_join_kernel(const void* __
     if constexpr (TOP) {
         __syncthreads();
         if (tid >= 64) return;
-        int at = lane * n;
-        const int end = lane < groups ? at + n : at;
-        uint32_t key = at < end ? l_key[at] : 0u, best = 0;
-        int head = at < end ? l_tok[at] : 0, id = 0;
+        // a lane's list: its head, the entry behind it (on its way), where the next one lies
+        int at = lane * n + 2, id = 0;
+        const int end = lane < groups ? lane * n + n : 0;
+        uint32_t key = at - 2 < end ? l_key[at - 2] : 0u, key2 = at - 1 < end ? l_key[at - 1] : 0u, best = 0;
+        int head = at - 2 < end ? l_tok[at - 2] : 0, head2 = at - 1 < end ? l_tok[at - 1] : 0;
         for (int i = 0; i < n; ++i) {
             const uint32_t m = wave_max_u32(key);
             const int from = (int)__builtin_ctzll(__ballot(key == m));
@@ -444,9 +510,11 @@ __global__ __launch_bounds__(TJ_THREADS) void logprob_join_kernel(const void* __
                 id = t;
             }
             if (lane == from) {
+                key = key2;
+                head = head2;
+                key2 = at < end ? l_key[at] : 0u;
+                head2 = at < end ? l_tok[at] : 0;
                 ++at;
-                key = at < end ? l_key[at] : 0u;
-                head = at < end ? l_tok[at] : 0;
             }
         }
         if (lane < n) {

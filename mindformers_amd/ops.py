@@ -6,6 +6,7 @@ the kernel on torch's current stream.  Nothing is computed in Python.
 """
 import contextlib
 import ctypes
+import functools
 import math
 import warnings
 from typing import NamedTuple
@@ -1053,7 +1054,15 @@ def token_logprobs(logits, tokens, n_top=0):
 
 
 # --------------------------------------------------------------------------------------------- low-rank adapters
-_INTS = [ctypes.c_int32 * n for n in range(9)]                # host arrays of slices
+@functools.lru_cache(maxsize=256)
+def _host_ints(values):
+    """A host array for the library, which only reads it."""
+    return (ctypes.c_int32 * len(values))(*values)
+
+
+@functools.lru_cache(maxsize=1024)
+def _adapter_bytes(*sizes):
+    return _lib.load().mf_adapter_workspace_bytes(*sizes)
 
 
 class AdapterRows(NamedTuple):
@@ -1114,14 +1123,15 @@ def adapter_linear(x, lora_a, lora_b, rows, base, widths=None, ranks=None, scale
         raise ValueError("scales must be a contiguous fp32 [n] on the adapters' device")
     if x.shape[-1:] != (k,) or base.shape[-1:] != (cols,):
         raise ValueError(f"x must be [T, {k}], base [T, {cols}]")
-    x, xs = _rows(x, k, "x")
+    x, xs = (x, k) if x.is_contiguous() else _rows(x, k, "x")
     at = x.data_ptr()
     if at % 16 or xs % 8:                                     # a slice whose rows are not on 16-byte borders
         x, xs = x.reshape(-1, k).clone(memory_format=torch.contiguous_format), k
         at = x.data_ptr()
-    base, bs = _rows(base, cols, "base")
+    whole = base.is_contiguous()
+    base, bs = (base, cols) if whole else _rows(base, cols, "base")
     if out is None:
-        out = torch.empty_like(base) if base.is_contiguous() else base.new_empty(base.shape)
+        out = torch.empty_like(base) if whole else base.new_empty(base.shape)
         got, os = out, cols
     else:
         got, os = _rows(out, cols, "out")
@@ -1132,10 +1142,10 @@ def adapter_linear(x, lora_a, lora_b, rows, base, widths=None, ranks=None, scale
     pa, pb = lora_a.data_ptr(), lora_b.data_ptr()
     _need((pa | pb) % 16 == 0, "lora_a and lora_b must lie on 16-byte borders")
     lib, dev = _lib.load(), lora_a.device
-    ws = workspace(lib.mf_adapter_workspace_bytes(t, n, tile, k, slices, r), dev, "adapter")
+    ws = workspace(_adapter_bytes(t, n, tile, k, slices, r), dev, "adapter")
     with _on(dev):
         check(lib.mf_adapter_linear(got.data_ptr(), at, pa, pb, base.data_ptr(), plan.data_ptr(), ptr(ranks), ptr(scales),
-                                    _INTS[slices](*widths), slices, t, n, tile, k, r, xs, bs, os, dtype_code(dtype), ws.data_ptr(),
+                                    _host_ints(widths), slices, t, n, tile, k, r, xs, bs, os, dtype_code(dtype), ws.data_ptr(),
                                     ws.numel(), stream_ptr(dev)), "mf_adapter_linear")
     return out
 
