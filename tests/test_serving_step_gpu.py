@@ -218,6 +218,50 @@ def test_logprobs_of_masked_infinite_and_equal_logits(dtype):
             _check_logprobs(x, tokens, n)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("v", [20011, 100003])
+def test_logprobs_of_many_equal_or_crowded_logits(dtype, v):
+    """More equal logits at the n-th place than a workgroup ranks at a time, and the best ones crowded: side by side, in one lane's columns, in
+    the last piece, as far apart as the type allows; a row that is masked but for a few."""
+    gen = torch.Generator().manual_seed(v)
+    x = (torch.rand(9, v, generator=gen) < 0.5).float() * 2 - 1
+    x[1] = torch.randint(0, 40, (v,), generator=gen).float() / 8
+    x[2] = torch.randn(v, generator=gen)
+    x[2, 7000:10000] += 20                                    # side by side
+    x[3] = torch.randn(v, generator=gen) / 16
+    x[3, 5::4096] = 30                                        # of one lane, all alike
+    x[4] = torch.randn(v, generator=gen) / 16
+    for i in range(8):
+        x[4, 40 + i::1024] = 10 + torch.arange(len(x[4, 40 + i::1024])).float() / 64
+    x[5] = torch.linspace(-30, 30, v)
+    x[6] = -float("inf")
+    x[6, [3, 7777, v - 1]] = torch.tensor([1.0, 2.0, 1.0])
+    x[7] = 0.0
+    x[7, ::3] = -0.0
+    x[8] = torch.randn(v, generator=gen)
+    x[8, -700:] = 50
+    x = x.to(dtype).cuda()
+    for n in (1, 20, 64):
+        _check_logprobs(x, np.array([0, 5, 9999, 5 + 4096, v - 1, v // 2, 3, 3, v - 1]), n)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+def test_logprobs_of_masked_rows_in_pieces(dtype):
+    """As the rows above, over several workgroups a row: pieces without a logit, and with fewer than are asked for."""
+    v = 70003
+    x = _logits(7, v, dtype, 6)
+    x[0, 5:] = -float("inf")
+    x[1, :69000] = float("nan")
+    x[2] = -float("inf")
+    x[3] = torch.finfo(dtype).min
+    x[4, 20000:] = -float("inf")
+    x[5, [9, 40000]] = float("inf")
+    x[6, ::2] = float("nan")
+    for tokens in (np.arange(7) * 10000, np.array([3, 69500, v - 1, 50000, 20001, 40000, 60001])):
+        for n in (0, 5, 64):
+            _check_logprobs(x, tokens, n)
+
+
 def test_logprobs_of_large_logits_of_both_signs():
     """Distances of the logits up to the range of float32 and past it: the smaller ones are out, -(a float) or -inf as the difference is."""
     x = _logits(4, 3000, F32, 3)
