@@ -6,7 +6,8 @@
 // One pass over the logits for the sums, the rank and the largest logit of every lane's steps; the best ones are looked for behind it, in
 // those steps of lanes whose largest reaches the n-th largest of the workgroup's 256 lanes: some more than n times 16 logits, read once
 // more.  (4137 x 152064 bf16 with 5, 20 and 64 alternatives: 211, 215 and 228 us; whole lanes read again, of whose 16 bytes a step
-// memory gives 128, 220, 297 and 403; a list kept on the way 280, 347 and 545; without alternatives 215.)  The waves of a workgroup take the steps of a piece of a
+// memory gives 128, 220, 297 and 403; a list kept on the way 280, 347 and 545; without alternatives 215; of rows of equal logits, which
+// reach it all, 233, 230 and 235.)  The waves of a workgroup take the steps of a piece of a
 // row in turn; each lane's sums are about a reference m of its own (moved when a logit passes it by more than 8: the sums stay
 // in range and H loses no more than that).  A row of one workgroup is done then, others are joined by a second kernel.  Sums in
 // float32: their errors are of the size of the rounding of what comes out.
@@ -101,6 +102,19 @@ __device__ __forceinline__ float below(float x) { return order32_back(order32(x 
 
 __device__ u32x4 tl_nothing;                                  // what a row without a whole vector loads in its place
 
+// the largest of a wave's values, in every lane
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+#define TL_DPP(ctrl) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xf, 0xf, false))
+    TL_DPP(0x111);                                            // from 1, 2, 4, 8 lanes below within sixteen
+    TL_DPP(0x112);
+    TL_DPP(0x114);
+    TL_DPP(0x118);
+    TL_DPP(0x142);                                            // the last lane of sixteen to the next sixteen, of 32 to the next 32
+    TL_DPP(0x143);
+#undef TL_DPP
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
 // The columns of a row that a workgroup has, and how its lanes take them: lane l of wave w has, of step k, vectors u at columns
 // c0 + (k TL_WAVES + w) STEP + (64 u + l) VEC.  Columns are counted from the 16-byte boundary at or before the row's start, `mis` elements in
 // front of it.
@@ -136,9 +150,9 @@ struct TopShared {
 __device__ __forceinline__ uint32_t order_high(uint16_t h) { return (uint16_t)(h ^ ((int16_t)h < 0 ? 0xffffu : 0x8000u)); }
 
 // Calls what(x, token) for the logits of the lanes and groups whose largest may reach key k: from a list, a vector a thread (four at a time),
-// or, where they are more than it takes, each lane for itself.  `per`: steps of a group.
-template <typename L, typename F>
-__device__ __forceinline__ void for_hits(const RowPiece& p, TopShared& sh, int per, uint32_t k, F&& what) {
+// or, where they are more than it takes, each lane for itself; `enough` says when to stop.  `per`: steps of a group.
+template <typename L, typename F, typename G>
+__device__ __forceinline__ void for_hits(const RowPiece& p, TopShared& sh, int per, uint32_t k, F&& what, G&& enough) {
     constexpr int VEC = L::VEC, VECS = L::VECS, STEP = 64 * VEC * VECS, AT_ONCE = 4;
     const int turns = (p.c1 - p.c0 + TL_WAVES * STEP - 1) / (TL_WAVES * STEP), groups = (turns + per - 1) / per;
     auto vector = [&](int g, int lane, int r) {               // column of vector r of a lane and group
@@ -164,7 +178,7 @@ __device__ __forceinline__ void for_hits(const RowPiece& p, TopShared& sh, int p
     __syncthreads();
     const int hits = sh.hits, each = per * VECS, items = hits * each;
     if (hits <= TL_HITS) {
-        for (int i0 = threadIdx.x; i0 < items; i0 += AT_ONCE * TL_WAVES * 64) {
+        for (int i0 = threadIdx.x; i0 < items && !enough(); i0 += AT_ONCE * TL_WAVES * 64) {
             u32x4 raw[AT_ONCE];
             int at[AT_ONCE];
 #pragma unroll
@@ -181,7 +195,7 @@ __device__ __forceinline__ void for_hits(const RowPiece& p, TopShared& sh, int p
     } else {
         for (int g = 0; g < groups; ++g)
             if (order_high(sh.most[g][threadIdx.x]) >= k >> 16)
-                for (int r = 0; r < each; ++r) {
+                for (int r = 0; r < each && !enough(); ++r) {
                     const int v = vector(g, threadIdx.x, r);
                     if (v < p.c1) use(v, load(v));
                 }
@@ -207,7 +221,8 @@ __device__ int best_of_piece(const RowPiece& p, TopShared& sh, int per, uint32_t
         if (c >= n) bound = trial;
         if (c == n) break;                                    // no bit below changes which lanes these are
     }
-    auto count_from = [&](uint32_t k) {                       // how many reach key k; the first TL_LIST of them go into the list
+    // how many reach key k (not all of them where it is more than TL_LIST, of which the first go into the list)
+    auto count_from = [&](uint32_t k) {
         __syncthreads();
         if (threadIdx.x == 0) sh.count = 0;
         for_hits<L>(p, sh, per, k, [&](float x, int tok) {
@@ -218,40 +233,58 @@ __device__ int best_of_piece(const RowPiece& p, TopShared& sh, int per, uint32_t
                     sh.tok[i] = tok;
                 }
             }
-        });
+        }, [&] { return __hip_atomic_load(&sh.count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) > TL_LIST; });
         return sh.count;
     };
     int c = count_from(bound);
     if (c <= TL_LIST) return c;
-    // More than fit: a higher bound that at least n reach, between `bound` and the largest key; the same in every thread.
-    uint32_t lo = bound, hi = 0xff800001u;                    // (no key is above that of +inf)
+    // More than fit: a higher bound that at least n reach, between `bound` and the largest key; the same in every thread.  In bits that the
+    // type's keys differ in.
+    constexpr int LOW = LowBit<L>::value;
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < TL_WAVES; ++i) most = max(most, k4[i]);
+    uint32_t lo = bound >> LOW, hi = (wave_max_u32(most) >> LOW) + 1;         // (no key is above that of +inf)
     while (hi - lo > 1) {
         const uint32_t mid = lo + (hi - lo) / 2;
-        c = count_from(mid);
+        c = count_from(mid << LOW);
         if (c >= n && c <= TL_LIST) return c;
         if (c > TL_LIST) lo = mid;
         else hi = mid;
     }
-    // Fewer than n above the logits of key `lo`, and more of those than fit: the lowest tokens of them, looked for in order.
-    c = count_from(hi);
-    const float level = order32_back(lo);
-    for (int v0 = p.c0 / L::VEC * L::VEC; v0 < p.c1 && c < n; v0 += TL_WAVES * 64) {
-        const int v = v0 + (int)threadIdx.x;
-        const bool in = v >= p.mis && v >= p.c0 && v < p.c1;
-        const bool tie = in && counted(L::at(p.base, min(max(v - p.mis, 0), p.vocab - 1))) == level;
-        const uint64_t t = __ballot(tie);
-        if (lane == 0) sh.key[threadIdx.x >> 6] = __popcll(t);
-        __syncthreads();
-        int before = c, all = 0;
+    // Fewer than n above the logits of key `lo`, and more of those than fit: the lowest tokens of them, looked for in order.  (A key's low
+    // bits: all ones of negative values.)
+    c = count_from(hi << LOW);
+    lo <<= LOW;
+    const float level = order32_back(lo >> 31 ? lo : lo | ((1u << LOW) - 1));
+    constexpr int AT_ONCE = 4;                                // columns a thread
+    for (int v0 = p.c0; v0 < p.c1 && c < n; v0 += AT_ONCE * TL_WAVES * 64) {
+        float x[AT_ONCE];
 #pragma unroll
-        for (int i = 0; i < TL_WAVES; ++i) {
-            if (i < (int)(threadIdx.x >> 6)) before += sh.key[i];
-            all += sh.key[i];
+        for (int j = 0; j < AT_ONCE; ++j)
+            x[j] = L::at(p.base, min(max(v0 + j * TL_WAVES * 64 + (int)threadIdx.x - p.mis, 0), p.vocab - 1));
+        uint64_t tie[AT_ONCE];
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            const int v = v0 + j * TL_WAVES * 64 + (int)threadIdx.x;
+            tie[j] = __ballot(v >= p.mis && v < p.c1 && counted(x[j]) == level);
+            if (lane == 0) sh.key[j * TL_WAVES + (threadIdx.x >> 6)] = __popcll(tie[j]);
         }
-        before += __popcll(t & ((1ull << lane) - 1ull));
-        if (tie && before < n) {
-            sh.x[before] = level;
-            sh.tok[before] = v - p.mis;
+        __syncthreads();
+        int all = 0;
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            int before = c + all;
+#pragma unroll
+            for (int i = 0; i < TL_WAVES; ++i) {
+                if (i < (int)(threadIdx.x >> 6)) before += sh.key[j * TL_WAVES + i];
+                all += sh.key[j * TL_WAVES + i];
+            }
+            before += __popcll(tie[j] & ((1ull << lane) - 1ull));
+            if ((tie[j] >> lane & 1) && before < n) {
+                sh.x[before] = level;
+                sh.tok[before] = v0 + j * TL_WAVES * 64 + (int)threadIdx.x - p.mis;
+            }
         }
         c = min(c + all, n);
         __syncthreads();
@@ -449,19 +482,6 @@ __global__ __launch_bounds__(TL_WAVES * 64) void logprob_kernel(const void* __re
             cand_tok[at + threadIdx.x] = -1;
         }
     }
-}
-
-// the largest of a wave's values, in every lane
-__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-#define TL_DPP(ctrl) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xf, 0xf, false))
-    TL_DPP(0x111);                                            // from 1, 2, 4, 8 lanes below within sixteen
-    TL_DPP(0x112);
-    TL_DPP(0x114);
-    TL_DPP(0x118);
-    TL_DPP(0x142);                                            // the last lane of sixteen to the next sixteen, of 32 to the next 32
-    TL_DPP(0x143);
-#undef TL_DPP
-    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 // Joins the workgroups of a row: their sums, and their lists, which are in order, by taking the best head n times (a lane a list; equal

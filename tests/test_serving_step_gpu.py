@@ -218,7 +218,7 @@ def test_logprobs_of_masked_infinite_and_equal_logits(dtype):
             _check_logprobs(x, tokens, n)
 
 
-@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
 @pytest.mark.parametrize("v", [20011, 100003])
 def test_logprobs_of_many_equal_or_crowded_logits(dtype, v):
     """More equal logits at the n-th place than a workgroup ranks at a time, and the best ones crowded: side by side, in one lane's columns, in
@@ -243,6 +243,24 @@ def test_logprobs_of_many_equal_or_crowded_logits(dtype, v):
     x = x.to(dtype).cuda()
     for n in (1, 20, 64):
         _check_logprobs(x, np.array([0, 5, 9999, 5 + 4096, v - 1, v // 2, 3, 3, v - 1]), n)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+@pytest.mark.parametrize("v", [2011, 20011, 100003])
+def test_logprobs_of_equal_logits_below_zero(dtype, v):
+    """More equal logits than a workgroup ranks at a time at values below zero, with none, few and many above them, and next to one."""
+    eps = torch.finfo(dtype).eps
+    x = torch.full((6, v), -1.5)
+    x[1, 700::900] = -1.25
+    x[2, 100:1700] = -1.5 * (1 + eps)                         # the values next to it
+    x[3, ::2] = -1.5 * (1 - eps)
+    x[4] = -40000.0
+    x[4, -3:] = -0.0
+    x[5] = -torch.finfo(dtype).tiny
+    x[5, 1::3] = 0.0
+    x = x.to(dtype).cuda()
+    for n in (1, 20, 64):
+        _check_logprobs(x, np.array([0, 700, 100, 2, v - 3, 1]), n)
 
 
 @pytest.mark.parametrize("dtype", [BF, FP, F32])
