@@ -36,9 +36,11 @@ __device__ __forceinline__ void sort_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// Lanes of the wave that have this lane's key (bits of it that any key may have: `bits`); lanes without a key are in nobody's.
+// Lanes of the wave that have this lane's key (bits of it that any key may have: `bits`); lanes without a key are in nobody's.  Prompts
+// have one key a wave.
 __device__ __forceinline__ uint64_t same_key(int key, int bits, bool on) {
     uint64_t m = __ballot(on);
+    if (__ballot(on && key != __builtin_amdgcn_readfirstlane(key)) == 0) return m;
     for (int b = 0; b < bits; ++b) {
         const uint64_t set = __ballot((key >> b) & 1);
         m &= (key >> b) & 1 ? set : ~set;
@@ -65,6 +67,7 @@ __global__ __launch_bounds__(WAVES * 64) void adapter_rows_kernel(int* __restric
     const int piece = ((tokens + WAVES - 1) / WAVES + 63) / 64 * 64;
     const int r0 = min(w * piece, tokens), r1 = min(r0 + piece, tokens);
     int key[AD_BATCH];
+    uint64_t same[AD_BATCH];
     auto load = [&](int rb) {
 #pragma unroll
         for (int i = 0; i < AD_BATCH; ++i) {
@@ -81,7 +84,7 @@ __global__ __launch_bounds__(WAVES * 64) void adapter_rows_kernel(int* __restric
         for (int i = 0; i < AD_BATCH; ++i) {
             const int r = rb + 64 * i + lane;
             if (rb + 64 * i >= r1) break;
-            const uint64_t m = same_key(key[i], bits, r < r1);
+            const uint64_t m = same[i] = same_key(key[i], bits, r < r1);
             sort_fence();
             if (r < r1 && (int)__builtin_ctzll(m) == lane) hist[w * n + key[i]] += __popcll(m);
             sort_fence();
@@ -123,12 +126,13 @@ __global__ __launch_bounds__(WAVES * 64) void adapter_rows_kernel(int* __restric
     if (tid == 0) start[n] = tokens;
     __syncthreads();
     for (int rb = r0; rb < r1; rb += 64 * AD_BATCH) {
-        if (piece > 64 * AD_BATCH) load(rb);                  // otherwise the keys are still there
+        const bool again = piece > 64 * AD_BATCH;             // otherwise the keys are still there
+        if (again) load(rb);
 #pragma unroll
         for (int i = 0; i < AD_BATCH; ++i) {
             const int r = rb + 64 * i + lane;
             if (rb + 64 * i >= r1) break;
-            const uint64_t m = same_key(key[i], bits, r < r1);
+            const uint64_t m = again ? same_key(key[i], bits, r < r1) : same[i];
             sort_fence();
             const int at = hist[w * n + key[i]];
             if (r < r1) order[start[key[i]] + at + __popcll(m & ((1ull << lane) - 1ull))] = r;
