@@ -164,7 +164,10 @@ class DecodeStackRunner:
         ids_t = None
         if adapter_ids is not None:
             if isinstance(adapter_ids, torch.Tensor) and adapter_ids.is_cuda:
-                ids_t = adapter_ids.reshape(-1).to(torch.int32)
+                ids_t = adapter_ids.reshape(-1)
+                if ids_t.dtype == torch.int64:
+                    ids_t = ids_t.clamp(-1, 2 ** 31 - 1)
+                ids_t = ids_t.to(torch.int32)
                 if ids_t.numel() == lens.size and q_lens is not None:
                     ids_t = torch.repeat_interleave(ids_t, torch.as_tensor(q_lens, device=self.device), output_size=t)
             else:
@@ -179,7 +182,7 @@ class DecodeStackRunner:
         slots = there["slots"] if "slots" in there else torch.as_tensor(slot_mapping, dtype=torch.int32, device=self.device)
         pos_t = there["pos"] if "pos" in there else torch.as_tensor(position_ids, device=self.device).reshape(-1)
         cos, sin = self._rope_rows(pos_t, there["freq"].view(torch.float32)) if self.rotary is None else (None, None)
-        h = self._run_layers(hidden_states, tables, lens_t, slots, cos, sin, q_starts, pos_t, there.get("ids", ids_t))
+        h = self._run_layers(hidden_states, tables, lens_t, slots, cos, sin, q_starts, **self._of_rows(pos_t, there.get("ids", ids_t)))
         if prefill:
             self.add_flags_custom(is_first_iteration=False)
         return h
@@ -198,7 +201,12 @@ class DecodeStackRunner:
         self.add_flags_custom(is_first_iteration=False)
         pos = torch.clamp(context_lens - 1, min=0)
         cos, sin = self._rope_rows(pos, self._freq_dev) if self.rotary is None else (None, None)
-        return self._run_layers(hidden_states, block_tables, context_lens, slot_mapping, cos, sin, None, pos, adapter_ids)
+        return self._run_layers(hidden_states, block_tables, context_lens, slot_mapping, cos, sin, None, **self._of_rows(pos, adapter_ids))
+
+    def _of_rows(self, positions, adapter_ids):
+        """What rows bring beside the rotary rows, named only where they do: a subclass's ``_run_layers`` may know nothing of it."""
+        named = {} if self.rotary is None else {"positions": positions}
+        return named if adapter_ids is None else {**named, "adapter_ids": adapter_ids}
 
     def _run_layers(self, h, tables, lens_t, slots, cos, sin, q_starts, positions=None, adapter_ids=None):
         normed, more = None, {}

@@ -269,3 +269,25 @@ def test_a_captured_step_with_adapters_follows_its_ids_and_lengths():
         torch.cuda.synchronize()
         for a, w in zip(got, step()):
             assert torch.equal(a, w)
+
+
+def test_ids_past_32_bits_and_a_runner_with_its_own_layer_loop():
+    layers = _layers(1, ("wo",))
+    x = torch.randn(3, HIDDEN, device="cuda").to(BF)
+    lens, tables, slots = np.array([1, 1, 1]), np.arange(3, dtype=np.int32).reshape(3, 1), np.arange(3, dtype=np.int32) * BS
+    plain = DecodeStackRunner(layers, npu_mem_size=0.002, cpu_mem_size=0, block_size=BS)
+    none = plain.forward(x, lens, tables, slots, prefill=False)
+    some = plain.forward(x, lens, tables, slots, prefill=False, adapter_ids=[1, -1, 2])
+    assert not torch.equal(some, none) and torch.equal(some[1], none[1])
+    wide = torch.tensor([1, 2 ** 32, -2 ** 32 + 2], device="cuda")           # the slots 0 and 2 in their lowest 32 bits
+    for ids in (wide, wide.cpu().numpy()):
+        got = plain.forward(x, lens, tables, slots, prefill=False, adapter_ids=ids)
+        assert torch.equal(got[0], some[0]) and torch.equal(got[1:], none[1:])
+
+    class Own(DecodeStackRunner):
+        def _run_layers(self, h, tables, lens_t, slots, cos, sin, q_starts):
+            return super()._run_layers(h, tables, lens_t, slots, cos, sin, q_starts)
+
+    own = Own(layers, npu_mem_size=0.002, cpu_mem_size=0, block_size=BS)
+    assert torch.equal(own.forward(x, lens, tables, slots, prefill=False), none)
+    assert torch.equal(own.decode(x, _i32(lens), _i32(tables), _i32(slots)), none)
