@@ -501,3 +501,42 @@ def test_operators_on_another_stream():
     other.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_rows_and_cache_rows_past_32_bits():
+    """Rows 2^31 elements apart, cache rows behind 2^31 elements: as the same rows side by side."""
+    big = torch.empty(2 * 2 ** 31 + 6000, dtype=BF, device="cuda")
+
+    def apart(x):
+        y = big.as_strided(x.shape, (2 ** 31, 1))
+        return y.copy_(x)
+
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    logits = torch.randn(3, 5003, generator=gen, device="cuda").to(BF)
+    tokens = _i32([7, 5002, -1])
+    for a, b in zip(ops.token_logprobs(apart(logits), tokens, n_top=5), ops.token_logprobs(logits, tokens, n_top=5)):
+        assert torch.equal(a, b)
+
+    rng = np.random.default_rng(4)
+    _, _, at, bt = _bank(rng, 2, (96,), 16, 64, BF, [16, 8])
+    ranks, rows = _i32([16, 8]), ops.adapter_rows(_i32([1, -1, 0]), 2)
+    x, base = logits[:, :64].contiguous(), logits[:, 64:160].contiguous()
+    want = ops.adapter_linear(x, at, bt, rows, base, ranks=ranks)
+    assert torch.equal(ops.adapter_linear(apart(x), at, bt, rows, base, ranks=ranks), want)
+    far = apart(base)
+    assert ops.adapter_linear(x, at, bt, rows, far, ranks=ranks, out=far) is far and torch.equal(far, want)
+
+    block, heads, d = 128, 8, 128
+    blocks = 2 ** 31 // (block * heads * d) + 2
+    kc, vc = (torch.empty(blocks, block, heads, d, dtype=BF, device="cuda") for _ in range(2))
+    slots, pos, inv = _i32([blocks * block - 1, 5, blocks * block - 129]), _i32([3, 1000, 70000]), torch.from_numpy(_inv(64)).cuda()
+    qkv = logits[:, :(4 + 2 * heads) * d].contiguous()
+    q, k, v = qkv[:, :4 * d], qkv[:, 4 * d:(4 + heads) * d], qkv[:, (4 + heads) * d:]
+    q_want, k_want = torch.empty(3, 4 * d, dtype=BF, device="cuda"), torch.empty(3, heads * d, dtype=BF, device="cuda")
+    ops.rotary_embedding(q, k, pos, inv, d, out=(q_want, k_want))
+    wide = apart(qkv)
+    ops.rotary_embedding(wide[:, :4 * d], wide[:, 4 * d:(4 + heads) * d], pos, inv, d, value=wide[:, (4 + heads) * d:], key_cache=kc, value_cache=vc,
+                         slot_mapping=slots)
+    assert torch.equal(wide[:, :4 * d], q_want) and torch.equal(wide[:, 4 * d:(4 + heads) * d], k_want)
+    at = slots.long()
+    assert torch.equal(kc.view(-1, heads * d)[at], k_want) and torch.equal(vc.view(-1, heads * d)[at], v)
