@@ -3,7 +3,7 @@
 //   out[t, s] = base[t, s] + scale[a] * B[a]_s (A[a]_s x[t]),   a = the adapter of row t, s = the slices of a fused projection
 //
 // A step's rows are sorted by adapter once (adapter_rows_kernel) into tiles of rows that share one; every projection of the step runs
-// two kernels on those tiles.  The first computes h = A x, [rows, slices x rank], with the K axis cut over workgroups and waves; the
+// two kernels on those tiles (a single row one kernel, adapter_row_kernel).  The first computes h = A x, [rows, slices x rank], with the K axis cut over workgroups and waves; the
 // second adds up the cuts, scales, and computes B h on top of the base rows.  Both products are on the matrix cores.  h stays in float32
 // between them and enters the second product as the sum of two 16-bit values (hi + lo), which fill the 32-deep instruction with 16
 // ranks: its rounding is 2^-17 of h (bf16) where one value would have 2^-9.
@@ -489,6 +489,88 @@ __global__ __launch_bounds__(AD_WAVES * 64) void adapter_expand_kernel(const Ada
     }
 }
 
+// Both products of a single row in one launch: a workgroup computes its slice's h for itself, in vector instructions, and then a column a
+// thread.  A wave computes RB ranks at a time, sixteen waves all of them, with eight steps' loads of 1 KB on their way, B's first
+// ranks and base in front of them; h stays in float32.  A's matrix is read by every workgroup, at about 90 KB a microsecond, so it is taken up to 2^17
+// elements.  (us with the gap behind it, of the two launches in brackets: K 4096, 4096 columns, ranks 8, 16 and 32: 4.5, 5.3, 7.3 (7.8, 7.7,
+// 8.1); 2 x 14336 columns 4.7, 5.6, 9.1 (8.2, 8.2, 8.2); K 14336, rank 16: 11.3 (8.6).  A call of one launch takes the host 3 us less.)
+constexpr int64_t AF_MOST = 1 << 17;
+constexpr int AF_WAVES = 16, AF_COLS = AF_WAVES * 64, AF_LOADS = 8;
+template <typename T, int RB>
+__global__ __launch_bounds__(AF_WAVES * 64) void adapter_row_kernel(const AdapterArgs A) {
+    constexpr int STEPS = AF_LOADS / RB;
+    __shared__ __align__(16) float h[AD_MAX_RANK];
+    const AdapterTile tile = A.tiles[0];
+    const int rank = tile.adapter < 0 ? 0 : adapter_rank(A, tile.adapter);
+    if (rank == 0 && A.out == A.base) return;
+    int block = blockIdx.x;
+    const int s = slice_of(A, block, AF_COLS);
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int cols = A.s.width[s], col = block * AF_COLS + threadIdx.x, at = A.s.first[s] + min(col, cols - 1);
+    const uint16_t base = A.base[at];
+    u32x4 bv[2];
+    const uint16_t* b = A.b + ((int64_t)max(tile.adapter, 0) * A.s.total + at) * A.rank;
+    if (rank) {
+        bv[0] = *(const u32x4*)b;
+        bv[1] = *(const u32x4*)(b + min(8, A.rank - 8));
+        const uint16_t* a0 = A.a + ((int64_t)tile.adapter * A.s.n + s) * A.rank * A.k;
+        const float scale = A.scales ? A.scales[tile.adapter] : 1.f;
+        for (int j0 = w * RB; j0 < rank; j0 += AF_WAVES * RB) {
+            float acc[RB];
+#pragma unroll
+            for (int j = 0; j < RB; ++j) acc[j] = 0.f;
+            for (int k1 = 0; k1 < A.k; k1 += STEPS * 512) {
+                const int k0 = k1 + 8 * lane;
+                u32x4 av[STEPS][RB], xv[STEPS];
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i) {
+                    const int k = min(k0 + 512 * i, A.k - 8);
+#pragma unroll
+                    for (int j = 0; j < RB; ++j) av[i][j] = *(const u32x4*)(a0 + (int64_t)min(j0 + j, rank - 1) * A.k + k);
+                    xv[i] = *(const u32x4*)(A.x + k);
+                }
+                __builtin_amdgcn_sched_barrier(0);            // all of them before the first use
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i) {
+                    if (k0 + 512 * i >= A.k) break;           // behind the row's end
+                    float x[8];
+                    unpack8<T>(xv[i], x);
+#pragma unroll
+                    for (int j = 0; j < RB; ++j) {
+                        float f[8];
+                        unpack8<T>(av[i][j], f);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) acc[j] = fmaf(f[e], x[e], acc[j]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < RB; ++j) {
+                const float sum = wave_sum(acc[j]) * scale;
+                if (lane == 0 && j0 + j < rank) h[j0 + j] = sum;
+            }
+        }
+    }
+    __syncthreads();
+    if (col >= cols) return;
+    float sum = 0.f;
+    for (int j0 = 0; j0 < rank; j0 += 16) {
+        if (j0) {
+            bv[0] = *(const u32x4*)(b + min(j0, A.rank - 8));
+            bv[1] = *(const u32x4*)(b + min(j0 + 8, A.rank - 8));
+        }
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+            float f[8];
+            unpack8<T>(bv[o], f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (j0 + 8 * o + e < rank) sum = fmaf(f[e], h[j0 + 8 * o + e], sum);      // (behind the adapter's rank: whatever lies there)
+        }
+    }
+    A.out[at] = rank ? T::from_float(T::to_float(base) + sum) : base;
+}
+
 // How the products are cut.  Two tiles of ranks a workgroup (three of 64 rows: x is read by fewer).  Cuts of K: 1024 workgroups where there
 // is that much, four units a wave and cut at least (eight where there are 128 tiles), 8 cuts at most: a cut is another float32 copy
 // of h.  Groups of columns a wave: up to four behind one sum of h, while 512 workgroups are left.  (us, of both kernels.  8191 rows, K 4096,
@@ -596,6 +678,20 @@ extern "C" int mf_adapter_linear(void* out, const void* x, const void* lora_a, c
     int64_t col_blocks = 0;
     for (int i = 0; i < slices; ++i) col_blocks += (A.s.width[i] + block_cols - 1) / block_cols;
     A.max_tiles = tiles, A.blocks = p.blocks, A.pitch = (rank + 31) / 32 * 32 + 8;
+    if (tokens == 1 && (int64_t)rank * k <= AF_MOST) {
+        int blocks = 0;
+        for (int i = 0; i < slices; ++i) blocks += (A.s.width[i] + AF_COLS - 1) / AF_COLS;
+#define AD_ROW(T, RB) hipLaunchKernelGGL((adapter_row_kernel<T, RB>), dim3(blocks), dim3(AF_WAVES * 64), 0, st, A)
+        if (dtype == MF_BF16) {
+            if (rank <= AF_WAVES) AD_ROW(BF16, 1);
+            else AD_ROW(BF16, 2);
+        } else {
+            if (rank <= AF_WAVES) AD_ROW(FP16, 1);
+            else AD_ROW(FP16, 2);
+        }
+#undef AD_ROW
+        return MF_LAUNCH_CHECK();
+    }
     const int64_t shrinks = ((int64_t)tiles * p.cuts + 7) / 8 * 8 * p.blocks;
     A.subs = tile / 16, A.col_blocks = (int)col_blocks;
     MF_REQUIRE(shrinks < (1 << 24) && tiles * A.subs * col_blocks < (1 << 24), "adapter_linear: %d rows of %lld columns", tokens,

@@ -399,6 +399,31 @@ def test_adapters_of_many_requests(dtype, t, n, r, k, widths):
     assert torch.equal(baset, got)                            # in place
 
 
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("n,r,k,widths", [(3, 8, 8, (1, 3)), (3, 32, 4096, (70, 1, 1025)), (2, 24, 4104, (1024, 1024)), (2, 128, 1024, (300,)),
+                                          (2, 128, 1032, (300,)), (4, 40, 520, (64, 64)), (2, 16, 8192, (2049,)), (2, 8, 14336, (100,))])
+def test_adapters_of_a_single_row(dtype, n, r, k, widths):
+    """Both sides of the size up to which one kernel computes a row's products, ranks that end inside the pieces they are taken in."""
+    rng = np.random.default_rng(k + r)
+    for rank in sorted({1, 5, 8, r // 2 + 3, r - 1, r} - {0}):
+        if rank > r:
+            continue
+        ranks = np.full(n, r)
+        ranks[n - 1] = rank
+        a, b, at, bt = _bank(rng, n, widths, r, k, dtype, ranks)
+        x, base = rounded(rng.normal(size=(1, k)), dtype), rounded(rng.normal(size=(1, sum(widths))), dtype)
+        xt, baset, scales = _dev(x, dtype), _dev(base, dtype), torch.full((n,), 0.75, device="cuda")
+        rows = ops.adapter_rows(_i32([n - 1]), n)
+        got = ops.adapter_linear(xt, at, bt, rows, baset, widths=widths, ranks=_i32(ranks), scales=scales)
+        want, mag = S.adapter_linear(x, a, b, [n - 1], base, widths, ranks, np.full(n, 0.75, np.float32))
+        _check_adapters(got, want, mag, x, k, dtype)
+        ops.adapter_linear(xt, at, bt, rows, baset, widths=widths, ranks=_i32(ranks), scales=scales, out=baset)
+        assert torch.equal(baset, got)
+        none = ops.adapter_linear(xt, at, bt, ops.adapter_rows(_i32([-1]), n), baset, widths=widths, ranks=_i32(ranks), scales=scales)
+        assert torch.equal(none, baset)
+
+
 @pytest.mark.parametrize("pad", [1, 4, 8])
 def test_adapters_of_column_slices(pad):
     """x, base and out as slices of wider rows, at alignments that are copied, moved element by element, and moved whole."""
