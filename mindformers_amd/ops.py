@@ -77,6 +77,22 @@ def _on(dev):
     return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
+# by themselves: what torch.cuda.current_device and a with statement add is a tenth of a small call
+_device_now = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_stream_now = _lib._raw_stream or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _on_index(index, entry, *args):
+    """Calls an entry point on the device ``index``, whose current stream is its last argument."""
+    if _device_now() == index:
+        rc = entry(*args, _stream_now(index))
+    else:
+        with torch.cuda.device(index):
+            rc = entry(*args, _stream_now(index))
+    if rc:
+        check(rc, entry.__name__)
+
+
 def rows_of(x, width):
     """x as [rows, width]: the tensor itself where it is that (a reshape to its own shape costs a microsecond of a small step)."""
     return x if x.dim() == 2 and x.shape[1] == width else x.reshape(-1, width)
@@ -174,20 +190,18 @@ def rotary_embedding(query, key, positions, inv_freq, head_dim, interleaved=Fals
     if not (index >= 0 and positions.get_device() == index and inv_freq.get_device() == index and positions.is_contiguous()
             and inv_freq.is_contiguous()):
         _need(_dev_of(query) == _dev_ok(positions, inv_freq), "all tensors must be on the same device")
-    if not (positions.dtype is torch.int32 and positions.dim() == 1 and inv_freq.dtype is torch.float64 and inv_freq.dim() == 1):
+    if not (positions.dtype is torch.int32 and len(positions.shape) == 1 and inv_freq.dtype is torch.float64 and len(inv_freq.shape) == 1):
         raise ValueError("positions must be int32 [T], inv_freq float64 [pairs]")
-    if not (dtype in _ACT and query.dim() > 0):
+    if dtype not in _ACT:
         raise ValueError("query must be bf16/fp16 [T, n_heads * head_dim]")
-    qw = query.shape[-1]
-    if not (0 < d <= 1024 and qw > 0 and qw % d == 0 and 0 < pairs and 0 <= offset and offset + 2 * pairs <= d):
-        raise ValueError(f"rows of {qw}, {pairs} pairs from column {offset} of heads of {d}: whole heads of up to 1024, and the pairs inside")
-    query, qs = _rows(query, qw, "query")
+    if not (0 < d <= 1024 and 0 < pairs and 0 <= offset and offset + 2 * pairs <= d):
+        raise ValueError(f"{pairs} pairs from column {offset} of heads of {d}: heads of up to 1024, and the pairs inside")
+    qw, qs = _head_rows(query, t, d, dtype, index, "query")
+    k = v = kc = vc = slot = None
     kw = ks = vs = slots = 0
-    if query.numel() != t * qw:
-        raise ValueError(f"query must hold a row for each of {t} positions")
     if key is not None:
-        kw = _head_rows(key, t, d, dtype, index, "key")
-        key, ks = _rows(key, kw, "key")
+        kw, ks = _head_rows(key, t, d, dtype, index, "key")
+        k = key.data_ptr()
     cached = key_cache is not None
     if cached or value_cache is not None or value is not None or slot_mapping is not None:
         if key is None or not cached or value_cache is None or value is None or slot_mapping is None:
@@ -198,41 +212,48 @@ def rotary_embedding(query, key, positions, inv_freq, head_dim, interleaved=Fals
         if not (key_cache.dtype is dtype and value_cache.dtype is dtype and key_cache.get_device() == index
                 and value_cache.get_device() == index and key_cache.is_contiguous() and value_cache.is_contiguous()):
             raise ValueError("caches must be contiguous, of query's type and on its device")
-        if not (slot_mapping.dtype is torch.int32 and slot_mapping.dim() == 1 and slot_mapping.numel() == t
-                and slot_mapping.get_device() == index and slot_mapping.is_contiguous()):
+        if not (slot_mapping.dtype is torch.int32 and slot_mapping.shape == (t,) and slot_mapping.get_device() == index
+                and slot_mapping.is_contiguous()):
             raise ValueError("slot_mapping must be a contiguous int32 [T] on query's device")
-        _need(_head_rows(value, t, d, dtype, index, "value") == kw, "value must have key's rows")
-        value, vs = _rows(value, kw, "value")
+        vw, vs = _head_rows(value, t, d, dtype, index, "value")
+        _need(vw == kw, "value must have key's rows")
+        v, kc, vc, slot = value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), slot_mapping.data_ptr()
         slots = shape[0] * shape[1]
+    q = query.data_ptr()
     if out is None:
-        q_out, k_out, qos, kos = query, key, qs, ks
+        q_out, k_out, qo, ko, qos, kos = query, key, q, k, qs, ks
     else:
         q_out, k_out = out
-        _need(_head_rows(q_out, t, d, dtype, index, "query_out") == qw, "query_out must have query's rows")
-        q_out, qos = _rows(q_out, qw, "query_out")
-        kos = 0
+        ko, kos = None, 0
+        ow, qos = _head_rows(q_out, t, d, dtype, index, "query_out")
+        _need(ow == qw, "query_out must have query's rows")
         if k_out is not None:
-            _need(key is not None and _head_rows(k_out, t, d, dtype, index, "key_out") == kw, "key_out must have key's rows")
-            k_out, kos = _rows(k_out, kw, "key_out")
+            ow, kos = _head_rows(k_out, t, d, dtype, index, "key_out")
+            _need(key is not None and ow == kw, "key_out must have key's rows")
+            ko = k_out.data_ptr()
         elif not (key is None or cached):
             raise ValueError("a key that goes neither to key_out nor into a cache")
-    lib, dev = _lib.load(), query.device
-    with _on(dev):
-        check(lib.mf_rotary_embedding(q_out.data_ptr(), ptr(k_out), query.data_ptr(), ptr(key), ptr(value), ptr(key_cache), ptr(value_cache),
-                                      positions.data_ptr(), inv_freq.data_ptr(), ptr(slot_mapping), t, qw // d, kw // d, d, pairs, int(offset),
-                                      1 if interleaved else 0, float(scale), slots, qs, ks, vs, qos, kos, dtype_code(dtype),
-                                      stream_ptr(dev)), "mf_rotary_embedding")
+        qo = q_out.data_ptr()
+    _on_index(index, _lib.load().mf_rotary_embedding, qo, ko, q, k, v, kc, vc, positions.data_ptr(), inv_freq.data_ptr(), slot, t, qw // d,
+              kw // d, d, pairs, int(offset), 1 if interleaved else 0, float(scale), slots, qs, ks, vs, qos, kos,
+              _lib.MF_BF16 if dtype is torch.bfloat16 else _lib.MF_FP16)
     return q_out, k_out
 
 
 def _head_rows(x, t, d, dtype, index, what):
-    """Width of a row of heads beside query, checked."""
-    if not (x.dtype is dtype and x.get_device() == index and x.dim() > 0):
+    """Width and distance of the rows of heads of a tensor beside query, checked."""
+    if not (x.dtype is dtype and x.get_device() == index):
         raise ValueError(f"{what} must have query's type and be on its device")
-    width = x.shape[-1]
+    shape = x.shape
+    if len(shape) == 2:                                       # nearly all: two looks at the tensor
+        rows, width = shape
+        row, col = x.stride()
+        if rows == t and col == 1 and width > 0 and width % d == 0 and (row >= width or t <= 1):
+            return width, row if t > 1 else width
+    width = shape[-1] if len(shape) else 0
     if not (width > 0 and width % d == 0 and x.numel() == t * width):
         raise ValueError(f"{what} must hold a row of heads of {d} for each of {t} positions")
-    return width
+    return width, _rows(x, width, what)[1]
 
 
 def rope_and_cache(query, key, value, cos, sin, key_cache, value_cache, slot_mapping, n_heads):
@@ -1024,33 +1045,44 @@ def token_logprobs(logits, tokens, n_top=0):
     """Log probabilities of ``tokens`` int32 [T] under softmax(logits[t]), their ranks, the entropy of every row and its ``n_top`` (up to
     64) most likely tokens; ties go to the lowest token.  logits [T, vocab], bf16, fp16 or fp32, may be a slice of wider rows.  A NaN logit
     counts as -inf, +inf as the largest float; a token outside the vocabulary (-1: a row of padding) gets -inf and rank -1."""
-    lib = _lib.load()
-    dev = _dev_of(logits, tokens)
-    _need(logits.dtype in _ACT or logits.dtype == torch.float32, "logits must be bf16, fp16 or fp32")
-    _need(logits.dim() == 2, "logits must be [T, vocab]")
-    t, v = logits.shape
-    _need(tokens.dtype == torch.int32 and tokens.dim() == 1 and tokens.numel() == t and tokens.is_contiguous(),
-          "tokens must be a contiguous int32 [T]")
-    _need(0 < v <= 0x7c000000 and t < 1 << 24, "1 to 0x7c000000 tokens of vocabulary and fewer than 2^24 rows")
-    stride = logits.stride(0) if t > 1 else v                 # one row: whatever its stride says
-    _need((logits.stride(1) == 1 or v == 1) and stride >= v, "logits rows must have a unit column stride and not overlap")
+    index, dtype = logits.get_device(), logits.dtype
+    if index < 0 or tokens.get_device() != index:
+        _dev_of(logits, tokens)                               # says what is wrong
+    if not (dtype in _ACT or dtype is torch.float32):
+        raise ValueError("logits must be bf16, fp16 or fp32")
+    if len(logits.shape) != 2:
+        raise ValueError("logits must be [T, vocab]")
+    (t, v), (stride, col) = logits.shape, logits.stride()
+    if not (tokens.dtype is torch.int32 and tokens.shape == (t,) and tokens.is_contiguous()):
+        raise ValueError("tokens must be a contiguous int32 [T]")
+    if not (0 < v <= 0x7c000000 and t < 1 << 24):
+        raise ValueError("1 to 0x7c000000 tokens of vocabulary and fewer than 2^24 rows")
+    if t <= 1:
+        stride = v                                            # one row: whatever its stride says
+    if not ((col == 1 or v == 1) and stride >= v):
+        raise ValueError("logits rows must have a unit column stride and not overlap")
     n = int(n_top)
     if not 0 <= n <= min(64, v):
         raise ValueError(f"n_top must be 0 to 64 and no more than the {v} tokens, got {n_top}")
+    dev, lib = logits.device, _lib.load()
     buf = torch.empty(t * (3 + 2 * n), dtype=torch.int32, device=dev)
     val, num = buf.view(torch.float32).as_strided, buf.as_strided
     res = TokenLogprobs(val((t,), (1,), 0), num((t,), (1,), t), val((t,), (1,), 2 * t), num((t, n), (n, 1), 3 * t),
                         val((t, n), (n, 1), (3 + n) * t))
     if t == 0:
         return res
-    code = dtype_code(logits.dtype)
-    need = lib.mf_token_logprobs_workspace_bytes(t, v, n, code)
+    code = dtype_code(dtype)
+    need = _logprob_bytes(t, v, n, code)
     ws = workspace(need, dev, "logprobs") if need else None
     a = buf.data_ptr()
-    with _on(dev):
-        check(lib.mf_token_logprobs(a, a + 4 * t, a + 8 * t, a + 12 * t, a + 4 * (3 + n) * t, ptr(logits), stride, ptr(tokens), t, v, n, code,
-                                    ptr(ws), ws.numel() if ws is not None else 0, stream_ptr(dev)), "mf_token_logprobs")
+    _on_index(index, lib.mf_token_logprobs, a, a + 4 * t, a + 8 * t, a + 12 * t, a + 4 * (3 + n) * t, logits.data_ptr(), stride,
+              tokens.data_ptr(), t, v, n, code, *((ws.data_ptr(), ws.numel()) if need else (None, 0)))
     return res
+
+
+@functools.lru_cache(maxsize=1024)
+def _logprob_bytes(*sizes):
+    return _lib.load().mf_token_logprobs_workspace_bytes(*sizes)
 
 
 # --------------------------------------------------------------------------------------------- low-rank adapters
@@ -1063,6 +1095,11 @@ def _host_ints(values):
 @functools.lru_cache(maxsize=1024)
 def _adapter_bytes(*sizes):
     return _lib.load().mf_adapter_workspace_bytes(*sizes)
+
+
+@functools.lru_cache(maxsize=1024)
+def _plan_ints(*sizes):
+    return _lib.load().mf_adapter_rows_ints(*sizes)
 
 
 class AdapterRows(NamedTuple):
@@ -1083,9 +1120,8 @@ def adapter_rows(adapter_ids, n_adapters):
     if not (0 < n <= 1024 and t <= 1 << 20):
         raise ValueError(f"1 to 1024 adapters and up to 2^20 rows, got {n_adapters} and {t}")
     tile = 16 if t <= 1024 else 64                            # prompts share weights and rows among 64, decode rows are of many adapters
-    plan = torch.empty(lib.mf_adapter_rows_ints(t, n, tile), dtype=torch.int32, device=dev)
-    with _on(dev):
-        check(lib.mf_adapter_rows(ptr(plan), ptr(adapter_ids), t, n, tile, stream_ptr(dev)), "mf_adapter_rows")
+    plan = torch.empty(_plan_ints(t, n, tile), dtype=torch.int32, device=dev)
+    _on_index(dev.index, lib.mf_adapter_rows, plan.data_ptr(), adapter_ids.data_ptr(), t, n, tile)
     return AdapterRows(plan, t, n, tile)
 
 
@@ -1121,33 +1157,41 @@ def adapter_linear(x, lora_a, lora_b, rows, base, widths=None, ranks=None, scale
         raise ValueError("ranks must be a contiguous int32 [n] on the adapters' device")
     if scales is not None and not (scales.dtype is torch.float32 and scales.numel() == n and scales.get_device() == index and scales.is_contiguous()):
         raise ValueError("scales must be a contiguous fp32 [n] on the adapters' device")
-    if x.shape[-1:] != (k,) or base.shape[-1:] != (cols,):
-        raise ValueError(f"x must be [T, {k}], base [T, {cols}]")
-    x, xs = (x, k) if x.is_contiguous() else _rows(x, k, "x")
+    x, xs, _ = _wide_rows(x, t, k, "x")
     at = x.data_ptr()
     if at % 16 or xs % 8:                                     # a slice whose rows are not on 16-byte borders
         x, xs = x.reshape(-1, k).clone(memory_format=torch.contiguous_format), k
         at = x.data_ptr()
-    whole = base.is_contiguous()
-    base, bs = (base, cols) if whole else _rows(base, cols, "base")
+    base, bs, whole = _wide_rows(base, t, cols, "base")
     if out is None:
         out = torch.empty_like(base) if whole else base.new_empty(base.shape)
-        got, os = out, cols
+        to, os = out.data_ptr(), cols
     else:
-        got, os = _rows(out, cols, "out")
-    if not (x.numel() == t * k and base.numel() == t * cols and got.numel() == t * cols and got.dtype is dtype):
-        raise ValueError(f"x, base and out must hold the {t} rows that adapter_rows was given, of one type")
+        if out.dtype is not dtype:
+            raise ValueError("out must have base's type")
+        to, os = out.data_ptr(), _wide_rows(out, t, cols, "out")[1]
     if t == 0:
         return out
     pa, pb = lora_a.data_ptr(), lora_b.data_ptr()
     _need((pa | pb) % 16 == 0, "lora_a and lora_b must lie on 16-byte borders")
-    lib, dev = _lib.load(), lora_a.device
-    ws = workspace(_adapter_bytes(t, n, tile, k, slices, r), dev, "adapter")
-    with _on(dev):
-        check(lib.mf_adapter_linear(got.data_ptr(), at, pa, pb, base.data_ptr(), plan.data_ptr(), ptr(ranks), ptr(scales),
-                                    _host_ints(widths), slices, t, n, tile, k, r, xs, bs, os, dtype_code(dtype), ws.data_ptr(),
-                                    ws.numel(), stream_ptr(dev)), "mf_adapter_linear")
+    ws = workspace(_adapter_bytes(t, n, tile, k, slices, r), lora_a.device, "adapter")
+    _on_index(index, _lib.load().mf_adapter_linear, to, at, pa, pb, base.data_ptr(), plan.data_ptr(), None if ranks is None else ranks.data_ptr(),
+              None if scales is None else scales.data_ptr(), _host_ints(widths), slices, t, n, tile, k, r, xs, bs, os,
+              _lib.MF_BF16 if dtype is torch.bfloat16 else _lib.MF_FP16, ws.data_ptr(), ws.numel())
     return out
+
+
+def _wide_rows(x, t, width, what):
+    """x, the distance of its rows of ``width``, and whether they lie one behind the other; checked to be ``t``."""
+    shape = x.shape
+    if len(shape) == 2:                                       # nearly all: two looks at the tensor
+        row, col = x.stride()
+        if shape == (t, width) and col == 1 and (row >= width or t <= 1):
+            return x, row if t > 1 else width, row == width or t <= 1
+    if shape[-1:] != (width,) or x.numel() != t * width:
+        raise ValueError(f"{what} must hold the {t} rows that adapter_rows was given, of {width}")
+    x, row = _rows(x, width, what)
+    return x, row, x.is_contiguous()
 
 
 # --------------------------------------------------------------------------------------------- norm / activation
