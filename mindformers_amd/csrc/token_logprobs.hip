@@ -544,9 +544,12 @@ __global__ __launch_bounds__(TJ_THREADS) void logprob_join_kernel(const void* __
     }
 }
 
-// Columns of a workgroup: 2048 workgroups where there is that much, rows in 64 at most.  Rows up to 32768 columns in one, which saves the second
-// kernel (1 x 32000 with 0, 5, 20 and 64 alternatives: 7, 11.4, 12.6 and 16 us, in eight pieces 5.6, 10.5, 13.3 and 23, beside a call's 3);
-// pieces of 16384 otherwise (1 x 152064 likewise 6.8, 12, 16 and 25 us, in pieces of 4096 5.6, 10.5, 14.5 and 40).
+// A row a workgroup up to 32768 columns, which saves the second kernel (1 x 32000 with 0, 5, 20 and 64 alternatives: 7, 11.4, 12.6 and
+// 16 us, in eight pieces 5.6, 10.5, 13.3 and 23, beside a call's 3), and where there is a row for 384 columns, so that rows alone fill the
+// device (1001 x 151643 fp32 91 us, in two pieces 103; 2000 x 152064 bf16 with 5 alternatives 117, in two 120; 200 x 50000 with 20 18.6, in four
+// 21.6).  Otherwise equal pieces of 16384 at least (1 x 152064 with 0, 5, 20 and 64: 6.8, 12, 16 and 25 us, in pieces of 4096 5.6,
+// 10.5, 14.5 and 40), for 1024 workgroups in all (300 x 152064 bf16 with 5 alternatives in one, two, four and ten: 41.0, 34.4, 30.4 and
+// 34.9).
 struct LogprobPlan {
     int cols, groups;
     size_t x, tok, bytes;
@@ -554,9 +557,10 @@ struct LogprobPlan {
 LogprobPlan logprob_plan(int64_t rows, int64_t vocab, int n, int dtype) {
     constexpr int64_t STEP = TL_WAVES * 64 * 16;              // logits of a workgroup's step, of either width
     const int64_t span = vocab + (dtype == MF_FP32 ? 3 : 7);
-    int64_t cols = std::max<int64_t>(STEP, rows * span / 2048);
-    cols = std::max({cols, (span + TL_MAX_GROUPS - 1) / TL_MAX_GROUPS, span <= 32768 ? span : 16384});
-    cols = std::min((cols + STEP - 1) / STEP * STEP, (span + STEP - 1) / STEP * STEP);
+    int64_t pieces = 1;
+    if (span > 32768 && rows * 384 < span)
+        pieces = std::min({(1024 + rows - 1) / rows, (span + 16383) / 16384, (int64_t)TL_MAX_GROUPS});
+    const int64_t cols = ((span + pieces - 1) / pieces + STEP - 1) / STEP * STEP;
     LogprobPlan p;
     p.cols = (int)cols;
     p.groups = (int)((span + cols - 1) / cols);
