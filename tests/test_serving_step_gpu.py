@@ -565,3 +565,51 @@ def test_rows_and_cache_rows_past_32_bits():
     assert torch.equal(wide[:, :4 * d], q_want) and torch.equal(wide[:, 4 * d:(4 + heads) * d], k_want)
     at = slots.long()
     assert torch.equal(kc.view(-1, heads * d)[at], k_want) and torch.equal(vc.view(-1, heads * d)[at], v)
+
+
+def _bad_rotary():
+    def case(**over):
+        z = lambda *shape, dtype=BF: torch.zeros(*shape, dtype=dtype, device="cuda")  # noqa: E731
+        a = dict(query=z(3, 128), key=z(3, 64), positions=z(3, dtype=torch.int32), inv_freq=z(32, dtype=torch.float64), head_dim=64)
+        for name, value in over.items():
+            a[name] = value(z) if callable(value) else value
+        return a
+    cache = dict(value=lambda z: z(3, 64), key_cache=lambda z: z(2, 4, 1, 64), value_cache=lambda z: z(2, 4, 1, 64),
+                 slot_mapping=lambda z: z(3, dtype=torch.int32))
+    return [case(positions=lambda z: z(3, dtype=torch.int64)), case(inv_freq=lambda z: z(32, dtype=F32)), case(query=lambda z: z(3, 100)),
+            case(query=lambda z: z(3, 128, dtype=F32)), case(query=lambda z: z(4, 128)), case(query=lambda z: z(1, 128).expand(3, 128)),
+            case(query=lambda z: z(128, 3).t()), case(key=lambda z: z(3, 64, dtype=FP)), case(key=lambda z: z(2, 64)),
+            case(key=lambda z: z(3, 64, dtype=BF).cpu()), case(positions=lambda z: z(3, dtype=torch.int32).cpu()), case(offset=1), case(offset=-1),
+            case(head_dim=0), case(inv_freq=lambda z: z(33, dtype=torch.float64)), case(inv_freq=lambda z: z(64, dtype=torch.float64)[::2]),
+            case(value=lambda z: z(3, 64)), case(**{**cache, "slot_mapping": None}), case(**{**cache, "value": lambda z: z(3, 128)}),
+            case(**{**cache, "key_cache": lambda z: z(2, 4, 1, 64, dtype=FP)}), case(**{**cache, "value_cache": lambda z: z(2, 5, 1, 64)}),
+            case(**{**cache, "slot_mapping": lambda z: z(3, dtype=torch.int64)}), case(**{**cache, "slot_mapping": lambda z: z(4, dtype=torch.int32)}),
+            case(**{**cache, "key": None}), case(out=lambda z: (z(3, 128), None)), case(out=lambda z: (z(3, 64), z(3, 64))),
+            case(out=lambda z: (z(3, 128), z(3, 128))), case(key=None, out=lambda z: (z(3, 128), z(3, 64)))]
+
+
+def test_refused_calls_on_the_gpu():
+    for a in _bad_rotary():
+        with pytest.raises(ValueError):
+            ops.rotary_embedding(**a)
+    z = lambda *shape, dtype=BF: torch.zeros(*shape, dtype=dtype, device="cuda")  # noqa: E731
+    t3 = z(3, dtype=torch.int32)
+    for args in ((z(3, 50), t3.long()), (z(3, 50), z(4, dtype=torch.int32)), (z(50), t3), (z(3, 50, dtype=torch.float64), t3), (z(3, 50), t3, 51),
+                 (z(3, 100), t3, 65), (z(3, 50), t3, -1), (z(50, 3).t(), t3), (z(1, 50).expand(3, 50), t3), (z(3, 50), t3.cpu()), (z(3, 0), t3),
+                 (z(3, 50), z(6, dtype=torch.int32)[::2])):
+        with pytest.raises(ValueError):
+            ops.token_logprobs(*args)
+    for args in ((t3.long(), 2), (t3, 0), (t3, 1025), (t3.view(1, 3), 2), (z(6, dtype=torch.int32)[::2], 2)):
+        with pytest.raises(ValueError):
+            ops.adapter_rows(*args)
+    rows = ops.adapter_rows(t3, 2)
+    good = dict(x=z(3, 64), lora_a=z(2, 16, 64), lora_b=z(2, 96, 16), rows=rows, base=z(3, 96))
+    ops.adapter_linear(**good)
+    for over in (dict(x=z(4, 64)), dict(x=z(3, 56)), dict(x=z(3, 64, dtype=FP)), dict(x=z(1, 64).expand(3, 64)), dict(base=z(3, 95)),
+                 dict(base=z(2, 96)), dict(base=z(3, 96).cpu()), dict(base=z(1, 96).expand(3, 96)), dict(out=z(3, 96, dtype=F32)),
+                 dict(out=z(2, 96)), dict(out=z(96, 3).t()), dict(lora_a=z(3, 16, 64)), dict(lora_a=z(2, 12, 64), lora_b=z(2, 96, 12)),
+                 dict(lora_a=z(2, 16, 60), x=z(3, 60)), dict(lora_b=z(2, 96, 8)), dict(lora_b=z(2, 16, 96).transpose(1, 2)), dict(widths=(96, 1)),
+                 dict(widths=(48, 48)), dict(widths=(96, 0)), dict(ranks=z(2, dtype=torch.int64)), dict(ranks=z(3, dtype=torch.int32)),
+                 dict(scales=z(2)), dict(scales=z(1, dtype=F32)), dict(lora_a=z(2, 136, 64), lora_b=z(2, 96, 136))):
+        with pytest.raises(ValueError):
+            ops.adapter_linear(**{**good, **over})
