@@ -147,8 +147,9 @@ __device__ __forceinline__ void rotary_finish(const RotaryArgs& A, RotaryUnit<VE
     }
 }
 
-// What bounds it: memory (8191 rows of 32 + 8 heads of 128 into a cache: 202 MB in 34 us, 5.9 TB/s).  Two units a thread are on their way at
-// once.
+// What bounds it: memory (8191 rows of 32 + 8 heads of 128 into a cache, 202 MB: 33 us where the last pass's rows are still in the last-level
+// cache, 44 otherwise; 16001 rows of 64 + 8 heads of 80, 369 MB: 75 us, 4.9 TB/s).  Two units a thread are on their way at once.  Several rows a
+// workgroup from 2048 on, in one row of units: 81 us for the second with a loop over rows.  One row: 3 us, of which a launch is most.
 template <typename T, int VEC, bool NEAR>
 __global__ __launch_bounds__(RO_THREADS) void rotary_kernel(const RotaryArgs A) {
     extern __shared__ float2 table[];                         // [rows][pairs]: s cos, s sin
