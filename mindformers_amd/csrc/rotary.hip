@@ -15,7 +15,7 @@
 namespace {
 
 constexpr int RO_THREADS = 256;
-constexpr int RO_ROWS = 4;                                    // rows of a workgroup, at most
+constexpr int RO_ROWS = 6;                                    // rows of a workgroup, at most
 constexpr int RO_MAX_PAIRS = 512;
 
 struct RotaryArgs {
@@ -147,9 +147,9 @@ __device__ __forceinline__ void rotary_finish(const RotaryArgs& A, RotaryUnit<VE
     }
 }
 
-// What bounds it: memory (8191 rows of 32 + 8 heads of 128 into a cache, 202 MB: 33 us where the last pass's rows are still in the last-level
-// cache, 44 otherwise; 16001 rows of 64 + 8 heads of 80, 369 MB: 75 us, 4.9 TB/s).  Two units a thread are on their way at once.  Several rows a
-// workgroup from 2048 on, in one row of units: 81 us for the second with a loop over rows.  One row: 3 us, of which a launch is most.
+// What bounds it: memory (8191 rows of 32 + 8 heads of 128 into a cache, 202 MB: 32 us where the last pass's rows are still in the last-level
+// cache, 41 otherwise; 16001 rows of 64 + 8 heads of 80, 369 MB: 72 us, 5.1 TB/s).  Two units a thread are on their way at once.  One row: 3 us,
+// of which a launch is most.
 template <typename T, int VEC, bool NEAR>
 __global__ __launch_bounds__(RO_THREADS) void rotary_kernel(const RotaryArgs A) {
     extern __shared__ float2 table[];                         // [rows][pairs]: s cos, s sin
@@ -242,8 +242,12 @@ extern "C" int mf_rotary_embedding(void* query_out, void* key_out, const void* q
     auto magic = [](int64_t units) { return (uint32_t)((0x100000000ll + units - 1) / units); };
     const int64_t each = (int64_t)(n_heads + n_kv_heads) * A.units + A.v_units;
     A.unit_magic = magic(A.units), A.row_magic = magic(each);
-    // several rows a workgroup where there are enough to fill the device: their angles take its threads at once
-    A.rows = num_tokens >= 2048 ? std::max(1, std::min(RO_ROWS, RO_THREADS / n_pairs)) : 1;
+    // Several rows a workgroup where they are short and there are enough to fill the device: as many as make a turn of its threads, two
+    // units each, and no more angles than threads.  (16001 rows in 1, 2, 4 and 6 a workgroup: 8 + 2 heads of 64, 76 units a row, 18.6, 15.6,
+    // 13.4 and 12.1 us; 7 + 1 of 256, 288 units, 41.0, 34.4, 35.3, 38.9; 32 + 8 of 128, 448 units, 71.1, 76.4, 79.3, 84.8.  2048 rows: 4.6,
+    // 4.4, 4.8, 4.9; 7.2, 7.8, 9.1, 11.1; 10.3, 11.3, 13.2, 16.4.)
+    A.rows = num_tokens < 4096 ? 1 : (int)std::min<int64_t>((2 * RO_THREADS + each / 2) / each, std::min(RO_ROWS, RO_THREADS / n_pairs));
+    A.rows = std::max(A.rows, 1);
     if (each > (1 << 14)) A.rows = 1;                         // the division by them is exact up to 2^32 / each
     const dim3 grid((unsigned)((num_tokens + A.rows - 1) / A.rows));
     const size_t lds = (size_t)A.rows * n_pairs * sizeof(float2);

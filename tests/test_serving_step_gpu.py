@@ -48,7 +48,8 @@ def _check_rotary(got, x, positions, inv, d, near, scale, offset, dtype, what):
 @pytest.mark.parametrize("t,heads,kv,d,pairs,offset", [(1, 32, 8, 128, 64, 0), (5, 28, 4, 128, 32, 0), (3, 7, 1, 80, 10, 0), (4, 4, 2, 64, 16, 32),
                                                        (2, 3, 3, 18, 9, 0), (2, 3, 1, 20, 5, 3), (6, 2, 2, 96, 24, 8), (3, 1, 1, 2, 1, 0),
                                                        (2049, 8, 2, 64, 32, 0), (2050, 3, 1, 256, 128, 0), (1, 1, 1, 1024, 512, 0),
-                                                       (2051, 2, 1, 640, 300, 40)])
+                                                       (2051, 2, 1, 640, 300, 40), (4097, 8, 2, 64, 32, 0), (4098, 3, 1, 256, 128, 0),
+                                                       (4099, 2, 1, 640, 300, 40), (4100, 1, 1, 16, 8, 0), (4101, 3, 1, 80, 10, 5), (5003, 12, 2, 64, 16, 8)])
 def test_rotary_layouts_and_parts(dtype, near, t, heads, kv, d, pairs, offset):
     rng = np.random.default_rng(t * 1000 + d)
     inv = _inv(pairs)
@@ -74,18 +75,18 @@ def test_rotary_far_and_negative_positions():
 
 @pytest.mark.parametrize("near", [False, True])
 @pytest.mark.parametrize("dtype", [BF, FP])
-@pytest.mark.parametrize("pad", [0, 1, 2, 4, 8])
-def test_rotary_of_column_slices_into_a_cache(dtype, near, pad):
+@pytest.mark.parametrize("t,pad", [(37, 0), (37, 1), (37, 2), (37, 4), (37, 8), (4111, 0), (4111, 2), (4111, 8)])
+def test_rotary_of_column_slices_into_a_cache(dtype, near, t, pad):
     """query, key and value as slices of a fused projection whose rows are `pad` columns further apart (every width of access), into outputs
     of their own and the cache; rows of slots outside of it leave the cache as it was."""
     rng = np.random.default_rng(pad)
-    t, h, kv, d, pairs, off = 37, 6, 2, 48, 16, 8
+    h, kv, d, pairs, off = 6, 2, 48, 16, 8
     inv = _inv(pairs)
     wide = rounded(rng.normal(size=(t, (h + 2 * kv) * d + pad)), dtype)
     qkv = _dev(wide, dtype)
     q, k, v = qkv[:, :h * d], qkv[:, h * d:(h + kv) * d], qkv[:, (h + kv) * d:(h + 2 * kv) * d]
     pos = rng.integers(0, 5000, t)
-    nb, bs = 5, 16
+    nb, bs = t // 16 + 3, 16
     slots = rng.permutation(nb * bs)[:t]
     slots[[3, 11, 20]] = [-1, nb * bs, 2 ** 31 - 1]
     kc, vc = (rounded(rng.normal(size=(nb, bs, kv, d)), dtype) for _ in range(2))
