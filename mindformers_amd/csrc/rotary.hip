@@ -14,7 +14,7 @@
 
 namespace {
 
-constexpr int RO_THREADS = 256;
+constexpr int RO_THREADS = 256, RO_MOST_THREADS = 512;
 constexpr int RO_ROWS = 6;                                    // rows of a workgroup, at most
 constexpr int RO_MAX_PAIRS = 512;
 
@@ -36,6 +36,7 @@ struct Piece {
     typedef __attribute__((ext_vector_type(N / 2))) uint32_t vec;
     vec v;
     __device__ __forceinline__ void load(const uint16_t* p) { v = *(const vec*)p; }
+    __device__ __forceinline__ void stream(const uint16_t* p) { v = __builtin_nontemporal_load((const vec*)p); }
     __device__ __forceinline__ void store(uint16_t* p) const { *(vec*)p = v; }
     __device__ __forceinline__ uint16_t at(int i) const { return (uint16_t)(v[i >> 1] >> (16 * (i & 1))); }
     template <typename T>
@@ -147,15 +148,15 @@ __device__ __forceinline__ void rotary_finish(const RotaryArgs& A, RotaryUnit<VE
     }
 }
 
-// What bounds it: memory (8191 rows of 32 + 8 heads of 128 into a cache, 202 MB: 32 us where the last pass's rows are still in the last-level
-// cache, 41 otherwise; 16001 rows of 64 + 8 heads of 80, 369 MB: 72 us, 5.1 TB/s).  Two units a thread are on their way at once.  One row: 3 us,
-// of which a launch is most.
-template <typename T, int VEC, bool NEAR>
-__global__ __launch_bounds__(RO_THREADS) void rotary_kernel(const RotaryArgs A) {
+// What bounds it: memory (8191 rows of 32 + 8 heads of 128 into a cache, 202 MB: 37 us; 16001 rows of 64 + 8 heads of 80, 369 MB: 68 us; 5.4 TB/s,
+// as a copy).  Two units a thread are on their way at once.  One row: 3 us, of which a launch is most.
+template <typename T, int VEC, bool NEAR, bool STREAM>
+__global__ __launch_bounds__(RO_MOST_THREADS) void rotary_kernel(const RotaryArgs A) {
     extern __shared__ float2 table[];                         // [rows][pairs]: s cos, s sin
+    const int threads = blockDim.x;
     const int64_t row0 = (int64_t)blockIdx.x * A.rows;
     const int rows = (int)min((int64_t)A.rows, A.tokens - row0);
-    for (int i = threadIdx.x; i < rows * A.pairs; i += RO_THREADS) {
+    for (int i = threadIdx.x; i < rows * A.pairs; i += threads) {
         const int r = i / A.pairs, p = i - r * A.pairs;
         const double turns = (double)A.positions[row0 + r] * (A.inv_freq[p] * 0.15915494309189535);
         float sn, cn;
@@ -164,18 +165,21 @@ __global__ __launch_bounds__(RO_THREADS) void rotary_kernel(const RotaryArgs A) 
     }
     __syncthreads();
     const int n_q = A.heads * A.units, n_qk = n_q + A.kv_heads * A.units, each = n_qk + A.v_units, all = rows * each;
-    for (int i = threadIdx.x; i < all; i += 2 * RO_THREADS) {
+    for (int i = threadIdx.x; i < all; i += 2 * threads) {
         RotaryUnit<VEC> U[2];
         int r[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            const int j = min(i + k * RO_THREADS, all - 1);
+            const int j = min(i + k * threads, all - 1);
             r[k] = A.rows == 1 ? 0 : each == 1 ? j : (int)__umulhi((uint32_t)j, A.row_magic);
             const int64_t row = row0 + r[k], slot = A.slots ? A.slots[row] : -1;
             const bool cached = slot >= 0 && slot < A.num_slots;
             rotary_take<VEC, NEAR>(A, U[k], j - r[k] * each, n_q, n_qk, row, cached ? slot * A.kv_heads * A.dim : 0, cached);
-            if (i + k * RO_THREADS >= all) U[k].in = nullptr;
-            if (U[k].in) {
+            if (i + k * threads >= all) U[k].in = nullptr;
+            if constexpr (STREAM) {
+                if (U[k].in) U[k].x.stream(U[k].in + U[k].c);
+                if (U[k].in && U[k].d >= 0) U[k].y.stream(U[k].in + U[k].d);
+            } else if (U[k].in) {
                 U[k].x.load(U[k].in + U[k].c);
                 if (U[k].d >= 0) U[k].y.load(U[k].in + U[k].d);
             }
@@ -249,15 +253,23 @@ extern "C" int mf_rotary_embedding(void* query_out, void* key_out, const void* q
     A.rows = num_tokens < 4096 ? 1 : (int)std::min<int64_t>((2 * RO_THREADS + each / 2) / each, std::min(RO_ROWS, RO_THREADS / n_pairs));
     A.rows = std::max(A.rows, 1);
     if (each > (1 << 14)) A.rows = 1;                         // the division by them is exact up to 2^32 / each
+    // long rows of few tokens: a turn of 512 threads (64 rows of 576 units 3.5 us, of 800 3.9; of 256 threads 4.3 and 4.7; 2048 rows 10.5
+    // and 13.3, of 256 threads 9.7 and 13.2)
+    const int threads = each > 2 * RO_THREADS && num_tokens < 2048 ? RO_MOST_THREADS : RO_THREADS;
+    // Inputs that the last-level cache does not keep beside the outputs are read past the caches (32 + 8 heads of 128 behind a copy that
+    // writes them, both: 16001 rows, 197 MB, 145.8 -> 140.8 us, 7000 rows, 86 MB, 54.2 -> 52.6; 4096 rows, 50 MB, 32.5 -> 32.8).  Outputs are not: what
+    // that gains, the attention behind it loses (8191 rows, both 572 -> 575 us).
+    const bool stream_in = (int64_t)num_tokens * (qw + kw + (key_cache ? kw : 0)) * 2 >= 80000000;
     const dim3 grid((unsigned)((num_tokens + A.rows - 1) / A.rows));
     const size_t lds = (size_t)A.rows * n_pairs * sizeof(float2);
     hipStream_t st = (hipStream_t)stream;
-#define RO_LAUNCH(T, N)                                                                                      \
-    do {                                                                                                     \
-        if (vec == 8) hipLaunchKernelGGL((rotary_kernel<T, 8, N>), grid, dim3(RO_THREADS), lds, st, A);      \
-        else if (vec == 4) hipLaunchKernelGGL((rotary_kernel<T, 4, N>), grid, dim3(RO_THREADS), lds, st, A); \
-        else if (vec == 2) hipLaunchKernelGGL((rotary_kernel<T, 2, N>), grid, dim3(RO_THREADS), lds, st, A); \
-        else hipLaunchKernelGGL((rotary_kernel<T, 1, N>), grid, dim3(RO_THREADS), lds, st, A);               \
+#define RO_LAUNCH(T, N)                                                                                                    \
+    do {                                                                                                                   \
+        if (vec == 8 && stream_in) hipLaunchKernelGGL((rotary_kernel<T, 8, N, true>), grid, dim3(threads), lds, st, A); \
+        else if (vec == 8) hipLaunchKernelGGL((rotary_kernel<T, 8, N, false>), grid, dim3(threads), lds, st, A);        \
+        else if (vec == 4) hipLaunchKernelGGL((rotary_kernel<T, 4, N, false>), grid, dim3(threads), lds, st, A);        \
+        else if (vec == 2) hipLaunchKernelGGL((rotary_kernel<T, 2, N, false>), grid, dim3(threads), lds, st, A);        \
+        else hipLaunchKernelGGL((rotary_kernel<T, 1, N, false>), grid, dim3(threads), lds, st, A);                      \
     } while (0)
     if (dtype == MF_BF16) {
         if (interleaved) RO_LAUNCH(BF16, true);

@@ -117,6 +117,31 @@ def test_rotary_of_column_slices_into_a_cache(dtype, near, t, pad):
     assert torch.equal(q_out, first[0]) and torch.equal(k_out, k)
 
 
+@pytest.mark.parametrize("dtype,near,d,pairs", [(BF, False, 128, 64), (FP, True, 128, 32), (BF, True, 80, 10)])
+def test_rotary_of_long_inputs_is_that_of_their_pieces(dtype, near, d, pairs):
+    """Inputs of more than 80 MB, which are read another way, and their thirds: the same bits, into outputs, a cache and in place."""
+    t, h, kv = 10007 * 128 // d, 28, 4
+    gen = torch.Generator(device="cuda").manual_seed(d)
+    qkv = torch.randn(t, (h + 2 * kv) * d, generator=gen, device="cuda").to(dtype)
+    pos, slots = torch.arange(t, dtype=torch.int32, device="cuda") * 7, torch.arange(t, dtype=torch.int32, device="cuda")
+    inv = torch.from_numpy(_inv(pairs)).cuda()
+
+    def turn(cuts):
+        q_out = torch.empty(t, h * d, dtype=dtype, device="cuda")
+        kc, vc = (torch.zeros(t // 16 + 1, 16, kv, d, dtype=dtype, device="cuda") for _ in range(2))
+        rows = qkv.clone()
+        for a, b in zip([0, *cuts], [*cuts, t]):
+            x = rows[a:b]
+            q, k, v = x[:, :h * d], x[:, h * d:(h + kv) * d], x[:, (h + kv) * d:]
+            more = dict(interleaved=near, value=v, key_cache=kc, value_cache=vc, slot_mapping=slots[a:b])
+            ops.rotary_embedding(q, k, pos[a:b], inv, d, out=(q_out[a:b], None), **more)
+            ops.rotary_embedding(q, k, pos[a:b], inv, d, interleaved=near)
+        return q_out, kc, vc, rows
+
+    for whole, thirds in zip(turn([]), turn([t // 3, t // 3 * 2])):
+        assert torch.equal(whole, thirds)
+
+
 def test_rotary_equals_the_cell_of_the_tables_at_near_positions():
     """Against apply_rotary_pos_emb on float32 rows of the same angles: the same formula, within the roundings of both."""
     rng = np.random.default_rng(1)
