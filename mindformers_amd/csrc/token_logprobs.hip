@@ -133,7 +133,7 @@ __device__ __forceinline__ void edge_vector(const RowPiece& p, int v, float* f) 
     for (int e = 0; e < L::VEC; ++e) f[e] = v + e >= p.mis && v + e < p.c1 ? f[e] : -INFINITY;
 }
 
-// the lowest bit of a key that two logits of the type differ in
+// the lowest bit of a key that two logits of the type differ in, but for +inf where it counts as the largest float32
 template <typename L> struct LowBit { static constexpr int value = 0; };
 template <> struct LowBit<Logit16<BF16>> { static constexpr int value = 16; };
 template <> struct LowBit<Logit16<FP16>> { static constexpr int value = 13; };
@@ -252,43 +252,47 @@ __device__ int best_of_piece(const RowPiece& p, TopShared& sh, int per, uint32_t
         if (c > TL_LIST) lo = mid;
         else hi = mid;
     }
-    // Fewer than n above the logits of key `lo`, and more of those than fit: the lowest tokens of them, looked for in order.  (A key's low
-    // bits: all ones of negative values.)
+    // Fewer than n above the logits of key `lo`, and more of those than fit: the lowest tokens of them, looked for in order.
     c = count_from(hi << LOW);
-    lo <<= LOW;
-    const float level = order32_back(lo >> 31 ? lo : lo | ((1u << LOW) - 1));
     constexpr int AT_ONCE = 4;                                // columns a thread
-    for (int v0 = p.c0; v0 < p.c1 && c < n; v0 += AT_ONCE * TL_WAVES * 64) {
-        float x[AT_ONCE];
+    auto take_equal = [&](float level) {
+        for (int v0 = p.c0; v0 < p.c1 && c < n; v0 += AT_ONCE * TL_WAVES * 64) {
+            float x[AT_ONCE];
 #pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j)
-            x[j] = L::at(p.base, min(max(v0 + j * TL_WAVES * 64 + (int)threadIdx.x - p.mis, 0), p.vocab - 1));
-        uint64_t tie[AT_ONCE];
+            for (int j = 0; j < AT_ONCE; ++j)
+                x[j] = L::at(p.base, min(max(v0 + j * TL_WAVES * 64 + (int)threadIdx.x - p.mis, 0), p.vocab - 1));
+            uint64_t tie[AT_ONCE];
 #pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j) {
-            const int v = v0 + j * TL_WAVES * 64 + (int)threadIdx.x;
-            tie[j] = __ballot(v >= p.mis && v < p.c1 && counted(x[j]) == level);
-            if (lane == 0) sh.key[j * TL_WAVES + (threadIdx.x >> 6)] = __popcll(tie[j]);
-        }
-        __syncthreads();
-        int all = 0;
-#pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j) {
-            int before = c + all;
-#pragma unroll
-            for (int i = 0; i < TL_WAVES; ++i) {
-                if (i < (int)(threadIdx.x >> 6)) before += sh.key[j * TL_WAVES + i];
-                all += sh.key[j * TL_WAVES + i];
+            for (int j = 0; j < AT_ONCE; ++j) {
+                const int v = v0 + j * TL_WAVES * 64 + (int)threadIdx.x;
+                tie[j] = __ballot(v >= p.mis && v < p.c1 && counted(x[j]) == level);
+                if (lane == 0) sh.key[j * TL_WAVES + (threadIdx.x >> 6)] = __popcll(tie[j]);
             }
-            before += __popcll(tie[j] & ((1ull << lane) - 1ull));
-            if ((tie[j] >> lane & 1) && before < n) {
-                sh.x[before] = level;
-                sh.tok[before] = v0 + j * TL_WAVES * 64 + (int)threadIdx.x - p.mis;
+            __syncthreads();
+            int all = 0;
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j) {
+                int before = c + all;
+#pragma unroll
+                for (int i = 0; i < TL_WAVES; ++i) {
+                    if (i < (int)(threadIdx.x >> 6)) before += sh.key[j * TL_WAVES + i];
+                    all += sh.key[j * TL_WAVES + i];
+                }
+                before += __popcll(tie[j] & ((1ull << lane) - 1ull));
+                if ((tie[j] >> lane & 1) && before < n) {
+                    sh.x[before] = level;
+                    sh.tok[before] = v0 + j * TL_WAVES * 64 + (int)threadIdx.x - p.mis;
+                }
             }
+            c = min(c + all, n);
+            __syncthreads();
         }
-        c = min(c + all, n);
-        __syncthreads();
-    }
+    };
+    // 16 bits: +inf, which counts as the largest float32, is no value of the type and has bits below LOW.  It comes in front of the type's own
+    // largest, whose upper bits it shares in bf16.
+    if (LOW && lo == order32(counted(INFINITY)) >> LOW) take_equal(counted(INFINITY));
+    lo <<= LOW;
+    take_equal(order32_back(lo >> 31 ? lo : lo | ((1u << LOW) - 1)));     // (a key's low bits: all ones of negative values)
     return c;
 }
 
