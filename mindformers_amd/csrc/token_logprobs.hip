@@ -372,8 +372,9 @@ __global__ __launch_bounds__(TL_WAVES * 64) void logprob_kernel(const void* __re
     }
 
     LaneSums sum;
-    // a lane's largest logit, and that of the steps that make a group (`per` of them) with their count and the group's number
-    const int turns = (p.c1 - p.c0 + TL_WAVES * STEP - 1) / (TL_WAVES * STEP), per = (turns + TL_TURNS - 1) / TL_TURNS;
+    // a lane's largest logit, and that of the steps that make a group (`per` of them; one at least: a row that ends where a piece begins
+    // leaves an empty one behind) with their count and the group's number
+    const int turns = (p.c1 - p.c0 + TL_WAVES * STEP - 1) / (TL_WAVES * STEP), per = max((turns + TL_TURNS - 1) / TL_TURNS, 1);
     float most = -INFINITY, group_most = -INFINITY;
     int steps = 0, step_group = 0;
     auto keep_group = [&] {

@@ -46,3 +46,18 @@ def test_logprobs_of_many_infinite_logits(dtype, v):
     wide[2, :700] = most
     for first in (1, 3):
         _check_logprobs(wide[:, first:first + v - 1], np.array([0, 5, v - 2]), 20)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+@pytest.mark.parametrize("v", [65536, 98304, 131072])
+def test_logprobs_of_rows_that_end_where_a_piece_begins(dtype, v):
+    """The last workgroup of an aligned row has no column then, of others a few."""
+    wide = _logits(3, v + 8, dtype, v)
+    for first in (0, 1, 8):
+        x = wide[:, first:first + v]
+        for n in (0, 5, 64):
+            _check_logprobs(x, np.array([0, v - 1, v // 2]), n)
+    x[0] = float("-inf")
+    x[1, :-3] = float("nan")
+    x[2, -1] = float("inf")
+    _check_logprobs(x, np.array([0, v - 2, v - 1]), 5)
