@@ -265,8 +265,14 @@ class QuantDecodeLayer(nn.Module):
             return y if adapters is None or name not in self.banks else self.banks[name](inp, y, adapters, out=y)
 
         nq, nkv = self.n_head * self.head_dim, self.n_kv_head * self.head_dim
-        n1 = normed if isinstance(normed, torch.Tensor) else ops.rms_norm(x, self.attn_norm, self.eps)
-        qkv = project(n1, "qkv")
+        if self.act_quant and (adapters is None or "qkv" not in self.banks):  # W8A8: the norm feeds the quantised projection only
+            if normed is None:
+                normed = ops.rms_norm_dynamic_quant(x, self.attn_norm, self.eps, self.qkv_smooth, tiled=True)
+            elif isinstance(normed, torch.Tensor):
+                normed = ops.dynamic_quant(normed, self.qkv_smooth, tiled=True)
+            qkv = self._linear(None, "qkv", quantized=normed)
+        else:                                                 # (adapters read the norm itself: what is handed over quantised does not do)
+            qkv = project(normed if isinstance(normed, torch.Tensor) else ops.rms_norm(x, self.attn_norm, self.eps), "qkv")
         q, k, v = qkv[:, :nq], qkv[:, nq:nq + nkv], qkv[:, nq + nkv:]
         if key_cache.dtype == torch.int8:                     # rotate, then quantize into the int8 caches
             if self.kv_scale is None:

@@ -220,10 +220,12 @@ class DecodeStackRunner:
                 raise ValueError(f"{adapter_ids.numel()} adapter_ids for {h.shape[0]} rows")
             more["adapters"] = ops.adapter_rows(adapter_ids.contiguous(), counts.pop())
         for i, layer in enumerate(self.layers):
-            # layer i also computes layer i + 1's attention norm (W8A8: and its quantisation), in the kernel that
-            # finishes its own last projection
+            # layer i also computes layer i + 1's attention norm (W8A8: and its quantisation, unless adapters read the norm itself), in the
+            # kernel that finishes its own last projection
             nxt = self.layers[i + 1] if i + 1 < self.num_layers else None
             chain = nxt is not None and layer.act_quant == nxt.act_quant
+            if chain and nxt.act_quant and "adapters" in more and "qkv" in nxt.banks:
+                chain = False
             nn = None
             if chain:
                 nn = (nxt.attn_norm, nxt.eps, nxt.qkv_smooth) if nxt.act_quant else (nxt.attn_norm, nxt.eps)

@@ -3,7 +3,12 @@ import numpy as np
 import pytest
 import torch
 
-from test_serving_step_gpu import BF, F32, FP, _check_logprobs, _logits
+from test_serving_step_gpu import BF, F32, FP, _check_logprobs, _i32, _logits
+from test_serving_step_modules_gpu import BS, D, HIDDEN, NKV, _layers
+
+from mindformers_amd import ops
+from mindformers_amd.modules import RotaryPositions
+from mindformers_amd.runner import DecodeStackRunner
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +66,45 @@ def test_logprobs_of_rows_that_end_where_a_piece_begins(dtype, v):
     x[1, :-3] = float("nan")
     x[2, -1] = float("inf")
     _check_logprobs(x, np.array([0, v - 2, v - 1]), 5)
+
+
+# ------------------------------------------------------------------------------------------------ the layer and the runner
+@pytest.mark.parametrize("banks", [(), ("wo", "fc2")])
+def test_a_w8a8_layer_takes_the_quantised_norm_it_is_handed(banks):
+    """The norm of other rows than x, so that it shows: as a tensor and quantised, the same bits."""
+    layer, = _layers(1, banks, act_quant=True)
+    x, y = (torch.randn(4, HIDDEN, device="cuda").to(BF) for _ in range(2))
+    kc, vc = (torch.randn(4, BS, NKV, D, device="cuda").to(BF) for _ in range(2))
+    args = (_i32([[0], [1], [2], [3]]), _i32([3, 16, 1, 9]), _i32([2, 31, 32, 56]), None, None)
+    view = dict(rotary=(_i32([2, 15, 0, 8]), RotaryPositions(D, interleaved=True)))
+    if banks:
+        view["adapters"] = ops.adapter_rows(_i32([0, 1, -1, 3]), 5)
+
+    def step(normed):
+        return layer(x, kc.clone(), vc.clone(), *args, normed=normed, **view)
+
+    whole = step(ops.rms_norm(y, layer.attn_norm, layer.eps))
+    assert torch.equal(step(ops.rms_norm_dynamic_quant(y, layer.attn_norm, layer.eps, layer.qkv_smooth, tiled=True)), whole)
+    assert torch.equal(step(ops.rms_norm(x, layer.attn_norm, layer.eps)), step(None)) and not torch.equal(step(None), whole)
+
+
+@pytest.mark.parametrize("banks,norms", [((), 2), (("wo",), 2), (("qkv", "fc1"), 0)])
+def test_a_runner_of_w8a8_layers_makes_each_norm_once(banks, norms, monkeypatch):
+    """Quantised where the layer takes it so, one a layer; none where adapters beside its first projection read the norm itself."""
+    layers = _layers(2, banks, act_quant=True)
+    rot = RotaryPositions(D, rotary_percent=0.5)
+    run = DecodeStackRunner(layers, npu_mem_size=0.002, cpu_mem_size=0, block_size=BS, rotary=rot)
+    x = torch.randn(3, HIDDEN, device="cuda").to(BF)
+    lens, tables, slots = _i32([1, 1, 1]), _i32([[0], [1], [2]]), _i32([0, BS, 2 * BS])
+    ids = _i32([0, -1, 3]) if banks else None
+    calls, real = {}, {n: getattr(ops, n) for n in ("rms_norm", "rms_norm_dynamic_quant")}
+    for name, fn in real.items():
+        monkeypatch.setattr(ops, name, lambda *a, _n=name, _f=fn, **kw: (calls.__setitem__(_n, calls.get(_n, 0) + 1), _f(*a, **kw))[1])
+    got = run.decode(x, lens, tables, slots, adapter_ids=ids)
+    assert calls.get("rms_norm_dynamic_quant", 0) == norms and calls["rms_norm"] == 4 - norms      # the second norm of each layer with them
+    rows = None if ids is None else ops.adapter_rows(ids, 5)
+    h = x
+    for i, layer in enumerate(layers):
+        caches = [torch.zeros_like(run.key_cache[i]) for _ in range(2)]
+        h = layer(h, *caches, tables, lens, slots, None, None, adapters=rows, rotary=(lens - 1, rot))
+    assert torch.equal(got, h)
