@@ -83,6 +83,17 @@ class AdapterBank(nn.Module):
 
     construct = forward
 
+    def _apply(self, fn, *args, **kw):
+        dtype = fn(self.lora_a.new_empty(0)).dtype
+        if dtype not in (torch.bfloat16, torch.float16):      # before anything is converted
+            raise TypeError("adapters are bfloat16 or float16")
+        scales = self.scales
+        super()._apply(fn, *args, **kw)
+        if self.scales.dtype != torch.float32:                # .half() and the like are for the matrices
+            self.scales = scales.to(self.lora_a.device)
+        self.dtype = dtype
+        return self
+
 
 class AdapterLinear(nn.Module):
     """A linear cell (float or quantised) with a bank of adapters beside it: ``forward(x, rows)`` is the cell's output plus each row's

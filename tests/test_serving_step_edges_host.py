@@ -1,0 +1,32 @@
+"""Calls of the serving-step modules at the edges of what their documentation allows, on the CPU."""
+import pytest
+import torch
+
+from mindformers_amd.modules import AdapterBank
+
+BF, FP, I32, F32, F64 = torch.bfloat16, torch.float16, torch.int32, torch.float32, torch.float64
+
+
+def _bank(dtype=BF):
+    return AdapterBank(2, 16, (8, 24), 8, dtype, device="cpu").load(1, [torch.ones(4, 16), None], [torch.ones(8, 4), None], scale=0.3)
+
+
+@pytest.mark.parametrize("convert", [lambda m: m.half(), lambda m: m.to(FP), lambda m: m.to("cpu", FP), lambda m: torch.nn.Sequential(m).half()[0]])
+def test_a_bank_changes_its_matrices_type(convert):
+    """The scales stay float32, as the products take them, and not by way of 16 bits; the ranks whole numbers."""
+    bank = convert(_bank())
+    assert bank.dtype == bank.lora_a.dtype == bank.lora_b.dtype == FP
+    assert bank.scales.dtype == F32 and bank.scales[1] == torch.tensor(0.3) and bank.ranks.dtype == I32 and bank.ranks.tolist() == [0, 4]
+    assert dict(bank.named_buffers())["scales"] is bank.scales
+    bank.load(0, [torch.ones(4, 16), None], [torch.ones(8, 4), None], scale=0.7)
+    assert bank.scales[0] == torch.tensor(0.7) and bank.bfloat16().dtype == BF and bank.scales[0] == torch.tensor(0.7)
+
+
+@pytest.mark.parametrize("convert", [lambda m: m.float(), lambda m: m.double(), lambda m: m.to(F64)])
+def test_a_bank_refuses_other_types_and_stays_as_it_was(convert):
+    bank = _bank()
+    before = {name: t.clone() for name, t in bank.named_buffers()}
+    with pytest.raises(TypeError):
+        convert(bank)
+    assert bank.dtype == BF and all(t.dtype == before[n].dtype and torch.equal(t, before[n]) for n, t in bank.named_buffers())
+    assert bank.to("cpu") is bank and bank.dtype == BF
