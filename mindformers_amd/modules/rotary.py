@@ -224,10 +224,9 @@ class RotaryPositions(nn.Module):
     construct = forward
 
     def _apply(self, fn, *args, **kw):
-        super()._apply(fn, *args, **kw)
-        if self.inv_freq.dtype != torch.float64:              # .half() and the like are for weights
+        if fn(self.inv_freq.new_empty(0)).dtype != torch.float64:             # .half() and the like are for weights; before anything is converted
             raise TypeError("the frequencies of RotaryPositions stay float64")
-        return self
+        return super()._apply(fn, *args, **kw)
 
 
 class FreqsMgr(nn.Module):

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from mindformers_amd.modules import AdapterBank
+from mindformers_amd.modules import AdapterBank, RotaryPositions
 
 BF, FP, I32, F32, F64 = torch.bfloat16, torch.float16, torch.int32, torch.float32, torch.float64
 
@@ -30,3 +30,13 @@ def test_a_bank_refuses_other_types_and_stays_as_it_was(convert):
         convert(bank)
     assert bank.dtype == BF and all(t.dtype == before[n].dtype and torch.equal(t, before[n]) for n, t in bank.named_buffers())
     assert bank.to("cpu") is bank and bank.dtype == BF
+
+
+@pytest.mark.parametrize("convert", [lambda m: m.half(), lambda m: m.float(), lambda m: m.to("cpu", BF)])
+def test_rotary_positions_refuse_other_types_and_stay_as_they_were(convert):
+    rot = RotaryPositions(32, base=5e5, device="cpu")
+    before = rot.inv_freq.clone()
+    with pytest.raises(TypeError):
+        convert(rot)
+    assert rot.inv_freq.dtype == F64 and torch.equal(rot.inv_freq, before)
+    assert rot.to("cpu") is rot and rot.double() is rot and torch.equal(rot.inv_freq, before)
