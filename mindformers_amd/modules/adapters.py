@@ -58,14 +58,14 @@ class AdapterBank(nn.Module):
             if not (ai.dim() == 2 and bi.dim() == 2 and 0 < r <= self.rank and ai.shape[1] == self.in_features and tuple(bi.shape) == (n, r)):
                 raise ValueError(f"lora_a {tuple(ai.shape)} and lora_b {tuple(bi.shape)}: [r, {self.in_features}] and [{n}, r] with r up to {self.rank}")
             most = max(most, r)
-        self.lora_a[slot].zero_()
-        self.lora_b[slot].zero_()
-        at = 0
+        new_a, new_b, at = torch.zeros_like(self.lora_a[slot]), torch.zeros_like(self.lora_b[slot]), 0
         for i, (ai, bi, n) in enumerate(zip(a, b, self.widths)):
             if ai is not None:
-                self.lora_a[slot, i, :ai.shape[0]].copy_(ai)
-                self.lora_b[slot, at:at + n, :ai.shape[0]].copy_(bi)
+                new_a[i, :ai.shape[0]].copy_(ai)
+                new_b[at:at + n, :ai.shape[0]].copy_(bi)
             at += n
+        self.lora_a[slot].copy_(new_a)                        # (only now: the matrices may be the slot's own)
+        self.lora_b[slot].copy_(new_b)
         self.ranks[slot] = most
         self.scales[slot] = float(scale)
         return self

@@ -32,6 +32,20 @@ def test_a_bank_refuses_other_types_and_stays_as_it_was(convert):
     assert bank.to("cpu") is bank and bank.dtype == BF
 
 
+def test_a_slot_takes_its_own_matrices_again():
+    """With another scale, or its slices in another order."""
+    bank = AdapterBank(2, 16, (8, 8), 8, device="cpu")
+    gen = torch.Generator().manual_seed(1)
+    a, b = [torch.randn(r, 16, generator=gen).to(BF) for r in (4, 6)], [torch.randn(8, r, generator=gen).to(BF) for r in (4, 6)]
+    bank.load(1, a, b)
+    own = [bank.lora_a[1, 0, :4], bank.lora_a[1, 1, :6]], [bank.lora_b[1, :8, :4], bank.lora_b[1, 8:, :6]]
+    bank.load(1, *own, scale=0.5)
+    assert all(torch.equal(x, y) for x, y in zip(own[0] + own[1], a + b)) and bank.scales[1] == 0.5
+    bank.load(1, own[0][::-1], own[1][::-1])
+    assert torch.equal(bank.lora_a[1, 0, :6], a[1]) and torch.equal(bank.lora_a[1, 1, :4], a[0]) and (bank.lora_a[1, 1, 4:] == 0).all()
+    assert torch.equal(bank.lora_b[1, :8, :6], b[1]) and torch.equal(bank.lora_b[1, 8:, :4], b[0]) and (bank.lora_b[1, 8:, 4:] == 0).all()
+
+
 @pytest.mark.parametrize("convert", [lambda m: m.half(), lambda m: m.float(), lambda m: m.to("cpu", BF)])
 def test_rotary_positions_refuse_other_types_and_stay_as_they_were(convert):
     rot = RotaryPositions(32, base=5e5, device="cpu")
