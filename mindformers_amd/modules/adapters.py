@@ -97,7 +97,8 @@ class AdapterBank(nn.Module):
 
 class AdapterLinear(nn.Module):
     """A linear cell (float or quantised) with a bank of adapters beside it: ``forward(x, rows)`` is the cell's output plus each row's
-    adapter, ``forward(x)`` the cell's alone."""
+    adapter, ``forward(x)`` the cell's alone.  Where x, and with it the float cells' output, is of another type than the bank (float32 rows
+    beside 16-bit weights), the adapters' part is computed in the bank's and added in the output's."""
 
     def __init__(self, layer, bank):
         super().__init__()
@@ -110,6 +111,12 @@ class AdapterLinear(nn.Module):
 
     def forward(self, x, rows=None, **kw):
         y = self.layer(x, **kw)
-        return y if rows is None else self.bank(x if x.dtype == self.bank.dtype else x.to(self.bank.dtype), y, rows, out=y)
+        if rows is None:
+            return y
+        dtype = self.bank.dtype
+        x = x if x.dtype == dtype else x.to(dtype)
+        if y.dtype != dtype:
+            return (y + self.bank(x, torch.zeros_like(y, dtype=dtype), rows)).to(y.dtype)  # (two 16-bit types: their sum is float32)
+        return self.bank(x, y, rows, out=y)
 
     construct = forward

@@ -3,11 +3,13 @@ import numpy as np
 import pytest
 import torch
 
+from helpers import EPS, dev, to_np
+from oracle import serving as S
 from test_serving_step_gpu import BF, F32, FP, _check_logprobs, _i32, _logits
 from test_serving_step_modules_gpu import BS, D, HIDDEN, NKV, _layers
 
 from mindformers_amd import ops
-from mindformers_amd.modules import RotaryPositions
+from mindformers_amd.modules import AdapterBank, AdapterLinear, ColumnParallelLinear, Linear, RotaryPositions, WeightQuantLinearCell
 from mindformers_amd.runner import DecodeStackRunner
 
 pytestmark = pytest.mark.gpu
@@ -66,6 +68,36 @@ def test_logprobs_of_rows_that_end_where_a_piece_begins(dtype, v):
     x[1, :-3] = float("nan")
     x[2, -1] = float("inf")
     _check_logprobs(x, np.array([0, v - 2, v - 1]), 5)
+
+
+# ------------------------------------------------------------------------------------------------ the cells
+@pytest.mark.parametrize("kind,dtype,x_dtype", [("float", FP, F32), ("float", BF, F32), ("parallel", BF, F32), ("parallel", FP, BF), ("w8", FP, BF),
+                                                ("w8", BF, F32)])
+def test_adapters_beside_a_cell_whose_rows_are_of_another_type(kind, dtype, x_dtype):
+    """The cell's own output, to the bit where a row has no adapter, plus the adapters' part, rounded to the bank's type (the cell's, where the
+    output is of it) and once more to the output's."""
+    rng = np.random.default_rng(2)
+    k, n = 128, 96
+    if kind == "float":
+        layer = Linear(k, n, has_bias=True, compute_dtype=dtype)
+    elif kind == "parallel":
+        layer = ColumnParallelLinear(k, n, compute_dtype=dtype)
+    else:
+        layer = WeightQuantLinearCell(k, n, compute_dtype=dtype).quantize_from_float(torch.randn(n, k))
+    bank = AdapterBank(3, k, n, 8, dtype)
+    bank.load(2, torch.from_numpy(rng.normal(size=(5, k)) / 16).cuda(), torch.from_numpy(rng.normal(size=(n, 5))).cuda(), scale=1.5)
+    x, ids = dev(rng.normal(size=(4, 5, k)), x_dtype), rng.integers(-1, 3, 20)
+    plain = layer(x)
+    got = AdapterLinear(layer, bank)(x, ops.adapter_rows(_i32(ids), 3))
+    assert got.dtype == plain.dtype and got.shape == plain.shape
+    bare = torch.from_numpy(ids != 2).cuda().view(4, 5)
+    assert torch.equal(got[bare], plain[bare])
+    delta, mag = S.adapter_linear(to_np(x.to(dtype)).reshape(20, k), to_np(bank.lora_a), to_np(bank.lora_b), ids, np.zeros((20, n)), (n,),
+                                  to_np(bank.ranks), to_np(bank.scales))
+    want = to_np(plain).reshape(20, n) + delta
+    # half a step of the adapters' part and of the output; the second product's operand and the float32 sums as in the product's own test
+    tol = EPS[dtype] * np.abs(delta) + EPS.get(plain.dtype, 2.0 ** -24) * np.abs(want) + 2.0 ** -14 * mag + 2.0 ** -25
+    assert (np.abs(to_np(got).reshape(20, n) - want) <= tol).all()
 
 
 # ------------------------------------------------------------------------------------------------ the layer and the runner
