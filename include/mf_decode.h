@@ -63,8 +63,8 @@ int mf_rope_rows(void* cos, void* sin, const int32_t* positions, const float* in
  * column `offset` on become scale * (a cos t - b sin t, b cos t + a sin t), t = positions[token] * inv_freq[pair] (radians, float64
  * [n_pairs]); the other columns pass.  interleaved 0: a pair is columns (i, i + n_pairs) of the part, otherwise (2i, 2i + 1).  Angles
  * in 64 bits, products in fp32, rounded once.  query, key, value: rows of n_heads / n_kv_heads / n_kv_heads x head_dim, *_row_stride
- * elements apart (0 = dense).  query_out, key_out: where they go, the inputs themselves (in place) or memory of their own; key_out may
- * be NULL, and without a key (n_kv_heads 0) so is key.  With caches (and value and slot_mapping) the key's and the value's rows also go
+ * elements apart (0 = dense).  query_out, key_out: where they go, the inputs themselves (in place) or memory of their own, of which
+ * none of the others (query, key, value, the caches) has a part; key_out may be NULL, and without a key (n_kv_heads 0) so is key.  With caches (and value and slot_mapping) the key's and the value's rows also go
  * to the cache rows slot_mapping names, as in mf_reshape_and_cache; slots outside [0, num_slots) are skipped. */
 int mf_rotary_embedding(void* query_out, void* key_out, const void* query, const void* key, const void* value, void* key_cache,
                         void* value_cache, const int32_t* positions, const double* inv_freq, const int32_t* slot_mapping,

@@ -237,6 +237,10 @@ extern "C" int mf_rotary_embedding(void* query_out, void* key_out, const void* q
     A.v_stride = v_row_stride > 0 ? v_row_stride : kw;
     MF_REQUIRE(A.q_stride >= qw && A.q_out_stride >= qw && A.k_stride >= kw && A.k_out_stride >= kw && A.v_stride >= kw,
                "rotary_embedding: rows overlap");
+    MF_REQUIRE(num_tokens == 1 || ((query_out != query || A.q_out_stride == A.q_stride) && (!key_out || key_out != key || A.k_out_stride == A.k_stride)),
+               "rotary_embedding: an output is its input with rows of another distance");
+    MF_REQUIRE(query_out != key_out && query_out != key && key_out != query && (!value || (value != query_out && value != key_out)),
+               "rotary_embedding: query, key and value share memory that is written");
     A.num_slots = num_slots, A.tokens = num_tokens, A.heads = n_heads, A.kv_heads = n_kv_heads, A.dim = head_dim, A.pairs = n_pairs;
     A.offset = offset, A.scale = scale;
     const int vec = rotary_vec(A, interleaved != 0);

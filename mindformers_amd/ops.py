@@ -184,7 +184,7 @@ def rotary_embedding(query, key, positions, inv_freq, head_dim, interleaved=Fals
     ``key`` [T, n_kv * D] (or None) the 2 * len(inv_freq) columns from ``offset`` on are turned in pairs by positions[t] * inv_freq[i]
     radians and multiplied with ``scale``; the others pass.  A pair is columns (i, i + len(inv_freq)) of that part, or (2 i, 2 i + 1) with
     ``interleaved``.  positions int32 [T], inv_freq float64.  In place, or into ``out`` = (query_out, key_out or None), which share no
-    memory with the inputs.  With ``key_cache`` / ``value_cache`` [num_blocks, block_size, n_kv, D] the turned key and ``value`` go to
+    memory with the inputs; in place query, key and value share none with each other.  With ``key_cache`` / ``value_cache`` [num_blocks, block_size, n_kv, D] the turned key and ``value`` go to
     the rows that ``slot_mapping`` names as well (a negative slot: to none).  Returns (query, key) where they went."""
     index, dtype, d, t, pairs = query.get_device(), query.dtype, int(head_dim), positions.numel(), inv_freq.numel()
     if not (index >= 0 and positions.get_device() == index and inv_freq.get_device() == index and positions.is_contiguous()

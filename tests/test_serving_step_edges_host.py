@@ -1,6 +1,10 @@
-"""Calls of the serving-step modules at the edges of what their documentation allows, on the CPU."""
+"""Calls of the serving-step operators and modules at the edges of what their documentation allows, on the CPU (nothing is launched)."""
+import ctypes
+
 import pytest
 import torch
+
+from test_serving_step_host import _rotary
 
 from mindformers_amd.modules import AdapterBank, RotaryPositions
 
@@ -54,3 +58,18 @@ def test_rotary_positions_refuse_other_types_and_stay_as_they_were(convert):
         convert(rot)
     assert rot.inv_freq.dtype == F64 and torch.equal(rot.inv_freq, before)
     assert rot.to("cpu") is rot and rot.double() is rot and torch.equal(rot.inv_freq, before)
+
+
+def _at(i):
+    """Addresses that no check reads through."""
+    return ctypes.c_void_p(0x10000 * (i + 1))
+
+
+@pytest.mark.parametrize("over", [dict(k=_at(0), k_out=_at(0)), dict(k=_at(0), k_out=None, **{n: _at(4 + i) for i, n in enumerate(("kc", "vc", "v", "slots"))}),
+                                  dict(v=_at(1), kc=_at(5), vc=_at(6), slots=_at(7), num=64), dict(v=_at(0), kc=_at(5), vc=_at(6), slots=_at(7), num=64),
+                                  dict(q_out=_at(1), k_out=_at(4)), dict(q_out=_at(4), k_out=_at(0)), dict(q_out=_at(4), k_out=_at(4)), dict(qs=128, qos=192),
+                                  dict(ks=64, kos=128)])
+def test_rotary_positions_refuse_shared_memory_that_is_written(over):
+    """In place the query, the key and the value are read while the others are written; an output with its input's address has its rows."""
+    rc, msg = _rotary(**{**dict(q_out=_at(0), q=_at(0), k_out=_at(1), k=_at(1), pos=_at(2), inv=_at(3), num=64), **over})
+    assert rc == 1 and msg.startswith("rotary_embedding") and ("share" in msg or "distance" in msg), msg
