@@ -352,7 +352,8 @@ __device__ __forceinline__ int slice_of(const AdapterArgs& A, int& block, int bl
 // and once with lo; its results go through LDS (of the wave's own) into rows of 128 bytes, eight lanes each, as base and out are moved.  A
 // group's first 64 ranks of B and its base rows are loaded behind the products and the results of the group before it, the first one's
 // in front of the sums of h (two groups ahead: no faster).  Workgroups go along the rows: over rows first, 2% slower, their pieces
-// of 2 KB lying a row apart.  Of prompts it is as fast as a copy of base to out.
+// of 2 KB lying a row apart.  Of 8191 rows of three adapters of rank 32, 6144 and 4096 columns, it takes 48 and 35 us, a copy of base to out
+// 39 and 27: every 16 rows load their columns' B anew, with 32 ranks as many bytes as base and out.
 constexpr int AD_PITCH = AD_GROUP + 4;                        // floats of a row of results
 template <typename T>
 __global__ __launch_bounds__(AD_WAVES * 64) void adapter_expand_kernel(const AdapterArgs A) {

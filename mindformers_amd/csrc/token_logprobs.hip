@@ -4,8 +4,9 @@
 //   rank(v) = number of tokens u with x[u] > x[v], or x[u] = x[v] and u < v
 //
 // One pass over the logits for the sums, the rank and the largest logit of every lane's steps; the best ones are looked for behind it, in
-// those steps of lanes whose largest reaches the n-th largest of the workgroup's 256 lanes: some more than n times 16 logits, read once
-// more.  (4137 x 152064 bf16 with 5, 20 and 64 alternatives: 211, 215 and 228 us; whole lanes read again, of whose 16 bytes a step
+// those groups of a lane's steps whose largest reaches the n-th largest of the workgroup's 256 lanes.  A group is one step of 16 logits for
+// each 98304 columns of the piece or part of them (24 groups a lane at most), so that is n times 16, 32, ... logits, read once more, and those of
+// groups whose largest has the upper 16 bits of that bound.  (4137 x 152064 bf16 with 5, 20 and 64 alternatives: 211, 215 and 228 us; whole lanes read again, of whose 16 bytes a step
 // memory gives 128, 220, 297 and 403; a list kept on the way 280, 347 and 545; without alternatives 215; of rows of equal logits, which
 // reach it all, 233, 230 and 235.)  The waves of a workgroup take the steps of a piece of a
 // row in turn; each lane's sums are about a reference m of its own (moved when a logit passes it by more than 8: the sums stay

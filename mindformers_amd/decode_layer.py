@@ -91,7 +91,8 @@ class QuantDecodeLayer(nn.Module):
     def set_adapters(self, banks):
         """Low-rank adapters beside this layer's projections: ``banks`` maps names out of NAMES to ``AdapterBank``s of as many slots each
         (slices, where a bank has them: q, k and v of "qkv", gate and up of "fc1").  A step that brings ``adapters`` (``ops.adapter_rows``)
-        adds every row's; one without is the layer's own."""
+        adds every row's; one without is the layer's own.  Before a step is captured into a graph: where fc1 gets or loses its bank in a
+        weight-only layer, its weights are packed anew."""
         for name, bank in banks.items():
             if name not in self.NAMES:
                 raise ValueError(f"no projection {name!r}: {self.NAMES}")
