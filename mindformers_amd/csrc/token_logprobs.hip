@@ -23,6 +23,7 @@ constexpr int TL_MAX_GROUPS = 64;                             // workgroups of a
 constexpr int TL_MAX_N = 64;                                  // alternatives
 constexpr int TL_LIST = 512;                                  // logits that a workgroup ranks at a time
 constexpr int TL_TURNS = 24;                                  // groups of steps that lanes' largest logits are kept of
+constexpr int TL_LATE = 8;                                    // steps whose sums are added up by themselves
 constexpr int TL_HITS = 1024;                                 // (lane, group)s that are looked into at once
 constexpr int64_t TL_MAX_VOCAB = 0x7c000000;                  // a column a piece behind the last in 32 bits
 
@@ -52,15 +53,23 @@ __device__ __forceinline__ void sums_to(RowSums& s, float m) {
 }
 
 // A lane's sums while it walks, in units of log 2: an exponent is x LOG2E - refl, one operation, with the product ref LOG2E rounded
-// once, to refl; `rest` is what that left out, which the sums make good when they are taken out.
+// once, to refl; `rest` is what that left out, which the sums make good when they are taken out.  The logits of a step are added up by
+// themselves, and TL_LATE steps of them: hundreds of like terms of a rounding's size beside one sum would all be rounded one way
+// (147000 logits 18 below a peak: log probabilities off by 3e-5).
 struct LaneSums {
-    float ref = 0.f, refl = 0.f, rest = 0.f, z = 0.f, w = 0.f;
+    float ref = 0.f, refl = 0.f, rest = 0.f, z = 0.f, w = 0.f, late_z = 0.f, late_w = 0.f;
     bool has = false;                                         // a finite logit was seen: ref is one
+    __device__ __forceinline__ void take_late() {
+        z += late_z;
+        w += late_w;
+        late_z = late_w = 0.f;
+    }
     __device__ __forceinline__ RowSums out(int above) const {
         const float e = __builtin_amdgcn_exp2f(-rest);
         return {has ? ref : -INFINITY, z * e, (w - rest * z) * e * LN2, above};
     }
     __device__ __forceinline__ void move(float to) {
+        take_late();
         RowSums s = out(0);
         sums_to(s, to);
         has = true;
@@ -373,6 +382,7 @@ __global__ __launch_bounds__(TL_WAVES * 64) void logprob_kernel(const void* __re
     }
 
     LaneSums sum;
+    int late = 0;
     // a lane's largest logit, and that of the steps that make a group (`per` of them; one at least: a row that ends where a piece begins
     // leaves an empty one behind) with their count and the group's number
     const int turns = (p.c1 - p.c0 + TL_WAVES * STEP - 1) / (TL_WAVES * STEP), per = max((turns + TL_TURNS - 1) / TL_TURNS, 1);
@@ -410,22 +420,26 @@ __global__ __launch_bounds__(TL_WAVES * 64) void logprob_kernel(const void* __re
             if (moves) sum.move(mx);
         }
         // 2^-150 is no float32 any more; -inf and NaN end there too
+        float step_z[2] = {}, step_w[2] = {};
         if (!__ballot(!(fabsf(sum.ref) < FAR))) {
 #pragma unroll
             for (int k = 0; k < E; ++k) {
                 const float d = fmaxf(fmaf(f[k], LOG2E, -sum.refl), -150.f), e = __builtin_amdgcn_exp2f(d);
-                sum.z += e;
-                sum.w = fmaf(d, e, sum.w);
+                step_z[k & 1] += e;
+                step_w[k & 1] = fmaf(d, e, step_w[k & 1]);
             }
         } else {
 #pragma unroll
             for (int k = 0; k < E; ++k) {
                 const float x = fabsf(sum.ref) < FAR ? fmaf(f[k], LOG2E, -sum.refl) : (f[k] - sum.ref) * LOG2E;
                 const float d = fmaxf(x, -150.f), e = __builtin_amdgcn_exp2f(d);
-                sum.z += e;
-                sum.w = fmaf(d, e, sum.w);
+                step_z[k & 1] += e;
+                step_w[k & 1] = fmaf(d, e, step_w[k & 1]);
             }
         }
+        sum.late_z += step_z[0] + step_z[1];
+        sum.late_w += step_w[0] + step_w[1];
+        if (++late % TL_LATE == 0) sum.take_late();
         if (__ballot(mx > counts)) {
 #pragma unroll
             for (int u = 0; u < VECS; ++u) {
@@ -436,6 +450,7 @@ __global__ __launch_bounds__(TL_WAVES * 64) void logprob_kernel(const void* __re
         }
     }
     // ---- the wave's sums, the workgroup's
+    sum.take_late();
     RowSums s = sum.out(above);
     sums_to(s, wave_max(s.m));
     s.z = wave_sum(s.z);

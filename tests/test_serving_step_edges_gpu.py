@@ -70,6 +70,26 @@ def test_logprobs_of_rows_that_end_where_a_piece_begins(dtype, v):
     _check_logprobs(x, np.array([0, v - 2, v - 1]), 5)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("t,v", [(40, 32000), (31, 47603), (400, 151643)])
+def test_sums_of_many_equal_small_terms_beside_a_large_one(dtype, t, v):
+    """Each lane begins at 0, goes on with logits of one low value, and one meets a peak: thousands of like terms of a rounding's size beside a
+    sum, whose errors all go one way.  Against the sums over the three values in float64; the tolerance is that of the other rows."""
+    low = torch.linspace(-10.0, -5.0, t).to(dtype)
+    peak = torch.linspace(7.9, 4.0, t).to(dtype)
+    x = low[:, None].repeat(1, v)
+    x[:, :4096:4] = 0.0
+    x[:, 7003] = peak
+    counts, values = np.array([[v - 1025, 1024, 1]]), np.stack([to_np(low), np.zeros(t), to_np(peak)], 1).astype(np.float64)
+    mass = counts * np.exp(values)
+    lp = values - np.log(mass.sum(axis=1, keepdims=True))
+    entropy = -(mass / mass.sum(axis=1, keepdims=True) * lp).sum(axis=1)
+    got = ops.token_logprobs(x.cuda(), _i32([7003] * t), n_top=1)
+    for a, b in ((got.logprobs, lp[:, 2]), (got.top_logprobs[:, 0], lp[:, 2]), (got.entropy, entropy)):
+        err = np.abs(to_np(a) - b)
+        assert (err <= 4e-6 + 4 * 2.0 ** -24 * np.abs(b)).all(), err.max()
+
+
 # ------------------------------------------------------------------------------------------------ the cells
 @pytest.mark.parametrize("kind,dtype,x_dtype", [("float", FP, F32), ("float", BF, F32), ("parallel", BF, F32), ("parallel", FP, BF), ("w8", FP, BF),
                                                 ("w8", BF, F32)])
